@@ -564,6 +564,85 @@ int gwa_dit_attention(const void* q, int64_t ldq, const void* k, int64_t ldk, co
                       int64_t ldo, int64_t S, int64_t Skv, int64_t heads, int64_t head_dim, float scale,
                       void* stream);
 
+/* ---- Rotary positions and a paged key/value cache ----------------------------
+ * No counterpart in the reference, whose layers are a denoiser's: what a decoder
+ * on the same quantized linears needs beside them.
+ *
+ * A cache is a pool of pages, each page_size key slots of every kv head; a
+ * sequence's keys are slots 0 .. kv_len - 1 of the pages its row of `table`
+ * lists. New tokens come packed: those of sequence b are rows q_start[b] ..
+ * q_start[b + 1] - 1, and their keys are the sequence's last ones (token i of n
+ * sits in slot kv_len - n + i), written before attention reads them.
+ * The device arrays (table, q_start, kv_len) are trusted for their meaning but
+ * not for memory: page ids are clamped into the pool, lengths into
+ * [0, table_width * page_size], q_start into [0, tokens]. */
+typedef struct gwa_paged_cache {
+  void* k;                /* [pages][kv_heads][page_size][head_dim] at the strides below */
+  void* v;                /* at the same strides */
+  float* w;               /* [pages][kv_heads][page_size] gathered attention weight, or NULL */
+  const int32_t* table;   /* [batch][table_width] page ids at row stride table_stride */
+  const int32_t* q_start; /* [batch + 1]; not read by gwa_paged_evict */
+  const int32_t* kv_len;  /* [batch] */
+  int64_t page_stride, head_stride, slot_stride; /* k and v, elements; multiples of 8 */
+  int64_t w_page_stride, w_head_stride;          /* w, elements */
+  int64_t pages, table_stride, table_width, batch;
+  int page_size;          /* a power of two, 8 .. 4096 */
+  int kv_heads, head_dim; /* head_dim % 8 == 0, 8 .. 256 */
+  int dtype;              /* GWA_DT_BF16 or GWA_DT_F16: k, v, and the q / k / v / o of the calls */
+} gwa_paged_cache;
+
+/* y = x with the first `rot` channels of every head rotated by its token's
+ * position: pairs (2i, 2i+1) with `interleaved`, else (i, i + rot/2), by the
+ * angle whose cosine / sine are cos_t / sin_t [table_rows, rot/2] (fp32) at row
+ * positions[t] (the token's index where positions is NULL; clamped into the
+ * table); `inverse` rotates back, which is also the gradient. Channels past rot
+ * are copied. x, y [tokens, heads, head_dim] at token / head strides (elements),
+ * y may be x; fp32 arithmetic, one rounding. dtype bf16, fp16 or fp32. */
+int gwa_rotary_embed(const void* x, int64_t ldxt, int64_t ldxh, const float* cos_t, const float* sin_t,
+                     int64_t table_rows, const int32_t* positions, void* y, int64_t ldyt, int64_t ldyh,
+                     int64_t tokens, int64_t heads, int64_t head_dim, int64_t rot, int interleaved, int inverse,
+                     int dtype, void* stream);
+
+/* New tokens into the cache: q_out = rotated q (contiguous [tokens, heads,
+ * head_dim]), rotated k and plain v into the tokens' slots, and 0 into the slots'
+ * gathered weights where the cache has them. rot == 0 rotates nothing (cos_t and
+ * sin_t may be NULL). A token whose slot would be negative (kv_len < its
+ * sequence's new tokens) or past the table is rotated but not stored. No two
+ * sequences of a call may list one page for slots that they write. */
+int gwa_paged_write(const gwa_paged_cache* cache, const void* q, int64_t ldqt, int64_t ldqh, const void* k,
+                    int64_t ldkt, int64_t ldkh, const void* v, int64_t ldvt, int64_t ldvh, const float* cos_t,
+                    const float* sin_t, int64_t table_rows, const int32_t* positions, void* q_out, int64_t tokens,
+                    int64_t heads, int64_t rot, int interleaved, void* stream);
+
+/* Attention of the new tokens over the cache: query head x reads kv head
+ * x / (heads / kv_heads); token i of n in a sequence of L keys sees keys
+ * 0 .. L - n + i with `causal`, else all L. o[t][x] = sum_j p_j v_j with
+ * p = softmax(scale * q . k), lse[t][x] = log sum_j exp(scale * q . k) (natural,
+ * fp32); a row that sees no key gives o = 0 and lse = -inf. With `gather`,
+ * w[key] += the sum of p over the sequence's new tokens and the kv head's query
+ * heads, in a fixed order (sequences of one call must not share pages then).
+ * fp32 scores, statistics and sums; p is rounded to the cache's dtype for the
+ * product with v. max_q / max_kv: the largest new-token count and kv_len of the
+ * batch as the host knows them; they shape the launch only (larger device values
+ * are still served). o contiguous [tokens, heads, head_dim], lse [tokens, heads].
+ * workspace: gwa_paged_attention_workspace bytes, 16-byte aligned; no state is
+ * kept in it. */
+int64_t gwa_paged_attention_workspace(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
+                                      int64_t head_dim, int64_t max_q, int64_t max_kv, int gather);
+int gwa_paged_attention(const gwa_paged_cache* cache, const void* q, int64_t ldqt, int64_t ldqh, void* o, float* lse,
+                        int64_t tokens, int64_t heads, int64_t max_q, int64_t max_kv, float scale, int causal,
+                        int gather, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Per sequence and kv head with more than `budget` keys: keeps the last `recent`
+ * and, of the others, the budget - recent of largest w (equal ones: the lowest
+ * slots; a NaN ranks above every number), and copies the kept rows of k, v and w
+ * in slot order into the pages of new_table [batch][new_width] (pages that no
+ * sequence of `table` uses); shorter sequences are copied whole. kept
+ * [batch][kv_heads][budget] int32: the old slots, -1 past new_len; new_len
+ * [batch] = min(kv_len, budget). */
+int gwa_paged_evict(const gwa_paged_cache* cache, const int32_t* new_table, int64_t new_stride, int64_t new_width,
+                    int64_t max_kv, int64_t budget, int64_t recent, int32_t* kept, int32_t* new_len, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -42,6 +42,17 @@ _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _flt = ctypes.c_float
 
+class PagedCacheArgs(ctypes.Structure):
+    """``gwa_paged_cache`` of the header."""
+
+    _fields_ = [("k", _vp), ("v", _vp), ("w", _vp), ("table", _vp), ("q_start", _vp), ("kv_len", _vp),
+                ("page_stride", _i64), ("head_stride", _i64), ("slot_stride", _i64), ("w_page_stride", _i64),
+                ("w_head_stride", _i64), ("pages", _i64), ("table_stride", _i64), ("table_width", _i64),
+                ("batch", _i64), ("page_size", _int), ("kv_heads", _int), ("head_dim", _int), ("dtype", _int)]
+
+
+_cache = ctypes.POINTER(PagedCacheArgs)
+
 # name -> argtypes (all return int status unless listed in _RESTYPES)
 _SIGNATURES: dict[str, tuple] = {
     "gwa_version": (),
@@ -98,13 +109,22 @@ _SIGNATURES: dict[str, tuple] = {
     "gwa_nvfp4_quant_act_dyn": (_vp, _i64, _vp, _vp, _vp, _vp, _int, _vp, _i64, _i64, _vp),
     "gwa_nvfp4_dequant": (_vp, _vp, _int, _vp, _i64, _i64, _vp),
     "gwa_nvfp4_scale_bias": (_vp, _vp, _vp, _vp, _i64, _i64, _vp),
+    "gwa_rotary_embed": (_vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _int, _int,
+                         _int, _vp),
+    "gwa_paged_write": (_cache, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _i64,
+                        _i64, _i64, _int, _vp),
+    "gwa_paged_attention_workspace": (_i64, _i64, _i64, _i64, _i64, _i64, _i64, _int),
+    "gwa_paged_attention": (_cache, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _flt, _int, _int, _vp, _i64,
+                            _vp),
+    "gwa_paged_evict": (_cache, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp),
 }
 _RESTYPES = {"gwa_build_info": ctypes.c_char_p, "gwa_last_error": ctypes.c_char_p,
              "gwa_svdq_quant_fp6_partials": ctypes.c_int64, "gwa_svdq_gemm_w4a4_fp6_next_partials": ctypes.c_int64,
              "gwa_nvfp4_blocked_scale_numel": ctypes.c_int64, "gwa_svdq_w4a4_linear_fp6_workspace": ctypes.c_int64,
              "gwa_svdq_w4a4_linear_fp6_noalloc_scratch_bytes": ctypes.c_int64,
              "gwa_svdq_quant_fp6_la_workspace": ctypes.c_int64,
-             "gwa_svdq_w4a4_linear_gemv_workspace": ctypes.c_int64}
+             "gwa_svdq_w4a4_linear_gemv_workspace": ctypes.c_int64,
+             "gwa_paged_attention_workspace": ctypes.c_int64}
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 
