@@ -625,10 +625,10 @@ int gwa_paged_write(const gwa_paged_cache* cache, const void* q, int64_t ldqt, i
  * product with v. max_q / max_kv: the largest new-token count and kv_len of the
  * batch as the host knows them; they shape the launch only (larger device values
  * are still served). o contiguous [tokens, heads, head_dim], lse [tokens, heads].
- * workspace: gwa_paged_attention_workspace bytes, 16-byte aligned; no state is
- * kept in it. */
+ * workspace: gwa_paged_attention_workspace bytes (capacity = table_width *
+ * page_size), 16-byte aligned; no state is kept in it. */
 int64_t gwa_paged_attention_workspace(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
-                                      int64_t head_dim, int64_t max_q, int64_t max_kv, int gather);
+                                      int64_t head_dim, int64_t max_q, int64_t max_kv, int64_t capacity, int gather);
 int gwa_paged_attention(const gwa_paged_cache* cache, const void* q, int64_t ldqt, int64_t ldqh, void* o, float* lse,
                         int64_t tokens, int64_t heads, int64_t max_q, int64_t max_kv, float scale, int causal,
                         int gather, void* workspace, int64_t workspace_bytes, void* stream);

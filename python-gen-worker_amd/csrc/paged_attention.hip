@@ -1,9 +1,52 @@
 // Attention of new tokens over a paged key/value cache, with the keys' attention weight gathered on request.
-#include "paged_common.h"
+#include <type_traits>
+
+#include "paged_mfma.h"
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// One call's operands, as the matrix-core kernels take them. Partial results of key split s: o_part
+// [s][tokens * heads][D] (fp32, each normalised by its own sum) and lse_part [s][tokens * heads] (log2 domain).
+struct AttnArgs {
+  PagedArgs c;
+  const uint16_t* q;
+  int64_t ldqt, ldqh;
+  uint16_t* o;
+  float* lse;
+  float* o_part;
+  float* lse_part;
+  float* scores;          // [tokens * heads][score_stride] in the log2 domain, or NULL
+  int64_t score_stride;
+  int tokens, heads, splits, split_keys, tiles;
+  float c_log2;
+  int causal;
+};
+
+// s + the dot product of eight 16-bit elements each, fp32
+template <class T>
+__device__ __forceinline__ float dot8(v4i x, v4i y, float s) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    s = fmaf(T::load((uint16_t)x[e]), T::load((uint16_t)y[e]), s);
+    s = fmaf(T::load((uint16_t)((uint32_t)x[e] >> 16)), T::load((uint16_t)((uint32_t)y[e] >> 16)), s);
+  }
+  return s;
+}
+
+// A row's result: into o and lse, or into its split's partials. `d0`: the first of 4 channels in o4.
+template <class T, int D>
+__device__ __forceinline__ void put_o(const AttnArgs& a, int split, int64_t row, int d0, float x, float y, float z,
+                                      float w) {
+  if (a.splits > 1)
+    *(float4*)(a.o_part + ((int64_t)split * a.tokens * a.heads + row) * D + d0) = make_float4(x, y, z, w);
+  else
+    *(uint2*)(a.o + row * D + d0) = make_uint2((uint32_t)Mfma<T>::pack(x, y), (uint32_t)Mfma<T>::pack(z, w));
+}
+__device__ __forceinline__ void put_lse(const AttnArgs& a, int split, int64_t row, float m, float l) {
+  const float lse2 = m == -INFINITY ? -INFINITY : m + __builtin_amdgcn_logf(l);
+  if (a.splits > 1) a.lse_part[(int64_t)split * a.tokens * a.heads + row] = lse2;
+  else a.lse[row] = lse2 * kLn2;
+}
 
 // ---------------------------------------------------------------------------
 // any head_dim: one wave per (new token, query head)
@@ -109,10 +152,680 @@ __global__ __launch_bounds__(64) void paged_gather_rows_kernel(PagedArgs c, cons
   }
 }
 
+// ---------------------------------------------------------------------------
+// head_dim 64 and 128, many rows: MFMA 32x32x16, 32 rows a wave
+// ---------------------------------------------------------------------------
+// One pass over the keys with a running softmax. A workgroup of NW waves owns 32 NW rows (new token, query head of the
+// group) of one sequence and kv head and walks its keys in tiles of BN, double buffered in LDS by direct copies
+// whose lanes look their key's page up a tile ahead. Per tile a wave computes, with fp32 accumulators:
+//   S^T = K q^T           (keys x rows: a lane holds one row, 16 keys of each 32)
+//   p   = 2^(S c - m)     (m: the row's running maximum; O and the sum l are rescaled where it moves)
+//   O^T = O^T + V^T p^T   (V^T by transposing reads, in the key order S^T leaves p in, so p stays in registers)
+// Tiles that every row of the workgroup sees whole run without a mask; the others compare each score's key with the
+// lane's limit. There 0 * v of a hidden key must not reach O: whoever copied a part of the tile sets values that are not
+// finite to 0 and says so, and rows that do see such a key get its values added one by one.
+template <int D, int BN, int NW>
+struct TileShape {
+  static constexpr int kRow = 2 * D, kRun = 1024 / kRow;  // row bytes; rows a 1 KB copy covers
+  static constexpr int kRuns = BN / kRun / NW;            // copies a wave, per K and per V tile
+  static constexpr int kTile = BN * kRow, kStage = 2 * kTile;
+  static constexpr int kNSB = BN / 32, kNC = BN / 16, kND = D / 32, kNQ = D / 16;
+};
+
+template <class T, int D, int BN, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void paged_attn_tile_kernel(AttnArgs a) {
+  using S = TileShape<D, BN, NW>;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * S::kStage];
+  __shared__ uint32_t flags[2][NW];  // whether a wave's part of a stage's values holds an infinity or NaN
+  const PagedArgs& c = a.c;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int j = lane & 31, hf = lane >> 5;  // MFMA column (row of the call, key or channel) and half
+  // workgroups of one sequence and kv head are `groups` apart in the grid, so with 8 kv heads (or 16, ...) they share
+  // an XCD's L2; a sequence's last rows, which see the most keys, start first
+  const int groups = c.batch * c.kv_heads;
+  const int grp = blockIdx.x % groups, rest = blockIdx.x / groups;
+  const int split = rest % a.splits, tile0 = a.tiles - 1 - rest / a.splits;
+  const int b = grp / c.kv_heads, h = grp % c.kv_heads, g = a.heads / c.kv_heads;
+  const Rows R = rows_of(c, b, a.tokens, g);
+  const bool causal = a.causal != 0;
+  const int32_t* pages = c.table + (int64_t)b * c.table_stride;
+  const uint8_t* kbase = (const uint8_t*)(c.k + h * c.head_stride);
+  const uint8_t* vbase = (const uint8_t*)(c.v + h * c.head_stride);
+  const int64_t page_bytes = 2 * c.page_stride;
+  const int slot_bytes = (int)(2 * c.slot_stride), slot_mask = (1 << c.page_shift) - 1;
+
+  // read offsets in a stage. K rows 32 sb + j, chunks 2 cd + hf. V^T operand (channel block db, 16-key step cc): lane
+  // p = lane % 16 of column half dh points at key 16 cc + 4 hf + p / 4 (+ 8), channels 32 db + 16 dh + 4 (p % 4) .. + 4;
+  // the swizzles depend on a row's low bits only, so steps of 16 rows are constant offsets
+  uint32_t kro[S::kNQ], vro[S::kND];
+#pragma unroll
+  for (int cd = 0; cd < S::kNQ; ++cd) kro[cd] = (uint32_t)(j * S::kRow + 16 * k_place<D>(2 * cd + hf, j));
+#pragma unroll
+  for (int db = 0; db < S::kND; ++db) {
+    const int r = 4 * hf + ((lane & 15) >> 2), col = 32 * db + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    vro[db] = (uint32_t)(S::kTile + r * S::kRow + 16 * v_place<D>(col >> 3, r) + 2 * (col & 7));
+  }
+  constexpr int CH = D / 8;
+  const int crow = lane / CH, cpl = lane % CH;  // the lane's row and chunk place in a 1 KB copy
+
+  for (int row0 = tile0 * 32 * NW; row0 < R.total; row0 += a.tiles * 32 * NW) {
+    const int row = row0 + 32 * wave + j, rc = min(row, R.total - 1);
+    const int tok = R.t0 + rc / g;
+    const int64_t out_row = (int64_t)tok * a.heads + h * g + rc % g;
+    const int lim = R.limit(rc, causal);
+    const int lim_lo = R.limit(row0, causal), lim_hi = R.limit(min(row0 + 32 * NW, R.total) - 1, causal);
+    // this split's keys [k_lo, k_hi) of those the last row sees, and the tiles of them that every row sees whole
+    const int k_lo = split * a.split_keys;
+    const int k_hi = split + 1 < a.splits ? min(k_lo + a.split_keys, lim_hi + 1) : lim_hi + 1;
+    const int ntiles = k_hi > k_lo ? (k_hi - k_lo + BN - 1) / BN : 0;
+    const int nfull = min(max(lim_lo + 1 - k_lo, 0) / BN, k_hi > k_lo ? (k_hi - k_lo) / BN : 0);
+
+    v4i qop[S::kNQ];  // q^T operand: q[row][16 cd + 8 hf .. + 8]
+    const uint16_t* qp = a.q + tok * a.ldqt + (h * g + rc % g) * a.ldqh + 8 * hf;
+#pragma unroll
+    for (int cd = 0; cd < S::kNQ; ++cd) qop[cd] = *(const v4i*)(qp + 16 * cd);
+
+    int pg[S::kRuns];
+    auto look_up = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < S::kRuns; ++u)
+        pg[u] = paged_page(c, pages, min(k_lo + t * BN + (wave + NW * u) * S::kRun + crow, k_hi - 1));
+    };
+    auto issue = [&](int t) __attribute__((always_inline)) {  // keys past the last repeat it (they are masked)
+      const uint32_t kb = (uint32_t)(uintptr_t)(lds + (t & 1) * S::kStage);
+#pragma unroll
+      for (int u = 0; u < S::kRuns; ++u) {
+        const int run = wave + NW * u, r = run * S::kRun + crow;
+        const int key = min(k_lo + t * BN + r, k_hi - 1);
+        const int64_t off = pg[u] * page_bytes + (int64_t)((key & slot_mask) * slot_bytes);
+        copy16(kb + run * 1024, kbase + off + 16 * k_place<D>(cpl, r));
+        copy16(kb + S::kTile + run * 1024, vbase + off + 16 * v_place<D>(cpl, r));
+      }
+    };
+    auto check_values = [&](int t) __attribute__((always_inline)) {
+      uint8_t* vb = lds + (t & 1) * S::kStage + S::kTile;
+      bool bad = false;
+#pragma unroll
+      for (int u = 0; u < S::kRuns; ++u) {
+        v4i* at = (v4i*)(vb + (wave + NW * u) * 1024 + lane * 16);
+        v4i x = *at;
+        if (take_nonfinite<T>(x)) *at = x, bad = true;
+      }
+      const bool any = __builtin_amdgcn_ballot_w64(bad) != 0;
+      if (lane == 0) flags[t & 1][wave] = any;
+    };
+
+    v16f oacc[S::kND];
+#pragma unroll
+    for (int db = 0; db < S::kND; ++db) oacc[db] = (v16f){};
+    float m_run = -INFINITY, l_run = 0.0f;
+
+    // MASK: the tile ends past some row's limit or the last key
+    auto step = [&](int t, auto mask_c) __attribute__((always_inline)) {
+      constexpr bool MASK = decltype(mask_c)::value;
+      const uint8_t* kb = lds + (t & 1) * S::kStage;
+      if (t + 1 < ntiles) issue(t + 1);
+      if (t + 2 < ntiles) look_up(t + 2);
+      const int vis = lim - (k_lo + t * BN);  // the lane's last visible key of the tile
+      v16f sc[S::kNSB];
+#pragma unroll
+      for (int sb = 0; sb < S::kNSB; ++sb) sc[sb] = (v16f){};
+#pragma unroll
+      for (int cd = 0; cd < S::kNQ; ++cd)
+#pragma unroll
+        for (int sb = 0; sb < S::kNSB; ++sb)
+          sc[sb] = Mfma<T>::wide(*(const v4i*)(kb + sb * 32 * S::kRow + kro[cd]), qop[cd], sc[sb]);
+      if (MASK) {
+#pragma unroll
+        for (int sb = 0; sb < S::kNSB; ++sb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (32 * sb + 8 * (i >> 2) + 4 * hf + (i & 3) > vis) sc[sb][i] = -INFINITY;
+      }
+      // the lane's maximum; the first level as med3(a, b, 3e38), which is max for scores below that and, unlike
+      // fmaxf, needs no quieting of raw MFMA results first
+      float m8[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        m8[i] = __builtin_amdgcn_fmed3f(sc[0][i], sc[0][i + 8], 3.0e38f);
+#pragma unroll
+        for (int sb = 1; sb < S::kNSB; ++sb)
+          m8[i] = fmaxf(m8[i], __builtin_amdgcn_fmed3f(sc[sb][i], sc[sb][i + 8], 3.0e38f));
+      }
+#pragma unroll
+      for (int w = 4; w >= 1; w >>= 1)
+#pragma unroll
+        for (int i = 0; i < w; ++i) m8[i] = fmaxf(m8[i], m8[i + w]);
+      const float x_max = fmaxf(m8[0], __shfl_xor(m8[0], 32)) * a.c_log2;
+      const bool bump = x_max > m_run;
+      const float m_new = bump ? x_max : m_run;
+      // a row that has seen no key yet subtracts 0: its scores are all -inf and its p all 0
+      const float ref = MASK && m_new == -INFINITY ? 0.0f : m_new;
+      const float alpha = __builtin_amdgcn_exp2f(m_run - ref);  // 0 on the first tile
+      m_run = m_new;
+      float ps[S::kNC];
+      v4i pop[S::kNC];
+#pragma unroll
+      for (int cc = 0; cc < S::kNC; ++cc) {
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[cc >> 1][8 * (cc & 1) + e], a.c_log2, -ref));
+        ps[cc] = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+        pop[cc] = (v4i){Mfma<T>::pack(p[0], p[1]), Mfma<T>::pack(p[2], p[3]), Mfma<T>::pack(p[4], p[5]),
+                        Mfma<T>::pack(p[6], p[7])};
+      }
+#pragma unroll
+      for (int w = S::kNC / 2; w >= 1; w >>= 1)
+#pragma unroll
+        for (int i = 0; i < w; ++i) ps[i] += ps[i + w];
+      l_run = __builtin_fmaf(l_run, alpha, ps[0]);
+      if (__builtin_amdgcn_ballot_w64(bump) != 0) {  // alpha is 1 in lanes whose maximum stayed
+#pragma unroll
+        for (int db = 0; db < S::kND; ++db) oacc[db] *= alpha;
+      }
+#pragma unroll
+      for (int db = 0; db < S::kND; ++db)
+#pragma unroll
+        for (int cc = 0; cc < S::kNC; ++cc) {
+          const v4s_ lo = lds_read_tr(kb + vro[db] + 16 * cc * S::kRow);
+          const v4s_ hi = lds_read_tr(kb + vro[db] + (16 * cc + 8) * S::kRow);
+          oacc[db] = Mfma<T>::wide(two_halves(lo, hi), pop[cc], oacc[db]);
+        }
+      if (MASK) {
+        bool taken = false;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) taken |= flags[t & 1][w] != 0;
+        if (taken) {
+          for (int kk = 0; kk < BN; ++kk) {
+            if (__builtin_amdgcn_ballot_w64(kk <= vis) == 0) break;
+            float s = 0.0f;
+#pragma unroll
+            for (int cd = 0; cd < S::kNQ; ++cd)
+              s = dot8<T>(qop[cd], *(const v4i*)(kb + kk * S::kRow + 16 * k_place<D>(2 * cd + hf, kk)), s);
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s + __shfl_xor(s, 32), a.c_log2, -ref));
+            if (kk <= vis) {  // the key exists: limits lie below the sequence's length
+              const int key = k_lo + t * BN + kk;
+              const uint16_t* vp = c.v + paged_at(c, paged_page(c, pages, key), h, key) + 4 * hf;
+#pragma unroll
+              for (int db = 0; db < S::kND; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  const float v = T::load(vp[32 * db + 8 * (i >> 2) + (i & 3)]);
+                  if (!(fabsf(v) < INFINITY)) oacc[db][i] = fmaf(p, v, oacc[db][i]);
+                }
+            }
+          }
+        }
+      }
+      wait_vm_lgkm0<0>();                                   // this wave's copies of tile t + 1 have landed
+      if (t + 1 >= nfull && t + 1 < ntiles) check_values(t + 1);  // a masked tile
+      __syncthreads();                                      // everyone's have; everyone is done with tile t's buffer
+    };
+
+    if (ntiles > 0) {
+      look_up(0);
+      issue(0);
+      if (ntiles > 1) look_up(1);
+      wait_vm_lgkm0<0>();
+      if (nfull == 0) check_values(0);
+      __syncthreads();
+    }
+    for (int t = 0; t < nfull; ++t) step(t, std::false_type{});
+    for (int t = nfull; t < ntiles; ++t) step(t, std::true_type{});
+
+    const float l_tot = l_run + __shfl_xor(l_run, 32);
+    const float inv = m_run == -INFINITY ? 0.0f : 1.0f / l_tot;
+    if (row < R.total) {
+#pragma unroll
+      for (int db = 0; db < S::kND; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+          put_o<T, D>(a, split, out_row, 32 * db + 2 * i + 4 * hf, oacc[db][i] * inv, oacc[db][i + 1] * inv,
+                      oacc[db][i + 2] * inv, oacc[db][i + 3] * inv);
+      if (hf == 0) put_lse(a, split, out_row, m_run, l_tot);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// head_dim 64 and 128, few rows: MFMA 16x16x32, 16 RB rows a workgroup, every wave its own keys
+// ---------------------------------------------------------------------------
+// Bound by reading K and V. A workgroup owns a split of one sequence's and kv head's keys; wave w takes its tiles w,
+// w + NW, ... of 32 keys through two LDS stages of its own (no barriers in the loop; the next tile is in flight
+// while one is computed), and the waves' O, m and l are joined at the end. The split's page ids are read into LDS
+// first, so that no ordinary load's wait falls among the copies'.
+constexpr int FW_KEYS = 32, FW_PAGES = 512;  // keys a tile; page ids staged at a time (whole tiles: page_size >= 8)
+
+template <int D, int RB, int NW>
+struct FewShape {
+  static constexpr int kRow = 2 * D, kRun = 1024 / kRow;
+  static constexpr int kRuns = FW_KEYS / kRun;  // copies a tile, per K and per V
+  static constexpr int kTile = FW_KEYS * kRow, kStage = 2 * kTile;
+  static constexpr int kND = D / 16, kNQ = D / 32;
+  static constexpr int kOut = 16 * RB * (D + 4) * 4;  // a wave's O at the end (rows padded against bank conflicts)
+  static constexpr int kWave = 2 * kStage > kOut ? 2 * kStage : kOut;
+};
+
+template <class T, int D, int RB, int NW>
+__global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(AttnArgs a) {
+  using S = FewShape<D, RB, NW>;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[NW * S::kWave];
+  __shared__ float stat[NW][2][16 * RB];  // m and l by wave
+  __shared__ int page_ids[FW_PAGES];
+  const PagedArgs& c = a.c;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int i16 = lane & 15, q4 = lane >> 4;  // MFMA column (row of the call, key or channel) and quarter
+  const int groups = c.batch * c.kv_heads;
+  const int grp = blockIdx.x % groups, split = blockIdx.x / groups;
+  const int b = grp / c.kv_heads, h = grp % c.kv_heads, g = a.heads / c.kv_heads;
+  const Rows R = rows_of(c, b, a.tokens, g);
+  const bool causal = a.causal != 0;
+  const int32_t* pages = c.table + (int64_t)b * c.table_stride;
+  const uint8_t* kbase = (const uint8_t*)(c.k + h * c.head_stride);
+  const uint8_t* vbase = (const uint8_t*)(c.v + h * c.head_stride);
+  const int64_t page_bytes = 2 * c.page_stride;
+  const int slot_bytes = (int)(2 * c.slot_stride), slot_mask = (1 << c.page_shift) - 1;
+  uint8_t* const mine = lds + wave * S::kWave;
+
+  // K operand: key 16 kb + i16, chunk 4 cd + q4. V^T operand (channels 16 db ..): lane p = i16 of quarter q4 points at key
+  // 4 q4 + p / 4 (and + 16), channels 16 db + 4 (p % 4) .. + 4
+  uint32_t kro[S::kNQ], vro[S::kND];
+#pragma unroll
+  for (int cd = 0; cd < S::kNQ; ++cd) kro[cd] = (uint32_t)(i16 * S::kRow + 16 * k_place<D>(4 * cd + q4, i16));
+#pragma unroll
+  for (int db = 0; db < S::kND; ++db) {
+    const int r = 4 * q4 + (i16 >> 2), col = 16 * db + 4 * (lane & 3);
+    vro[db] = (uint32_t)(S::kTile + r * S::kRow + 16 * v_place<D>(col >> 3, r) + 2 * (col & 7));
+  }
+  constexpr int CH = D / 8;
+  const int crow = lane / CH, cpl = lane % CH;
+
+  for (int row0 = 0; row0 < R.total; row0 += 16 * RB) {
+    int lim[RB];
+    int64_t out_row[RB];
+    v4i qop[RB][S::kNQ];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      const int rc = min(row0 + 16 * rb + i16, R.total - 1), tok = R.t0 + rc / g;
+      lim[rb] = R.limit(rc, causal);
+      out_row[rb] = (int64_t)tok * a.heads + h * g + rc % g;
+      const uint16_t* qp = a.q + tok * a.ldqt + (h * g + rc % g) * a.ldqh + 8 * q4;
+#pragma unroll
+      for (int cd = 0; cd < S::kNQ; ++cd) qop[rb][cd] = *(const v4i*)(qp + 32 * cd);
+    }
+    const int lim_lo = R.limit(row0, causal), lim_hi = R.limit(min(row0 + 16 * RB, R.total) - 1, causal);
+    const int k_lo = split * a.split_keys;
+    const int k_hi = split + 1 < a.splits ? min(k_lo + a.split_keys, lim_hi + 1) : lim_hi + 1;
+
+    v4f oacc[RB][S::kND];
+    float m_run[RB], l_run[RB];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      m_run[rb] = -INFINITY, l_run[rb] = 0.0f;
+#pragma unroll
+      for (int db = 0; db < S::kND; ++db) oacc[rb][db] = (v4f){};
+    }
+
+    const int seg_keys = FW_PAGES << c.page_shift;  // keys whose page ids are staged at a time
+    for (int s_lo = k_lo; s_lo < k_hi; s_lo += seg_keys) {
+      const int s_hi = min(s_lo + seg_keys, k_hi), p0 = s_lo >> c.page_shift;
+      __syncthreads();  // the ids of the last segment are no longer read
+      for (int i = tid; i <= ((s_hi - 1) >> c.page_shift) - p0; i += 64 * NW)
+        page_ids[i] = min(max(pages[p0 + i], 0), c.pages - 1);
+      __syncthreads();
+      const int ntiles = (s_hi - s_lo + FW_KEYS - 1) / FW_KEYS;
+      auto issue = [&](int t) __attribute__((always_inline)) {  // keys past the last repeat it (they are masked)
+        uint8_t* st = mine + ((t / NW) & 1) * S::kStage;
+        const uint32_t kb = (uint32_t)(uintptr_t)st;
+#pragma unroll
+        for (int u = 0; u < S::kRuns; ++u) {
+          const int r = u * S::kRun + crow, key = min(s_lo + t * FW_KEYS + r, s_hi - 1);
+          const int64_t off = page_ids[(key >> c.page_shift) - p0] * page_bytes +
+                              (int64_t)((key & slot_mask) * slot_bytes);
+          copy16(kb + u * 1024, kbase + off + 16 * k_place<D>(cpl, r));
+          copy16(kb + S::kTile + u * 1024, vbase + off + 16 * v_place<D>(cpl, r));
+        }
+      };
+      auto step = [&](int t, auto mask_c) __attribute__((always_inline)) {
+        constexpr bool MASK = decltype(mask_c)::value;
+        uint8_t* kb = mine + ((t / NW) & 1) * S::kStage;
+        const int k0 = s_lo + t * FW_KEYS;
+        v4i pop[RB];
+        float ref[RB];
+        bool taken = false;
+        if (MASK) {
+#pragma unroll
+          for (int u = 0; u < S::kRuns; ++u) {
+            v4i* at = (v4i*)(kb + S::kTile + u * 1024 + lane * 16);
+            v4i x = *at;
+            if (take_nonfinite<T>(x)) *at = x, taken = true;
+          }
+          taken = __builtin_amdgcn_ballot_w64(taken) != 0;
+        }
+        v4f sc[RB][2];
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) sc[rb][0] = sc[rb][1] = (v4f){};
+#pragma unroll
+        for (int cd = 0; cd < S::kNQ; ++cd)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const v4i kop = *(const v4i*)(kb + 16 * x * S::kRow + kro[cd]);
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) sc[rb][x] = Mfma<T>::tall(kop, qop[rb][cd], sc[rb][x]);
+          }
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+          // the lane's scores: its row, keys 16 x + 4 q4 + r
+          if (a.scores && row0 + 16 * rb + i16 < R.total) {
+            float* sp = a.scores + out_row[rb] * a.score_stride + k0 + 4 * q4;
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              if (k0 + 16 * x + 4 * q4 < a.score_stride)
+                *(float4*)(sp + 16 * x) = make_float4(sc[rb][x][0] * a.c_log2, sc[rb][x][1] * a.c_log2,
+                                                      sc[rb][x][2] * a.c_log2, sc[rb][x][3] * a.c_log2);
+          }
+          float mx = -INFINITY;
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              if (MASK && k0 + 16 * x + 4 * q4 + r > lim[rb]) sc[rb][x][r] = -INFINITY;
+              mx = fmaxf(mx, sc[rb][x][r]);
+            }
+          mx = fmaxf(mx, __shfl_xor(mx, 16));
+          mx = fmaxf(mx, __shfl_xor(mx, 32)) * a.c_log2;
+          const bool bump = mx > m_run[rb];
+          const float m_new = bump ? mx : m_run[rb];
+          ref[rb] = MASK && m_new == -INFINITY ? 0.0f : m_new;
+          const float alpha = __builtin_amdgcn_exp2f(m_run[rb] - ref[rb]);
+          m_run[rb] = m_new;
+          float p[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rb][e >> 2][e & 3], a.c_log2, -ref[rb]));
+          l_run[rb] = __builtin_fmaf(l_run[rb], alpha, ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])));
+          pop[rb] = (v4i){Mfma<T>::pack(p[0], p[1]), Mfma<T>::pack(p[2], p[3]), Mfma<T>::pack(p[4], p[5]),
+                          Mfma<T>::pack(p[6], p[7])};
+          if (__builtin_amdgcn_ballot_w64(bump) != 0) {
+#pragma unroll
+            for (int db = 0; db < S::kND; ++db) oacc[rb][db] *= alpha;
+          }
+        }
+#pragma unroll
+        for (int db = 0; db < S::kND; ++db) {
+          const v4s_ lo = lds_read_tr(kb + vro[db]), hi = lds_read_tr(kb + vro[db] + 16 * S::kRow);
+          const v4i vop = two_halves(lo, hi);
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) oacc[rb][db] = Mfma<T>::tall(vop, pop[rb], oacc[rb][db]);
+        }
+        if (MASK && taken) {
+          for (int kk = 0; kk < FW_KEYS; ++kk) {
+            const int key = k0 + kk;
+            if (key > lim_hi) break;
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+              float s = 0.0f;
+#pragma unroll
+              for (int cd = 0; cd < S::kNQ; ++cd)
+                s = dot8<T>(qop[rb][cd], *(const v4i*)(kb + kk * S::kRow + 16 * k_place<D>(4 * cd + q4, kk)), s);
+              s += __shfl_xor(s, 16);
+              s += __shfl_xor(s, 32);
+              const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s, a.c_log2, -ref[rb]));
+              if (key <= lim[rb]) {
+                const uint16_t* vp = c.v + paged_at(c, paged_page(c, pages, key), h, key) + 4 * q4;
+#pragma unroll
+                for (int db = 0; db < S::kND; ++db)
+#pragma unroll
+                  for (int r = 0; r < 4; ++r) {
+                    const float v = T::load(vp[16 * db + r]);
+                    if (!(fabsf(v) < INFINITY)) oacc[rb][db][r] = fmaf(p, v, oacc[rb][db][r]);
+                  }
+              }
+            }
+          }
+        }
+      };
+      // tiles wave, wave + NW, ...: the next one's copies go out before this one's are waited for
+      if (wave < ntiles) issue(wave);
+      for (int t = wave; t < ntiles; t += NW) {
+        if (t + NW < ntiles) {
+          issue(t + NW);
+          wait_vm_lgkm0<2 * S::kRuns>();
+        } else {
+          wait_vm_lgkm0<0>();
+        }
+        asm volatile("" ::: "memory");
+        const int k1 = s_lo + (t + 1) * FW_KEYS;
+        if (k1 <= lim_lo + 1 && k1 <= s_hi) step(t, std::false_type{});
+        else step(t, std::true_type{});
+        wait_vm_lgkm0<63>();  // this tile's LDS reads are done before its stage is copied into again
+        asm volatile("" ::: "memory");
+      }
+    }
+
+    // join the waves: each leaves its O [row][channel] with its m and l, thread by thread they are summed in wave order
+    __syncthreads();
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      float* op = (float*)mine + (16 * rb + i16) * (D + 4);
+#pragma unroll
+      for (int db = 0; db < S::kND; ++db) *(v4f*)(op + 16 * db + 4 * q4) = oacc[rb][db];
+      l_run[rb] += __shfl_xor(l_run[rb], 16);
+      l_run[rb] += __shfl_xor(l_run[rb], 32);
+      if (q4 == 0) stat[wave][0][16 * rb + i16] = m_run[rb], stat[wave][1][16 * rb + i16] = l_run[rb];
+    }
+    __syncthreads();
+    const int nrows = min(16 * RB, R.total - row0);
+    for (int i = tid; i < nrows * (D / 4); i += 64 * NW) {
+      const int r = i / (D / 4), d = i % (D / 4) * 4;
+      float m = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) m = fmaxf(m, stat[w][0][r]);
+      const float ref = m == -INFINITY ? 0.0f : m;
+      float l = 0.0f;
+      v4f o = {};
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float f = __builtin_amdgcn_exp2f(stat[w][0][r] - ref);
+        l = __builtin_fmaf(stat[w][1][r], f, l);
+        o += *(const v4f*)((const float*)(lds + w * S::kWave) + r * (D + 4) + d) * f;
+      }
+      const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
+      const int64_t at = (int64_t)(R.t0 + (row0 + r) / g) * a.heads + h * g + (row0 + r) % g;
+      put_o<T, D>(a, split, at, d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+      if (d == 0) put_lse(a, split, at, m, l);
+    }
+    if (row0 + 16 * RB < R.total) __syncthreads();  // the stages are copied into again
+  }
+}
+
+// Joins a row's splits, in their order: one wave a row.
+template <class T, int D>
+__global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t rows = (int64_t)a.tokens * a.heads, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  float m = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.lse_part[s * rows + row]);
+  const float ref = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f, o[D / 64] = {};
+  for (int s = 0; s < a.splits; ++s) {
+    const float f = __builtin_amdgcn_exp2f(a.lse_part[s * rows + row] - ref);
+    l += f;
+    const float* p = a.o_part + (s * rows + row) * D + lane * (D / 64);
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) o[e] = __builtin_fmaf(p[e], f, o[e]);
+  }
+  const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
+  if constexpr (D == 128) ((uint32_t*)(a.o + row * D))[lane] = (uint32_t)Mfma<T>::pack(o[0] * inv, o[1] * inv);
+  else a.o[row * D + lane] = (uint16_t)Mfma<T>::pack(o[0] * inv, 0.0f);
+  if (lane == 0) a.lse[row] = m == -INFINITY ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// ---------------------------------------------------------------------------
+// gathered weights: w[key] += sum over the rows that see it of 2^(s c - lse)
+// ---------------------------------------------------------------------------
+
+// From the scores that the few-rows kernel left: 4 keys a thread, the rows in order.
+__global__ __launch_bounds__(256) void paged_gather_scores_kernel(AttnArgs a) {
+  const PagedArgs& c = a.c;
+  const int b = blockIdx.y / c.kv_heads, h = blockIdx.y % c.kv_heads, g = a.heads / c.kv_heads;
+  const Rows R = rows_of(c, b, a.tokens, g);
+  for (int j0 = (blockIdx.x * 256 + threadIdx.x) * 4; j0 < R.len; j0 += gridDim.x * 1024) {
+    float sum[4] = {};
+    for (int r = 0; r < R.total; ++r) {
+      const int lim = R.limit(r, a.causal != 0);
+      if (j0 > lim) continue;
+      const int64_t row = (int64_t)(R.t0 + r / g) * a.heads + h * g + r % g;
+      const float lse2 = a.lse[row] * kLog2e;
+      const float4 s = *(const float4*)(a.scores + row * a.score_stride + j0);
+      const float x[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (j0 + e <= lim) sum[e] += __builtin_amdgcn_exp2f(x[e] - lse2);
+    }
+    const int page = paged_page(c, c.table + (int64_t)b * c.table_stride, j0);  // page_size >= 8: all four in one page
+    float* w = c.w + paged_w_at(c, page, h, j0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (j0 + e < R.len) w[e] += sum[e];
+  }
+}
+
+// Recomputed: a wave holds 32 keys as the MFMA's A operand and walks all rows in blocks of 32 (q^T as B, straight from
+// memory: the 4 waves of a workgroup and the key blocks of one kv head read the same rows). A lane sums its row's
+// probabilities for 16 keys; the 32 rows' lanes are joined at the end.
+constexpr int GT_WAVES = 4;
+
+template <class T, int D>
+__global__ __launch_bounds__(64 * GT_WAVES) void paged_gather_tile_kernel(AttnArgs a) {
+  constexpr int NQ = D / 16;
+  const PagedArgs& c = a.c;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, j = lane & 31, hf = lane >> 5;
+  const int groups = c.batch * c.kv_heads;
+  const int grp = blockIdx.x % groups, b = grp / c.kv_heads, h = grp % c.kv_heads, g = a.heads / c.kv_heads;
+  const Rows R = rows_of(c, b, a.tokens, g);
+  const bool causal = a.causal != 0;
+  const int32_t* pages = c.table + (int64_t)b * c.table_stride;
+  for (int j0 = (blockIdx.x / groups * GT_WAVES + wave) * 32; j0 < R.len; j0 += a.tiles * GT_WAVES * 32) {
+    const int key = min(j0 + j, R.len - 1);
+    const uint16_t* kp = c.k + paged_at(c, paged_page(c, pages, key), h, key) + 8 * hf;
+    v4i kop[NQ];
+#pragma unroll
+    for (int cd = 0; cd < NQ; ++cd) kop[cd] = *(const v4i*)(kp + 16 * cd);
+    float sum[16] = {};
+    // rows that see no key of this block come first
+    const int first = causal ? max(j0 - (R.len - R.n), 0) * g : 0;
+    for (int row0 = first; row0 < R.total; row0 += 32) {
+      const int rc = min(row0 + j, R.total - 1), tok = R.t0 + rc / g, x = h * g + rc % g;
+      const uint16_t* qp = a.q + tok * a.ldqt + x * a.ldqh + 8 * hf;
+      v16f s = {};
+#pragma unroll
+      for (int cd = 0; cd < NQ; ++cd) s = Mfma<T>::wide(kop[cd], *(const v4i*)(qp + 16 * cd), s);
+      const float lse2 = a.lse[(int64_t)tok * a.heads + x] * kLog2e;
+      const int vis = row0 + j < R.total ? R.limit(rc, causal) - j0 : -1;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c_log2, -lse2));
+        sum[i] += 8 * (i >> 2) + 4 * hf + (i & 3) <= vis ? p : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+#pragma unroll
+      for (int w = 16; w; w >>= 1) sum[i] += __shfl_xor(sum[i], w);
+    if (j == 0) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int at = j0 + 8 * (i >> 2) + 4 * hf + (i & 3);
+        if (at < R.len) c.w[paged_w_at(c, paged_page(c, pages, at), h, at)] += sum[i];
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// the choice of kernel and splits
+// ---------------------------------------------------------------------------
+constexpr int64_t kScoreBytes = 256ll << 20;  // most workspace spent on kept scores
+
+struct Plan {
+  bool matrix, few, keep_scores;
+  int row_blocks;  // few: 16-row blocks a workgroup (1 or 2)
+  int waves;       // tile: 4 or 8
+  int splits, split_keys, tiles;
+  int64_t score_stride, part_floats, bytes;
+};
+
+Plan plan_of(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t d, int64_t max_q, int64_t max_kv,
+             int64_t capacity, bool gather) {
+  Plan p = {};
+  p.matrix = d == 64 || d == 128;
+  p.splits = 1, p.split_keys = 1 << 30, p.tiles = 1;
+  if (!p.matrix || batch == 0 || tokens == 0) return p;
+  const int64_t rows = max_q * (heads / kv_heads), groups = batch * kv_heads;
+  max_kv = max_kv < 1 ? 1 : max_kv;
+  p.few = rows <= 32;
+  if (p.few) {
+    p.row_blocks = rows <= 16 ? 1 : 2;
+    // splits of one length for all sequences, so that ragged lengths still make even work: about 2048 of them in all if
+    // every sequence were the longest, of at least 256 keys
+    int64_t keys = (groups * max_kv / 2048 + 127) / 128 * 128;
+    if (keys < 256) keys = 256;
+    p.split_keys = (int)keys;
+    p.splits = (int)((max_kv + keys - 1) / keys);
+    p.score_stride = (capacity + 3) / 4 * 4;
+    p.keep_scores = gather && tokens * heads * p.score_stride * 4 <= kScoreBytes;
+  } else {
+    p.waves = rows <= 128 ? 4 : 8;
+    p.tiles = (int)((rows + 32 * p.waves - 1) / (32 * p.waves));
+    const int64_t blocks = p.tiles * groups;
+    int64_t want = (512 + blocks - 1) / blocks, most = (max_kv + 511) / 512;
+    if (want > most) want = most;
+    if (blocks >= 256 || want < 1) want = 1;
+    p.split_keys = (int)(((max_kv + want - 1) / want + 127) / 128 * 128);
+    p.splits = (int)((max_kv + p.split_keys - 1) / p.split_keys);
+  }
+  if (p.splits > 1) p.part_floats = p.splits * tokens * heads * (d + 1);
+  p.bytes = (p.part_floats + (p.keep_scores ? tokens * heads * p.score_stride : 0)) * 4;
+  return p;
+}
+
+template <class T, int D>
+void launch_matrix(const Plan& p, AttnArgs a, int64_t max_kv, bool gather, hipStream_t st) {
+  const unsigned groups = (unsigned)(a.c.batch * a.c.kv_heads);
+  if (p.few) {
+    const dim3 grid(groups * (unsigned)p.splits);
+    constexpr int NW = 4;
+    if (p.row_blocks == 1) hipLaunchKernelGGL((paged_attn_few_kernel<T, D, 1, NW>), grid, dim3(64 * NW), 0, st, a);
+    else hipLaunchKernelGGL((paged_attn_few_kernel<T, D, 2, NW>), grid, dim3(64 * NW), 0, st, a);
+  } else {
+    const dim3 grid(groups * (unsigned)(p.splits * p.tiles));
+    if (p.waves == 4) hipLaunchKernelGGL((paged_attn_tile_kernel<T, D, 64, 4>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((paged_attn_tile_kernel<T, D, 128, 8>), grid, dim3(512), 0, st, a);
+  }
+  if (p.splits > 1)
+    hipLaunchKernelGGL((paged_attn_join_kernel<T, D>), dim3((unsigned)(((int64_t)a.tokens * a.heads + 3) / 4)), dim3(256),
+                       0, st, a);
+  if (!gather) return;
+  if (p.keep_scores) {
+    const unsigned blocks = (unsigned)((max_kv + 1023) / 1024);
+    hipLaunchKernelGGL(paged_gather_scores_kernel, dim3(blocks ? blocks : 1, groups), dim3(256), 0, st, a);
+  } else {
+    a.tiles = (int)((max_kv + 32 * GT_WAVES - 1) / (32 * GT_WAVES));
+    if (a.tiles < 1) a.tiles = 1;
+    hipLaunchKernelGGL((paged_gather_tile_kernel<T, D>), dim3(groups * (unsigned)a.tiles), dim3(64 * GT_WAVES), 0, st, a);
+  }
+}
+
 }  // namespace
 
-extern "C" int64_t gwa_paged_attention_workspace(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int) {
-  return 0;
+extern "C" int64_t gwa_paged_attention_workspace(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
+                                                 int64_t head_dim, int64_t max_q, int64_t max_kv, int64_t capacity,
+                                                 int gather) {
+  if (batch < 0 || tokens < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || max_q < 0 || max_kv < 0) return 0;
+  return plan_of(batch, tokens, heads, kv_heads, head_dim, max_q, max_kv, capacity, gather != 0).bytes;
 }
 
 extern "C" int gwa_paged_attention(const gwa_paged_cache* cache, const void* q, int64_t ldqt, int64_t ldqh, void* o,
@@ -142,6 +855,29 @@ extern "C" int gwa_paged_attention(const gwa_paged_cache* cache, const void* q, 
               "%s: q and o must be 16-byte aligned", what);
   hipStream_t st = (hipStream_t)stream;
   const float c_log2 = scale * kLog2e;
+  const Plan p = plan_of(c.batch, tokens, heads, c.kv_heads, d, max_q, max_kv, c.capacity, gather != 0);
+  if (p.matrix && c.batch > 0) {
+    GWA_REQUIRE(groups * p.splits * p.tiles < (1ll << 31) && rows * p.splits < (1ll << 31),
+                "%s: %lld rows in %d splits are too many", what, (long long)rows, p.splits);
+    GWA_REQUIRE(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes && GWA_ALIGNED(workspace, 16)),
+                "%s: a workspace of %lld bytes, %lld are needed (16-byte aligned)", what, (long long)workspace_bytes,
+                (long long)p.bytes);
+    float* ws = (float*)workspace;
+    const int64_t n_o = p.splits > 1 ? p.splits * rows * d : 0;
+    // scores first: their rows are read and written 16 bytes at a time
+    const int64_t n_s = p.keep_scores ? rows * p.score_stride : 0;
+    const AttnArgs a = {c, (const uint16_t*)q, ldqt, ldqh, (uint16_t*)o, lse, ws + n_s, ws + n_s + n_o,
+                        p.keep_scores ? ws : nullptr, p.score_stride, (int)tokens, (int)heads, p.splits, p.split_keys,
+                        p.tiles, c_log2, causal};
+    if (cache->dtype == GWA_DT_BF16) {
+      if (d == 128) launch_matrix<Bf16, 128>(p, a, max_kv, gather != 0, st);
+      else launch_matrix<Bf16, 64>(p, a, max_kv, gather != 0, st);
+    } else {
+      if (d == 128) launch_matrix<Fp16, 128>(p, a, max_kv, gather != 0, st);
+      else launch_matrix<Fp16, 64>(p, a, max_kv, gather != 0, st);
+    }
+    return gwa_check_launch(what);
+  }
   const dim3 grid((unsigned)((rows + RW_WAVES - 1) / RW_WAVES)), block(64 * RW_WAVES);
   const dim3 ggrid((unsigned)((max_kv + 63) / 64 > 0 ? (max_kv + 63) / 64 : 1), (unsigned)groups);
   auto run = [&](auto t) {

@@ -113,7 +113,7 @@ _SIGNATURES: dict[str, tuple] = {
                          _int, _vp),
     "gwa_paged_write": (_cache, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _i64,
                         _i64, _i64, _int, _vp),
-    "gwa_paged_attention_workspace": (_i64, _i64, _i64, _i64, _i64, _i64, _i64, _int),
+    "gwa_paged_attention_workspace": (_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int),
     "gwa_paged_attention": (_cache, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _flt, _int, _int, _vp, _i64,
                             _vp),
     "gwa_paged_evict": (_cache, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp),
