@@ -12,6 +12,7 @@
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
@@ -42,6 +43,11 @@ struct Abi {
   decltype(&gwa_w8a8_quant) w8a8_quant;
   decltype(&gwa_w8a8_gemm) w8a8_gemm;
   decltype(&gwa_awq_w4a16_mm) awq_w4a16_mm;
+  decltype(&gwa_rotary_embed) rotary_embed;
+  decltype(&gwa_paged_write) paged_write;
+  decltype(&gwa_paged_attention_workspace) paged_attention_workspace;
+  decltype(&gwa_paged_attention) paged_attention;
+  decltype(&gwa_paged_evict) paged_evict;
 };
 Abi g_abi;
 bool g_bound = false;
@@ -346,6 +352,270 @@ PyObject* awq_forward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------------------
+// rotary positions and the paged cache: the functions of paged.py, whose checks these are; None where one fails
+// ---------------------------------------------------------------------------
+
+bool ints_on(const Tensor& t, const at::Device& dev, at::IntArrayRef sizes) {
+  return t.scalar_type() == at::kInt && t.layout() == at::kStrided && t.device() == dev && t.sizes().equals(sizes) &&
+         (t.dim() == 0 || t.numel() == 0 || t.stride(-1) == 1);
+}
+bool heads_on(const Tensor& t, at::ScalarType dt, const at::Device& dev, int64_t tokens, int64_t heads, int64_t dim) {
+  return t.scalar_type() == dt && t.layout() == at::kStrided && t.device() == dev &&
+         t.sizes().equals({tokens, heads, dim}) && (t.numel() == 0 || t.stride(2) == 1);
+}
+template <class P>
+P* address(const Tensor& t) {
+  return (P*)t.data_ptr();
+}
+
+// tensor arguments in order: exact tensors that no subclass, transform or (with `grad` unset) autograd has a say in,
+// undefined for None where `optional` has the argument's bit
+bool plain_args(PyObject* const* args, int n, unsigned optional, Tensor* out, bool grad = false) {
+  if (c10::impl::TorchDispatchModeTLS::stack_len() != 0 || at::impl::torch_function_mode_enabled() ||
+      torch::jit::tracer::isTracing())
+    return false;
+  for (int i = 0; i < n; ++i) {
+    if (args[i] == Py_None) {
+      if (!(optional >> i & 1)) return false;
+      continue;
+    }
+    if (!THPVariable_CheckExact(args[i])) return false;
+    const Tensor& t = THPVariable_Unpack(args[i]);
+    if (t.key_set().has_any(kNotPlain) || (t.requires_grad() && at::GradMode::is_enabled() && !(grad && i == 0)))
+      return false;
+    out[i] = t;
+  }
+  return true;
+}
+
+// (rotated channels, table rows) of fitting tables for `tokens` tokens
+bool tables_fit(const Tensor& cos, const Tensor& sin, const Tensor& positions, int64_t tokens, int64_t dim,
+                const at::Device& dev, int64_t& rot, int64_t& rows) {
+  rot = rows = 0;
+  if (positions.defined() && !ints_on(positions, dev, {tokens})) return false;
+  if (cos.defined() != sin.defined()) return false;
+  if (!cos.defined()) return true;
+  if (cos.dim() != 2 || !dense_on(cos, at::kFloat, dev) || !dense_on(sin, at::kFloat, dev) ||
+      !cos.sizes().equals(sin.sizes()))
+    return false;
+  rows = cos.size(0), rot = 2 * cos.size(1);
+  return rot <= dim && (rot == 0 || tokens == 0 || (rows > 0 && (positions.defined() || rows >= tokens)));
+}
+
+// y of a call that fits, undefined otherwise
+Tensor rotated(const Tensor& x0, const Tensor& cos, const Tensor& sin, const Tensor& positions, bool interleaved,
+               bool inverse) {
+  int64_t rot, rows;
+  const int dt = dt_code(x0.scalar_type());
+  if (!x0.is_cuda() || x0.layout() != at::kStrided || x0.dim() != 3 || dt < 0 || !cos.defined() ||
+      !tables_fit(cos, sin, positions, x0.size(0), x0.size(2), x0.device(), rot, rows))
+    return Tensor();
+  const int64_t t = x0.size(0), h = x0.size(1), d = x0.size(2);
+  if (d < 2 || d > 1024 || d % 2) return Tensor();
+  const Tensor x = x0.stride(2) == 1 ? x0 : x0.contiguous();
+  Tensor y = empty_like_device({t, h, d}, x.scalar_type(), x);
+  if (y.numel() &&
+      g_abi.rotary_embed(x.data_ptr(), x.stride(0), x.stride(1), address<float>(cos), address<float>(sin), rows,
+                         positions.defined() ? address<int32_t>(positions) : nullptr, y.data_ptr(), h * d, d, t, h, d,
+                         rot, interleaved, inverse, dt, stream_of(x)) != GWA_OK)
+    return Tensor();
+  return y;
+}
+
+OptTensor some(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
+
+// the recorded rotation: its gradient is the rotation back, recorded again where a graph of it is asked for
+struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& cos, const Tensor& sin,
+                        const OptTensor& positions, bool interleaved, bool inverse) {
+    const Tensor at = positions.value_or(Tensor());
+    ctx->save_for_backward({cos, sin, at});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["inverse"] = inverse;
+    Tensor y = rotated(x, cos, sin, at, interleaved, inverse);
+    TORCH_CHECK(y.defined(), "rotary_embed: the library refused a checked call");
+    return y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    Tensor dx;
+    if (grads[0].defined())
+      dx = RotaryFunction::apply(grads[0], saved[0], saved[1], some(saved[2]), ctx->saved_data["interleaved"].toBool(),
+                                 !ctx->saved_data["inverse"].toBool());
+    return {dx, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// rotary_embed(x, cos, sin, positions, interleaved, inverse) -> y
+PyObject* rotary_embed(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Tensor t[4];
+  if (nargs != 6 || !g_bound || !plain_args(args, 4, 8u, t, true)) Py_RETURN_NONE;
+  const bool interleaved = PyObject_IsTrue(args[4]) == 1, inverse = PyObject_IsTrue(args[5]) == 1;
+  Tensor y;
+  {
+    pybind11::gil_scoped_release no_gil;
+    if (t[0].requires_grad() && at::GradMode::is_enabled()) {
+      int64_t rot, rows;
+      const bool fits = t[0].is_cuda() && t[0].layout() == at::kStrided && t[0].dim() == 3 && t[1].defined() &&
+                        dt_code(t[0].scalar_type()) >= 0 && t[0].size(2) >= 2 && t[0].size(2) <= 1024 &&
+                        t[0].size(2) % 2 == 0 &&
+                        tables_fit(t[1], t[2], t[3], t[0].size(0), t[0].size(2), t[0].device(), rot, rows);
+      if (fits) y = RotaryFunction::apply(t[0], t[1], t[2], some(t[3]), interleaved, inverse);
+    } else {
+      y = rotated(t[0], t[1], t[2], t[3], interleaved, inverse);
+    }
+  }
+  if (!y.defined()) Py_RETURN_NONE;
+  return THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+// the C interface's cache of fitting tensors
+bool cache_fits(const Tensor& k, const Tensor& v, const Tensor& w, const Tensor& table, const Tensor& q_start,
+                const Tensor& kv_len, gwa_paged_cache& c) {
+  const at::Device dev = k.device();
+  if (!k.is_cuda() || k.layout() != at::kStrided || (k.scalar_type() != at::kBFloat16 && k.scalar_type() != at::kHalf) ||
+      k.dim() != 4 || k.stride(3) != 1 || v.scalar_type() != k.scalar_type() || v.device() != dev ||
+      v.layout() != at::kStrided || !v.sizes().equals(k.sizes()) || !v.strides().equals(k.strides()) ||
+      kv_len.dim() != 1 || table.dim() != 2)
+    return false;
+  const int64_t batch = kv_len.size(0);
+  if (!ints_on(kv_len, dev, {batch}) || !ints_on(table, dev, {batch, table.size(1)}) ||
+      (q_start.defined() && !ints_on(q_start, dev, {batch + 1})))
+    return false;
+  if (w.defined() && (w.scalar_type() != at::kFloat || w.layout() != at::kStrided || w.device() != dev ||
+                      !w.sizes().equals({k.size(0), k.size(1), k.size(2)}) || (k.size(2) != 1 && w.stride(2) != 1)))
+    return false;
+  if (k.size(2) > 4096 || k.size(1) > 65535 || k.size(3) > 256) return false;  // the struct's ints; refused in Python
+  c = gwa_paged_cache{k.data_ptr(), v.data_ptr(), w.defined() ? address<float>(w) : nullptr, address<int32_t>(table),
+                      q_start.defined() ? address<int32_t>(q_start) : nullptr, address<int32_t>(kv_len), k.stride(0),
+                      k.stride(1), k.stride(2), w.defined() ? w.stride(0) : 0, w.defined() ? w.stride(1) : 0, k.size(0),
+                      std::max(table.stride(0), table.size(1)), table.size(1), batch, (int)k.size(2), (int)k.size(1),
+                      (int)k.size(3), dt_code(k.scalar_type())};
+  return true;
+}
+
+// paged_write(q, k, v, cos, sin, positions, k_pages, v_pages, table, q_start, kv_len, weights, interleaved) -> q rotated
+PyObject* paged_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Tensor t[12];
+  if (nargs != 13 || !g_bound || !plain_args(args, 12, 1u << 3 | 1u << 4 | 1u << 5 | 1u << 11, t)) Py_RETURN_NONE;
+  const bool interleaved = PyObject_IsTrue(args[12]) == 1;
+  const Tensor &q = t[0], &k = t[1], &v = t[2];
+  Tensor out;
+  {
+    pybind11::gil_scoped_release no_gil;
+    gwa_paged_cache c;
+    int64_t rot, rows;
+    const at::ScalarType dt = t[6].scalar_type();
+    const at::Device dev = t[6].device();
+    if (q.dim() == 3 && cache_fits(t[6], t[7], t[11], t[8], t[9], t[10], c)) {
+      const int64_t n = q.size(0), h = q.size(1), d = c.head_dim;
+      if (heads_on(q, dt, dev, n, h, d) && heads_on(k, dt, dev, n, c.kv_heads, d) &&
+          heads_on(v, dt, dev, n, c.kv_heads, d) && tables_fit(t[3], t[4], t[5], n, d, dev, rot, rows)) {
+        out = empty_like_device({n, h, d}, dt, q);
+        if (g_abi.paged_write(&c, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+                              v.data_ptr(), v.stride(0), v.stride(1), t[3].defined() ? address<float>(t[3]) : nullptr,
+                              t[4].defined() ? address<float>(t[4]) : nullptr, rows,
+                              t[5].defined() ? address<int32_t>(t[5]) : nullptr, out.data_ptr(), n, h, rot, interleaved,
+                              stream_of(t[6])) != GWA_OK)
+          out = Tensor();
+      }
+    }
+  }
+  if (!out.defined()) Py_RETURN_NONE;
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* pair(Tensor a, Tensor b) {
+  PyObject *x = THPVariable_Wrap(std::move(a)), *y = THPVariable_Wrap(std::move(b));
+  PyObject* both = PyTuple_New(2);
+  PyTuple_SET_ITEM(both, 0, x);
+  PyTuple_SET_ITEM(both, 1, y);
+  return both;
+}
+
+// paged_attention(q, k_pages, v_pages, table, q_start, kv_len, weights, max_q, max_kv, scale, causal) -> (o, lse)
+PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Tensor t[7];
+  if (nargs != 11 || !g_bound || !plain_args(args, 7, 1u << 6, t) || !PyLong_Check(args[7]) || !PyLong_Check(args[8]))
+    Py_RETURN_NONE;
+  const long long max_q = PyLong_AsLongLong(args[7]), max_kv = PyLong_AsLongLong(args[8]);
+  const double scale = PyFloat_AsDouble(args[9]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  const bool causal = PyObject_IsTrue(args[10]) == 1;
+  const Tensor& q = t[0];
+  Tensor o, lse;
+  {
+    pybind11::gil_scoped_release no_gil;
+    gwa_paged_cache c;
+    if (q.dim() == 3 && q.size(1) > 0 && cache_fits(t[1], t[2], t[6], t[3], t[4], t[5], c) && c.kv_heads > 0 &&
+        q.size(1) % c.kv_heads == 0 &&
+        heads_on(q, t[1].scalar_type(), t[1].device(), q.size(0), q.size(1), c.head_dim) && q.size(0) > 0 &&
+        q.stride(0) > 0 && q.stride(1) > 0 && q.stride(0) % 8 == 0 && q.stride(1) % 8 == 0 &&
+        (uintptr_t)q.data_ptr() % 16 == 0) {
+      const int64_t n = q.size(0), h = q.size(1);
+      const bool gather = t[6].defined();
+      o = empty_like_device({n, h, c.head_dim}, q.scalar_type(), q);
+      lse = empty_like_device({n, h}, at::kFloat, q);
+      const int64_t bytes = g_abi.paged_attention_workspace(c.batch, n, h, c.kv_heads, c.head_dim, max_q, max_kv,
+                                                            c.table_width * c.page_size, gather);
+      Tensor ws;
+      if (bytes > 0) ws = empty_like_device({bytes}, at::kByte, q);
+      if (g_abi.paged_attention(&c, q.data_ptr(), q.stride(0), q.stride(1), o.data_ptr(), address<float>(lse), n, h, max_q,
+                                max_kv, (float)scale, causal, gather, bytes > 0 ? ws.data_ptr() : nullptr, bytes,
+                                stream_of(q)) != GWA_OK)
+        o = Tensor();
+    }
+  }
+  if (!o.defined()) Py_RETURN_NONE;
+  return pair(std::move(o), std::move(lse));
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_evict(k_pages, v_pages, weights, table, kv_len, new_table, max_kv, budget, recent) -> (kept, new_len)
+PyObject* paged_evict(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Tensor t[6];
+  if (nargs != 9 || !g_bound || !plain_args(args, 6, 0, t)) Py_RETURN_NONE;
+  long long num[3];
+  for (int i = 0; i < 3; ++i) {
+    if (!PyLong_Check(args[6 + i])) Py_RETURN_NONE;
+    num[i] = PyLong_AsLongLong(args[6 + i]);
+  }
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  const long long max_kv = num[0], budget = num[1], recent = num[2];
+  const Tensor& next = t[5];
+  Tensor kept, len;
+  {
+    pybind11::gil_scoped_release no_gil;
+    gwa_paged_cache c;
+    if (budget > 0 && recent >= 0 && recent <= budget && next.dim() == 2 &&
+        cache_fits(t[0], t[1], t[2], t[3], Tensor(), t[4], c) &&
+        ints_on(next, t[0].device(), {c.batch, next.size(1)})) {
+      kept = empty_like_device({c.batch, c.kv_heads, budget}, at::kInt, next);
+      len = empty_like_device({c.batch}, at::kInt, next);
+      if (g_abi.paged_evict(&c, address<int32_t>(next), std::max(next.stride(0), next.size(1)), next.size(1), max_kv,
+                            budget, recent, address<int32_t>(kept), address<int32_t>(len), stream_of(t[0])) != GWA_OK)
+        kept = Tensor();
+    }
+  }
+  if (!kept.defined()) Py_RETURN_NONE;
+  return pair(std::move(kept), std::move(len));
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef bound_methods[] = {
     {"run", (PyCFunction)(void (*)(void))bound_run, METH_FASTCALL,
      "run(x, module.__dict__) -> the layer's output, or None where its general path has to decide"},
@@ -449,6 +719,11 @@ PyObject* host_bind(PyObject*, PyObject* args) {
   GWA_BIND(w8a8_quant);
   GWA_BIND(w8a8_gemm);
   GWA_BIND(awq_w4a16_mm);
+  GWA_BIND(rotary_embed);
+  GWA_BIND(paged_write);
+  GWA_BIND(paged_attention_workspace);
+  GWA_BIND(paged_attention);
+  GWA_BIND(paged_evict);
 #undef GWA_BIND
   Py_INCREF(bodies);
   Py_INCREF(records);
@@ -466,6 +741,17 @@ PyObject* host_bind(PyObject*, PyObject* args) {
 PyMethodDef module_methods[] = {{"bind", host_bind, METH_VARARGS, "bind(addresses, bodies, ref_records)"},
                                 {"awq_forward", (PyCFunction)(void (*)(void))awq_forward, METH_FASTCALL,
                                  "awq_forward(x, weight, wscales, wzeros, bias, max_rows) -> output or None"},
+                                {"rotary_embed", (PyCFunction)(void (*)(void))rotary_embed, METH_FASTCALL,
+                                 "rotary_embed(x, cos, sin, positions, interleaved, inverse) -> output or None"},
+                                {"paged_write", (PyCFunction)(void (*)(void))paged_write, METH_FASTCALL,
+                                 "paged_write(q, k, v, cos, sin, positions, k_pages, v_pages, table, q_start, kv_len, "
+                                 "weights, interleaved) -> rotated q or None"},
+                                {"paged_attention", (PyCFunction)(void (*)(void))paged_attention, METH_FASTCALL,
+                                 "paged_attention(q, k_pages, v_pages, table, q_start, kv_len, weights, max_q, max_kv, "
+                                 "scale, causal) -> (o, lse) or None"},
+                                {"paged_evict", (PyCFunction)(void (*)(void))paged_evict, METH_FASTCALL,
+                                 "paged_evict(k_pages, v_pages, weights, table, kv_len, new_table, max_kv, budget, "
+                                 "recent) -> (kept, new_len) or None"},
                                 {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host_calls", "Native host side of eager calls.", -1, module_methods};
 

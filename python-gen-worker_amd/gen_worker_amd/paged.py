@@ -30,6 +30,7 @@ import torch
 from torch import Tensor
 
 from . import _native as nat
+from . import ops
 
 _DTYPES = {torch.bfloat16: nat.DT_BF16, torch.float16: nat.DT_F16, torch.float32: nat.DT_F32}
 
@@ -78,6 +79,13 @@ def _tables(name: str, cos: Optional[Tensor], sin: Optional[Tensor], positions: 
     _require(positions is not None or rows >= tokens or half == 0, name,
              f"{tokens} tokens without positions over a table of {rows}")
     return 2 * half, rows
+
+
+def _host():
+    """The native host calls, which make these calls in a few microseconds; None while the library is not loaded,
+    without them, and under compilation. Theirs return None for whatever the Python way has to decide or refuse."""
+    host = ops._host
+    return None if host is None or torch.compiler.is_compiling() else host
 
 
 def _plain(*tensors: Optional[Tensor]) -> bool:
@@ -142,6 +150,7 @@ def _rotary_body(x: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor
     _require(x.dim() == 3 and x.dtype in _DTYPES and x.is_cuda, name,
              f"x must be a bf16, fp16 or fp32 CUDA tensor [tokens, heads, head_dim], got {x.dtype} {list(x.shape)} on "
              f"{x.device}")
+    _require(cos is not None and sin is not None, name, "cos and sin are needed")
     t, h, d = x.shape
     rot, rows = _tables(name, cos, sin, positions, t, d, x.device)
     _require(d % 2 == 0 and 2 <= d <= 1024, name, f"head_dim {d} (an even number up to 1024)")
@@ -186,6 +195,11 @@ def rotary_embed(x: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor
     ``2 * cos.shape[1]`` channels of every head rotated by their token's position, the others copied. Pairs are
     (2i, 2i + 1) with ``interleaved``, else (i, i + half). ``positions``: int32 [tokens] rows of the tables (held inside
     them), or None for 0, 1, 2, ... ``inverse`` rotates back. Computed in fp32, rounded once; differentiable in x."""
+    host = _host()
+    if host is not None:
+        y = host.rotary_embed(x, cos, sin, positions, interleaved, inverse)
+        if y is not None:
+            return y
     if _plain(x, cos, sin, positions):
         return _rotary_body(x, cos, sin, positions, interleaved, inverse)
     return _rotary_op(x, cos, sin, positions, interleaved, inverse)
@@ -268,6 +282,11 @@ def paged_write(q: Tensor, k: Tensor, v: Tensor, cos: Optional[Tensor], sin: Opt
     and keys are rotated as ``rotary_embed`` does (cos = sin = None: not at all); the new slots' gathered ``weights``
     [pages, kv_heads, page_size] start at 0. No two sequences may write one page."""
     a = (q, k, v, cos, sin, positions, k_pages, v_pages, table, q_start, kv_len, weights)
+    host = _host()
+    if host is not None:
+        out = host.paged_write(*a, interleaved)
+        if out is not None:
+            return out
     return _write_body(*a, interleaved) if _plain(*a) else _write_op(*a, interleaved)
 
 
@@ -322,6 +341,11 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, 
     is defined."""
     if scale is None:
         scale = float(q.shape[-1]) ** -0.5
+    host = _host()
+    if host is not None:
+        out = host.paged_attention(q, k_pages, v_pages, table, q_start, kv_len, weights, max_q, max_kv, scale, causal)
+        if out is not None:
+            return out
     if _plain(q, k_pages, v_pages, table, q_start, kv_len, weights):
         return _attention_body(q, k_pages, v_pages, table, q_start, kv_len, max_q, max_kv, scale, causal, weights)
     return _attention_op(q, k_pages, v_pages, table, q_start, kv_len, max_q, max_kv, scale, causal, weights)
@@ -362,6 +386,11 @@ def paged_evict(k_pages: Tensor, v_pages: Tensor, weights: Tensor, table: Tensor
     the pages of ``new_table`` int32 [batch, width], which must be pages that ``table`` does not use. Returns (kept int32
     [batch, kv_heads, budget]: the old slots, -1 past the end; the new kv_len)."""
     a = (k_pages, v_pages, weights, table, kv_len)
+    host = _host()
+    if host is not None:
+        out = host.paged_evict(*a, new_table, max_kv, budget, recent)
+        if out is not None:
+            return out
     if _plain(*a, new_table):
         return _evict_body(*a, max_kv, new_table, budget, recent)
     return _evict_op(*a, max_kv, new_table, budget, recent)

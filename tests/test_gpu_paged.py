@@ -133,7 +133,7 @@ def test_rotary_gradient(interleaved):
         up, down = (rotary_embed(x + s * 4.0 * v, cos, sin, at.int(), interleaved=interleaved) for s in (1, -1))
         slope = float((dy.double() * (up.double() - down.double())).sum()) / 8.0
     want = float((dx.double() * v.double()).sum())
-    assert abs(slope - want) <= 16 * E * float((dy.abs().double() * (x.abs().sum() / x.numel() + 4 * v.abs()).double()).sum())
+    assert abs(slope - want) <= 16 * E * float((dy.abs().double() * (x.detach().abs().mean() + 4 * v.abs()).double()).sum())
     (de,) = torch.autograd.grad(rotary_embed(x, cos, sin, at.int(), interleaved=interleaved).sum(), x)
     _check_turned(de, *_turn(torch.ones_like(x), cos, sin, at, interleaved, inverse=True))
 
@@ -566,3 +566,47 @@ def test_cache_steps_like_one_long_sequence():
     cache.drop(a)
     cache.drop(b)
     assert cache.free_pages == 64
+
+
+def test_native_host_calls_and_python_bodies_agree(monkeypatch):
+    """Every function with the native host calls and without them: the same bits; what the native ones do not take
+    (operands of another type, a missing table, autograd through attention) is decided by Python either way."""
+    from gen_worker_amd import ops, paged
+
+    assert ops._host is not None
+    r = Ragged([3, 1], [50, 700], 4, 2, 64, 16, BF16, seed=8)
+    w0, k0 = r.w.clone(), r.k.clone()
+    cos, sin = paged.rotary_table(64, 32, device=DEV)
+    at = torch.arange(r.tokens, device=DEV).int()
+    new = _ints([[0, 1], [2, 3]])
+    x = torch.randn(5, 3, 48, generator=r.g, device=DEV, requires_grad=True)
+
+    def everything():
+        r.w.copy_(w0), r.k.copy_(k0)
+        out = [paged.rotary_embed(r.q, cos, sin, at, interleaved=True), paged.rotary_embed(r.q, cos, sin, inverse=True)]
+        y = paged.rotary_embed(x, cos, sin)
+        (dx,) = torch.autograd.grad((y * y).sum(), x, create_graph=True)
+        assert dx.requires_grad and y.requires_grad
+        out += [y.detach(), dx.detach(), torch.autograd.grad(dx.square().sum(), x)[0]]
+        out.append(paged.paged_write(r.q, r.q[:, :2], r.q[:, 2:], cos, sin, at, r.k, r.v, r.table, r.q_start, r.kv_len,
+                                     weights=r.w))
+        out += [*r.attend(gather=True), r.w.clone()]
+        dst_k, dst_v, dst_w = (torch.cat([t, torch.zeros_like(t[:4])]) for t in (r.k, r.v, r.w))
+        out += [*paged.paged_evict(dst_k, dst_v, dst_w, r.table, r.kv_len, 700, new + r.k.shape[0], 32, 5), dst_k, dst_v]
+        for bad in (lambda: r.attend(q=r.q.to(F16)), lambda: paged.rotary_embed(r.q, cos, sin.double()),
+                    lambda: paged.rotary_embed(r.q, cos, sin, at.long()), lambda: r.attend(q=r.q[:, :3]),
+                    lambda: paged.paged_write(r.q, r.q, r.q, cos, sin, at, r.k, r.v, r.table, r.q_start, r.kv_len),
+                    lambda: paged.paged_evict(r.k, r.v, r.w, r.table, r.kv_len, 700, new, 4, 5),
+                    lambda: paged.rotary_embed(r.q, None, None)):
+            with pytest.raises(ValueError):
+                bad()
+        return out
+
+    with_host = everything()
+    monkeypatch.setattr(ops, "_host", None)
+    without = everything()
+    for a, b in zip(with_host, without):
+        assert torch.equal(a.nan_to_num(), b.nan_to_num())
+    (dx,) = torch.autograd.grad(paged.rotary_embed(x, cos, sin).square().sum(), x)
+    # the rotation keeps lengths: d |y|^2 / dx = 2 x, to rounding of two rotations of values below 6
+    assert bool(((dx - 2 * x).abs() <= 64 * E * 6).all())
