@@ -5,8 +5,11 @@
 
 namespace {
 
-// One call's operands, as the matrix-core kernels take them. Partial results of key split s: o_part
-// [s][tokens * heads][D] (fp32, each normalised by its own sum) and lse_part [s][tokens * heads] (log2 domain).
+constexpr int kCus = 256;  // MI355X
+
+// One call's operands, as the matrix-core kernels take them. Partial results (fp32, each normalised by its own sum, with
+// the log2 of that sum) of key split s in o_part [s][tokens * heads][D] and lse_part [s][tokens * heads]; of a share
+// (many rows) in [2 * shares][rows of a tile].
 struct AttnArgs {
   PagedArgs c;
   const uint16_t* q;
@@ -16,8 +19,9 @@ struct AttnArgs {
   float* o_part;
   float* lse_part;
   float* scores;          // [tokens * heads][score_stride] in the log2 domain, or NULL
+  float* w_part;
   int64_t score_stride;
-  int tokens, heads, splits, split_keys, tiles;
+  int tokens, heads, splits, split_keys, tiles, shares;
   float c_log2;
   int causal;
 };
@@ -161,229 +165,401 @@ __global__ __launch_bounds__(64) void paged_gather_rows_kernel(PagedArgs c, cons
 //   S^T = K q^T           (keys x rows: a lane holds one row, 16 keys of each 32)
 //   p   = 2^(S c - m)     (m: the row's running maximum; O and the sum l are rescaled where it moves)
 //   O^T = O^T + V^T p^T   (V^T by transposing reads, in the key order S^T leaves p in, so p stays in registers)
+// A tile takes two slots, each ended by a barrier: the matrix slot (O of the tile before, S of this one) and the softmax
+// slot. With 8 waves the SIMD's second wave runs one slot behind the first, so that one has the matrix cores while
+// the other has the vector unit.
 // Tiles that every row of the workgroup sees whole run without a mask; the others compare each score's key with the
 // lane's limit. There 0 * v of a hidden key must not reach O: whoever copied a part of the tile sets values that are not
-// finite to 0 and says so, and rows that do see such a key get its values added one by one.
+// finite to 0 and says so, and rows that do see such a key get its values added one by one at the end.
 template <int D, int BN, int NW>
 struct TileShape {
   static constexpr int kRow = 2 * D, kRun = 1024 / kRow;  // row bytes; rows a 1 KB copy covers
   static constexpr int kRuns = BN / kRun / NW;            // copies a wave, per K and per V tile
-  static constexpr int kTile = BN * kRow, kStage = 2 * kTile;
+  static constexpr int kTile = BN * kRow;                 // LDS: K tiles 0 and 1, then V tiles 0 and 1
   static constexpr int kNSB = BN / 32, kNC = BN / 16, kND = D / 32, kNQ = D / 16;
 };
 
 template <class T, int D, int BN, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void paged_attn_tile_kernel(AttnArgs a) {
   using S = TileShape<D, BN, NW>;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * S::kStage];
-  __shared__ uint32_t flags[2][NW];  // whether a wave's part of a stage's values holds an infinity or NaN
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * S::kTile];
+  __shared__ uint32_t aside;  // whether any value of a masked tile was set aside
   const PagedArgs& c = a.c;
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63;
+  const int behind = wave >> 2;             // slots this wave runs behind the workgroup's first
   const int j = lane & 31, hf = lane >> 5;  // MFMA column (row of the call, key or channel) and half
-  // workgroups of one sequence and kv head are `groups` apart in the grid, so with 8 kv heads (or 16, ...) they share
-  // an XCD's L2; a sequence's last rows, which see the most keys, start first
-  const int groups = c.batch * c.kv_heads;
-  const int grp = blockIdx.x % groups, rest = blockIdx.x / groups;
-  const int split = rest % a.splits, tile0 = a.tiles - 1 - rest / a.splits;
-  const int b = grp / c.kv_heads, h = grp % c.kv_heads, g = a.heads / c.kv_heads;
-  const Rows R = rows_of(c, b, a.tokens, g);
+  constexpr int BM = 32 * NW;
+  const int g = a.heads / c.kv_heads;
   const bool causal = a.causal != 0;
-  const int32_t* pages = c.table + (int64_t)b * c.table_stride;
-  const uint8_t* kbase = (const uint8_t*)(c.k + h * c.head_stride);
-  const uint8_t* vbase = (const uint8_t*)(c.v + h * c.head_stride);
-  const int64_t page_bytes = 2 * c.page_stride;
-  const int slot_bytes = (int)(2 * c.slot_stride), slot_mask = (1 << c.page_shift) - 1;
+  const uint32_t page_bytes = (uint32_t)(2 * c.page_stride), slot_bytes = (uint32_t)(2 * c.slot_stride);
+  const uint32_t slot_mask = (1u << c.page_shift) - 1;
 
-  // read offsets in a stage. K rows 32 sb + j, chunks 2 cd + hf. V^T operand (channel block db, 16-key step cc): lane
-  // p = lane % 16 of column half dh points at key 16 cc + 4 hf + p / 4 (+ 8), channels 32 db + 16 dh + 4 (p % 4) .. + 4;
-  // the swizzles depend on a row's low bits only, so steps of 16 rows are constant offsets
-  uint32_t kro[S::kNQ], vro[S::kND];
-#pragma unroll
-  for (int cd = 0; cd < S::kNQ; ++cd) kro[cd] = (uint32_t)(j * S::kRow + 16 * k_place<D>(2 * cd + hf, j));
-#pragma unroll
-  for (int db = 0; db < S::kND; ++db) {
-    const int r = 4 * hf + ((lane & 15) >> 2), col = 32 * db + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-    vro[db] = (uint32_t)(S::kTile + r * S::kRow + 16 * v_place<D>(col >> 3, r) + 2 * (col & 7));
-  }
+  // read offsets in a tile: K row j, chunk hf (chunk 2 cd + hf: the address xor 32 cd; rows 32 sb + j: a constant
+  // more). V^T operand (channel block db, 16-key step cc): lane p = lane % 16 of column half dh points at key 4 hf + p / 4
+  // (16 cc and 8 more: constants), channels 16 dh + 4 (p % 4) .. + 4 (block db: the address xor 64 db)
+  const uint32_t kro = (uint32_t)(j * S::kRow + 16 * k_place<D>(hf, j));
+  const int vr = 4 * hf + ((lane & 15) >> 2), vc = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  const uint32_t vro = (uint32_t)(vr * S::kRow + 16 * v_place<D>(vc >> 3, vr) + 2 * (vc & 7));
   constexpr int CH = D / 8;
   const int crow = lane / CH, cpl = lane % CH;  // the lane's row and chunk place in a 1 KB copy
+  // (a wave's copies are a multiple of 4 KB apart, so the swizzles of the lane's row are the same in all)
+  const uint32_t klane = crow * slot_bytes + 16 * k_place<D>(cpl, wave * S::kRun + crow);
+  const uint32_t vlane = crow * slot_bytes + 16 * v_place<D>(cpl, wave * S::kRun + crow);
 
-  for (int row0 = tile0 * 32 * NW; row0 < R.total; row0 += a.tiles * 32 * NW) {
-    const int row = row0 + 32 * wave + j, rc = min(row, R.total - 1);
-    const int tok = R.t0 + rc / g;
-    const int64_t out_row = (int64_t)tok * a.heads + h * g + rc % g;
-    const int lim = R.limit(rc, causal);
-    const int lim_lo = R.limit(row0, causal), lim_hi = R.limit(min(row0 + 32 * NW, R.total) - 1, causal);
-    // this split's keys [k_lo, k_hi) of those the last row sees, and the tiles of them that every row sees whole
-    const int k_lo = split * a.split_keys;
-    const int k_hi = split + 1 < a.splits ? min(k_lo + a.split_keys, lim_hi + 1) : lim_hi + 1;
-    const int ntiles = k_hi > k_lo ? (k_hi - k_lo + BN - 1) / BN : 0;
-    const int nfull = min(max(lim_lo + 1 - k_lo, 0) / BN, k_hi > k_lo ? (k_hi - k_lo) / BN : 0);
+  // this workgroup's share. An XCD's workgroups (every 8th) take neighbouring shares, which are of one head where there
+  // are 8 (or 16, ...), so that K and V are shared in its L2
+  const int share = blockIdx.x % kXcds * (a.shares / kXcds) + blockIdx.x / kXcds, tt = BM / g;
+  int64_t unused;
+  const int64_t per_head = head_line(c, a.tokens, tt, causal, 0, unused), all = per_head * c.kv_heads;
+  const int64_t x0 = share_start(all, share, a.shares), x1 = share_start(all, share + 1, a.shares);
+  if (x0 >= x1) return;
+  Place at = place_of<BN>(c, a.tokens, tt, causal, per_head, x0);
+  const Place end = place_of<BN>(c, a.tokens, tt, causal, per_head, x1);
+  Rows R = uniform_rows_of(c, at.b, a.tokens, g);
 
-    v4i qop[S::kNQ];  // q^T operand: q[row][16 cd + 8 hf .. + 8]
-    const uint16_t* qp = a.q + tok * a.ldqt + (h * g + rc % g) * a.ldqh + 8 * hf;
-#pragma unroll
-    for (int cd = 0; cd < S::kNQ; ++cd) qop[cd] = *(const v4i*)(qp + 16 * cd);
+  while (true) {  // one part of a row tile's keys: BN-key units [at.unit, to)
+    const int h = at.h, i0 = at.tile * tt, i1 = min(i0 + tt, R.n);
+    const bool last = at.h == end.h && at.b == end.b && at.tile == end.tile;
+    const int lim_lo = R.token_limit(i0, causal), lim_hi = R.token_limit(i1 - 1, causal);
+    const int units = max(1, (lim_hi + BN) / BN), to = last ? min(end.unit, units) : units;
+    if (at.unit < to) {
+      const int32_t* pages = c.table + (int64_t)at.b * c.table_stride;
+      const uint8_t* kbase = (const uint8_t*)(c.k + h * c.head_stride);
+      const uint8_t* vbase = (const uint8_t*)(c.v + h * c.head_stride);
+      const int r = 32 * wave + j, ri = i0 + r / g, rc = min(ri, i1 - 1);  // the lane's row, its token
+      const int tok = R.t0 + rc, head = h * g + r % g;
+      const int lim = R.token_limit(rc, causal);
+      // the part's keys [k_lo, k_hi) and the tiles of them that every row sees whole
+      const int k_lo = at.unit * BN, k_hi = min(to * BN, lim_hi + 1);
+      const int ntiles = k_hi > k_lo ? to - at.unit : 0;
+      const int nfull = min(max(lim_lo + 1 - k_lo, 0) / BN, k_hi > k_lo ? (k_hi - k_lo) / BN : 0);
 
-    int pg[S::kRuns];
-    auto look_up = [&](int t) __attribute__((always_inline)) {
+      v4i qop[S::kNQ];  // q^T operand: q[row][16 cd + 8 hf .. + 8]
+      const uint16_t* qp = a.q + tok * a.ldqt + head * a.ldqh + 8 * hf;
 #pragma unroll
-      for (int u = 0; u < S::kRuns; ++u)
-        pg[u] = paged_page(c, pages, min(k_lo + t * BN + (wave + NW * u) * S::kRun + crow, k_hi - 1));
-    };
-    auto issue = [&](int t) __attribute__((always_inline)) {  // keys past the last repeat it (they are masked)
-      const uint32_t kb = (uint32_t)(uintptr_t)(lds + (t & 1) * S::kStage);
-#pragma unroll
-      for (int u = 0; u < S::kRuns; ++u) {
-        const int run = wave + NW * u, r = run * S::kRun + crow;
-        const int key = min(k_lo + t * BN + r, k_hi - 1);
-        const int64_t off = pg[u] * page_bytes + (int64_t)((key & slot_mask) * slot_bytes);
-        copy16(kb + run * 1024, kbase + off + 16 * k_place<D>(cpl, r));
-        copy16(kb + S::kTile + run * 1024, vbase + off + 16 * v_place<D>(cpl, r));
-      }
-    };
-    auto check_values = [&](int t) __attribute__((always_inline)) {
-      uint8_t* vb = lds + (t & 1) * S::kStage + S::kTile;
-      bool bad = false;
-#pragma unroll
-      for (int u = 0; u < S::kRuns; ++u) {
-        v4i* at = (v4i*)(vb + (wave + NW * u) * 1024 + lane * 16);
-        v4i x = *at;
-        if (take_nonfinite<T>(x)) *at = x, bad = true;
-      }
-      const bool any = __builtin_amdgcn_ballot_w64(bad) != 0;
-      if (lane == 0) flags[t & 1][wave] = any;
-    };
+      for (int cd = 0; cd < S::kNQ; ++cd) qop[cd] = *(const v4i*)(qp + 16 * cd);
 
-    v16f oacc[S::kND];
+      // Copies of 1 KB cover kRun rows from a multiple of kRun on, which lie in one page (page_size >= 8), so a copy's page
+      // and address are the wave's, and a lane adds a constant. Ids of the tile whose values are copied next, and of the
+      // one after it, whose keys are; copies wholly past the last key repeat that key's.
+      int pgv[S::kRuns], pgk[S::kRuns];
+      auto run_key = [&](int t, int u) __attribute__((always_inline)) {
+        return min(k_lo + t * BN + (wave + NW * u) * S::kRun, (k_hi - 1) & ~(S::kRun - 1));
+      };
+      auto place = [&](int t, int u, int page) __attribute__((always_inline)) {
+        return (uint64_t)(uint32_t)min(max(uniform(page), 0), c.pages - 1) * page_bytes +
+               ((uint32_t)run_key(t, u) & slot_mask) * slot_bytes;
+      };
+      auto look_up = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
-    for (int db = 0; db < S::kND; ++db) oacc[db] = (v16f){};
-    float m_run = -INFINITY, l_run = 0.0f;
+        for (int u = 0; u < S::kRuns; ++u) pgk[u] = pages[run_key(t, u) >> c.page_shift];
+      };
+      auto copy_keys = [&](int t) __attribute__((always_inline)) {
+        const uint32_t st = (uint32_t)(uintptr_t)(lds + (t & 1) * S::kTile);
+#pragma unroll
+        for (int u = 0; u < S::kRuns; ++u) copy16(st + (wave + NW * u) * 1024, kbase + place(t, u, pgk[u]), klane);
+      };
+      auto copy_values = [&](int t) __attribute__((always_inline)) {
+        const uint32_t st = (uint32_t)(uintptr_t)(lds + (2 + (t & 1)) * S::kTile);
+#pragma unroll
+        for (int u = 0; u < S::kRuns; ++u) copy16(st + (wave + NW * u) * 1024, vbase + place(t, u, pgv[u]), vlane);
+      };
+      // the copies that go out in tile t's first slot: its values and the next tile's keys, into the places of the
+      // tiles read up to the slot before
+      auto copies = [&](int t) __attribute__((always_inline)) {
+        copy_values(t);
+        if (t + 1 < ntiles) copy_keys(t + 1);
+#pragma unroll
+        for (int u = 0; u < S::kRuns; ++u) pgv[u] = pgk[u];
+        if (t + 2 < ntiles) look_up(t + 2);
+      };
+      // the end of its second slot: they have landed, here and (after the barrier) everywhere
+      auto landed = [&](int t) __attribute__((always_inline)) {
+        wait_vm_lgkm0<0>();
+        if (t >= nfull && t < ntiles) {  // a masked tile
+          uint8_t* vb = lds + (2 + (t & 1)) * S::kTile;
+          bool bad = false;
+#pragma unroll
+          for (int u = 0; u < S::kRuns; ++u) {
+            v4i* p = (v4i*)(vb + (wave + NW * u) * 1024 + lane * 16);
+            v4i x = *p;
+            if (k_lo + t * BN + (wave + NW * u) * S::kRun + crow >= k_hi) *p = (v4i){};  // whatever a page holds past the end
+            else if (take_nonfinite<T>(x)) *p = x, bad = true;
+          }
+          if (bad) aside = 1;
+        }
+        __syncthreads();
+      };
 
-    // MASK: the tile ends past some row's limit or the last key
-    auto step = [&](int t, auto mask_c) __attribute__((always_inline)) {
-      constexpr bool MASK = decltype(mask_c)::value;
-      const uint8_t* kb = lds + (t & 1) * S::kStage;
-      if (t + 1 < ntiles) issue(t + 1);
-      if (t + 2 < ntiles) look_up(t + 2);
-      const int vis = lim - (k_lo + t * BN);  // the lane's last visible key of the tile
-      v16f sc[S::kNSB];
-#pragma unroll
-      for (int sb = 0; sb < S::kNSB; ++sb) sc[sb] = (v16f){};
-#pragma unroll
-      for (int cd = 0; cd < S::kNQ; ++cd)
-#pragma unroll
-        for (int sb = 0; sb < S::kNSB; ++sb)
-          sc[sb] = Mfma<T>::wide(*(const v4i*)(kb + sb * 32 * S::kRow + kro[cd]), qop[cd], sc[sb]);
-      if (MASK) {
-#pragma unroll
-        for (int sb = 0; sb < S::kNSB; ++sb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (32 * sb + 8 * (i >> 2) + 4 * hf + (i & 3) > vis) sc[sb][i] = -INFINITY;
-      }
-      // the lane's maximum; the first level as med3(a, b, 3e38), which is max for scores below that and, unlike
-      // fmaxf, needs no quieting of raw MFMA results first
-      float m8[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        m8[i] = __builtin_amdgcn_fmed3f(sc[0][i], sc[0][i + 8], 3.0e38f);
-#pragma unroll
-        for (int sb = 1; sb < S::kNSB; ++sb)
-          m8[i] = fmaxf(m8[i], __builtin_amdgcn_fmed3f(sc[sb][i], sc[sb][i + 8], 3.0e38f));
-      }
-#pragma unroll
-      for (int w = 4; w >= 1; w >>= 1)
-#pragma unroll
-        for (int i = 0; i < w; ++i) m8[i] = fmaxf(m8[i], m8[i + w]);
-      const float x_max = fmaxf(m8[0], __shfl_xor(m8[0], 32)) * a.c_log2;
-      const bool bump = x_max > m_run;
-      const float m_new = bump ? x_max : m_run;
-      // a row that has seen no key yet subtracts 0: its scores are all -inf and its p all 0
-      const float ref = MASK && m_new == -INFINITY ? 0.0f : m_new;
-      const float alpha = __builtin_amdgcn_exp2f(m_run - ref);  // 0 on the first tile
-      m_run = m_new;
-      float ps[S::kNC];
+      v16f oacc[S::kND], sc[S::kNSB];
       v4i pop[S::kNC];
 #pragma unroll
-      for (int cc = 0; cc < S::kNC; ++cc) {
-        float p[8];
+      for (int db = 0; db < S::kND; ++db) oacc[db] = (v16f){};
+      float m_run = -INFINITY, l_run = 0.0f;
+
+      // matrix slot: O of tile t - 1 (VALUES), then S of tile t (KEYS). The operands are read from LDS kAhead MFMAs ahead
+      // of their use, in an order the scheduler may not change: left to itself, short of registers, it waits for
+      // each operand right after asking for it
+      auto matrix = [&](int t, auto values_c, auto keys_c) __attribute__((always_inline)) {
+        constexpr bool VALUES = decltype(values_c)::value, KEYS = decltype(keys_c)::value;
+        constexpr int kAhead = 6, kV = VALUES ? S::kND * S::kNC : 0, kAll = kV + (KEYS ? S::kNQ * S::kNSB : 0);
+        const uint8_t* vb = lds + (2 + ((t - 1) & 1)) * S::kTile;
+        const uint8_t* kb = lds + (t & 1) * S::kTile;
+        v4i ring[kAhead];
+        auto read = [&](int i) __attribute__((always_inline)) {
+          if (i < kV) {
+            const uint8_t* p = vb + (vro ^ (uint32_t)(64 * (i / S::kNC))) + 16 * (i % S::kNC) * S::kRow;
+            ring[i % kAhead] = two_halves(lds_read_tr(p), lds_read_tr(p + 8 * S::kRow));
+          } else {
+            const int k = i - kV;
+            ring[i % kAhead] = *(const v4i*)(kb + (kro ^ (uint32_t)(32 * (k / S::kNSB))) + k % S::kNSB * 32 * S::kRow);
+          }
+        };
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[cc >> 1][8 * (cc & 1) + e], a.c_log2, -ref));
-        ps[cc] = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-        pop[cc] = (v4i){Mfma<T>::pack(p[0], p[1]), Mfma<T>::pack(p[2], p[3]), Mfma<T>::pack(p[4], p[5]),
-                        Mfma<T>::pack(p[6], p[7])};
-      }
+        for (int i = 0; i < kAhead; ++i) read(i);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int w = S::kNC / 2; w >= 1; w >>= 1)
+        for (int i = 0; i < kAll; ++i) {
+          if (i < kV) {
+            oacc[i / S::kNC] = Mfma<T>::wide(ring[i % kAhead], pop[i % S::kNC], oacc[i / S::kNC]);
+          } else {
+            const int k = i - kV;
+            sc[k % S::kNSB] = Mfma<T>::wide(ring[i % kAhead], qop[k / S::kNSB], k < S::kNSB ? (v16f){} : sc[k % S::kNSB]);
+          }
+          if (i + kAhead < kAll) read(i + kAhead);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      };
+      const std::true_type yes;
+      const std::false_type no;
+      auto softmax_of = [&](int t, auto mask_c) __attribute__((always_inline)) {
+        constexpr bool MASK = decltype(mask_c)::value;
+        if (MASK) {
+          const int vis = lim - (k_lo + t * BN) - 4 * hf;  // the lane's last visible key of the tile, less its keys' common part
 #pragma unroll
-        for (int i = 0; i < w; ++i) ps[i] += ps[i + w];
-      l_run = __builtin_fmaf(l_run, alpha, ps[0]);
-      if (__builtin_amdgcn_ballot_w64(bump) != 0) {  // alpha is 1 in lanes whose maximum stayed
+          for (int sb = 0; sb < S::kNSB; ++sb)
 #pragma unroll
-        for (int db = 0; db < S::kND; ++db) oacc[db] *= alpha;
-      }
+            for (int i = 0; i < 16; ++i)
+              if (32 * sb + 8 * (i >> 2) + (i & 3) > vis) sc[sb][i] = -INFINITY;
+        }
+        // the lane's maximum; the first level as med3(a, b, 3e38), which is max for scores below that and, unlike
+        // fmaxf, needs no quieting of raw MFMA results first
+        float m8[8];
 #pragma unroll
-      for (int db = 0; db < S::kND; ++db)
+        for (int i = 0; i < 8; ++i) {
+          m8[i] = __builtin_amdgcn_fmed3f(sc[0][i], sc[0][i + 8], 3.0e38f);
+#pragma unroll
+          for (int sb = 1; sb < S::kNSB; ++sb)
+            m8[i] = fmaxf(m8[i], __builtin_amdgcn_fmed3f(sc[sb][i], sc[sb][i + 8], 3.0e38f));
+        }
+#pragma unroll
+        for (int w = 4; w >= 1; w >>= 1)
+#pragma unroll
+          for (int i = 0; i < w; ++i) m8[i] = fmaxf(m8[i], m8[i + w]);
+        const float x_max = fmaxf(m8[0], __shfl_xor(m8[0], 32)) * a.c_log2;
+        const bool bump = x_max > m_run;
+        const float m_new = bump ? x_max : m_run;
+        // a row that has seen no key yet subtracts 0: its scores are all -inf and its p all 0
+        const float ref = MASK && m_new == -INFINITY ? 0.0f : m_new;
+        const float alpha = __builtin_amdgcn_exp2f(m_run - ref);  // 0 on the first tile
+        m_run = m_new;
+        float ps[S::kNC];
 #pragma unroll
         for (int cc = 0; cc < S::kNC; ++cc) {
-          const v4s_ lo = lds_read_tr(kb + vro[db] + 16 * cc * S::kRow);
-          const v4s_ hi = lds_read_tr(kb + vro[db] + (16 * cc + 8) * S::kRow);
-          oacc[db] = Mfma<T>::wide(two_halves(lo, hi), pop[cc], oacc[db]);
-        }
-      if (MASK) {
-        bool taken = false;
+          float p[8];
 #pragma unroll
-        for (int w = 0; w < NW; ++w) taken |= flags[t & 1][w] != 0;
-        if (taken) {
-          for (int kk = 0; kk < BN; ++kk) {
-            if (__builtin_amdgcn_ballot_w64(kk <= vis) == 0) break;
+          for (int e = 0; e < 8; ++e)
+            p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[cc >> 1][8 * (cc & 1) + e], a.c_log2, -ref));
+          ps[cc] = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+          pop[cc] = (v4i){Mfma<T>::pack(p[0], p[1]), Mfma<T>::pack(p[2], p[3]), Mfma<T>::pack(p[4], p[5]),
+                          Mfma<T>::pack(p[6], p[7])};
+        }
+#pragma unroll
+        for (int w = S::kNC / 2; w >= 1; w >>= 1)
+#pragma unroll
+          for (int i = 0; i < w; ++i) ps[i] += ps[i + w];
+        l_run = __builtin_fmaf(l_run, alpha, ps[0]);
+        if (__builtin_amdgcn_ballot_w64(bump) != 0) {  // alpha is 1 in lanes whose maximum stayed
+#pragma unroll
+          for (int db = 0; db < S::kND; ++db) oacc[db] *= alpha;
+        }
+      };
+      auto softmax = [&](int t) __attribute__((always_inline)) {
+        if (t < nfull) softmax_of(t, no);
+        else softmax_of(t, yes);
+      };
+
+      if (ntiles > 0) {
+        if (tid == 0) aside = 0;
+        look_up(0);
+        copy_keys(0);
+#pragma unroll
+        for (int u = 0; u < S::kRuns; ++u) pgv[u] = pgk[u];
+        if (ntiles > 1) look_up(1);
+        wait_vm_lgkm0<0>();
+        __syncthreads();
+        // tile t: slots 2 t and 2 t + 1 of the waves that run ahead, one later of those behind; all pass the same barriers
+        if (behind == 0) {
+          copies(0);
+          matrix(0, no, yes);
+          barrier_lds();
+          for (int t = 0; t + 1 < ntiles; ++t) {
+            softmax(t);
+            landed(t);
+            copies(t + 1);
+            matrix(t + 1, yes, yes);
+            barrier_lds();
+          }
+          softmax_of(ntiles - 1, yes);
+          landed(ntiles - 1);
+          matrix(ntiles, yes, no);
+          barrier_lds();
+          __syncthreads();
+        } else {
+          copies(0);
+          barrier_lds();
+          matrix(0, no, yes);
+          landed(0);
+          for (int t = 0; t + 1 < ntiles; ++t) {
+            copies(t + 1);
+            softmax(t);
+            barrier_lds();
+            matrix(t + 1, yes, yes);
+            landed(t + 1);
+          }
+          softmax_of(ntiles - 1, yes);
+          barrier_lds();
+          matrix(ntiles, yes, no);
+          __syncthreads();
+        }
+        if (aside) {  // rows that see keys whose values were set aside: those values, one by one
+          for (int key = k_lo + nfull * BN; key < k_hi; ++key) {
+            const int64_t at_key = paged_at(c, paged_page(c, pages, key), h, key);
             float s = 0.0f;
 #pragma unroll
-            for (int cd = 0; cd < S::kNQ; ++cd)
-              s = dot8<T>(qop[cd], *(const v4i*)(kb + kk * S::kRow + 16 * k_place<D>(2 * cd + hf, kk)), s);
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s + __shfl_xor(s, 32), a.c_log2, -ref));
-            if (kk <= vis) {  // the key exists: limits lie below the sequence's length
-              const int key = k_lo + t * BN + kk;
-              const uint16_t* vp = c.v + paged_at(c, paged_page(c, pages, key), h, key) + 4 * hf;
+            for (int cd = 0; cd < S::kNQ; ++cd) s = dot8<T>(qop[cd], *(const v4i*)(c.k + at_key + 8 * hf + 16 * cd), s);
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s + __shfl_xor(s, 32), a.c_log2, -m_run));
+            if (key <= lim) {
 #pragma unroll
               for (int db = 0; db < S::kND; ++db)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                  const float v = T::load(vp[32 * db + 8 * (i >> 2) + (i & 3)]);
+                  const float v = T::load(c.v[at_key + 32 * db + 8 * (i >> 2) + 4 * hf + (i & 3)]);
                   if (!(fabsf(v) < INFINITY)) oacc[db][i] = fmaf(p, v, oacc[db][i]);
                 }
             }
           }
         }
+        __syncthreads();  // `aside` has been read
       }
-      wait_vm_lgkm0<0>();                                   // this wave's copies of tile t + 1 have landed
-      if (t + 1 >= nfull && t + 1 < ntiles) check_values(t + 1);  // a masked tile
-      __syncthreads();                                      // everyone's have; everyone is done with tile t's buffer
-    };
 
-    if (ntiles > 0) {
-      look_up(0);
-      issue(0);
-      if (ntiles > 1) look_up(1);
-      wait_vm_lgkm0<0>();
-      if (nfull == 0) check_values(0);
-      __syncthreads();
+      const float l_tot = l_run + __shfl_xor(l_run, 32);
+      const float inv = m_run == -INFINITY ? 0.0f : 1.0f / l_tot;
+      const float lse2 = m_run == -INFINITY ? -INFINITY : m_run + __builtin_amdgcn_logf(l_tot);
+      if (at.unit > 0 || to < units) {
+        // a part: into the share's slot, the first for a tile that an earlier share began, else the second
+        const int64_t prow = (int64_t)(2 * share + (at.unit > 0 ? 0 : 1)) * BM + r;
+        float* op = a.o_part + prow * D + 4 * hf;
+#pragma unroll
+        for (int db = 0; db < S::kND; ++db)
+#pragma unroll
+          for (int i = 0; i < 16; i += 4)
+            *(float4*)(op + 32 * db + 2 * i) = make_float4(oacc[db][i] * inv, oacc[db][i + 1] * inv,
+                                                           oacc[db][i + 2] * inv, oacc[db][i + 3] * inv);
+        if (hf == 0) a.lse_part[prow] = lse2;
+      } else if (r < tt * g && ri < i1) {
+        const int64_t out_row = (int64_t)tok * a.heads + head;
+        uint16_t* op = a.o + out_row * D + 4 * hf;
+#pragma unroll
+        for (int db = 0; db < S::kND; ++db)
+#pragma unroll
+          for (int i = 0; i < 16; i += 4)
+            *(uint2*)(op + 32 * db + 2 * i) =
+                make_uint2((uint32_t)Mfma<T>::pack(oacc[db][i] * inv, oacc[db][i + 1] * inv),
+                           (uint32_t)Mfma<T>::pack(oacc[db][i + 2] * inv, oacc[db][i + 3] * inv));
+        if (hf == 0) a.lse[out_row] = lse2 * kLn2;
+      }
     }
-    for (int t = 0; t < nfull; ++t) step(t, std::false_type{});
-    for (int t = nfull; t < ntiles; ++t) step(t, std::true_type{});
+    if (last) break;
+    at.unit = 0;
+    if (i1 < R.n) {
+      ++at.tile;
+    } else {
+      at.tile = 0;
+      do {  // the next sequence with new tokens, of the next head after the last
+        if (++at.b == c.batch) at.b = 0, ++at.h;
+        if (at.h == c.kv_heads) return;  // the line's end
+        R = uniform_rows_of(c, at.b, a.tokens, g);
+      } while (R.n == 0);
+    }
+  }
+}
 
-    const float l_tot = l_run + __shfl_xor(l_run, 32);
-    const float inv = m_run == -INFINITY ? 0.0f : 1.0f / l_tot;
-    if (row < R.total) {
-#pragma unroll
-      for (int db = 0; db < S::kND; ++db)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4)
-          put_o<T, D>(a, split, out_row, 32 * db + 2 * i + 4 * hf, oacc[db][i] * inv, oacc[db][i + 1] * inv,
-                      oacc[db][i + 2] * inv, oacc[db][i + 3] * inv);
-      if (hf == 0) put_lse(a, split, out_row, m_run, l_tot);
+// Joins the parts of row tiles that the shares' ends cut, in the shares' order. A workgroup takes JT_ROWS rows of a tile
+// and finds from the same division which shares hold a part of it.
+constexpr int JT_ROWS = 32;
+
+template <class T, int D, int BM, int BN>
+__global__ __launch_bounds__(256) void paged_attn_join_parts_kernel(AttnArgs a) {
+  const PagedArgs& c = a.c;
+  const int g = a.heads / c.kv_heads, groups = c.batch * c.kv_heads, tt = BM / g;
+  const bool causal = a.causal != 0;
+  const int chunk = blockIdx.x % (BM / JT_ROWS), rest = blockIdx.x / (BM / JT_ROWS);
+  const int b = rest % groups % c.batch, h = rest % groups / c.batch;
+  const Rows R = uniform_rows_of(c, b, a.tokens, g);
+  if (rest / groups * tt >= R.n) return;
+  int64_t before;
+  const int64_t per_head = head_line(c, a.tokens, tt, causal, b, before), all = per_head * c.kv_heads;
+  const TileLine line = tile_line(R, tt, causal);
+  __shared__ int slots[2 * kCus];  // the slots of a tile's parts, in order
+  __shared__ int nslots;
+  for (int tile = rest / groups; tile * tt < R.n; tile += a.tiles) {
+    const int64_t x0 = h * per_head + before + line.before(tile), x1 = h * per_head + before + line.before(tile + 1);
+    const int i0 = tile * tt, i1 = min(i0 + tt, R.n);
+    const int units = max(1, (R.token_limit(i1 - 1, causal) + BN) / BN);
+    // shares whose start lies in (x0, x1) cut the tile; s0 is the one before them. A share starts at or before x where
+    // all * s / n <= x
+    const int s0 = (int)(((x0 + 1) * a.shares - 1) / all), s1 = (int)((x1 * a.shares - 1) / all);
+    if (s0 == s1) continue;
+    auto cut = [&](int s) {  // the unit at which share s begins, of those in s0 .. s1 + 1
+      if (s <= s0) return 0;
+      return s > s1 ? units : min(units, (int)(share_start(all, s, a.shares) - x0) / BN);
+    };
+    __syncthreads();  // the list of the tile before is no longer read
+    if (threadIdx.x < 64) {
+      int n = 0;
+      for (int s = s0; s <= s1; s += 64) {
+        const int mine = s + threadIdx.x, lo = cut(mine);
+        const bool part = mine <= s1 && cut(mine + 1) > lo;
+        const uint64_t parts = __ballot(part);
+        if (part) slots[n + __popcll(parts & ((1ull << threadIdx.x) - 1))] = 2 * mine + (lo > 0 ? 0 : 1);
+        n += __popcll(parts);
+      }
+      if (threadIdx.x == 0) nslots = n;
+    }
+    __syncthreads();
+    const int parts = nslots;
+    if (parts < 2) continue;  // whole after all: cuts before its first keys or behind its last
+    const int rows = min(JT_ROWS, (i1 - i0) * g - chunk * JT_ROWS);
+    for (int i = threadIdx.x; i < rows * (D / 4); i += 256) {
+      const int r = chunk * JT_ROWS + i / (D / 4), d = i % (D / 4) * 4;
+      float m = -INFINITY;
+      for (int k = 0; k < parts; ++k) m = fmaxf(m, a.lse_part[(int64_t)slots[k] * BM + r]);
+      const float ref = m == -INFINITY ? 0.0f : m;
+      float l = 0.0f;
+      v4f o = {};
+#pragma unroll 4
+      for (int k = 0; k < parts; ++k) {
+        const int64_t prow = (int64_t)slots[k] * BM + r;
+        const float f = __builtin_amdgcn_exp2f(a.lse_part[prow] - ref);
+        l += f;
+        o += *(const v4f*)(a.o_part + prow * D + d) * f;
+      }
+      const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
+      const int64_t out_row = (int64_t)(R.t0 + i0 + r / g) * a.heads + h * g + r % g;
+      *(uint2*)(a.o + out_row * D + d) = make_uint2((uint32_t)Mfma<T>::pack(o[0] * inv, o[1] * inv),
+                                                    (uint32_t)Mfma<T>::pack(o[2] * inv, o[3] * inv));
+      if (d == 0) a.lse[out_row] = m == -INFINITY ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
     }
   }
 }
@@ -475,6 +651,10 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(AttnArgs a) {
         page_ids[i] = min(max(pages[p0 + i], 0), c.pages - 1);
       __syncthreads();
       const int ntiles = (s_hi - s_lo + FW_KEYS - 1) / FW_KEYS;
+      bool aside = false;  // whether values of a masked tile were set aside (see the many-rows kernel)
+      auto whole = [&](int t) {  // every row sees the whole tile
+        return s_lo + (t + 1) * FW_KEYS <= min(lim_lo + 1, s_hi);
+      };
       auto issue = [&](int t) __attribute__((always_inline)) {  // keys past the last repeat it (they are masked)
         uint8_t* st = mine + ((t / NW) & 1) * S::kStage;
         const uint32_t kb = (uint32_t)(uintptr_t)st;
@@ -493,15 +673,13 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(AttnArgs a) {
         const int k0 = s_lo + t * FW_KEYS;
         v4i pop[RB];
         float ref[RB];
-        bool taken = false;
         if (MASK) {
 #pragma unroll
           for (int u = 0; u < S::kRuns; ++u) {
             v4i* at = (v4i*)(kb + S::kTile + u * 1024 + lane * 16);
             v4i x = *at;
-            if (take_nonfinite<T>(x)) *at = x, taken = true;
+            if (take_nonfinite<T>(x)) *at = x, aside = true;
           }
-          taken = __builtin_amdgcn_ballot_w64(taken) != 0;
         }
         v4f sc[RB][2];
 #pragma unroll
@@ -530,7 +708,7 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(AttnArgs a) {
           for (int x = 0; x < 2; ++x)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              if (MASK && k0 + 16 * x + 4 * q4 + r > lim[rb]) sc[rb][x][r] = -INFINITY;
+              if (MASK && 16 * x + r > lim[rb] - k0 - 4 * q4) sc[rb][x][r] = -INFINITY;
               mx = fmaxf(mx, sc[rb][x][r]);
             }
           mx = fmaxf(mx, __shfl_xor(mx, 16));
@@ -559,32 +737,6 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(AttnArgs a) {
 #pragma unroll
           for (int rb = 0; rb < RB; ++rb) oacc[rb][db] = Mfma<T>::tall(vop, pop[rb], oacc[rb][db]);
         }
-        if (MASK && taken) {
-          for (int kk = 0; kk < FW_KEYS; ++kk) {
-            const int key = k0 + kk;
-            if (key > lim_hi) break;
-#pragma unroll
-            for (int rb = 0; rb < RB; ++rb) {
-              float s = 0.0f;
-#pragma unroll
-              for (int cd = 0; cd < S::kNQ; ++cd)
-                s = dot8<T>(qop[rb][cd], *(const v4i*)(kb + kk * S::kRow + 16 * k_place<D>(4 * cd + q4, kk)), s);
-              s += __shfl_xor(s, 16);
-              s += __shfl_xor(s, 32);
-              const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s, a.c_log2, -ref[rb]));
-              if (key <= lim[rb]) {
-                const uint16_t* vp = c.v + paged_at(c, paged_page(c, pages, key), h, key) + 4 * q4;
-#pragma unroll
-                for (int db = 0; db < S::kND; ++db)
-#pragma unroll
-                  for (int r = 0; r < 4; ++r) {
-                    const float v = T::load(vp[16 * db + r]);
-                    if (!(fabsf(v) < INFINITY)) oacc[rb][db][r] = fmaf(p, v, oacc[rb][db][r]);
-                  }
-              }
-            }
-          }
-        }
       };
       // tiles wave, wave + NW, ...: the next one's copies go out before this one's are waited for
       if (wave < ntiles) issue(wave);
@@ -596,11 +748,37 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(AttnArgs a) {
           wait_vm_lgkm0<0>();
         }
         asm volatile("" ::: "memory");
-        const int k1 = s_lo + (t + 1) * FW_KEYS;
-        if (k1 <= lim_lo + 1 && k1 <= s_hi) step(t, std::false_type{});
+        if (whole(t)) step(t, std::false_type{});
         else step(t, std::true_type{});
         wait_vm_lgkm0<63>();  // this tile's LDS reads are done before its stage is copied into again
         asm volatile("" ::: "memory");
+      }
+      if (__builtin_amdgcn_ballot_w64(aside) != 0) {  // rows that see keys whose values were set aside: those values
+        for (int t = wave; t < ntiles; t += NW) {
+          if (whole(t)) continue;
+          for (int key = s_lo + t * FW_KEYS; key < min(s_lo + (t + 1) * FW_KEYS, s_hi); ++key) {
+            const int64_t at_key = paged_at(c, paged_page(c, pages, key), h, key);
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+              float s = 0.0f;
+#pragma unroll
+              for (int cd = 0; cd < S::kNQ; ++cd)
+                s = dot8<T>(qop[rb][cd], *(const v4i*)(c.k + at_key + 8 * q4 + 32 * cd), s);
+              s += __shfl_xor(s, 16);
+              s += __shfl_xor(s, 32);
+              const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s, a.c_log2, -m_run[rb]));
+              if (key <= lim[rb]) {
+#pragma unroll
+                for (int db = 0; db < S::kND; ++db)
+#pragma unroll
+                  for (int r = 0; r < 4; ++r) {
+                    const float v = T::load(c.v[at_key + 16 * db + 4 * q4 + r]);
+                    if (!(fabsf(v) < INFINITY)) oacc[rb][db][r] = fmaf(p, v, oacc[rb][db][r]);
+                  }
+              }
+            }
+          }
+        }
       }
     }
 
@@ -633,34 +811,47 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(AttnArgs a) {
       }
       const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
       const int64_t at = (int64_t)(R.t0 + (row0 + r) / g) * a.heads + h * g + (row0 + r) % g;
-      put_o<T, D>(a, split, at, d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+      if (k_hi > k_lo || a.splits == 1) put_o<T, D>(a, split, at, d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
       if (d == 0) put_lse(a, split, at, m, l);
     }
     if (row0 + 16 * RB < R.total) __syncthreads();  // the stages are copied into again
   }
 }
 
-// Joins a row's splits, in their order: one wave a row.
+// Joins a row's splits, in their order: D / 4 lanes a row, 4 channels each, 4 splits' loads in flight.
 template <class T, int D>
 __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t rows = (int64_t)a.tokens * a.heads, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  constexpr int L = D / 4;
+  const int64_t rows = (int64_t)a.tokens * a.heads, row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
   if (row >= rows) return;
+  const int d = threadIdx.x % L * 4;
   float m = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.lse_part[s * rows + row]);
-  const float ref = m == -INFINITY ? 0.0f : m;
-  float l = 0.0f, o[D / 64] = {};
-  for (int s = 0; s < a.splits; ++s) {
-    const float f = __builtin_amdgcn_exp2f(a.lse_part[s * rows + row] - ref);
-    l += f;
-    const float* p = a.o_part + (s * rows + row) * D + lane * (D / 64);
+  for (int s = 0; s < a.splits; s += 4) {
+    float x[4];
 #pragma unroll
-    for (int e = 0; e < D / 64; ++e) o[e] = __builtin_fmaf(p[e], f, o[e]);
+    for (int e = 0; e < 4; ++e) x[e] = a.lse_part[min(s + e, a.splits - 1) * rows + row];
+    m = fmaxf(fmaxf(fmaxf(m, x[0]), fmaxf(x[1], x[2])), x[3]);
+  }
+  const float ref = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f;
+  v4f o = {};
+  for (int s = 0; s < a.splits; s += 4) {
+    float f[4];
+    v4f x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f[e] = s + e < a.splits ? __builtin_amdgcn_exp2f(a.lse_part[min(s + e, a.splits - 1) * rows + row] - ref) : 0.0f;
+      x[e] = (v4f){};
+      // a split without keys for the row has not written its part
+      if (f[e] != 0.0f) x[e] = *(const v4f*)(a.o_part + ((s + e) * rows + row) * D + d);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) l += f[e], o += x[e] * f[e];
   }
   const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
-  if constexpr (D == 128) ((uint32_t*)(a.o + row * D))[lane] = (uint32_t)Mfma<T>::pack(o[0] * inv, o[1] * inv);
-  else a.o[row * D + lane] = (uint16_t)Mfma<T>::pack(o[0] * inv, 0.0f);
-  if (lane == 0) a.lse[row] = m == -INFINITY ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+  *(uint2*)(a.o + row * D + d) = make_uint2((uint32_t)Mfma<T>::pack(o[0] * inv, o[1] * inv),
+                                            (uint32_t)Mfma<T>::pack(o[2] * inv, o[3] * inv));
+  if (d == 0) a.lse[row] = m == -INFINITY ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 // ---------------------------------------------------------------------------
@@ -693,44 +884,94 @@ __global__ __launch_bounds__(256) void paged_gather_scores_kernel(AttnArgs a) {
   }
 }
 
-// Recomputed: a wave holds 32 keys as the MFMA's A operand and walks all rows in blocks of 32 (q^T as B, straight from
-// memory: the 4 waves of a workgroup and the key blocks of one kv head read the same rows). A lane sums its row's
-// probabilities for 16 keys; the 32 rows' lanes are joined at the end.
-constexpr int GT_WAVES = 4;
+// Recomputed: a wave holds 32 keys as the MFMA's A operand and walks the rows in tiles of 64, which a workgroup of 4
+// waves (128 keys) copies to LDS, double buffered (q^T as B). A lane sums its row's probabilities for 16 keys; the
+// lanes of the 32 rows are joined at the end. The rows are divided over `splits` workgroups where the keys alone are
+// too few to fill the chip: each leaves its sums in w_part [split][group][score_stride], joined in order.
+constexpr int GT_WAVES = 4, GT_ROWS = 64, GT_KEYS = 32 * GT_WAVES;
 
 template <class T, int D>
 __global__ __launch_bounds__(64 * GT_WAVES) void paged_gather_tile_kernel(AttnArgs a) {
-  constexpr int NQ = D / 16;
+  constexpr int NQ = D / 16, kRow = 2 * D, kRun = 1024 / kRow, kRuns = GT_ROWS / kRun / GT_WAVES, kStage = GT_ROWS * kRow;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
   const PagedArgs& c = a.c;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, j = lane & 31, hf = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, j = lane & 31, hf = lane >> 5;
   const int groups = c.batch * c.kv_heads;
-  const int grp = blockIdx.x % groups, b = grp / c.kv_heads, h = grp % c.kv_heads, g = a.heads / c.kv_heads;
+  const int grp = blockIdx.x % groups, rest = blockIdx.x / groups, split = rest % a.splits;
+  const int b = grp / c.kv_heads, h = grp % c.kv_heads, g = a.heads / c.kv_heads;
   const Rows R = rows_of(c, b, a.tokens, g);
   const bool causal = a.causal != 0;
   const int32_t* pages = c.table + (int64_t)b * c.table_stride;
-  for (int j0 = (blockIdx.x / groups * GT_WAVES + wave) * 32; j0 < R.len; j0 += a.tiles * GT_WAVES * 32) {
-    const int key = min(j0 + j, R.len - 1);
-    const uint16_t* kp = c.k + paged_at(c, paged_page(c, pages, key), h, key) + 8 * hf;
+  constexpr int CH = D / 8;
+  const int crow = lane / CH, cpl = lane % CH;
+  uint32_t qro[NQ];
+#pragma unroll
+  for (int cd = 0; cd < NQ; ++cd) qro[cd] = (uint32_t)(j * kRow + 16 * k_place<D>(2 * cd + hf, j));
+
+  for (int w0 = rest / a.splits * GT_KEYS; w0 < R.len; w0 += a.tiles * GT_KEYS) {
+    const int j0 = w0 + 32 * wave, key = min(j0 + j, R.len - 1);
+    const int64_t kat = paged_at(c, paged_page(c, pages, key), h, key);
     v4i kop[NQ];
 #pragma unroll
-    for (int cd = 0; cd < NQ; ++cd) kop[cd] = *(const v4i*)(kp + 16 * cd);
-    float sum[16] = {};
-    // rows that see no key of this block come first
-    const int first = causal ? max(j0 - (R.len - R.n), 0) * g : 0;
-    for (int row0 = first; row0 < R.total; row0 += 32) {
-      const int rc = min(row0 + j, R.total - 1), tok = R.t0 + rc / g, x = h * g + rc % g;
-      const uint16_t* qp = a.q + tok * a.ldqt + x * a.ldqh + 8 * hf;
-      v16f s = {};
+    for (int cd = 0; cd < NQ; ++cd) kop[cd] = *(const v4i*)(c.k + kat + 8 * hf + 16 * cd);
+    // rows that see a key of this workgroup's come last; this split's share of their tiles
+    const int first = causal ? max(w0 - (R.len - R.n), 0) * g : 0;
+    const int all = first < R.total ? (R.total - first + GT_ROWS - 1) / GT_ROWS : 0;
+    const int t_lo = (int)((int64_t)all * split / a.splits), t_hi = (int)((int64_t)all * (split + 1) / a.splits);
+    float sum[16] = {}, lse2[2], next2[2];
+    auto lse_of = [&](int t, float (&out)[2]) __attribute__((always_inline)) {
 #pragma unroll
-      for (int cd = 0; cd < NQ; ++cd) s = Mfma<T>::wide(kop[cd], *(const v4i*)(qp + 16 * cd), s);
-      const float lse2 = a.lse[(int64_t)tok * a.heads + x] * kLog2e;
-      const int vis = row0 + j < R.total ? R.limit(rc, causal) - j0 : -1;
+      for (int x = 0; x < 2; ++x) {
+        const int rc = min(first + t * GT_ROWS + 32 * x + j, R.total - 1);
+        out[x] = a.lse[(int64_t)(R.t0 + rc / g) * a.heads + h * g + rc % g] * kLog2e;
+      }
+    };
+    auto issue = [&](int t) __attribute__((always_inline)) {
+      const uint32_t st = (uint32_t)(uintptr_t)(lds + (t & 1) * kStage);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c_log2, -lse2));
-        sum[i] += 8 * (i >> 2) + 4 * hf + (i & 3) <= vis ? p : 0.0f;
+      for (int u = 0; u < kRuns; ++u) {
+        const int run = wave + GT_WAVES * u, r = run * kRun + crow, rc = min(first + t * GT_ROWS + r, R.total - 1);
+        copy16(st + run * 1024, a.q + (R.t0 + rc / g) * a.ldqt + (h * g + rc % g) * a.ldqh + 8 * k_place<D>(cpl, r));
+      }
+    };
+    if (t_lo < t_hi) {
+      lse_of(t_lo, next2);
+      issue(t_lo);
+    }
+    for (int t = t_lo; t < t_hi; ++t) {
+      wait_vm_lgkm0<0>();
+      __syncthreads();  // tile t is there; everyone is done with the other stage
+      lse2[0] = next2[0], lse2[1] = next2[1];
+      if (t + 1 < t_hi) {
+        lse_of(t + 1, next2);
+        issue(t + 1);
+      }
+      const uint8_t* st = lds + (t & 1) * kStage;
+      const int row0 = first + t * GT_ROWS;
+      v16f s[2] = {};
+#pragma unroll
+      for (int cd = 0; cd < NQ; ++cd)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) s[x] = Mfma<T>::wide(kop[cd], *(const v4i*)(st + 32 * x * kRow + qro[cd]), s[x]);
+      // whole tiles every row of which sees all of the wave's keys need no mask
+      if (row0 + GT_ROWS <= R.total && R.limit(row0, causal) >= j0 + 31) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sum[i] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][i], a.c_log2, -lse2[x]));
+      } else {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int r = row0 + 32 * x + j, vis = r < R.total ? R.limit(r, causal) - j0 - 4 * hf : -1;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][i], a.c_log2, -lse2[x]));
+            sum[i] += 8 * (i >> 2) + (i & 3) <= vis ? p : 0.0f;
+          }
+        }
       }
     }
+    __syncthreads();  // the next keys' first tile is copied into a stage that this one's last may still be read from
 #pragma unroll
     for (int i = 0; i < 16; ++i)
 #pragma unroll
@@ -739,9 +980,22 @@ __global__ __launch_bounds__(64 * GT_WAVES) void paged_gather_tile_kernel(AttnAr
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int at = j0 + 8 * (i >> 2) + 4 * hf + (i & 3);
-        if (at < R.len) c.w[paged_w_at(c, paged_page(c, pages, at), h, at)] += sum[i];
+        if (at >= R.len) continue;
+        if (a.splits > 1) a.w_part[((int64_t)split * groups + grp) * a.score_stride + at] = sum[i];
+        else c.w[paged_w_at(c, paged_page(c, pages, at), h, at)] += sum[i];
       }
     }
+  }
+}
+
+__global__ __launch_bounds__(256) void paged_gather_join_kernel(AttnArgs a) {
+  const PagedArgs& c = a.c;
+  const int grp = blockIdx.y, b = grp / c.kv_heads, h = grp % c.kv_heads, groups = c.batch * c.kv_heads;
+  const int len = paged_kv_len(c, b);
+  for (int j = blockIdx.x * 256 + threadIdx.x; j < len; j += gridDim.x * 256) {
+    float sum = 0.0f;
+    for (int s = 0; s < a.splits; ++s) sum += a.w_part[((int64_t)s * groups + grp) * a.score_stride + j];
+    c.w[paged_w_at(c, paged_page(c, c.table + (int64_t)b * c.table_stride, j), h, j)] += sum;
   }
 }
 
@@ -754,14 +1008,16 @@ struct Plan {
   bool matrix, few, keep_scores;
   int row_blocks;  // few: 16-row blocks a workgroup (1 or 2)
   int waves;       // tile: 4 or 8
-  int splits, split_keys, tiles;
+  int splits, split_keys, tiles, shares;
+  int row_splits, key_tiles;  // of the recomputing gather
   int64_t score_stride, part_floats, bytes;
 };
 
 Plan plan_of(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t d, int64_t max_q, int64_t max_kv,
              int64_t capacity, bool gather) {
   Plan p = {};
-  p.matrix = d == 64 || d == 128;
+  // a row tile holds a token's whole group of query heads
+  p.matrix = (d == 64 || d == 128) && heads / kv_heads <= 256;
   p.splits = 1, p.split_keys = 1 << 30, p.tiles = 1;
   if (!p.matrix || batch == 0 || tokens == 0) return p;
   const int64_t rows = max_q * (heads / kv_heads), groups = batch * kv_heads;
@@ -775,20 +1031,29 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int
     if (keys < 256) keys = 256;
     p.split_keys = (int)keys;
     p.splits = (int)((max_kv + keys - 1) / keys);
-    p.score_stride = (capacity + 3) / 4 * 4;
-    p.keep_scores = gather && tokens * heads * p.score_stride * 4 <= kScoreBytes;
+    p.keep_scores = gather && tokens * heads * ((capacity + 3) / 4 * 4) * 4 <= kScoreBytes;
   } else {
     p.waves = rows <= 128 ? 4 : 8;
-    p.tiles = (int)((rows + 32 * p.waves - 1) / (32 * p.waves));
-    const int64_t blocks = p.tiles * groups;
-    int64_t want = (512 + blocks - 1) / blocks, most = (max_kv + 511) / 512;
-    if (want > most) want = most;
-    if (blocks >= 256 || want < 1) want = 1;
-    p.split_keys = (int)(((max_kv + want - 1) / want + 127) / 128 * 128);
-    p.splits = (int)((max_kv + p.split_keys - 1) / p.split_keys);
+    const int64_t tt = 32 * p.waves / (heads / kv_heads);
+    p.tiles = (int)((max_q + tt - 1) / tt);
+    p.shares = p.waves == 4 ? 2 * kCus : kCus;  // as many workgroups as fit at once
+    p.part_floats = 2 * p.shares * (32 * p.waves) * (d + 1);
   }
   if (p.splits > 1) p.part_floats = p.splits * tokens * heads * (d + 1);
-  p.bytes = (p.part_floats + (p.keep_scores ? tokens * heads * p.score_stride : 0)) * 4;
+  int64_t gathered = 0;
+  p.score_stride = (capacity + 3) / 4 * 4;
+  if (p.keep_scores) {
+    gathered = tokens * heads * p.score_stride;
+  } else if (gather) {
+    p.key_tiles = (int)((max_kv + GT_KEYS - 1) / GT_KEYS);
+    // four workgroups a CU, of at least 4 row tiles each
+    int64_t want = (1024 + p.key_tiles * groups - 1) / (p.key_tiles * groups), most = rows / (4 * GT_ROWS);
+    if (want > most) want = most;
+    if (want < 1 || want * groups * p.score_stride * 4 > kScoreBytes) want = 1;
+    p.row_splits = (int)want;
+    if (want > 1) gathered = want * groups * p.score_stride;
+  }
+  p.bytes = (p.part_floats + gathered) * 4;
   return p;
 }
 
@@ -801,21 +1066,28 @@ void launch_matrix(const Plan& p, AttnArgs a, int64_t max_kv, bool gather, hipSt
     if (p.row_blocks == 1) hipLaunchKernelGGL((paged_attn_few_kernel<T, D, 1, NW>), grid, dim3(64 * NW), 0, st, a);
     else hipLaunchKernelGGL((paged_attn_few_kernel<T, D, 2, NW>), grid, dim3(64 * NW), 0, st, a);
   } else {
-    const dim3 grid(groups * (unsigned)(p.splits * p.tiles));
-    if (p.waves == 4) hipLaunchKernelGGL((paged_attn_tile_kernel<T, D, 64, 4>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((paged_attn_tile_kernel<T, D, 128, 8>), grid, dim3(512), 0, st, a);
+    const dim3 grid((unsigned)p.shares), jgrid(groups * (unsigned)(p.tiles * (32 * p.waves / JT_ROWS)));
+    if (p.waves == 4) {
+      hipLaunchKernelGGL((paged_attn_tile_kernel<T, D, 64, 4>), grid, dim3(256), 0, st, a);
+      hipLaunchKernelGGL((paged_attn_join_parts_kernel<T, D, 128, 64>), jgrid, dim3(256), 0, st, a);
+    } else {
+      hipLaunchKernelGGL((paged_attn_tile_kernel<T, D, 64, 8>), grid, dim3(512), 0, st, a);
+      hipLaunchKernelGGL((paged_attn_join_parts_kernel<T, D, 256, 64>), jgrid, dim3(256), 0, st, a);
+    }
   }
   if (p.splits > 1)
-    hipLaunchKernelGGL((paged_attn_join_kernel<T, D>), dim3((unsigned)(((int64_t)a.tokens * a.heads + 3) / 4)), dim3(256),
-                       0, st, a);
+    hipLaunchKernelGGL((paged_attn_join_kernel<T, D>), dim3((unsigned)(((int64_t)a.tokens * a.heads * D + 1023) / 1024)),
+                       dim3(256), 0, st, a);
   if (!gather) return;
   if (p.keep_scores) {
     const unsigned blocks = (unsigned)((max_kv + 1023) / 1024);
     hipLaunchKernelGGL(paged_gather_scores_kernel, dim3(blocks ? blocks : 1, groups), dim3(256), 0, st, a);
   } else {
-    a.tiles = (int)((max_kv + 32 * GT_WAVES - 1) / (32 * GT_WAVES));
-    if (a.tiles < 1) a.tiles = 1;
-    hipLaunchKernelGGL((paged_gather_tile_kernel<T, D>), dim3(groups * (unsigned)a.tiles), dim3(64 * GT_WAVES), 0, st, a);
+    a.tiles = p.key_tiles, a.splits = p.row_splits;
+    hipLaunchKernelGGL((paged_gather_tile_kernel<T, D>), dim3(groups * (unsigned)(a.tiles * a.splits)),
+                       dim3(64 * GT_WAVES), 0, st, a);
+    if (a.splits > 1)
+      hipLaunchKernelGGL(paged_gather_join_kernel, dim3((unsigned)((max_kv + 255) / 256), groups), dim3(256), 0, st, a);
   }
 }
 
@@ -857,18 +1129,18 @@ extern "C" int gwa_paged_attention(const gwa_paged_cache* cache, const void* q, 
   const float c_log2 = scale * kLog2e;
   const Plan p = plan_of(c.batch, tokens, heads, c.kv_heads, d, max_q, max_kv, c.capacity, gather != 0);
   if (p.matrix && c.batch > 0) {
-    GWA_REQUIRE(groups * p.splits * p.tiles < (1ll << 31) && rows * p.splits < (1ll << 31),
+    GWA_REQUIRE(groups * p.splits * p.tiles < (1ll << 27) && rows * p.splits < (1ll << 31),
                 "%s: %lld rows in %d splits are too many", what, (long long)rows, p.splits);
     GWA_REQUIRE(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes && GWA_ALIGNED(workspace, 16)),
                 "%s: a workspace of %lld bytes, %lld are needed (16-byte aligned)", what, (long long)workspace_bytes,
                 (long long)p.bytes);
     float* ws = (float*)workspace;
-    const int64_t n_o = p.splits > 1 ? p.splits * rows * d : 0;
-    // scores first: their rows are read and written 16 bytes at a time
-    const int64_t n_s = p.keep_scores ? rows * p.score_stride : 0;
+    const int64_t n_o = p.part_floats / (d + 1) * d;
+    // scores or gathered parts first: scores' rows are read and written 16 bytes at a time
+    const int64_t n_s = p.bytes / 4 - p.part_floats;
     const AttnArgs a = {c, (const uint16_t*)q, ldqt, ldqh, (uint16_t*)o, lse, ws + n_s, ws + n_s + n_o,
-                        p.keep_scores ? ws : nullptr, p.score_stride, (int)tokens, (int)heads, p.splits, p.split_keys,
-                        p.tiles, c_log2, causal};
+                        p.keep_scores ? ws : nullptr, ws, p.score_stride, (int)tokens, (int)heads, p.splits, p.split_keys,
+                        p.tiles, p.shares, c_log2, causal};
     if (cache->dtype == GWA_DT_BF16) {
       if (d == 128) launch_matrix<Bf16, 128>(p, a, max_kv, gather != 0, st);
       else launch_matrix<Bf16, 64>(p, a, max_kv, gather != 0, st);

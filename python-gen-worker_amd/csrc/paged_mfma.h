@@ -42,8 +42,18 @@ struct Mfma<Fp16> {
   static constexpr uint32_t kExp = 0x7c00u;
 };
 
-// Direct-to-LDS copy of 16 bytes a lane from a 64-bit address: LDS [lds_addr + 16 lane, +16) <- [p, +16). As asm for
-// dma16's reason: the waits are the kernel's, so the compiler's wait counts must not include it.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+  return (int64_t)((uint64_t)(uint32_t)uniform((int)(uint32_t)(uint64_t)x) | (uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32);
+}
+
+// Direct-to-LDS copy of 16 bytes a lane: LDS [lds_addr + 16 lane, +16) <- [base + off, +16), base the same for the wave
+// (a 64-bit address: pools pass 4 GiB). As asm for dma16's reason: the waits are the kernel's, so the compiler's wait
+// counts must not include it.
+__device__ __forceinline__ void copy16(uint32_t lds_addr, const void* base, uint32_t off) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds_addr), "v"(off), "s"(base) : "memory", "m0");
+}
+// the same from an address of the lane's own
 __device__ __forceinline__ void copy16(uint32_t lds_addr, const void* p) {
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds_addr), "v"(p) : "memory", "m0");
 }
@@ -85,9 +95,10 @@ __device__ __forceinline__ bool take_nonfinite(v4i& x) {
 // Sequence b's part of a call for one kv head: its rows (new token i, query head of the group) flattened as i * group + g
 struct Rows {
   int t0, n, len, group, total;
-  __device__ __forceinline__ int limit(int row, bool causal) const {  // last key the row sees, -1 for none
-    return causal ? max(len - n + row / group, -1) : len - 1;
+  __device__ __forceinline__ int token_limit(int i, bool causal) const {  // last key new token i sees, -1 for none
+    return causal ? max(len - n + i, -1) : len - 1;
   }
+  __device__ __forceinline__ int limit(int row, bool causal) const { return token_limit(row / group, causal); }
 };
 __device__ __forceinline__ Rows rows_of(const PagedArgs& c, int b, int tokens, int group) {
   Rows r;
@@ -97,5 +108,113 @@ __device__ __forceinline__ Rows rows_of(const PagedArgs& c, int b, int tokens, i
   r.total = r.n * group;
   return r;
 }
+
+// the same, for a sequence the whole wave works on: in scalar registers, which the copies' LDS addresses need
+__device__ __forceinline__ Rows uniform_rows_of(const PagedArgs& c, int b, int tokens, int group) {
+  const Rows r = rows_of(c, b, tokens, group);
+  return Rows{uniform(r.t0), uniform(r.n), uniform(r.len), group, uniform(r.total)};
+}
+
+// The division of many-row work. A row tile is the rows of TT consecutive new tokens of one sequence and kv head; tiles
+// are laid end to end (heads, then sequences, then tokens), each as long as the keys its last token sees plus a constant,
+// and the line is cut into `shares` runs of equal length, one a workgroup. A cut inside a tile lies at the last whole
+// BN keys before it. Lengths of tiles are linear in their index, so positions have closed forms; the last tile of a
+// sequence counts as if it were whole.
+struct TileLine {
+  int first_keys, slope, none, tiles;  // keys of tile 0 (may be negative), keys more a tile, tiles without keys
+  static constexpr int kFixed = 64;    // a tile's constant part, in keys: its queries, its first copies, its output
+  // length of the first t tiles
+  __device__ __forceinline__ int64_t before(int t) const {
+    int64_t x = (int64_t)kFixed * t;
+    if (t > none) x += (int64_t)(t - none) * first_keys + (int64_t)slope * ((int64_t)t * (t - 1) - (int64_t)none * (none - 1)) / 2;
+    return x;
+  }
+  // the tile that position x < before(tiles) falls into
+  __device__ __forceinline__ int tile_at(int64_t x) const {
+    int lo = 0, hi = tiles - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (before(mid) <= x) lo = mid;
+      else hi = mid - 1;
+    }
+    return lo;
+  }
+};
+__device__ __forceinline__ TileLine tile_line(const Rows& r, int tt, bool causal) {
+  TileLine l;
+  l.tiles = (r.n + tt - 1) / tt;
+  l.slope = causal ? tt : 0;
+  l.first_keys = causal ? r.len - r.n + tt : r.len;
+  // tile t has keys where first_keys + slope t > 0
+  l.none = l.first_keys > 0 ? 0 : causal ? min(l.tiles, -l.first_keys / tt + 1) : l.tiles;
+  return l;
+}
+// one head's length in all, and that of the sequences before b; the whole wave calls it
+__device__ __forceinline__ int64_t head_line(const PagedArgs& c, int tokens, int tt, bool causal, int b, int64_t& before) {
+  int64_t all = 0;
+  before = 0;
+  for (int i = 0; i < c.batch; i += 64) {
+    const int mine = i + (threadIdx.x & 63);
+    int64_t u = 0;
+    if (mine < c.batch) {
+      const TileLine l = tile_line(rows_of(c, mine, tokens, 1), tt, causal);
+      u = l.before(l.tiles);
+    }
+    int64_t e = mine < b ? u : 0;
+#pragma unroll
+    for (int w = 32; w; w >>= 1) u += __shfl_xor(u, w), e += __shfl_xor(e, w);
+    all += u;
+    before += e;
+  }
+  all = uniform64(all);
+  before = uniform64(before);
+  return all;
+}
+// A place on the line: a head's sequence, a tile of it, and how many whole BN keys of the tile lie before it (which may be
+// more than the tile has)
+struct Place {
+  int h, b, tile, unit;
+};
+template <int BN>
+__device__ __forceinline__ Place place_of(const PagedArgs& c, int tokens, int tt, bool causal, int64_t per_head, int64_t x) {
+  Place p;
+  p.h = uniform((int)(x / per_head));
+  p.b = c.batch, p.tile = p.unit = 0;
+  x -= p.h * per_head;
+  if (p.h >= c.kv_heads) return p;  // the line's end
+  for (int i = 0; i < c.batch; i += 64) {
+    const int lane = threadIdx.x & 63, mine = i + lane;
+    int64_t u = 0;
+    TileLine l = {};
+    if (mine < c.batch) {
+      l = tile_line(rows_of(c, mine, tokens, 1), tt, causal);
+      u = l.before(l.tiles);
+    }
+    int64_t upto = u;
+#pragma unroll
+    for (int w = 1; w < 64; w <<= 1) {
+      const int64_t y = __shfl_up(upto, w);
+      if (lane >= w) upto += y;
+    }
+    const uint64_t past = __ballot(upto > x);
+    if (past) {
+      const int at = uniform(__ffsll((unsigned long long)past) - 1);
+      x = uniform64(x - __shfl(upto - u, at));
+      l.first_keys = uniform(__shfl(l.first_keys, at));
+      l.slope = uniform(__shfl(l.slope, at));
+      l.none = uniform(__shfl(l.none, at));
+      l.tiles = uniform(__shfl(l.tiles, at));
+      p.b = i + at;
+      p.tile = l.tile_at(x);
+      p.unit = (int)((x - l.before(p.tile)) / BN);
+      break;
+    }
+    x = uniform64(x - __shfl(upto, 63));
+  }
+  p.b = uniform(p.b), p.tile = uniform(p.tile), p.unit = uniform(p.unit);
+  return p;
+}
+// start of share i of n, a power of two
+__device__ __forceinline__ int64_t share_start(int64_t all, int i, int n) { return all * i >> (__ffs(n) - 1); }
 
 }  // namespace
