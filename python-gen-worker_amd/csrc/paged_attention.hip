@@ -884,29 +884,37 @@ __global__ __launch_bounds__(256) void paged_gather_scores_kernel(AttnArgs a) {
   }
 }
 
-// Recomputed: a wave holds 32 keys as the MFMA's A operand and walks the rows in tiles of 64, which a workgroup of 4
-// waves (128 keys) copies to LDS, double buffered (q^T as B). A lane sums its row's probabilities for 16 keys; the
-// lanes of the 32 rows are joined at the end. The rows are divided over `splits` workgroups where the keys alone are
-// too few to fill the chip: each leaves its sums in w_part [split][group][score_stride], joined in order.
+// Recomputed: a wave holds 32 keys as the MFMA's A operand and walks the rows in tiles of 64 (64 / group new tokens with
+// all heads of the group), which a workgroup of 4 waves (128 keys) copies to LDS, double buffered (q^T as B). A lane sums
+// its row's probabilities for 16 keys; the lanes of the 32 rows are joined at the end. The tokens are divided over
+// `splits` workgroups where the keys alone are too few to fill the chip: each leaves its sums in w_part
+// [split][group][score_stride], joined in order.
 constexpr int GT_WAVES = 4, GT_ROWS = 64, GT_KEYS = 32 * GT_WAVES;
 
 template <class T, int D>
-__global__ __launch_bounds__(64 * GT_WAVES) void paged_gather_tile_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * GT_WAVES, 3) void paged_gather_tile_kernel(AttnArgs a) {
   constexpr int NQ = D / 16, kRow = 2 * D, kRun = 1024 / kRow, kRuns = GT_ROWS / kRun / GT_WAVES, kStage = GT_ROWS * kRow;
+  constexpr int kAhead = 4;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
   const PagedArgs& c = a.c;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, j = lane & 31, hf = lane >> 5;
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, j = lane & 31, hf = lane >> 5;
   const int groups = c.batch * c.kv_heads;
   const int grp = blockIdx.x % groups, rest = blockIdx.x / groups, split = rest % a.splits;
-  const int b = grp / c.kv_heads, h = grp % c.kv_heads, g = a.heads / c.kv_heads;
-  const Rows R = rows_of(c, b, a.tokens, g);
+  const int b = grp / c.kv_heads, h = grp % c.kv_heads, g = a.heads / c.kv_heads, tt = GT_ROWS / g;
+  const Rows R = uniform_rows_of(c, b, a.tokens, g);
   const bool causal = a.causal != 0;
   const int32_t* pages = c.table + (int64_t)b * c.table_stride;
   constexpr int CH = D / 8;
   const int crow = lane / CH, cpl = lane % CH;
-  uint32_t qro[NQ];
+  const uint32_t qro = (uint32_t)(j * kRow + 16 * k_place<D>(hf, j));  // chunk 2 cd + hf: xor 32 cd
+  const uint16_t* q0 = a.q + R.t0 * a.ldqt + h * g * a.ldqh;
+  const float* lse0 = a.lse + (int64_t)R.t0 * a.heads + h * g;
+  int64_t qoff[kRuns];  // the lane's part of a whole tile's copies
 #pragma unroll
-  for (int cd = 0; cd < NQ; ++cd) qro[cd] = (uint32_t)(j * kRow + 16 * k_place<D>(2 * cd + hf, j));
+  for (int u = 0; u < kRuns; ++u) {
+    const int place = (wave + GT_WAVES * u) * kRun + crow, r = min(place, tt * g - 1);
+    qoff[u] = r / g * a.ldqt + r % g * a.ldqh + 8 * k_place<D>(cpl, place);
+  }
 
   for (int w0 = rest / a.splits * GT_KEYS; w0 < R.len; w0 += a.tiles * GT_KEYS) {
     const int j0 = w0 + 32 * wave, key = min(j0 + j, R.len - 1);
@@ -914,28 +922,33 @@ __global__ __launch_bounds__(64 * GT_WAVES) void paged_gather_tile_kernel(AttnAr
     v4i kop[NQ];
 #pragma unroll
     for (int cd = 0; cd < NQ; ++cd) kop[cd] = *(const v4i*)(c.k + kat + 8 * hf + 16 * cd);
-    // rows that see a key of this workgroup's come last; this split's share of their tiles
-    const int first = causal ? max(w0 - (R.len - R.n), 0) * g : 0;
-    const int all = first < R.total ? (R.total - first + GT_ROWS - 1) / GT_ROWS : 0;
+    // tokens that see a key of this workgroup's come last; this split's share of their tiles
+    const int first = causal ? max(w0 - (R.len - R.n), 0) : 0;
+    const int all = first < R.n ? (R.n - first + tt - 1) / tt : 0;
     const int t_lo = (int)((int64_t)all * split / a.splits), t_hi = (int)((int64_t)all * (split + 1) / a.splits);
-    float sum[16] = {}, lse2[2], next2[2];
-    auto lse_of = [&](int t, float (&out)[2]) __attribute__((always_inline)) {
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int rc = min(first + t * GT_ROWS + 32 * x + j, R.total - 1);
-        out[x] = a.lse[(int64_t)(R.t0 + rc / g) * a.heads + h * g + rc % g] * kLog2e;
-      }
-    };
+    // row r of a tile: its token i + r / g (the last of the sequence where that is past it), head r % g; rows past the
+    // tile's tokens repeat its last
     auto issue = [&](int t) __attribute__((always_inline)) {
       const uint32_t st = (uint32_t)(uintptr_t)(lds + (t & 1) * kStage);
+      const int i = first + t * tt, most = R.n - 1 - i;
 #pragma unroll
       for (int u = 0; u < kRuns; ++u) {
-        const int run = wave + GT_WAVES * u, r = run * kRun + crow, rc = min(first + t * GT_ROWS + r, R.total - 1);
-        copy16(st + run * 1024, a.q + (R.t0 + rc / g) * a.ldqt + (h * g + rc % g) * a.ldqh + 8 * k_place<D>(cpl, r));
+        const int run = wave + GT_WAVES * u, r = min(run * kRun + crow, tt * g - 1);
+        const int64_t off = most >= tt - 1 ? qoff[u] : min(r / g, most) * a.ldqt + r % g * a.ldqh + 8 * k_place<D>(cpl, run * kRun + crow);
+        copy16(st + run * 1024, q0 + i * a.ldqt + off);
+      }
+    };
+    float sum[16] = {}, lse2[2], next2[2];
+    auto lse_of = [&](int t) __attribute__((always_inline)) {
+      const int i = first + t * tt, most = R.n - 1 - i;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int r = 32 * x + j;  // rows past the tile's tokens: a probability of 0
+        next2[x] = r < tt * g ? lse0[(int64_t)(i + min(r / g, most)) * a.heads + r % g] * kLog2e : INFINITY;
       }
     };
     if (t_lo < t_hi) {
-      lse_of(t_lo, next2);
+      lse_of(t_lo);
       issue(t_lo);
     }
     for (int t = t_lo; t < t_hi; ++t) {
@@ -943,18 +956,27 @@ __global__ __launch_bounds__(64 * GT_WAVES) void paged_gather_tile_kernel(AttnAr
       __syncthreads();  // tile t is there; everyone is done with the other stage
       lse2[0] = next2[0], lse2[1] = next2[1];
       if (t + 1 < t_hi) {
-        lse_of(t + 1, next2);
+        lse_of(t + 1);
         issue(t + 1);
       }
       const uint8_t* st = lds + (t & 1) * kStage;
-      const int row0 = first + t * GT_ROWS;
-      v16f s[2] = {};
+      const int i0 = first + t * tt;
+      v16f s[2];
+      v4i ring[kAhead];  // operands read ahead of their MFMAs, in this order
+      auto read = [&](int k) __attribute__((always_inline)) {
+        ring[k % kAhead] = *(const v4i*)(st + 32 * (k % 2) * kRow + (qro ^ (uint32_t)(32 * (k / 2))));
+      };
 #pragma unroll
-      for (int cd = 0; cd < NQ; ++cd)
+      for (int k = 0; k < kAhead; ++k) read(k);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int x = 0; x < 2; ++x) s[x] = Mfma<T>::wide(kop[cd], *(const v4i*)(st + 32 * x * kRow + qro[cd]), s[x]);
-      // whole tiles every row of which sees all of the wave's keys need no mask
-      if (row0 + GT_ROWS <= R.total && R.limit(row0, causal) >= j0 + 31) {
+      for (int k = 0; k < 2 * NQ; ++k) {
+        s[k % 2] = Mfma<T>::wide(kop[k / 2], ring[k % kAhead], k < 2 ? (v16f){} : s[k % 2]);
+        if (k + kAhead < 2 * NQ) read(k + kAhead);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      // tiles all of whose tokens see all of the wave's keys need no mask
+      if (i0 + tt <= R.n && R.token_limit(i0, causal) >= j0 + 31) {
 #pragma unroll
         for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -962,11 +984,12 @@ __global__ __launch_bounds__(64 * GT_WAVES) void paged_gather_tile_kernel(AttnAr
       } else {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const int r = row0 + 32 * x + j, vis = r < R.total ? R.limit(r, causal) - j0 - 4 * hf : -1;
+          const int r = 32 * x + j, i = i0 + r / g;
+          const int vis = r < tt * g && i < R.n ? R.token_limit(i, causal) - j0 - 4 * hf : -64;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][i], a.c_log2, -lse2[x]));
-            sum[i] += 8 * (i >> 2) + (i & 3) <= vis ? p : 0.0f;
+          for (int e = 0; e < 16; ++e) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e], a.c_log2, -lse2[x]));
+            sum[e] += 8 * (e >> 2) + (e & 3) <= vis ? p : 0.0f;
           }
         }
       }
@@ -1045,9 +1068,9 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int
   if (p.keep_scores) {
     gathered = tokens * heads * p.score_stride;
   } else if (gather) {
-    p.key_tiles = (int)((max_kv + GT_KEYS - 1) / GT_KEYS);
-    // four workgroups a CU, of at least 4 row tiles each
-    int64_t want = (1024 + p.key_tiles * groups - 1) / (p.key_tiles * groups), most = rows / (4 * GT_ROWS);
+    p.key_tiles = (int)(max_kv > 0 ? (max_kv + GT_KEYS - 1) / GT_KEYS : 1);
+    // six workgroups a CU, of at least 4 row tiles each
+    int64_t want = (1536 + p.key_tiles * groups - 1) / (p.key_tiles * groups), most = rows / (4 * GT_ROWS);
     if (want > most) want = most;
     if (want < 1 || want * groups * p.score_stride * 4 > kScoreBytes) want = 1;
     p.row_splits = (int)want;
@@ -1084,6 +1107,11 @@ void launch_matrix(const Plan& p, AttnArgs a, int64_t max_kv, bool gather, hipSt
     hipLaunchKernelGGL(paged_gather_scores_kernel, dim3(blocks ? blocks : 1, groups), dim3(256), 0, st, a);
   } else {
     a.tiles = p.key_tiles, a.splits = p.row_splits;
+    if (a.heads / a.c.kv_heads > GT_ROWS) {
+      hipLaunchKernelGGL((paged_gather_rows_kernel<T>), dim3((unsigned)((max_kv + 63) / 64 > 0 ? (max_kv + 63) / 64 : 1), groups),
+                         dim3(64), 0, st, a.c, a.q, a.ldqt, a.ldqh, a.lse, a.tokens, a.heads, D, a.c_log2, a.causal);
+      return;
+    }
     hipLaunchKernelGGL((paged_gather_tile_kernel<T, D>), dim3(groups * (unsigned)(a.tiles * a.splits)),
                        dim3(64 * GT_WAVES), 0, st, a);
     if (a.splits > 1)
