@@ -292,9 +292,14 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t mine, uint32_t* cells, ui
 // found digit by digit (11 + 11 + 10 bits, a histogram each: 11 bits hold the sign, the exponent and two bits of the
 // mantissa, so weights of one magnitude still spread over several counters); keys above it and, from the lowest
 // slot on, as many equal to it as are still wanted are kept. Each wave owns a run of slots, so that after one sum
-// over the waves every wave knows where its kept slots go: `kept` ascends and no order depends on timing.
-__global__ __launch_bounds__(EV_THREADS) void evict_select_kernel(PagedArgs c, int budget, int recent, int32_t* kept,
-                                                                  int32_t* new_len) {
+// over the waves every wave knows where its kept slots go: `kept` ascends and no order depends on timing. Bound by
+// latency: the first EV_HELD ranks are read once, 8 loads of a thread in flight, and held in LDS for all passes (32768 keys
+// read again in every pass took 76 us; held in registers, whose passes are unrolled code, 38 us and 13 for 640 keys).
+constexpr int EV_HELD = 32768, EV_GROUP = 8;
+
+__global__ __launch_bounds__(EV_THREADS) void evict_select_kernel(PagedArgs c, int budget, int recent, int held,
+                                                                  int32_t* kept, int32_t* new_len) {
+  extern __shared__ uint32_t ranks[];  // held
   __shared__ uint32_t bins[EV_BINS];
   __shared__ uint32_t cells[EV_WAVES];
   __shared__ uint32_t found[2];
@@ -309,7 +314,38 @@ __global__ __launch_bounds__(EV_THREADS) void evict_select_kernel(PagedArgs c, i
   }
   const int32_t* row = c.table + b * c.table_stride;
   const int first = n - recent;  // keys before the recent ones: more than budget - recent of them
-  auto rank_of = [&](int j) { return weight_rank(c.w[paged_w_at(c, paged_page(c, row, j), h, j)]); };
+  const int run = ((n + EV_WAVES - 1) / EV_WAVES + 63) & ~63;
+  const int j0 = min(wave * run, n), j1 = min(j0 + run, n);
+  // rank of slot j < n, out of LDS for the first `held` slots; those of recent keys are never looked at
+  auto rank_of = [&](int j) __attribute__((always_inline)) {
+    return weight_rank(c.w[paged_w_at(c, paged_page(c, row, j), h, j)]);
+  };
+  const int in_lds = min(n, held);
+  for (int j = tid; j < in_lds; j += EV_GROUP * EV_THREADS) {  // a step's loads all in flight together
+    int page[EV_GROUP];
+    float w[EV_GROUP];
+#pragma unroll
+    for (int k = 0; k < EV_GROUP; ++k) page[k] = paged_page(c, row, min(j + k * EV_THREADS, in_lds - 1));
+#pragma unroll
+    for (int k = 0; k < EV_GROUP; ++k) {
+      const int at = min(j + k * EV_THREADS, in_lds - 1);
+      w[k] = c.w[paged_w_at(c, page[k], h, at)];
+    }
+#pragma unroll
+    for (int k = 0; k < EV_GROUP; ++k)
+      if (j + k * EV_THREADS < in_lds) ranks[j + k * EV_THREADS] = weight_rank(w[k]);
+  }
+  // f(slot of the wave's first lane, the lane's rank) over the wave's run, 64 slots at a time
+  auto each = [&](auto f) __attribute__((always_inline)) {
+    const int mid = min(j1, in_lds / 64 * 64);
+    int j = j0;
+#pragma unroll 4
+    for (; j < mid; j += 64) f(j, ranks[j + lane]);
+    for (; j < j1; j += 64) {
+      const int at = min(j + lane, n - 1);
+      f(j, at < in_lds ? ranks[at] : rank_of(at));
+    }
+  };
 
   uint32_t want = (uint32_t)(budget - recent), prefix = 0;
   int shift = 21;
@@ -318,10 +354,10 @@ __global__ __launch_bounds__(EV_THREADS) void evict_select_kernel(PagedArgs c, i
       const int bits = pass == 2 ? 10 : 11;
       for (int i = tid; i < EV_BINS; i += EV_THREADS) bins[i] = 0;
       __syncthreads();
-      for (int j = tid; j < first; j += EV_THREADS) {
-        const uint32_t u = rank_of(j);
-        if (pass == 0 || (u >> (shift + bits)) == prefix) atomicAdd(&bins[(u >> shift) & ((1u << bits) - 1)], 1u);
-      }
+      each([&](int j, uint32_t u) __attribute__((always_inline)) {
+        if (j + lane < min(first, j1) && (pass == 0 || (u >> (shift + bits)) == prefix))
+          atomicAdd(&bins[(u >> shift) & ((1u << bits) - 1)], 1u);
+      });
       __syncthreads();
       // counters from the top, two a thread: the one at which the count reaches `want`
       const int i1 = EV_BINS - 1 - 2 * tid, i0 = i1 - 1;
@@ -346,33 +382,26 @@ __global__ __launch_bounds__(EV_THREADS) void evict_select_kernel(PagedArgs c, i
     prefix = 0xffffffffu;  // nothing but the recent keys
   }
   // now: keys ranked above `prefix` are kept, and the first `want` equal to it
-  const int run = ((n + EV_WAVES - 1) / EV_WAVES + 63) & ~63;
-  const int j0 = min(wave * run, n), j1 = min(j0 + run, n);
   const bool any = budget > recent;
   uint32_t above = 0, equal = 0;
-  for (int j = j0; j < j1; j += 64) {
-    const bool in = j + lane < j1, old = in && j + lane < first;
-    const uint32_t u = old ? rank_of(j + lane) : 0;
+  each([&](int j, uint32_t u) __attribute__((always_inline)) {
+    const bool in = j + lane < j1, old = j + lane < first;
     above += __popcll(__ballot(in && (!old || (any && u > prefix))));
-    equal += __popcll(__ballot(old && any && u == prefix));
-  }
+    equal += __popcll(__ballot(old && in && any && u == prefix));
+  });
   uint32_t all;
-  uint32_t eq = wave_scan(equal, cells, all);
-  // of the equal ones before this wave's run, at most `want` are kept
-  const uint32_t eq_before = eq;
-  const uint32_t above_before = wave_scan(above, cells, all);
-  uint32_t at = above_before + min(eq_before, want);
-  for (int j = j0; j < j1; j += 64) {
-    const bool in = j + lane < j1, old = in && j + lane < first;
-    const uint32_t u = old ? rank_of(j + lane) : 0;
-    const bool is_eq = old && any && u == prefix;
+  uint32_t eq = wave_scan(equal, cells, all);  // equal ones before this wave's run, of which at most `want` are kept
+  uint32_t at = wave_scan(above, cells, all) + min(eq, want);
+  each([&](int j, uint32_t u) __attribute__((always_inline)) {
+    const bool in = j + lane < j1, old = j + lane < first;
+    const bool is_eq = old && in && any && u == prefix;
     const uint64_t eqs = __ballot(is_eq), below = (1ull << lane) - 1;
     const bool keep = (in && (!old || (any && u > prefix))) || (is_eq && eq + __popcll(eqs & below) < want);
     const uint64_t keeps = __ballot(keep);
     if (keep) out[at + __popcll(keeps & below)] = j + lane;
     at += __popcll(keeps);
     eq += __popcll(eqs);
-  }
+  });
 }
 
 constexpr int EC_THREADS = 256;
@@ -418,8 +447,9 @@ extern "C" int gwa_paged_evict(const gwa_paged_cache* cache, const int32_t* new_
   const int64_t blocks = (most * pieces + EC_THREADS - 1) / EC_THREADS;
   GWA_REQUIRE(groups < 65536 && blocks < (1ll << 31), "%s: %lld heads of sequences are too many", what,
               (long long)groups);
-  hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)groups), dim3(EV_THREADS), 0, (hipStream_t)stream, c,
-                     (int)budget, (int)recent, kept, new_len);
+  const int held = (int)(max_kv < EV_HELD ? max_kv : EV_HELD);
+  hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)groups), dim3(EV_THREADS), (size_t)held * 4,
+                     (hipStream_t)stream, c, (int)budget, (int)recent, held, kept, new_len);
   const int rc = gwa_check_launch(what);
   if (rc != GWA_OK || blocks == 0) return rc;
   hipLaunchKernelGGL(evict_copy_kernel, dim3((unsigned)blocks, (unsigned)groups), dim3(EC_THREADS), 0,
