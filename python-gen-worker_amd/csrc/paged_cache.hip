@@ -1,5 +1,7 @@
 // Rotary positions, the write of new tokens into a paged key/value cache, and the eviction of its least attended
 // keys. All three move each value once and compute next to nothing: they are bound by memory.
+#include <type_traits>
+
 #include "paged_common.h"
 
 namespace {
@@ -295,7 +297,7 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t mine, uint32_t* cells, ui
 // over the waves every wave knows where its kept slots go: `kept` ascends and no order depends on timing. Bound by
 // latency: the first EV_HELD ranks are read once, 8 loads of a thread in flight, and held in LDS for all passes (32768 keys
 // read again in every pass took 76 us; held in registers, whose passes are unrolled code, 38 us and 13 for 640 keys).
-constexpr int EV_HELD = 32768, EV_GROUP = 8;
+constexpr int EV_HELD = 32768;
 
 __global__ __launch_bounds__(EV_THREADS) void evict_select_kernel(PagedArgs c, int budget, int recent, int held,
                                                                   int32_t* kept, int32_t* new_len) {
@@ -321,20 +323,22 @@ __global__ __launch_bounds__(EV_THREADS) void evict_select_kernel(PagedArgs c, i
     return weight_rank(c.w[paged_w_at(c, paged_page(c, row, j), h, j)]);
   };
   const int in_lds = min(n, held);
-  for (int j = tid; j < in_lds; j += EV_GROUP * EV_THREADS) {  // a step's loads all in flight together
-    int page[EV_GROUP];
-    float w[EV_GROUP];
+  auto fill = [&](auto group_c) __attribute__((always_inline)) {  // a step's loads all in flight together
+    constexpr int G = decltype(group_c)::value;
+    for (int j = tid; j < in_lds; j += G * EV_THREADS) {
+      int page[G];
+      float w[G];
 #pragma unroll
-    for (int k = 0; k < EV_GROUP; ++k) page[k] = paged_page(c, row, min(j + k * EV_THREADS, in_lds - 1));
+      for (int k = 0; k < G; ++k) page[k] = paged_page(c, row, min(j + k * EV_THREADS, in_lds - 1));
 #pragma unroll
-    for (int k = 0; k < EV_GROUP; ++k) {
-      const int at = min(j + k * EV_THREADS, in_lds - 1);
-      w[k] = c.w[paged_w_at(c, page[k], h, at)];
+      for (int k = 0; k < G; ++k) w[k] = c.w[paged_w_at(c, page[k], h, min(j + k * EV_THREADS, in_lds - 1))];
+#pragma unroll
+      for (int k = 0; k < G; ++k)
+        if (j + k * EV_THREADS < in_lds) ranks[j + k * EV_THREADS] = weight_rank(w[k]);
     }
-#pragma unroll
-    for (int k = 0; k < EV_GROUP; ++k)
-      if (j + k * EV_THREADS < in_lds) ranks[j + k * EV_THREADS] = weight_rank(w[k]);
-  }
+  };
+  if (in_lds > 4 * EV_THREADS) fill(std::integral_constant<int, 16>{});
+  else fill(std::integral_constant<int, 2>{});
   // f(slot of the wave's first lane, the lane's rank) over the wave's run, 64 slots at a time
   auto each = [&](auto f) __attribute__((always_inline)) {
     const int mid = min(j1, in_lds / 64 * 64);
@@ -379,28 +383,34 @@ __global__ __launch_bounds__(EV_THREADS) void evict_select_kernel(PagedArgs c, i
       __syncthreads();
     }
   } else {
-    prefix = 0xffffffffu;  // nothing but the recent keys
+    prefix = 0xffffffffu;  // nothing but the recent keys: no rank is above it, and no equal one is wanted
   }
-  // now: keys ranked above `prefix` are kept, and the first `want` equal to it
-  const bool any = budget > recent;
-  uint32_t above = 0, equal = 0;
+  // now: of the keys before the recent ones, those ranked above `prefix` are kept (none where nothing is wanted: the
+  // highest rank is), and the first `want` equal to it
+  const int o1 = min(j1, first);  // the run's end among them
+  uint32_t above = 0, equal = 0;  // by lane
   each([&](int j, uint32_t u) __attribute__((always_inline)) {
-    const bool in = j + lane < j1, old = j + lane < first;
-    above += __popcll(__ballot(in && (!old || (any && u > prefix))));
-    equal += __popcll(__ballot(old && in && any && u == prefix));
+    const bool old = j + lane < o1;
+    above += old && u > prefix;
+    equal += old && u == prefix;
   });
+#pragma unroll
+  for (int w = 32; w; w >>= 1) above += __shfl_xor(above, w), equal += __shfl_xor(equal, w);
   uint32_t all;
   uint32_t eq = wave_scan(equal, cells, all);  // equal ones before this wave's run, of which at most `want` are kept
-  uint32_t at = wave_scan(above, cells, all) + min(eq, want);
+  uint32_t at = wave_scan(above + (uint32_t)(j1 - max(o1, j0)), cells, all) + min(eq, want);
+  auto lanes_below = [](uint64_t m) { return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0)); };
   each([&](int j, uint32_t u) __attribute__((always_inline)) {
-    const bool in = j + lane < j1, old = j + lane < first;
-    const bool is_eq = old && in && any && u == prefix;
-    const uint64_t eqs = __ballot(is_eq), below = (1ull << lane) - 1;
-    const bool keep = (in && (!old || (any && u > prefix))) || (is_eq && eq + __popcll(eqs & below) < want);
+    const bool old = j + lane < o1, recent_key = j + lane >= first && j + lane < j1;
+    bool keep = (old && u > prefix) || recent_key;
+    const uint64_t eqs = __ballot(old && u == prefix);
+    if (eqs) {  // the same for the whole wave
+      keep |= (eqs >> lane & 1) && eq + lanes_below(eqs) < want;
+      eq += __popcll(eqs);
+    }
     const uint64_t keeps = __ballot(keep);
-    if (keep) out[at + __popcll(keeps & below)] = j + lane;
+    if (keep) out[at + lanes_below(keeps)] = j + lane;
     at += __popcll(keeps);
-    eq += __popcll(eqs);
   });
 }
 
@@ -413,7 +423,7 @@ __global__ __launch_bounds__(EC_THREADS) void evict_copy_kernel(PagedArgs c, con
   const int h = blockIdx.y % c.kv_heads, b = blockIdx.y / c.kv_heads;
   const int i = blockIdx.x * EC_THREADS + threadIdx.x, r = i / pieces, p = i - r * pieces;
   if (r >= min(min(paged_kv_len(c, b), budget), new_capacity)) return;
-  const int j = kept[(int64_t)blockIdx.y * budget + r];
+  const int j = min(max(kept[(int64_t)blockIdx.y * budget + r], 0), paged_kv_len(c, b) - 1);
   const int from = paged_page(c, c.table + b * c.table_stride, j);
   const int to = paged_page(c, new_table + b * new_stride, r);
   const int64_t src = paged_at(c, from, h, j) + 8 * p, dst = paged_at(c, to, h, r) + 8 * p;
