@@ -37,21 +37,6 @@ __device__ __forceinline__ float dot8(v4i x, v4i y, float s) {
   return s;
 }
 
-// A row's result: into o and lse, or into its split's partials. `d0`: the first of 4 channels in o4.
-template <class T, int D>
-__device__ __forceinline__ void put_o(const AttnArgs& a, int split, int64_t row, int d0, float x, float y, float z,
-                                      float w) {
-  if (a.splits > 1)
-    *(float4*)(a.o_part + ((int64_t)split * a.tokens * a.heads + row) * D + d0) = make_float4(x, y, z, w);
-  else
-    *(uint2*)(a.o + row * D + d0) = make_uint2((uint32_t)Mfma<T>::pack(x, y), (uint32_t)Mfma<T>::pack(z, w));
-}
-__device__ __forceinline__ void put_lse(const AttnArgs& a, int split, int64_t row, float m, float l) {
-  const float lse2 = m == -INFINITY ? -INFINITY : m + __builtin_amdgcn_logf(l);
-  if (a.splits > 1) a.lse_part[(int64_t)split * a.tokens * a.heads + row] = lse2;
-  else a.lse[row] = lse2 * kLn2;
-}
-
 // ---------------------------------------------------------------------------
 // any head_dim: one wave per (new token, query head)
 // ---------------------------------------------------------------------------
@@ -495,12 +480,13 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_attn_tile_kernel(AttnArgs a)
   }
 }
 
+constexpr int join_rows(int bm) { return bm < 32 ? bm : 32; }
+
 // Joins the parts of row tiles that the shares' ends cut, in the shares' order. A workgroup takes JT_ROWS rows of a tile
 // and finds from the same division which shares hold a part of it.
-constexpr int JT_ROWS = 32;
-
 template <class T, int D, int BM, int BN>
 __global__ __launch_bounds__(256) void paged_attn_join_parts_kernel(AttnArgs a) {
+  constexpr int JT_ROWS = join_rows(BM);
   const PagedArgs& c = a.c;
   const int g = a.heads / c.kv_heads, groups = c.batch * c.kv_heads, tt = BM / g;
   const bool causal = a.causal != 0;
@@ -567,13 +553,18 @@ __global__ __launch_bounds__(256) void paged_attn_join_parts_kernel(AttnArgs a) 
 // ---------------------------------------------------------------------------
 // head_dim 64 and 128, few rows: MFMA 16x16x32, 16 RB rows a workgroup, every wave its own keys
 // ---------------------------------------------------------------------------
-// Bound by reading K and V. A workgroup owns a split of one sequence's and kv head's keys; wave w takes its tiles w,
+// Bound by reading K and V. A workgroup owns a run of one sequence's and kv head's keys; wave w takes its tiles w,
 // w + NW, ... of 32 keys through two LDS stages of its own (no barriers in the loop; the next tile is in flight
-// while one is computed), and the waves' O, m and l are joined at the end. The split's page ids are read into LDS
+// while one is computed), and the waves' O, m and l are joined at the end. The run's page ids are read into LDS
 // first, so that no ordinary load's wait falls among the copies'.
+// Runs: with SHARES the line of all keys is cut into one equal share for each CU, as for many rows: a workgroup's start
+// costs a few microseconds, so one round of workgroups that all end together reads fastest (32 sequences of up to
+// 32768 keys: runs of 4096 keys, 866 workgroups, took 321 us, of 16384 keys, 328 workgroups, 303). Where the keys are so few
+// that runs of 256 are all there at once, a run is a split of that length, which a workgroup finds without the line.
 constexpr int FW_KEYS = 32, FW_PAGES = 512;  // keys a tile; page ids staged at a time (whole tiles: page_size >= 8)
+constexpr int FW_WAVES = 4, FW_UNIT = FW_KEYS * FW_WAVES;
 
-template <int D, int RB, int NW>
+template <int D, int RB>
 struct FewShape {
   static constexpr int kRow = 2 * D, kRun = 1024 / kRow;
   static constexpr int kRuns = FW_KEYS / kRun;  // copies a tile, per K and per V
@@ -583,32 +574,26 @@ struct FewShape {
   static constexpr int kWave = 2 * kStage > kOut ? 2 * kStage : kOut;
 };
 
-template <class T, int D, int RB, int NW>
-__global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(AttnArgs a) {
-  using S = FewShape<D, RB, NW>;
+template <class T, int D, int RB, bool SHARES>
+__global__ __launch_bounds__(64 * FW_WAVES) void paged_attn_few_kernel(AttnArgs a) {
+  using S = FewShape<D, RB>;
+  constexpr int NW = FW_WAVES, BM = 16 * RB;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[NW * S::kWave];
-  __shared__ float stat[NW][2][16 * RB];  // m and l by wave
+  __shared__ float stat[NW][2][BM];  // m and l by wave
   __shared__ int page_ids[FW_PAGES];
   const PagedArgs& c = a.c;
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63;
   const int i16 = lane & 15, q4 = lane >> 4;  // MFMA column (row of the call, key or channel) and quarter
-  const int groups = c.batch * c.kv_heads;
-  const int grp = blockIdx.x % groups, split = blockIdx.x / groups;
-  const int b = grp / c.kv_heads, h = grp % c.kv_heads, g = a.heads / c.kv_heads;
-  const Rows R = rows_of(c, b, a.tokens, g);
+  const int g = a.heads / c.kv_heads, tt = BM / g;  // new tokens a row tile holds
   const bool causal = a.causal != 0;
-  const int32_t* pages = c.table + (int64_t)b * c.table_stride;
-  const uint8_t* kbase = (const uint8_t*)(c.k + h * c.head_stride);
-  const uint8_t* vbase = (const uint8_t*)(c.v + h * c.head_stride);
-  const int64_t page_bytes = 2 * c.page_stride;
-  const int slot_bytes = (int)(2 * c.slot_stride), slot_mask = (1 << c.page_shift) - 1;
+  const uint32_t page_bytes = (uint32_t)(2 * c.page_stride), slot_bytes = (uint32_t)(2 * c.slot_stride);
+  const uint32_t slot_mask = (1u << c.page_shift) - 1;
   uint8_t* const mine = lds + wave * S::kWave;
 
-  // K operand: key 16 kb + i16, chunk 4 cd + q4. V^T operand (channels 16 db ..): lane p = i16 of quarter q4 points at key
-  // 4 q4 + p / 4 (and + 16), channels 16 db + 4 (p % 4) .. + 4
-  uint32_t kro[S::kNQ], vro[S::kND];
-#pragma unroll
-  for (int cd = 0; cd < S::kNQ; ++cd) kro[cd] = (uint32_t)(i16 * S::kRow + 16 * k_place<D>(4 * cd + q4, i16));
+  // K operand: key 16 x + i16, chunk q4 (chunk 4 cd + q4: the address xor 64 cd). V^T operand (channels 16 db ..): lane
+  // p = i16 of quarter q4 points at key 4 q4 + p / 4 (and + 16), channels 16 db + 4 (p % 4) .. + 4
+  const uint32_t kro = (uint32_t)(i16 * S::kRow + 16 * k_place<D>(q4, i16));
+  uint32_t vro[S::kND];
 #pragma unroll
   for (int db = 0; db < S::kND; ++db) {
     const int r = 4 * q4 + (i16 >> 2), col = 16 * db + 4 * (lane & 3);
@@ -616,23 +601,33 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(AttnArgs a) {
   }
   constexpr int CH = D / 8;
   const int crow = lane / CH, cpl = lane % CH;
+  uint32_t klane[S::kRuns], vlane[S::kRuns];  // the lane's part of each copy's addresses
+#pragma unroll
+  for (int u = 0; u < S::kRuns; ++u) {
+    klane[u] = crow * slot_bytes + 16 * k_place<D>(cpl, u * S::kRun + crow);
+    vlane[u] = crow * slot_bytes + 16 * v_place<D>(cpl, u * S::kRun + crow);
+  }
 
-  for (int row0 = 0; row0 < R.total; row0 += 16 * RB) {
+  // the rows of tokens [i0, i1) of sequence b and kv head h over keys [k_lo, k_hi); `slot`: where the partial result
+  // goes, -1 for a whole one
+  auto run = [&](const Rows& R, int b, int h, int i0, int i1, int k_lo, int k_hi, int slot) __attribute__((always_inline)) {
+    const int32_t* pages = c.table + (int64_t)b * c.table_stride;
+    const uint8_t* kbase = (const uint8_t*)(c.k + h * c.head_stride);
+    const uint8_t* vbase = (const uint8_t*)(c.v + h * c.head_stride);
+    const int nrows = (i1 - i0) * g;
     int lim[RB];
     int64_t out_row[RB];
     v4i qop[RB][S::kNQ];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      const int rc = min(row0 + 16 * rb + i16, R.total - 1), tok = R.t0 + rc / g;
-      lim[rb] = R.limit(rc, causal);
-      out_row[rb] = (int64_t)tok * a.heads + h * g + rc % g;
-      const uint16_t* qp = a.q + tok * a.ldqt + (h * g + rc % g) * a.ldqh + 8 * q4;
+      const int r = min(16 * rb + i16, nrows - 1), tok = R.t0 + i0 + r / g, head = h * g + r % g;
+      lim[rb] = R.token_limit(i0 + r / g, causal);
+      out_row[rb] = (int64_t)tok * a.heads + head;
+      const uint16_t* qp = a.q + tok * a.ldqt + head * a.ldqh + 8 * q4;
 #pragma unroll
       for (int cd = 0; cd < S::kNQ; ++cd) qop[rb][cd] = *(const v4i*)(qp + 32 * cd);
     }
-    const int lim_lo = R.limit(row0, causal), lim_hi = R.limit(min(row0 + 16 * RB, R.total) - 1, causal);
-    const int k_lo = split * a.split_keys;
-    const int k_hi = split + 1 < a.splits ? min(k_lo + a.split_keys, lim_hi + 1) : lim_hi + 1;
+    const int lim_lo = R.token_limit(i0, causal);
 
     v4f oacc[RB][S::kND];
     float m_run[RB], l_run[RB];
@@ -646,7 +641,7 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(AttnArgs a) {
     const int seg_keys = FW_PAGES << c.page_shift;  // keys whose page ids are staged at a time
     for (int s_lo = k_lo; s_lo < k_hi; s_lo += seg_keys) {
       const int s_hi = min(s_lo + seg_keys, k_hi), p0 = s_lo >> c.page_shift;
-      __syncthreads();  // the ids of the last segment are no longer read
+      if (s_lo > k_lo) __syncthreads();  // the ids of the last segment are no longer read
       for (int i = tid; i <= ((s_hi - 1) >> c.page_shift) - p0; i += 64 * NW)
         page_ids[i] = min(max(pages[p0 + i], 0), c.pages - 1);
       __syncthreads();
@@ -655,16 +650,17 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(AttnArgs a) {
       auto whole = [&](int t) {  // every row sees the whole tile
         return s_lo + (t + 1) * FW_KEYS <= min(lim_lo + 1, s_hi);
       };
-      auto issue = [&](int t) __attribute__((always_inline)) {  // keys past the last repeat it (they are masked)
-        uint8_t* st = mine + ((t / NW) & 1) * S::kStage;
-        const uint32_t kb = (uint32_t)(uintptr_t)st;
+      // a copy's rows lie in one page (page_size >= 8): its address is the wave's; copies wholly past the last key repeat
+      // that key's
+      auto issue = [&](int t) __attribute__((always_inline)) {
+        const uint32_t st = (uint32_t)(uintptr_t)(mine + ((t / NW) & 1) * S::kStage);
 #pragma unroll
         for (int u = 0; u < S::kRuns; ++u) {
-          const int r = u * S::kRun + crow, key = min(s_lo + t * FW_KEYS + r, s_hi - 1);
-          const int64_t off = page_ids[(key >> c.page_shift) - p0] * page_bytes +
-                              (int64_t)((key & slot_mask) * slot_bytes);
-          copy16(kb + u * 1024, kbase + off + 16 * k_place<D>(cpl, r));
-          copy16(kb + S::kTile + u * 1024, vbase + off + 16 * v_place<D>(cpl, r));
+          const uint32_t key = (uint32_t)min(s_lo + t * FW_KEYS + u * S::kRun, (s_hi - 1) & ~(S::kRun - 1));
+          const uint64_t off = (uint64_t)(uint32_t)uniform(page_ids[(key >> c.page_shift) - p0]) * page_bytes +
+                               (key & slot_mask) * slot_bytes;
+          copy16(st + u * 1024, kbase + off, klane[u]);
+          copy16(st + S::kTile + u * 1024, vbase + off, vlane[u]);
         }
       };
       auto step = [&](int t, auto mask_c) __attribute__((always_inline)) {
@@ -672,13 +668,13 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(AttnArgs a) {
         uint8_t* kb = mine + ((t / NW) & 1) * S::kStage;
         const int k0 = s_lo + t * FW_KEYS;
         v4i pop[RB];
-        float ref[RB];
         if (MASK) {
 #pragma unroll
           for (int u = 0; u < S::kRuns; ++u) {
             v4i* at = (v4i*)(kb + S::kTile + u * 1024 + lane * 16);
             v4i x = *at;
-            if (take_nonfinite<T>(x)) *at = x, aside = true;
+            if (k0 + u * S::kRun + crow >= s_hi) *at = (v4i){};  // whatever a page holds past the end
+            else if (take_nonfinite<T>(x)) *at = x, aside = true;
           }
         }
         v4f sc[RB][2];
@@ -688,14 +684,14 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(AttnArgs a) {
         for (int cd = 0; cd < S::kNQ; ++cd)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const v4i kop = *(const v4i*)(kb + 16 * x * S::kRow + kro[cd]);
+            const v4i kop = *(const v4i*)(kb + 16 * x * S::kRow + (kro ^ (uint32_t)(64 * cd)));
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) sc[rb][x] = Mfma<T>::tall(kop, qop[rb][cd], sc[rb][x]);
           }
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
           // the lane's scores: its row, keys 16 x + 4 q4 + r
-          if (a.scores && row0 + 16 * rb + i16 < R.total) {
+          if (a.scores && 16 * rb + i16 < nrows) {
             float* sp = a.scores + out_row[rb] * a.score_stride + k0 + 4 * q4;
 #pragma unroll
             for (int x = 0; x < 2; ++x)
@@ -715,13 +711,13 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(AttnArgs a) {
           mx = fmaxf(mx, __shfl_xor(mx, 32)) * a.c_log2;
           const bool bump = mx > m_run[rb];
           const float m_new = bump ? mx : m_run[rb];
-          ref[rb] = MASK && m_new == -INFINITY ? 0.0f : m_new;
-          const float alpha = __builtin_amdgcn_exp2f(m_run[rb] - ref[rb]);
+          const float ref = MASK && m_new == -INFINITY ? 0.0f : m_new;
+          const float alpha = __builtin_amdgcn_exp2f(m_run[rb] - ref);
           m_run[rb] = m_new;
           float p[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rb][e >> 2][e & 3], a.c_log2, -ref[rb]));
+            p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rb][e >> 2][e & 3], a.c_log2, -ref));
           l_run[rb] = __builtin_fmaf(l_run[rb], alpha, ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])));
           pop[rb] = (v4i){Mfma<T>::pack(p[0], p[1]), Mfma<T>::pack(p[2], p[3]), Mfma<T>::pack(p[4], p[5]),
                           Mfma<T>::pack(p[6], p[7])};
@@ -783,7 +779,6 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(AttnArgs a) {
     }
 
     // join the waves: each leaves its O [row][channel] with its m and l, thread by thread they are summed in wave order
-    __syncthreads();
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       float* op = (float*)mine + (16 * rb + i16) * (D + 4);
@@ -794,7 +789,6 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(AttnArgs a) {
       if (q4 == 0) stat[wave][0][16 * rb + i16] = m_run[rb], stat[wave][1][16 * rb + i16] = l_run[rb];
     }
     __syncthreads();
-    const int nrows = min(16 * RB, R.total - row0);
     for (int i = tid; i < nrows * (D / 4); i += 64 * NW) {
       const int r = i / (D / 4), d = i % (D / 4) * 4;
       float m = -INFINITY;
@@ -810,11 +804,64 @@ __global__ __launch_bounds__(64 * NW) void paged_attn_few_kernel(AttnArgs a) {
         o += *(const v4f*)((const float*)(lds + w * S::kWave) + r * (D + 4) + d) * f;
       }
       const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
-      const int64_t at = (int64_t)(R.t0 + (row0 + r) / g) * a.heads + h * g + (row0 + r) % g;
-      if (k_hi > k_lo || a.splits == 1) put_o<T, D>(a, split, at, d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-      if (d == 0) put_lse(a, split, at, m, l);
+      const float lse2 = m == -INFINITY ? -INFINITY : m + __builtin_amdgcn_logf(l);
+      const int64_t row = (int64_t)(R.t0 + i0 + r / g) * a.heads + h * g + r % g;
+      if (slot < 0) {
+        *(uint2*)(a.o + row * D + d) = make_uint2((uint32_t)Mfma<T>::pack(o[0] * inv, o[1] * inv),
+                                                  (uint32_t)Mfma<T>::pack(o[2] * inv, o[3] * inv));
+        if (d == 0) a.lse[row] = lse2 * kLn2;
+      } else {
+        const int64_t prow = SHARES ? (int64_t)slot * BM + r : (int64_t)slot * a.tokens * a.heads + row;
+        // a split without keys leaves only its lse
+        if (SHARES || k_hi > k_lo) *(v4f*)(a.o_part + prow * D + d) = o * inv;
+        if (d == 0) a.lse_part[prow] = lse2;
+      }
     }
-    if (row0 + 16 * RB < R.total) __syncthreads();  // the stages are copied into again
+  };
+
+  if constexpr (!SHARES) {
+    const int groups = c.batch * c.kv_heads;
+    const int grp = blockIdx.x % groups, split = blockIdx.x / groups, b = grp / c.kv_heads, h = grp % c.kv_heads;
+    const Rows R = uniform_rows_of(c, b, a.tokens, g);
+    for (int i0 = 0; i0 < R.n; i0 += tt) {
+      const int i1 = min(i0 + tt, R.n), lim_hi = R.token_limit(i1 - 1, causal), k_lo = split * a.split_keys;
+      const int k_hi = split + 1 < a.splits ? min(k_lo + a.split_keys, lim_hi + 1) : lim_hi + 1;
+      if (i0 > 0) __syncthreads();  // the stages are copied into again
+      run(R, b, h, i0, i1, k_lo, k_hi, a.splits > 1 ? split : -1);
+    }
+  } else {
+    const int share = blockIdx.x % kXcds * (a.shares / kXcds) + blockIdx.x / kXcds;
+    int64_t unused;
+    const int64_t per_head = head_line(c, a.tokens, tt, causal, 0, unused), all = per_head * c.kv_heads;
+    const int64_t x0 = share_start(all, share, a.shares), x1 = share_start(all, share + 1, a.shares);
+    if (x0 >= x1) return;
+    Place at = place_of<FW_UNIT>(c, a.tokens, tt, causal, per_head, x0);
+    const Place end = place_of<FW_UNIT>(c, a.tokens, tt, causal, per_head, x1);
+    Rows R = uniform_rows_of(c, at.b, a.tokens, g);
+    while (true) {
+      const int i0 = at.tile * tt, i1 = min(i0 + tt, R.n), lim_hi = R.token_limit(i1 - 1, causal);
+      const bool last = at.h == end.h && at.b == end.b && at.tile == end.tile;
+      const int units = max(1, (lim_hi + FW_UNIT) / FW_UNIT), to = last ? min(end.unit, units) : units;
+      if (at.unit < to) {
+        // a part goes into the share's slot: the first for a tile that an earlier share began, else the second
+        const bool part = at.unit > 0 || to < units;
+        run(R, at.b, at.h, i0, i1, at.unit * FW_UNIT, min(to * FW_UNIT, lim_hi + 1),
+            part ? 2 * share + (at.unit > 0 ? 0 : 1) : -1);
+        __syncthreads();  // the stages are copied into again
+      }
+      if (last) break;
+      at.unit = 0;
+      if (i1 < R.n) {
+        ++at.tile;
+      } else {
+        at.tile = 0;
+        do {  // the next sequence with new tokens, of the next head after the last
+          if (++at.b == c.batch) at.b = 0, ++at.h;
+          if (at.h == c.kv_heads) return;  // the line's end
+          R = uniform_rows_of(c, at.b, a.tokens, g);
+        } while (R.n == 0);
+      }
+    }
   }
 }
 
@@ -1029,8 +1076,7 @@ constexpr int64_t kScoreBytes = 256ll << 20;  // most workspace spent on kept sc
 
 struct Plan {
   bool matrix, few, keep_scores;
-  int row_blocks;  // few: 16-row blocks a workgroup (1 or 2)
-  int waves;       // tile: 4 or 8
+  int64_t tile_rows;  // rows a workgroup: 16 or 32 (few), 128 or 256
   int splits, split_keys, tiles, shares;
   int row_splits, key_tiles;  // of the recomputing gather
   int64_t score_stride, part_floats, bytes;
@@ -1043,26 +1089,20 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int
   p.matrix = (d == 64 || d == 128) && heads / kv_heads <= 256;
   p.splits = 1, p.split_keys = 1 << 30, p.tiles = 1;
   if (!p.matrix || batch == 0 || tokens == 0) return p;
-  const int64_t rows = max_q * (heads / kv_heads), groups = batch * kv_heads;
+  const int64_t group = heads / kv_heads, rows = (max_q < 1 ? 1 : max_q) * group, groups = batch * kv_heads;
   max_kv = max_kv < 1 ? 1 : max_kv;
   p.few = rows <= 32;
-  if (p.few) {
-    p.row_blocks = rows <= 16 ? 1 : 2;
-    // splits of one length for all sequences, so that ragged lengths still make even work: about 2048 of them in all if
-    // every sequence were the longest, of at least 256 keys
-    int64_t keys = (groups * max_kv / 2048 + 127) / 128 * 128;
-    if (keys < 256) keys = 256;
-    p.split_keys = (int)keys;
-    p.splits = (int)((max_kv + keys - 1) / keys);
-    p.keep_scores = gather && tokens * heads * ((capacity + 3) / 4 * 4) * 4 <= kScoreBytes;
+  p.tile_rows = p.few ? (rows <= 16 ? 16 : 32) : rows <= 128 ? 128 : 256;
+  p.tiles = (int)(((max_q < 1 ? 1 : max_q) + p.tile_rows / group - 1) / (p.tile_rows / group));
+  if (p.few) p.keep_scores = gather && tokens * heads * ((capacity + 3) / 4 * 4) * 4 <= kScoreBytes;
+  if (p.few && groups * ((max_kv + 255) / 256) <= kCus) {
+    p.split_keys = 256;
+    p.splits = (int)((max_kv + 255) / 256);
+    if (p.splits > 1) p.part_floats = p.splits * tokens * heads * (d + 1);
   } else {
-    p.waves = rows <= 128 ? 4 : 8;
-    const int64_t tt = 32 * p.waves / (heads / kv_heads);
-    p.tiles = (int)((max_q + tt - 1) / tt);
-    p.shares = p.waves == 4 ? 2 * kCus : kCus;  // as many workgroups as fit at once
-    p.part_floats = 2 * p.shares * (32 * p.waves) * (d + 1);
+    p.shares = p.tile_rows == 128 ? 2 * kCus : kCus;  // as many workgroups as fit at once
+    p.part_floats = 2 * p.shares * p.tile_rows * (d + 1);
   }
-  if (p.splits > 1) p.part_floats = p.splits * tokens * heads * (d + 1);
   int64_t gathered = 0;
   p.score_stride = (capacity + 3) / 4 * 4;
   if (p.keep_scores) {
@@ -1083,14 +1123,23 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int
 template <class T, int D>
 void launch_matrix(const Plan& p, AttnArgs a, int64_t max_kv, bool gather, hipStream_t st) {
   const unsigned groups = (unsigned)(a.c.batch * a.c.kv_heads);
-  if (p.few) {
-    const dim3 grid(groups * (unsigned)p.splits);
-    constexpr int NW = 4;
-    if (p.row_blocks == 1) hipLaunchKernelGGL((paged_attn_few_kernel<T, D, 1, NW>), grid, dim3(64 * NW), 0, st, a);
-    else hipLaunchKernelGGL((paged_attn_few_kernel<T, D, 2, NW>), grid, dim3(64 * NW), 0, st, a);
+  if (p.few && p.shares == 0) {
+    const dim3 grid(groups * (unsigned)p.splits), block(64 * FW_WAVES);
+    if (p.tile_rows == 16) hipLaunchKernelGGL((paged_attn_few_kernel<T, D, 1, false>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((paged_attn_few_kernel<T, D, 2, false>), grid, block, 0, st, a);
+    if (p.splits > 1)
+      hipLaunchKernelGGL((paged_attn_join_kernel<T, D>), dim3((unsigned)(((int64_t)a.tokens * a.heads * D + 1023) / 1024)),
+                         dim3(256), 0, st, a);
   } else {
-    const dim3 grid((unsigned)p.shares), jgrid(groups * (unsigned)(p.tiles * (32 * p.waves / JT_ROWS)));
-    if (p.waves == 4) {
+    const dim3 grid((unsigned)p.shares);
+    const dim3 jgrid(groups * (unsigned)(p.tiles * (p.tile_rows / join_rows((int)p.tile_rows))));
+    if (p.tile_rows == 16) {
+      hipLaunchKernelGGL((paged_attn_few_kernel<T, D, 1, true>), grid, dim3(64 * FW_WAVES), 0, st, a);
+      hipLaunchKernelGGL((paged_attn_join_parts_kernel<T, D, 16, FW_UNIT>), jgrid, dim3(256), 0, st, a);
+    } else if (p.tile_rows == 32) {
+      hipLaunchKernelGGL((paged_attn_few_kernel<T, D, 2, true>), grid, dim3(64 * FW_WAVES), 0, st, a);
+      hipLaunchKernelGGL((paged_attn_join_parts_kernel<T, D, 32, FW_UNIT>), jgrid, dim3(256), 0, st, a);
+    } else if (p.tile_rows == 128) {
       hipLaunchKernelGGL((paged_attn_tile_kernel<T, D, 64, 4>), grid, dim3(256), 0, st, a);
       hipLaunchKernelGGL((paged_attn_join_parts_kernel<T, D, 128, 64>), jgrid, dim3(256), 0, st, a);
     } else {
@@ -1098,9 +1147,6 @@ void launch_matrix(const Plan& p, AttnArgs a, int64_t max_kv, bool gather, hipSt
       hipLaunchKernelGGL((paged_attn_join_parts_kernel<T, D, 256, 64>), jgrid, dim3(256), 0, st, a);
     }
   }
-  if (p.splits > 1)
-    hipLaunchKernelGGL((paged_attn_join_kernel<T, D>), dim3((unsigned)(((int64_t)a.tokens * a.heads * D + 1023) / 1024)),
-                       dim3(256), 0, st, a);
   if (!gather) return;
   if (p.keep_scores) {
     const unsigned blocks = (unsigned)((max_kv + 1023) / 1024);
