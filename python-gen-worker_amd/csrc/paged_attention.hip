@@ -18,6 +18,7 @@ struct AttnArgs {
   float* lse;
   float* o_part;
   float* lse_part;
+  int4* cuts;             // [shares]: a share's cut tiles, see Cut
   float* scores;          // [tokens * heads][score_stride] in the log2 domain, or NULL
   float* w_part;
   int64_t score_stride;
@@ -35,6 +36,21 @@ __device__ __forceinline__ float dot8(v4i x, v4i y, float s) {
     s = fmaf(T::load((uint16_t)((uint32_t)x[e] >> 16)), T::load((uint16_t)((uint32_t)y[e] >> 16)), s);
   }
   return s;
+}
+
+// What a share says of the row tiles that its ends cut, for the join: x: 0, 1 or 2: no part of a tile that an earlier share
+// began, one that later shares continue, one that ends the tile; y: rows of a tile that it begins and later shares
+// continue (0: none), which start at token z, kv head w. Every share's workgroup sets its own; thread 0 writes.
+__device__ __forceinline__ void no_cuts(const AttnArgs& a, int share) {
+  if (threadIdx.x == 0) a.cuts[share] = make_int4(0, 0, 0, 0);
+}
+__device__ __forceinline__ void set_cut(const AttnArgs& a, int share, bool begun, bool ends, int rows, int token, int h) {
+  if (threadIdx.x != 0) return;
+  if (begun) {
+    a.cuts[share].x = ends ? 2 : 1;
+  } else {
+    a.cuts[share].y = rows, a.cuts[share].z = token, a.cuts[share].w = h;
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -194,9 +210,9 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_attn_tile_kernel(AttnArgs a)
   // this workgroup's share. An XCD's workgroups (every 8th) take neighbouring shares, which are of one head where there
   // are 8 (or 16, ...), so that K and V are shared in its L2
   const int share = blockIdx.x % kXcds * (a.shares / kXcds) + blockIdx.x / kXcds, tt = BM / g;
-  int64_t unused;
-  const int64_t per_head = head_line(c, a.tokens, tt, causal, 0, unused), all = per_head * c.kv_heads;
+  const int64_t per_head = head_line(c, a.tokens, tt, causal), all = per_head * c.kv_heads;
   const int64_t x0 = share_start(all, share, a.shares), x1 = share_start(all, share + 1, a.shares);
+  no_cuts(a, share);
   if (x0 >= x1) return;
   Place at = place_of<BN>(c, a.tokens, tt, causal, per_head, x0);
   const Place end = place_of<BN>(c, a.tokens, tt, causal, per_head, x1);
@@ -443,6 +459,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_attn_tile_kernel(AttnArgs a)
       const float lse2 = m_run == -INFINITY ? -INFINITY : m_run + __builtin_amdgcn_logf(l_tot);
       if (at.unit > 0 || to < units) {
         // a part: into the share's slot, the first for a tile that an earlier share began, else the second
+        set_cut(a, share, at.unit > 0, to == units, (i1 - i0) * g, R.t0 + i0, h);
         const int64_t prow = (int64_t)(2 * share + (at.unit > 0 ? 0 : 1)) * BM + r;
         float* op = a.o_part + prow * D + 4 * hf;
 #pragma unroll
@@ -482,71 +499,53 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_attn_tile_kernel(AttnArgs a)
 
 constexpr int join_rows(int bm) { return bm < 32 ? bm : 32; }
 
-// Joins the parts of row tiles that the shares' ends cut, in the shares' order. A workgroup takes JT_ROWS rows of a tile
-// and finds from the same division which shares hold a part of it.
-template <class T, int D, int BM, int BN>
+// Joins the parts of row tiles that the shares' ends cut, in the shares' order: a workgroup for JT rows of the tile that
+// its share begins and others continue.
+template <class T, int D, int BM>
 __global__ __launch_bounds__(256) void paged_attn_join_parts_kernel(AttnArgs a) {
-  constexpr int JT_ROWS = join_rows(BM);
-  const PagedArgs& c = a.c;
-  const int g = a.heads / c.kv_heads, groups = c.batch * c.kv_heads, tt = BM / g;
-  const bool causal = a.causal != 0;
-  const int chunk = blockIdx.x % (BM / JT_ROWS), rest = blockIdx.x / (BM / JT_ROWS);
-  const int b = rest % groups % c.batch, h = rest % groups / c.batch;
-  const Rows R = uniform_rows_of(c, b, a.tokens, g);
-  if (rest / groups * tt >= R.n) return;
-  int64_t before;
-  const int64_t per_head = head_line(c, a.tokens, tt, causal, b, before), all = per_head * c.kv_heads;
-  const TileLine line = tile_line(R, tt, causal);
-  __shared__ int slots[2 * kCus];  // the slots of a tile's parts, in order
+  constexpr int JT = join_rows(BM);
+  __shared__ int slots[2 * kCus + 1];  // the slots of the tile's parts, in order
   __shared__ int nslots;
-  for (int tile = rest / groups; tile * tt < R.n; tile += a.tiles) {
-    const int64_t x0 = h * per_head + before + line.before(tile), x1 = h * per_head + before + line.before(tile + 1);
-    const int i0 = tile * tt, i1 = min(i0 + tt, R.n);
-    const int units = max(1, (R.token_limit(i1 - 1, causal) + BN) / BN);
-    // shares whose start lies in (x0, x1) cut the tile; s0 is the one before them. A share starts at or before x where
-    // all * s / n <= x
-    const int s0 = (int)(((x0 + 1) * a.shares - 1) / all), s1 = (int)((x1 * a.shares - 1) / all);
-    if (s0 == s1) continue;
-    auto cut = [&](int s) {  // the unit at which share s begins, of those in s0 .. s1 + 1
-      if (s <= s0) return 0;
-      return s > s1 ? units : min(units, (int)(share_start(all, s, a.shares) - x0) / BN);
-    };
-    __syncthreads();  // the list of the tile before is no longer read
-    if (threadIdx.x < 64) {
-      int n = 0;
-      for (int s = s0; s <= s1; s += 64) {
-        const int mine = s + threadIdx.x, lo = cut(mine);
-        const bool part = mine <= s1 && cut(mine + 1) > lo;
-        const uint64_t parts = __ballot(part);
-        if (part) slots[n + __popcll(parts & ((1ull << threadIdx.x) - 1))] = 2 * mine + (lo > 0 ? 0 : 1);
-        n += __popcll(parts);
-      }
-      if (threadIdx.x == 0) nslots = n;
+  const int share = blockIdx.x / (BM / JT), r0 = blockIdx.x % (BM / JT) * JT;
+  const int4 cut = a.cuts[share];
+  if (cut.y <= r0) return;
+  if (threadIdx.x < 64) {
+    int n = 1;
+    bool ended = false;
+    for (int s = share + 1; s < a.shares && !ended; s += 64) {
+      const int mine = s + threadIdx.x, kind = mine < a.shares ? a.cuts[mine].x : 0;
+      const uint64_t ends = __ballot(kind == 2);
+      // up to the first share that ends a tile: the parts before it are all of this one
+      const uint64_t upto = ends ? ends ^ (ends - 1) : ~0ull;
+      const uint64_t parts = __ballot(kind != 0) & upto;
+      if (parts >> threadIdx.x & 1) slots[n + __popcll(parts & ((1ull << threadIdx.x) - 1))] = 2 * mine;
+      n += __popcll(parts);
+      ended = ends != 0;
     }
-    __syncthreads();
-    const int parts = nslots;
-    if (parts < 2) continue;  // whole after all: cuts before its first keys or behind its last
-    const int rows = min(JT_ROWS, (i1 - i0) * g - chunk * JT_ROWS);
-    for (int i = threadIdx.x; i < rows * (D / 4); i += 256) {
-      const int r = chunk * JT_ROWS + i / (D / 4), d = i % (D / 4) * 4;
-      float m = -INFINITY;
-      for (int k = 0; k < parts; ++k) m = fmaxf(m, a.lse_part[(int64_t)slots[k] * BM + r]);
-      const float ref = m == -INFINITY ? 0.0f : m;
-      float l = 0.0f;
-      v4f o = {};
+    if (threadIdx.x == 0) slots[0] = 2 * share + 1, nslots = n;
+  }
+  __syncthreads();
+  const int parts = nslots, g = a.heads / a.c.kv_heads, rows = min(JT, cut.y - r0);
+  for (int i = threadIdx.x; i < rows * (D / 4); i += 256) {
+    const int r = r0 + i / (D / 4), d = i % (D / 4) * 4;
+    float m = -INFINITY;
 #pragma unroll 4
-      for (int k = 0; k < parts; ++k) {
-        const int64_t prow = (int64_t)slots[k] * BM + r;
-        const float f = __builtin_amdgcn_exp2f(a.lse_part[prow] - ref);
-        l += f;
-        o += *(const v4f*)(a.o_part + prow * D + d) * f;
-      }
-      const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
-      const int64_t out_row = (int64_t)(R.t0 + i0 + r / g) * a.heads + h * g + r % g;
-      *(uint2*)(a.o + out_row * D + d) = make_uint2((uint32_t)Mfma<T>::pack(o[0] * inv, o[1] * inv),
-                                                    (uint32_t)Mfma<T>::pack(o[2] * inv, o[3] * inv));
-      if (d == 0) a.lse[out_row] = m == -INFINITY ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+    for (int k = 0; k < parts; ++k) m = fmaxf(m, a.lse_part[(int64_t)slots[k] * BM + r]);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f;
+    v4f o = {};
+#pragma unroll 4
+    for (int k = 0; k < parts; ++k) {
+      const int64_t prow = (int64_t)slots[k] * BM + r;
+      const float f = __builtin_amdgcn_exp2f(a.lse_part[prow] - ref);
+      l += f;
+      o += *(const v4f*)(a.o_part + prow * D + d) * f;
     }
+    const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
+    const int64_t out_row = (int64_t)(cut.z + r / g) * a.heads + cut.w * g + r % g;
+    *(uint2*)(a.o + out_row * D + d) = make_uint2((uint32_t)Mfma<T>::pack(o[0] * inv, o[1] * inv),
+                                                  (uint32_t)Mfma<T>::pack(o[2] * inv, o[3] * inv));
+    if (d == 0) a.lse[out_row] = m == -INFINITY ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
   }
 }
 
@@ -831,9 +830,9 @@ __global__ __launch_bounds__(64 * FW_WAVES) void paged_attn_few_kernel(AttnArgs 
     }
   } else {
     const int share = blockIdx.x % kXcds * (a.shares / kXcds) + blockIdx.x / kXcds;
-    int64_t unused;
-    const int64_t per_head = head_line(c, a.tokens, tt, causal, 0, unused), all = per_head * c.kv_heads;
+      const int64_t per_head = head_line(c, a.tokens, tt, causal), all = per_head * c.kv_heads;
     const int64_t x0 = share_start(all, share, a.shares), x1 = share_start(all, share + 1, a.shares);
+    no_cuts(a, share);
     if (x0 >= x1) return;
     Place at = place_of<FW_UNIT>(c, a.tokens, tt, causal, per_head, x0);
     const Place end = place_of<FW_UNIT>(c, a.tokens, tt, causal, per_head, x1);
@@ -845,6 +844,7 @@ __global__ __launch_bounds__(64 * FW_WAVES) void paged_attn_few_kernel(AttnArgs 
       if (at.unit < to) {
         // a part goes into the share's slot: the first for a tile that an earlier share began, else the second
         const bool part = at.unit > 0 || to < units;
+        if (part) set_cut(a, share, at.unit > 0, to == units, (i1 - i0) * g, R.t0 + i0, at.h);
         run(R, at.b, at.h, i0, i1, at.unit * FW_UNIT, min(to * FW_UNIT, lim_hi + 1),
             part ? 2 * share + (at.unit > 0 ? 0 : 1) : -1);
         __syncthreads();  // the stages are copied into again
@@ -1077,9 +1077,9 @@ constexpr int64_t kScoreBytes = 256ll << 20;  // most workspace spent on kept sc
 struct Plan {
   bool matrix, few, keep_scores;
   int64_t tile_rows;  // rows a workgroup: 16 or 32 (few), 128 or 256
-  int splits, split_keys, tiles, shares;
+  int splits, split_keys, shares;
   int row_splits, key_tiles;  // of the recomputing gather
-  int64_t score_stride, part_floats, bytes;
+  int64_t score_stride, gathered, part_floats, bytes;
 };
 
 Plan plan_of(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t d, int64_t max_q, int64_t max_kv,
@@ -1087,13 +1087,12 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int
   Plan p = {};
   // a row tile holds a token's whole group of query heads
   p.matrix = (d == 64 || d == 128) && heads / kv_heads <= 256;
-  p.splits = 1, p.split_keys = 1 << 30, p.tiles = 1;
+  p.splits = 1, p.split_keys = 1 << 30;
   if (!p.matrix || batch == 0 || tokens == 0) return p;
   const int64_t group = heads / kv_heads, rows = (max_q < 1 ? 1 : max_q) * group, groups = batch * kv_heads;
   max_kv = max_kv < 1 ? 1 : max_kv;
   p.few = rows <= 32;
   p.tile_rows = p.few ? (rows <= 16 ? 16 : 32) : rows <= 128 ? 128 : 256;
-  p.tiles = (int)(((max_q < 1 ? 1 : max_q) + p.tile_rows / group - 1) / (p.tile_rows / group));
   if (p.few) p.keep_scores = gather && tokens * heads * ((capacity + 3) / 4 * 4) * 4 <= kScoreBytes;
   if (p.few && groups * ((max_kv + 255) / 256) <= kCus) {
     p.split_keys = 256;
@@ -1103,10 +1102,9 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int
     p.shares = p.tile_rows == 128 ? 2 * kCus : kCus;  // as many workgroups as fit at once
     p.part_floats = 2 * p.shares * p.tile_rows * (d + 1);
   }
-  int64_t gathered = 0;
   p.score_stride = (capacity + 3) / 4 * 4;
   if (p.keep_scores) {
-    gathered = tokens * heads * p.score_stride;
+    p.gathered = tokens * heads * p.score_stride;
   } else if (gather) {
     p.key_tiles = (int)(max_kv > 0 ? (max_kv + GT_KEYS - 1) / GT_KEYS : 1);
     // six workgroups a CU, of at least 4 row tiles each
@@ -1114,9 +1112,9 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int
     if (want > most) want = most;
     if (want < 1 || want * groups * p.score_stride * 4 > kScoreBytes) want = 1;
     p.row_splits = (int)want;
-    if (want > 1) gathered = want * groups * p.score_stride;
+    if (want > 1) p.gathered = want * groups * p.score_stride;
   }
-  p.bytes = (p.part_floats + gathered) * 4;
+  p.bytes = (p.gathered + p.part_floats) * 4 + p.shares * 16;
   return p;
 }
 
@@ -1132,19 +1130,19 @@ void launch_matrix(const Plan& p, AttnArgs a, int64_t max_kv, bool gather, hipSt
                          dim3(256), 0, st, a);
   } else {
     const dim3 grid((unsigned)p.shares);
-    const dim3 jgrid(groups * (unsigned)(p.tiles * (p.tile_rows / join_rows((int)p.tile_rows))));
+    const dim3 jgrid((unsigned)(p.shares * (p.tile_rows / join_rows((int)p.tile_rows))));
     if (p.tile_rows == 16) {
       hipLaunchKernelGGL((paged_attn_few_kernel<T, D, 1, true>), grid, dim3(64 * FW_WAVES), 0, st, a);
-      hipLaunchKernelGGL((paged_attn_join_parts_kernel<T, D, 16, FW_UNIT>), jgrid, dim3(256), 0, st, a);
+      hipLaunchKernelGGL((paged_attn_join_parts_kernel<T, D, 16>), jgrid, dim3(256), 0, st, a);
     } else if (p.tile_rows == 32) {
       hipLaunchKernelGGL((paged_attn_few_kernel<T, D, 2, true>), grid, dim3(64 * FW_WAVES), 0, st, a);
-      hipLaunchKernelGGL((paged_attn_join_parts_kernel<T, D, 32, FW_UNIT>), jgrid, dim3(256), 0, st, a);
+      hipLaunchKernelGGL((paged_attn_join_parts_kernel<T, D, 32>), jgrid, dim3(256), 0, st, a);
     } else if (p.tile_rows == 128) {
       hipLaunchKernelGGL((paged_attn_tile_kernel<T, D, 64, 4>), grid, dim3(256), 0, st, a);
-      hipLaunchKernelGGL((paged_attn_join_parts_kernel<T, D, 128, 64>), jgrid, dim3(256), 0, st, a);
+      hipLaunchKernelGGL((paged_attn_join_parts_kernel<T, D, 128>), jgrid, dim3(256), 0, st, a);
     } else {
       hipLaunchKernelGGL((paged_attn_tile_kernel<T, D, 64, 8>), grid, dim3(512), 0, st, a);
-      hipLaunchKernelGGL((paged_attn_join_parts_kernel<T, D, 256, 64>), jgrid, dim3(256), 0, st, a);
+      hipLaunchKernelGGL((paged_attn_join_parts_kernel<T, D, 256>), jgrid, dim3(256), 0, st, a);
     }
   }
   if (!gather) return;
@@ -1203,18 +1201,19 @@ extern "C" int gwa_paged_attention(const gwa_paged_cache* cache, const void* q, 
   const float c_log2 = scale * kLog2e;
   const Plan p = plan_of(c.batch, tokens, heads, c.kv_heads, d, max_q, max_kv, c.capacity, gather != 0);
   if (p.matrix && c.batch > 0) {
-    GWA_REQUIRE(groups * p.splits * p.tiles < (1ll << 27) && rows * p.splits < (1ll << 31),
-                "%s: %lld rows in %d splits are too many", what, (long long)rows, p.splits);
+    GWA_REQUIRE(rows * p.splits < (1ll << 31) && groups * (p.key_tiles + 1) * (p.row_splits + 1) < (1ll << 31),
+                "%s: %lld rows over %lld sequences' heads are too many", what, (long long)rows, (long long)groups);
     GWA_REQUIRE(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes && GWA_ALIGNED(workspace, 16)),
                 "%s: a workspace of %lld bytes, %lld are needed (16-byte aligned)", what, (long long)workspace_bytes,
                 (long long)p.bytes);
     float* ws = (float*)workspace;
     const int64_t n_o = p.part_floats / (d + 1) * d;
     // scores or gathered parts first: scores' rows are read and written 16 bytes at a time
-    const int64_t n_s = p.bytes / 4 - p.part_floats;
+    const int64_t n_s = p.gathered;
     const AttnArgs a = {c, (const uint16_t*)q, ldqt, ldqh, (uint16_t*)o, lse, ws + n_s, ws + n_s + n_o,
+                        (int4*)(ws + n_s + p.part_floats),
                         p.keep_scores ? ws : nullptr, ws, p.score_stride, (int)tokens, (int)heads, p.splits, p.split_keys,
-                        p.tiles, p.shares, c_log2, causal};
+                        1, p.shares, c_log2, causal};
     if (cache->dtype == GWA_DT_BF16) {
       if (d == 128) launch_matrix<Bf16, 128>(p, a, max_kv, gather != 0, st);
       else launch_matrix<Bf16, 64>(p, a, max_kv, gather != 0, st);

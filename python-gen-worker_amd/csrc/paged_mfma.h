@@ -149,10 +149,9 @@ __device__ __forceinline__ TileLine tile_line(const Rows& r, int tt, bool causal
   l.none = l.first_keys > 0 ? 0 : causal ? min(l.tiles, -l.first_keys / tt + 1) : l.tiles;
   return l;
 }
-// one head's length in all, and that of the sequences before b; the whole wave calls it
-__device__ __forceinline__ int64_t head_line(const PagedArgs& c, int tokens, int tt, bool causal, int b, int64_t& before) {
+// one head's length in all; the whole wave calls it
+__device__ __forceinline__ int64_t head_line(const PagedArgs& c, int tokens, int tt, bool causal) {
   int64_t all = 0;
-  before = 0;
   for (int i = 0; i < c.batch; i += 64) {
     const int mine = i + (threadIdx.x & 63);
     int64_t u = 0;
@@ -160,15 +159,11 @@ __device__ __forceinline__ int64_t head_line(const PagedArgs& c, int tokens, int
       const TileLine l = tile_line(rows_of(c, mine, tokens, 1), tt, causal);
       u = l.before(l.tiles);
     }
-    int64_t e = mine < b ? u : 0;
 #pragma unroll
-    for (int w = 32; w; w >>= 1) u += __shfl_xor(u, w), e += __shfl_xor(e, w);
+    for (int w = 32; w; w >>= 1) u += __shfl_xor(u, w);
     all += u;
-    before += e;
   }
-  all = uniform64(all);
-  before = uniform64(before);
-  return all;
+  return uniform64(all);
 }
 // A place on the line: a head's sequence, a tile of it, and how many whole BN keys of the tile lie before it (which may be
 // more than the tile has)
