@@ -210,12 +210,13 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_attn_tile_kernel(AttnArgs a)
   // this workgroup's share. An XCD's workgroups (every 8th) take neighbouring shares, which are of one head where there
   // are 8 (or 16, ...), so that K and V are shared in its L2
   const int share = blockIdx.x % kXcds * (a.shares / kXcds) + blockIdx.x / kXcds, tt = BM / g;
-  const int64_t per_head = head_line(c, a.tokens, tt, causal), all = per_head * c.kv_heads;
+  const LineLanes lanes = line_lanes(c, a.tokens, tt, causal, 0);
+  const int64_t per_head = head_line(c, a.tokens, tt, causal, lanes), all = per_head * c.kv_heads;
   const int64_t x0 = share_start(all, share, a.shares), x1 = share_start(all, share + 1, a.shares);
   no_cuts(a, share);
   if (x0 >= x1) return;
-  Place at = place_of<BN>(c, a.tokens, tt, causal, per_head, x0);
-  const Place end = place_of<BN>(c, a.tokens, tt, causal, per_head, x1);
+  Place at = place_of<BN>(c, a.tokens, tt, causal, per_head, lanes, x0);
+  const Place end = place_of<BN>(c, a.tokens, tt, causal, per_head, lanes, x1);
   Rows R = uniform_rows_of(c, at.b, a.tokens, g);
 
   while (true) {  // one part of a row tile's keys: BN-key units [at.unit, to)
@@ -830,12 +831,13 @@ __global__ __launch_bounds__(64 * FW_WAVES) void paged_attn_few_kernel(AttnArgs 
     }
   } else {
     const int share = blockIdx.x % kXcds * (a.shares / kXcds) + blockIdx.x / kXcds;
-      const int64_t per_head = head_line(c, a.tokens, tt, causal), all = per_head * c.kv_heads;
+      const LineLanes lanes = line_lanes(c, a.tokens, tt, causal, 0);
+  const int64_t per_head = head_line(c, a.tokens, tt, causal, lanes), all = per_head * c.kv_heads;
     const int64_t x0 = share_start(all, share, a.shares), x1 = share_start(all, share + 1, a.shares);
     no_cuts(a, share);
     if (x0 >= x1) return;
-    Place at = place_of<FW_UNIT>(c, a.tokens, tt, causal, per_head, x0);
-    const Place end = place_of<FW_UNIT>(c, a.tokens, tt, causal, per_head, x1);
+    Place at = place_of<FW_UNIT>(c, a.tokens, tt, causal, per_head, lanes, x0);
+    const Place end = place_of<FW_UNIT>(c, a.tokens, tt, causal, per_head, lanes, x1);
     Rows R = uniform_rows_of(c, at.b, a.tokens, g);
     while (true) {
       const int i0 = at.tile * tt, i1 = min(i0 + tt, R.n), lim_hi = R.token_limit(i1 - 1, causal);
@@ -1099,7 +1101,11 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int
     p.splits = (int)((max_kv + 255) / 256);
     if (p.splits > 1) p.part_floats = p.splits * tokens * heads * (d + 1);
   } else {
-    p.shares = p.tile_rows == 128 ? 2 * kCus : kCus;  // as many workgroups as fit at once
+    // as many workgroups as fit at once, but no more than 16 to a row tile: 2 sequences of 95 tokens over 5619 keys, 6
+    // heads over 2, cut into 44 parts a tile took 41.8 us, into 11 parts 31.4; the join reads every part
+    const int64_t tt = p.tile_rows / group, row_tiles = groups * (((max_q < 1 ? 1 : max_q) + tt - 1) / tt);
+    p.shares = p.tile_rows == 128 ? 2 * kCus : kCus;
+    while (p.shares > 8 && p.shares > 16 * row_tiles) p.shares /= 2;
     p.part_floats = 2 * p.shares * p.tile_rows * (d + 1);
   }
   p.score_stride = (capacity + 3) / 4 * 4;

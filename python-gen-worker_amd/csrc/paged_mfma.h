@@ -129,13 +129,14 @@ struct TileLine {
     if (t > none) x += (int64_t)(t - none) * first_keys + (int64_t)slope * ((int64_t)t * (t - 1) - (int64_t)none * (none - 1)) / 2;
     return x;
   }
-  // the tile that position x < before(tiles) falls into
+  // the tile that position x < before(tiles) falls into; the whole wave calls it, 64 candidates at a time
   __device__ __forceinline__ int tile_at(int64_t x) const {
-    int lo = 0, hi = tiles - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (before(mid) <= x) lo = mid;
-      else hi = mid - 1;
+    int lo = 0, width = tiles;  // among tiles [lo, lo + width)
+    while (width > 1) {
+      const int step = (width + 63) / 64, mine = (int)(threadIdx.x & 63) * step;
+      const int at = __popcll(__ballot(mine < width && before(lo + mine) <= x)) - 1;
+      lo += at * step;
+      width = min(step, width - at * step);
     }
     return lo;
   }
@@ -149,62 +150,68 @@ __device__ __forceinline__ TileLine tile_line(const Rows& r, int tt, bool causal
   l.none = l.first_keys > 0 ? 0 : causal ? min(l.tiles, -l.first_keys / tt + 1) : l.tiles;
   return l;
 }
-// one head's length in all; the whole wave calls it
-__device__ __forceinline__ int64_t head_line(const PagedArgs& c, int tokens, int tt, bool causal) {
-  int64_t all = 0;
-  for (int i = 0; i < c.batch; i += 64) {
-    const int mine = i + (threadIdx.x & 63);
-    int64_t u = 0;
-    if (mine < c.batch) {
-      const TileLine l = tile_line(rows_of(c, mine, tokens, 1), tt, causal);
-      u = l.before(l.tiles);
-    }
-#pragma unroll
-    for (int w = 32; w; w >>= 1) u += __shfl_xor(u, w);
-    all += u;
+// The sequences i .. i + 63 of a batch, one a lane: the lane's line, its length, and the length up to its end
+struct LineLanes {
+  TileLine line;
+  int64_t own, upto;
+};
+__device__ __forceinline__ LineLanes line_lanes(const PagedArgs& c, int tokens, int tt, bool causal, int i) {
+  const int lane = threadIdx.x & 63;
+  LineLanes r = {};
+  if (i + lane < c.batch) {
+    r.line = tile_line(rows_of(c, i + lane, tokens, 1), tt, causal);
+    r.own = r.line.before(r.line.tiles);
   }
-  return uniform64(all);
+  r.upto = r.own;
+#pragma unroll
+  for (int w = 1; w < 64; w <<= 1) {
+    const int64_t y = __shfl_up(r.upto, w);
+    if (lane >= w) r.upto += y;
+  }
+  return r;
 }
 // A place on the line: a head's sequence, a tile of it, and how many whole BN keys of the tile lie before it (which may be
 // more than the tile has)
 struct Place {
   int h, b, tile, unit;
 };
+// One head's length, and the places of a share's start and of the next one's. The whole wave calls these; `first` are the
+// lanes of the batch's first 64 sequences, which are all there are as a rule.
+__device__ __forceinline__ int64_t head_line(const PagedArgs& c, int tokens, int tt, bool causal, const LineLanes& first) {
+  int64_t all = uniform64(__shfl(first.upto, 63));
+  for (int i = 64; i < c.batch; i += 64) all += uniform64(__shfl(line_lanes(c, tokens, tt, causal, i).upto, 63));
+  return all;
+}
 template <int BN>
-__device__ __forceinline__ Place place_of(const PagedArgs& c, int tokens, int tt, bool causal, int64_t per_head, int64_t x) {
+__device__ __forceinline__ Place place_of(const PagedArgs& c, int tokens, int tt, bool causal, int64_t per_head,
+                                          const LineLanes& first, int64_t x) {
   Place p;
-  p.h = uniform((int)(x / per_head));
+  // the head: as many as end at or before x
+  p.h = 0;
+  for (int i = 0; i < c.kv_heads; i += 64)
+    p.h += __popcll(__ballot(i + (int)(threadIdx.x & 63) < c.kv_heads && (i + (int)(threadIdx.x & 63) + 1) * per_head <= x));
+  p.h = uniform(p.h);
   p.b = c.batch, p.tile = p.unit = 0;
-  x -= p.h * per_head;
   if (p.h >= c.kv_heads) return p;  // the line's end
+  x -= p.h * per_head;
   for (int i = 0; i < c.batch; i += 64) {
-    const int lane = threadIdx.x & 63, mine = i + lane;
-    int64_t u = 0;
-    TileLine l = {};
-    if (mine < c.batch) {
-      l = tile_line(rows_of(c, mine, tokens, 1), tt, causal);
-      u = l.before(l.tiles);
-    }
-    int64_t upto = u;
-#pragma unroll
-    for (int w = 1; w < 64; w <<= 1) {
-      const int64_t y = __shfl_up(upto, w);
-      if (lane >= w) upto += y;
-    }
-    const uint64_t past = __ballot(upto > x);
+    LineLanes s = first;
+    if (i > 0) s = line_lanes(c, tokens, tt, causal, i);
+    const uint64_t past = __ballot(s.upto > x);
     if (past) {
       const int at = uniform(__ffsll((unsigned long long)past) - 1);
-      x = uniform64(x - __shfl(upto - u, at));
-      l.first_keys = uniform(__shfl(l.first_keys, at));
-      l.slope = uniform(__shfl(l.slope, at));
-      l.none = uniform(__shfl(l.none, at));
-      l.tiles = uniform(__shfl(l.tiles, at));
+      x = uniform64(x - __shfl(s.upto - s.own, at));
+      TileLine l;
+      l.first_keys = uniform(__shfl(s.line.first_keys, at));
+      l.slope = uniform(__shfl(s.line.slope, at));
+      l.none = uniform(__shfl(s.line.none, at));
+      l.tiles = uniform(__shfl(s.line.tiles, at));
       p.b = i + at;
-      p.tile = l.tile_at(x);
-      p.unit = (int)((x - l.before(p.tile)) / BN);
+      p.tile = uniform(l.tile_at(x));
+      p.unit = (int)(x - l.before(p.tile)) / BN;
       break;
     }
-    x = uniform64(x - __shfl(upto, 63));
+    x = uniform64(x - __shfl(s.upto, 63));
   }
   p.b = uniform(p.b), p.tile = uniform(p.tile), p.unit = uniform(p.unit);
   return p;
