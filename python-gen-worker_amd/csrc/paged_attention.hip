@@ -498,13 +498,14 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_attn_tile_kernel(AttnArgs a)
   }
 }
 
-constexpr int join_rows(int bm) { return bm < 32 ? bm : 32; }
-
 // Joins the parts of row tiles that the shares' ends cut, in the shares' order: a workgroup for JT rows of the tile that
-// its share begins and others continue.
+// its share begins and others continue. All parts' sums are read at once and turned into their factors in LDS, so that a
+// part's values wait for nothing (read in turn, 12 parts of a tile of 28 rows took 14 us, so 6).
+constexpr int JT = 16;
+
 template <class T, int D, int BM>
 __global__ __launch_bounds__(256) void paged_attn_join_parts_kernel(AttnArgs a) {
-  constexpr int JT = join_rows(BM);
+  __shared__ float part[2 * kCus + 1][JT];  // a part's sum, then its factor, by row
   __shared__ int slots[2 * kCus + 1];  // the slots of the tile's parts, in order
   __shared__ int nslots;
   const int share = blockIdx.x / (BM / JT), r0 = blockIdx.x % (BM / JT) * JT;
@@ -527,26 +528,36 @@ __global__ __launch_bounds__(256) void paged_attn_join_parts_kernel(AttnArgs a) 
   }
   __syncthreads();
   const int parts = nslots, g = a.heads / a.c.kv_heads, rows = min(JT, cut.y - r0);
-  for (int i = threadIdx.x; i < rows * (D / 4); i += 256) {
-    const int r = r0 + i / (D / 4), d = i % (D / 4) * 4;
+  for (int i = threadIdx.x; i < parts * JT; i += 256) {
+    const int k = i / JT, r = i % JT;
+    part[k][r] = r < rows ? a.lse_part[(int64_t)slots[k] * BM + r0 + r] : 0.0f;
+  }
+  __syncthreads();
+  {
+    const int r = threadIdx.x / 16, lane = threadIdx.x % 16;  // 16 lanes a row
     float m = -INFINITY;
-#pragma unroll 4
-    for (int k = 0; k < parts; ++k) m = fmaxf(m, a.lse_part[(int64_t)slots[k] * BM + r]);
+    for (int k = lane; k < parts; k += 16) m = fmaxf(m, part[k][r]);
+#pragma unroll
+    for (int w = 8; w; w >>= 1) m = fmaxf(m, __shfl_xor(m, w));
     const float ref = m == -INFINITY ? 0.0f : m;
     float l = 0.0f;
-    v4f o = {};
-#pragma unroll 4
-    for (int k = 0; k < parts; ++k) {
-      const int64_t prow = (int64_t)slots[k] * BM + r;
-      const float f = __builtin_amdgcn_exp2f(a.lse_part[prow] - ref);
-      l += f;
-      o += *(const v4f*)(a.o_part + prow * D + d) * f;
-    }
+    for (int k = lane; k < parts; k += 16) l += __builtin_amdgcn_exp2f(part[k][r] - ref);
+#pragma unroll
+    for (int w = 8; w; w >>= 1) l += __shfl_xor(l, w);
     const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
+    for (int k = lane; k < parts; k += 16) part[k][r] = __builtin_amdgcn_exp2f(part[k][r] - ref) * inv;
+    if (lane == 0 && r < rows)
+      a.lse[(int64_t)(cut.z + (r0 + r) / g) * a.heads + cut.w * g + (r0 + r) % g] =
+          m == -INFINITY ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * (D / 4); i += 256) {
+    const int rr = i / (D / 4), r = r0 + rr, d = i % (D / 4) * 4;
+    v4f o = {};
+#pragma unroll 8
+    for (int k = 0; k < parts; ++k) o += *(const v4f*)(a.o_part + ((int64_t)slots[k] * BM + r) * D + d) * part[k][rr];
     const int64_t out_row = (int64_t)(cut.z + r / g) * a.heads + cut.w * g + r % g;
-    *(uint2*)(a.o + out_row * D + d) = make_uint2((uint32_t)Mfma<T>::pack(o[0] * inv, o[1] * inv),
-                                                  (uint32_t)Mfma<T>::pack(o[2] * inv, o[3] * inv));
-    if (d == 0) a.lse[out_row] = m == -INFINITY ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+    *(uint2*)(a.o + out_row * D + d) = make_uint2((uint32_t)Mfma<T>::pack(o[0], o[1]), (uint32_t)Mfma<T>::pack(o[2], o[3]));
   }
 }
 
@@ -1136,7 +1147,7 @@ void launch_matrix(const Plan& p, AttnArgs a, int64_t max_kv, bool gather, hipSt
                          dim3(256), 0, st, a);
   } else {
     const dim3 grid((unsigned)p.shares);
-    const dim3 jgrid((unsigned)(p.shares * (p.tile_rows / join_rows((int)p.tile_rows))));
+    const dim3 jgrid((unsigned)(p.shares * (p.tile_rows / JT)));
     if (p.tile_rows == 16) {
       hipLaunchKernelGGL((paged_attn_few_kernel<T, D, 1, true>), grid, dim3(64 * FW_WAVES), 0, st, a);
       hipLaunchKernelGGL((paged_attn_join_parts_kernel<T, D, 16>), jgrid, dim3(256), 0, st, a);
