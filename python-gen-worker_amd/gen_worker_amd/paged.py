@@ -337,8 +337,9 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, 
     head_dim^-0.5. ``max_q`` and ``max_kv``: the batch's largest new-token count and kv_len, which choose the launch.
     ``weights`` fp32 [pages, kv_heads, page_size]: every key's slot gets, added, the probability it drew from the
     sequence's new tokens over the kv head's query heads, in an order that does not depend on timing; sequences may
-    share pages only without it. head_dim: a multiple of 8 up to 256 (the matrix cores serve 64 and 128). No gradient
-    is defined."""
+    share pages only without it. head_dim: a multiple of 8 up to 256 (the matrix cores serve 64 and 128, up to 256 query
+    heads to a kv head). Rows of q that belong to no sequence (before q_start[0], behind q_start[batch]) are not written. No
+    gradient is defined."""
     if scale is None:
         scale = float(q.shape[-1]) ** -0.5
     host = _host()
@@ -543,9 +544,13 @@ class PagedCache:
         kv_len, flat, new = self._device_rows([lens, table, fresh])
         flat, new = flat.view(len(cut), old_width), new.view(len(cut), width)
         kept = None
-        for cache in [self] + self._twins:
-            got = paged_evict(cache.k, cache.v, cache.weights, flat, kv_len, max(lens), new, budget, recent)[0]
-            kept = got if kept is None else kept
+        try:
+            for cache in [self] + self._twins:
+                got = paged_evict(cache.k, cache.v, cache.weights, flat, kv_len, max(lens), new, budget, recent)[0]
+                kept = got if kept is None else kept
+        except Exception:
+            self._free.extend(fresh)   # nothing has moved: the sequences keep their pages
+            raise
         for i, s in enumerate(cut):
             e = self._seqs[s]
             self._free.extend(reversed(e[0]))
