@@ -638,7 +638,9 @@ int gwa_paged_attention(const gwa_paged_cache* cache, const void* q, int64_t ldq
  * and, of the others, the budget - recent of largest w (equal ones: the lowest
  * slots; a NaN ranks above every number), and copies the kept rows of k, v and w
  * in slot order into the pages of new_table [batch][new_width] (pages that no
- * sequence of `table` uses); shorter sequences are copied whole. kept
+ * sequence of `table` uses, room for min(budget, the largest kv_len) keys);
+ * shorter sequences are copied whole. max_kv: the largest kv_len as the host
+ * knows it; it shapes the launch only. kept
  * [batch][kv_heads][budget] int32: the old slots, -1 past new_len; new_len
  * [batch] = min(kv_len, budget). */
 int gwa_paged_evict(const gwa_paged_cache* cache, const int32_t* new_table, int64_t new_stride, int64_t new_width,

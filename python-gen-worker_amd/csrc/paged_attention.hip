@@ -1,4 +1,5 @@
 // Attention of new tokens over a paged key/value cache, with the keys' attention weight gathered on request.
+#include <algorithm>
 #include <type_traits>
 
 #include "paged_mfma.h"
@@ -207,21 +208,32 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_attn_tile_kernel(AttnArgs a)
   const uint32_t klane = crow * slot_bytes + 16 * k_place<D>(cpl, wave * S::kRun + crow);
   const uint32_t vlane = crow * slot_bytes + 16 * v_place<D>(cpl, wave * S::kRun + crow);
 
-  // this workgroup's share. An XCD's workgroups (every 8th) take neighbouring shares, which are of one head where there
-  // are 8 (or 16, ...), so that K and V are shared in its L2
-  const int share = blockIdx.x % kXcds * (a.shares / kXcds) + blockIdx.x / kXcds, tt = BM / g;
-  const LineLanes lanes = line_lanes(c, a.tokens, tt, causal, 0);
-  const int64_t per_head = head_line(c, a.tokens, tt, causal, lanes), all = per_head * c.kv_heads;
-  const int64_t x0 = share_start(all, share, a.shares), x1 = share_start(all, share + 1, a.shares);
-  no_cuts(a, share);
-  if (x0 >= x1) return;
-  Place at = place_of<BN>(c, a.tokens, tt, causal, per_head, lanes, x0);
-  const Place end = place_of<BN>(c, a.tokens, tt, causal, per_head, lanes, x1);
+  const int tt = BM / g;  // new tokens a row tile holds
+  const bool shared = a.shares > 0;
+  int share = 0;
+  Place at, end;
+  if (shared) {
+    // this workgroup's share. An XCD's workgroups (every 8th) take neighbouring shares, which are of one head where
+    // there are 8 (or 16, ...), so that K and V are shared in its L2
+    share = blockIdx.x % kXcds * (a.shares / kXcds) + blockIdx.x / kXcds;
+    const LineLanes lanes = line_lanes(c, a.tokens, tt, causal, 0);
+    const int64_t per_head = head_line(c, a.tokens, tt, causal, lanes), all = per_head * c.kv_heads;
+    const int64_t x0 = share_start(all, share, a.shares), x1 = share_start(all, share + 1, a.shares);
+    no_cuts(a, share);
+    if (x0 >= x1) return;
+    at = place_of<BN>(c, a.tokens, tt, causal, per_head, lanes, x0);
+    end = place_of<BN>(c, a.tokens, tt, causal, per_head, lanes, x1);
+  } else {  // a workgroup a row tile, all of its keys; the tiles that see the most start first
+    const int groups = c.batch * c.kv_heads, grp = blockIdx.x % groups;
+    at = Place{grp % c.kv_heads, grp / c.kv_heads, a.tiles - 1 - (int)(blockIdx.x / groups), 0};
+    end = at;
+  }
   Rows R = uniform_rows_of(c, at.b, a.tokens, g);
+  if (!shared && at.tile * tt >= R.n) return;
 
   while (true) {  // one part of a row tile's keys: BN-key units [at.unit, to)
     const int h = at.h, i0 = at.tile * tt, i1 = min(i0 + tt, R.n);
-    const bool last = at.h == end.h && at.b == end.b && at.tile == end.tile;
+    const bool last = shared && at.h == end.h && at.b == end.b && at.tile == end.tile;
     const int lim_lo = R.token_limit(i0, causal), lim_hi = R.token_limit(i1 - 1, causal);
     const int units = max(1, (lim_hi + BN) / BN), to = last ? min(end.unit, units) : units;
     if (at.unit < to) {
@@ -485,7 +497,10 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_attn_tile_kernel(AttnArgs a)
     }
     if (last) break;
     at.unit = 0;
-    if (i1 < R.n) {
+    if (!shared) {
+      at.tile += a.tiles;  // more tiles than the host knew of
+      if (at.tile * tt >= R.n) break;
+    } else if (i1 < R.n) {
       ++at.tile;
     } else {
       at.tile = 0;
@@ -505,7 +520,8 @@ constexpr int JT = 16;
 
 template <class T, int D, int BM>
 __global__ __launch_bounds__(256) void paged_attn_join_parts_kernel(AttnArgs a) {
-  __shared__ float part[2 * kCus + 1][JT];  // a part's sum, then its factor, by row
+  constexpr int kAtOnce = 64, kItems = JT * D / 4 / 256;  // parts whose factors are held; a thread's pieces of 4 channels
+  __shared__ float factor[kAtOnce][JT];
   __shared__ int slots[2 * kCus + 1];  // the slots of the tile's parts, in order
   __shared__ int nslots;
   const int share = blockIdx.x / (BM / JT), r0 = blockIdx.x % (BM / JT) * JT;
@@ -528,36 +544,40 @@ __global__ __launch_bounds__(256) void paged_attn_join_parts_kernel(AttnArgs a) 
   }
   __syncthreads();
   const int parts = nslots, g = a.heads / a.c.kv_heads, rows = min(JT, cut.y - r0);
-  for (int i = threadIdx.x; i < parts * JT; i += 256) {
-    const int k = i / JT, r = i % JT;
-    part[k][r] = r < rows ? a.lse_part[(int64_t)slots[k] * BM + r0 + r] : 0.0f;
-  }
-  __syncthreads();
-  {
-    const int r = threadIdx.x / 16, lane = threadIdx.x % 16;  // 16 lanes a row
-    float m = -INFINITY;
-    for (int k = lane; k < parts; k += 16) m = fmaxf(m, part[k][r]);
+  const int fr = threadIdx.x / 16, lane = threadIdx.x % 16;  // 16 lanes a row find its factors
+  auto sum_of = [&](int k) { return fr < rows ? a.lse_part[(int64_t)slots[k] * BM + r0 + fr] : 0.0f; };
+  float m = -INFINITY;
+  for (int k = lane; k < parts; k += 16) m = fmaxf(m, sum_of(k));
 #pragma unroll
-    for (int w = 8; w; w >>= 1) m = fmaxf(m, __shfl_xor(m, w));
-    const float ref = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f;
-    for (int k = lane; k < parts; k += 16) l += __builtin_amdgcn_exp2f(part[k][r] - ref);
+  for (int w = 8; w; w >>= 1) m = fmaxf(m, __shfl_xor(m, w));
+  const float ref = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f;
+  for (int k = lane; k < parts; k += 16) l += __builtin_amdgcn_exp2f(sum_of(k) - ref);
 #pragma unroll
-    for (int w = 8; w; w >>= 1) l += __shfl_xor(l, w);
-    const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
-    for (int k = lane; k < parts; k += 16) part[k][r] = __builtin_amdgcn_exp2f(part[k][r] - ref) * inv;
-    if (lane == 0 && r < rows)
-      a.lse[(int64_t)(cut.z + (r0 + r) / g) * a.heads + cut.w * g + (r0 + r) % g] =
-          m == -INFINITY ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < rows * (D / 4); i += 256) {
-    const int rr = i / (D / 4), r = r0 + rr, d = i % (D / 4) * 4;
-    v4f o = {};
+  for (int w = 8; w; w >>= 1) l += __shfl_xor(l, w);
+  const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
+  auto out_row = [&](int r) { return (int64_t)(cut.z + (r0 + r) / g) * a.heads + cut.w * g + (r0 + r) % g; };
+  if (lane == 0 && fr < rows) a.lse[out_row(fr)] = m == -INFINITY ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+  v4f o[kItems] = {};
+  for (int k0 = 0; k0 < parts; k0 += kAtOnce) {
+    const int n = min(kAtOnce, parts - k0);
+    if (k0 > 0) __syncthreads();
+    for (int k = lane; k < n; k += 16) factor[k][fr] = __builtin_amdgcn_exp2f(sum_of(k0 + k) - ref) * inv;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kItems; ++e) {
+      const int i = threadIdx.x + 256 * e, r = i / (D / 4), d = i % (D / 4) * 4;
+      if (r >= rows) continue;
 #pragma unroll 8
-    for (int k = 0; k < parts; ++k) o += *(const v4f*)(a.o_part + ((int64_t)slots[k] * BM + r) * D + d) * part[k][rr];
-    const int64_t out_row = (int64_t)(cut.z + r / g) * a.heads + cut.w * g + r % g;
-    *(uint2*)(a.o + out_row * D + d) = make_uint2((uint32_t)Mfma<T>::pack(o[0], o[1]), (uint32_t)Mfma<T>::pack(o[2], o[3]));
+      for (int k = 0; k < n; ++k) o[e] += *(const v4f*)(a.o_part + ((int64_t)slots[k0 + k] * BM + r0 + r) * D + d) * factor[k][r];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < kItems; ++e) {
+    const int i = threadIdx.x + 256 * e, r = i / (D / 4), d = i % (D / 4) * 4;
+    if (r < rows)
+      *(uint2*)(a.o + out_row(r) * D + d) = make_uint2((uint32_t)Mfma<T>::pack(o[e][0], o[e][1]),
+                                                       (uint32_t)Mfma<T>::pack(o[e][2], o[e][3]));
   }
 }
 
@@ -1090,7 +1110,7 @@ constexpr int64_t kScoreBytes = 256ll << 20;  // most workspace spent on kept sc
 struct Plan {
   bool matrix, few, keep_scores;
   int64_t tile_rows;  // rows a workgroup: 16 or 32 (few), 128 or 256
-  int splits, split_keys, shares;
+  int splits, split_keys, shares, tiles;
   int row_splits, key_tiles;  // of the recomputing gather
   int64_t score_stride, gathered, part_floats, bytes;
 };
@@ -1107,25 +1127,37 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int
   p.few = rows <= 32;
   p.tile_rows = p.few ? (rows <= 16 ? 16 : 32) : rows <= 128 ? 128 : 256;
   if (p.few) p.keep_scores = gather && tokens * heads * ((capacity + 3) / 4 * 4) * 4 <= kScoreBytes;
-  if (p.few && groups * ((max_kv + 255) / 256) <= kCus) {
+  // few splits only: their join reads them in turn (72 of 2 sequences of 18361 keys: 39 us in all, as shares 19)
+  if (p.few && groups * ((max_kv + 255) / 256) <= kCus && max_kv <= 8 * 256) {
     p.split_keys = 256;
     p.splits = (int)((max_kv + 255) / 256);
     if (p.splits > 1) p.part_floats = p.splits * tokens * heads * (d + 1);
   } else {
-    // as many workgroups as fit at once, but no more than 16 to a row tile: 2 sequences of 95 tokens over 5619 keys, 6
-    // heads over 2, cut into 44 parts a tile took 41.8 us, into 11 parts 31.4; the join reads every part
-    const int64_t tt = p.tile_rows / group, row_tiles = groups * (((max_q < 1 ? 1 : max_q) + tt - 1) / tt);
+    // as many workgroups as fit at once, but no more than 32 to a row tile: 2 sequences of 95 tokens over 5619 keys, 6
+    // heads over 2, cut into 64 parts a tile take 26 us, into 32 23, into 8 32; the join reads every part
+    const int64_t tt = p.tile_rows / group, tiles = ((max_q < 1 ? 1 : max_q) + tt - 1) / tt;
+    const int64_t row_tiles = kv_heads * std::min(batch * tiles, tokens / tt + batch), units = (max_kv + 63) / 64;
     p.shares = p.tile_rows == 128 ? 2 * kCus : kCus;
-    while (p.shares > 8 && p.shares > 16 * row_tiles) p.shares /= 2;
-    p.part_floats = 2 * p.shares * p.tile_rows * (d + 1);
+    // Many rows: a workgroup a row tile where that takes no longer. 64 keys take it about 2 us, and it goes through
+    // whole rounds of workgroups; shares always end together, but take 8 us to find and to join and 6 % more for
+    // their cut tiles (4096 tokens over 16500 keys, 32 heads over 8, 512 tiles: 894 us against 965; 150 tokens over 152
+    // keys, 8 heads over 4: 16.9 against 20.3)
+    const int64_t rounds = (row_tiles + p.shares - 1) / p.shares;
+    if (!p.few && 200 * units * rounds * p.shares < 212 * units * row_tiles + 800 * p.shares && groups * tiles < (1ll << 31)) {
+      p.tiles = (int)tiles;
+      p.shares = 0;
+    } else {
+      while (p.shares > 8 && p.shares > 32 * row_tiles) p.shares /= 2;
+      p.part_floats = 2 * p.shares * p.tile_rows * (d + 1);
+    }
   }
   p.score_stride = (capacity + 3) / 4 * 4;
   if (p.keep_scores) {
     p.gathered = tokens * heads * p.score_stride;
   } else if (gather) {
     p.key_tiles = (int)(max_kv > 0 ? (max_kv + GT_KEYS - 1) / GT_KEYS : 1);
-    // six workgroups a CU, of at least 4 row tiles each
-    int64_t want = (1536 + p.key_tiles * groups - 1) / (p.key_tiles * groups), most = rows / (4 * GT_ROWS);
+    // six workgroups a CU, of at least 2 row tiles each
+    int64_t want = (1536 + p.key_tiles * groups - 1) / (p.key_tiles * groups), most = rows / (2 * GT_ROWS);
     if (want > most) want = most;
     if (want < 1 || want * groups * p.score_stride * 4 > kScoreBytes) want = 1;
     p.row_splits = (int)want;
@@ -1145,6 +1177,10 @@ void launch_matrix(const Plan& p, AttnArgs a, int64_t max_kv, bool gather, hipSt
     if (p.splits > 1)
       hipLaunchKernelGGL((paged_attn_join_kernel<T, D>), dim3((unsigned)(((int64_t)a.tokens * a.heads * D + 1023) / 1024)),
                          dim3(256), 0, st, a);
+  } else if (p.shares == 0) {
+    const dim3 grid(groups * (unsigned)p.tiles);
+    if (p.tile_rows == 128) hipLaunchKernelGGL((paged_attn_tile_kernel<T, D, 64, 4>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((paged_attn_tile_kernel<T, D, 64, 8>), grid, dim3(512), 0, st, a);
   } else {
     const dim3 grid((unsigned)p.shares);
     const dim3 jgrid((unsigned)(p.shares * (p.tile_rows / JT)));
@@ -1230,7 +1266,7 @@ extern "C" int gwa_paged_attention(const gwa_paged_cache* cache, const void* q, 
     const AttnArgs a = {c, (const uint16_t*)q, ldqt, ldqh, (uint16_t*)o, lse, ws + n_s, ws + n_s + n_o,
                         (int4*)(ws + n_s + p.part_floats),
                         p.keep_scores ? ws : nullptr, ws, p.score_stride, (int)tokens, (int)heads, p.splits, p.split_keys,
-                        1, p.shares, c_log2, causal};
+                        p.tiles, p.shares, c_log2, causal};
     if (cache->dtype == GWA_DT_BF16) {
       if (d == 128) launch_matrix<Bf16, 128>(p, a, max_kv, gather != 0, st);
       else launch_matrix<Bf16, 64>(p, a, max_kv, gather != 0, st);

@@ -1,5 +1,6 @@
 // Rotary positions, the write of new tokens into a paged key/value cache, and the eviction of its least attended
 // keys. All three move each value once and compute next to nothing: they are bound by memory.
+#include <algorithm>
 #include <type_traits>
 
 #include "paged_common.h"
@@ -421,16 +422,19 @@ __global__ __launch_bounds__(EC_THREADS) void evict_copy_kernel(PagedArgs c, con
                                                                 int64_t new_stride, int new_capacity,
                                                                 const int32_t* kept, int budget, int pieces) {
   const int h = blockIdx.y % c.kv_heads, b = blockIdx.y / c.kv_heads;
-  const int i = blockIdx.x * EC_THREADS + threadIdx.x, r = i / pieces, p = i - r * pieces;
-  if (r >= min(min(paged_kv_len(c, b), budget), new_capacity)) return;
-  const int j = min(max(kept[(int64_t)blockIdx.y * budget + r], 0), paged_kv_len(c, b) - 1);
-  const int from = paged_page(c, c.table + b * c.table_stride, j);
-  const int to = paged_page(c, new_table + b * new_stride, r);
-  const int64_t src = paged_at(c, from, h, j) + 8 * p, dst = paged_at(c, to, h, r) + 8 * p;
-  const v4i kk = *(const v4i*)(c.k + src), vv = *(const v4i*)(c.v + src);
-  *(v4i*)(c.k + dst) = kk;
-  *(v4i*)(c.v + dst) = vv;
-  if (p == 0) c.w[paged_w_at(c, to, h, r)] = c.w[paged_w_at(c, from, h, j)];
+  const int rows = min(min(paged_kv_len(c, b), budget), new_capacity);
+  // one step where the host's max_kv holds
+  for (int64_t i = (int64_t)blockIdx.x * EC_THREADS + threadIdx.x; i < (int64_t)rows * pieces; i += (int64_t)gridDim.x * EC_THREADS) {
+    const int r = (int)(i / pieces), p = (int)(i - (int64_t)r * pieces);
+    const int j = min(max(kept[(int64_t)blockIdx.y * budget + r], 0), paged_kv_len(c, b) - 1);
+    const int from = paged_page(c, c.table + b * c.table_stride, j);
+    const int to = paged_page(c, new_table + b * new_stride, r);
+    const int64_t src = paged_at(c, from, h, j) + 8 * p, dst = paged_at(c, to, h, r) + 8 * p;
+    const v4i kk = *(const v4i*)(c.k + src), vv = *(const v4i*)(c.v + src);
+    *(v4i*)(c.k + dst) = kk;
+    *(v4i*)(c.v + dst) = vv;
+    if (p == 0) c.w[paged_w_at(c, to, h, r)] = c.w[paged_w_at(c, from, h, j)];
+  }
 }
 
 }  // namespace
@@ -454,14 +458,14 @@ extern "C" int gwa_paged_evict(const gwa_paged_cache* cache, const int32_t* new_
   GWA_REQUIRE(kept && new_len && (new_table || new_width == 0), "%s: null pointer", what);
   const int64_t groups = (int64_t)c.batch * c.kv_heads;
   const int pieces = cache->head_dim / 8;
-  const int64_t blocks = (most * pieces + EC_THREADS - 1) / EC_THREADS;
+  const int64_t blocks = (std::max<int64_t>(most, 1) * pieces + EC_THREADS - 1) / EC_THREADS;
   GWA_REQUIRE(groups < 65536 && blocks < (1ll << 31), "%s: %lld heads of sequences are too many", what,
               (long long)groups);
   const int held = (int)(max_kv < EV_HELD ? max_kv : EV_HELD);
   hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)groups), dim3(EV_THREADS), (size_t)held * 4,
                      (hipStream_t)stream, c, (int)budget, (int)recent, held, kept, new_len);
   const int rc = gwa_check_launch(what);
-  if (rc != GWA_OK || blocks == 0) return rc;
+  if (rc != GWA_OK || new_width == 0) return rc;
   hipLaunchKernelGGL(evict_copy_kernel, dim3((unsigned)blocks, (unsigned)groups), dim3(EC_THREADS), 0,
                      (hipStream_t)stream, c, new_table, new_stride, (int)(new_width * cache->page_size), kept,
                      (int)budget, pieces);

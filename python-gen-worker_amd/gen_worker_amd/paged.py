@@ -384,7 +384,8 @@ def paged_evict(k_pages: Tensor, v_pages: Tensor, weights: Tensor, table: Tensor
     """Cuts every sequence with more than ``budget`` keys back to it, for each kv head on its own: the last
     ``recent`` keys stay, and of the others the ``budget - recent`` of largest gathered weight (equal ones: the lowest
     slots; NaN ranks highest). What stays (k, v and weights, in slot order; all of a shorter sequence) is copied into
-    the pages of ``new_table`` int32 [batch, width], which must be pages that ``table`` does not use. Returns (kept int32
+    the pages of ``new_table`` int32 [batch, width], which must be pages that ``table`` does not use and hold
+    min(budget, the largest kv_len) keys a row; ``max_kv``: the largest kv_len, which shapes the launch. Returns (kept int32
     [batch, kv_heads, budget]: the old slots, -1 past the end; the new kv_len)."""
     a = (k_pages, v_pages, weights, table, kv_len)
     host = _host()

@@ -264,6 +264,46 @@ def test_attention_matches_64_bits(q, kv, heads, hk, dim, page, dtype, causal, g
         assert bool(torch.isnan(r.w[untouched]).all())
 
 
+def _many(n, lo, hi, seed):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randint(lo, hi + 1, (n,), generator=g).tolist()
+
+
+@pytest.mark.parametrize("q,kv,heads,hk,dim,page,dtype", [
+    # more than 64 sequences (one token each; chunks), more than 64 kv heads, groups past 64 and past 256 query heads, one
+    # sequence with nearly all of the keys among many short ones
+    ([1] * 130, _many(130, 0, 400, 1), 4, 2, 128, 16, BF16),
+    (_many(70, 0, 20, 2), [3000] + _many(69, 20, 90, 3), 4, 1, 64, 16, F16),
+    ([1, 2, 1], [600, 31, 257], 70, 70, 64, 16, BF16),
+    ([3, 1], [200, 90], 80, 1, 64, 16, F16), ([2, 1], [70, 40], 260, 1, 64, 16, BF16),
+    ([2] + [1] * 40, [9000] + [5] * 40, 8, 8, 64, 64, BF16), ([200] + [30] * 6, [7000] + [30] * 6, 2, 2, 128, 64, BF16)])
+@pytest.mark.parametrize("gather", [False, True])
+def test_many_sequences_heads_and_uneven_lengths(q, kv, heads, hk, dim, page, dtype, gather):
+    kv = [max(a, b) for a, b in zip(q, kv)]
+    r = Ragged(q, kv, heads, hk, dim, page, dtype, seed=heads)
+    w0 = r.w.clone() if gather else None
+    for causal in (True, False):
+        if gather:
+            r.w.copy_(w0)
+        o, lse = r.attend(causal=causal, gather=gather)
+        r.check(o, lse, causal, w0=w0, heads=range(0, heads, 13))
+
+
+def test_gather_without_room_for_the_scores():
+    """A table that could address so many keys that few-row scores are not kept: recomputed, the same sums."""
+    r = Ragged([1, 3], [700, 90], 8, 2, 64, 4096, BF16, seed=6)
+    w0 = r.w.clone()
+    r.attend(gather=True)
+    kept = r.w.clone()
+    r.w.copy_(w0)
+    r.table = torch.cat([r.table, torch.full((2, 4000), -1, dtype=torch.int32, device=DEV)], 1)
+    o, lse = r.attend(gather=True)
+    r.check(o, lse, w0=w0)
+    p, s = r.places(0)
+    # both are sums of 8 probabilities of a key, each within its own bound of the exact ones
+    assert bool(((r.w - kept)[p, :, s].abs() <= 1e-4 * kept[p, :, s] + 1e-6).all())
+
+
 @pytest.mark.parametrize("dim,page", [(128, 16), (64, 32), (40, 16)])
 @pytest.mark.parametrize("gather", [False, True])
 def test_rows_that_see_nothing(dim, page, gather):
@@ -471,7 +511,9 @@ def test_evict_keeps_the_heaviest(kv, hk, dim, page, budget, recent, dtype, weig
     k, v, w = grow(r.k), grow(r.v), grow(r.w)
     wk, wv, ww = k.clone(), v.clone(), w.clone()
     new = _ints(rows)
-    kept, new_len = paged_evict(k, v, w, r.table, r.kv_len, max(kv), new, budget, recent)
+    # the host's idea of the largest kv_len shapes the launch only
+    stated = max(kv) if weights != "ties" else min(max(kv), budget, width * page) // 3
+    kept, new_len = paged_evict(k, v, w, r.table, r.kv_len, stated, new, budget, recent)
     assert new_len.tolist() == m
     for b, n in enumerate(kv):
         p, s = r.places(b)
