@@ -72,7 +72,6 @@ def _tables(name: str, cos: Optional[Tensor], sin: Optional[Tensor], positions: 
                  and t.is_contiguous(), name,
                  f"{what} must be a contiguous float32 [positions, rotated / 2] table on {device}, got {t.dtype} "
                  f"{list(t.shape)} on {t.device}")
-        _require(not (t.requires_grad and torch.is_grad_enabled()), name, f"{what} has no gradient")
     rows, half = int(cos.shape[0]), int(cos.shape[1])
     _require(2 * half <= dim, name, f"tables for {2 * half} channels of {dim}")
     _require(rows > 0 or tokens == 0 or half == 0, name, "tables without positions")
@@ -195,6 +194,8 @@ def rotary_embed(x: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor
     ``2 * cos.shape[1]`` channels of every head rotated by their token's position, the others copied. Pairs are
     (2i, 2i + 1) with ``interleaved``, else (i, i + half). ``positions``: int32 [tokens] rows of the tables (held inside
     them), or None for 0, 1, 2, ... ``inverse`` rotates back. Computed in fp32, rounded once; differentiable in x."""
+    _require(not torch.is_grad_enabled() or not (cos is not None and cos.requires_grad or sin is not None
+                                                 and sin.requires_grad), "rotary_embed", "the tables have no gradient")
     host = _host()
     if host is not None:
         y = host.rotary_embed(x, cos, sin, positions, interleaved, inverse)

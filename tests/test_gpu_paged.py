@@ -639,7 +639,8 @@ def test_native_host_calls_and_python_bodies_agree(monkeypatch):
                     lambda: paged.rotary_embed(r.q, cos, sin, at.long()), lambda: r.attend(q=r.q[:, :3]),
                     lambda: paged.paged_write(r.q, r.q, r.q, cos, sin, at, r.k, r.v, r.table, r.q_start, r.kv_len),
                     lambda: paged.paged_evict(r.k, r.v, r.w, r.table, r.kv_len, 700, new, 4, 5),
-                    lambda: paged.rotary_embed(r.q, None, None)):
+                    lambda: paged.rotary_embed(r.q, None, None),
+                    lambda: paged.rotary_embed(r.q, cos.clone().requires_grad_(True), sin)):
             with pytest.raises(ValueError):
                 bad()
         return out
