@@ -300,9 +300,12 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t mine, uint32_t* cells, ui
 // mantissa, so weights of one magnitude still spread over several counters); keys above it and, from the lowest
 // slot on, as many equal to it as are still wanted are kept. Each wave owns a run of slots, so that after one sum
 // over the waves every wave knows where its kept slots go: `kept` ascends and no order depends on timing. Bound by
-// latency: the first EV_HELD ranks are read once, 8 loads of a thread in flight, and held in LDS for all passes (32768 keys
-// read again in every pass took 76 us; held in registers, whose passes are unrolled code, 38 us and 13 for 640 keys).
+// latency and, at many keys, by the few instructions a key takes on one CU: the first EV_HELD ranks are read once, up to
+// 16 loads of a thread in flight, and held in LDS for all passes (32768 keys read again in every pass took 76 us; held in
+// registers, whose passes are unrolled code, 38 us and 13 for 640 keys). EV_AHEAD LDS reads go before what a pass does
+// with them (2 us of 30 over one at a time; 8 and 16 the same).
 constexpr int EV_HELD = 32768;
+constexpr int EV_AHEAD = 4;
 
 __global__ __launch_bounds__(EV_THREADS) void evict_select_kernel(PagedArgs c, int budget, int recent, int held,
                                                                   int32_t* kept, int32_t* new_len) {
@@ -320,95 +323,96 @@ __global__ __launch_bounds__(EV_THREADS) void evict_select_kernel(PagedArgs c, i
     return;
   }
   const int32_t* row = c.table + b * c.table_stride;
-  const int first = n - recent;  // keys before the recent ones: more than budget - recent of them
-  const int run = ((n + EV_WAVES - 1) / EV_WAVES + 63) & ~63;
-  const int j0 = min(wave * run, n), j1 = min(j0 + run, n);
-  // rank of slot j < n, out of LDS for the first `held` slots; those of recent keys are never looked at
+  // Only the `first` keys before the recent ones are ranked: more than budget - recent of them. Rank 0, which no
+  // weight has, fills their last 64 slots up.
+  const int first = n - recent, padded = (first + 63) & ~63;
+  for (int i = tid; i < recent; i += EV_THREADS) out[budget - recent + i] = first + i;
+  uint32_t want = (uint32_t)(budget - recent);
+  if (want == 0) return;
+  const int run = ((first + EV_WAVES - 1) / EV_WAVES + 63) & ~63;
+  const int j0 = min(wave * run, padded), j1 = min(j0 + run, padded);
   auto rank_of = [&](int j) __attribute__((always_inline)) {
-    return weight_rank(c.w[paged_w_at(c, paged_page(c, row, j), h, j)]);
+    const int at = min(j, first - 1);
+    const uint32_t u = weight_rank(c.w[paged_w_at(c, paged_page(c, row, at), h, at)]);
+    return j < first ? u : 0;
   };
-  const int in_lds = min(n, held);
+  const int in_lds = min(padded, held);
   auto fill = [&](auto group_c) __attribute__((always_inline)) {  // a step's loads all in flight together
     constexpr int G = decltype(group_c)::value;
     for (int j = tid; j < in_lds; j += G * EV_THREADS) {
       int page[G];
       float w[G];
 #pragma unroll
-      for (int k = 0; k < G; ++k) page[k] = paged_page(c, row, min(j + k * EV_THREADS, in_lds - 1));
+      for (int k = 0; k < G; ++k) page[k] = paged_page(c, row, min(j + k * EV_THREADS, first - 1));
 #pragma unroll
-      for (int k = 0; k < G; ++k) w[k] = c.w[paged_w_at(c, page[k], h, min(j + k * EV_THREADS, in_lds - 1))];
+      for (int k = 0; k < G; ++k) w[k] = c.w[paged_w_at(c, page[k], h, min(j + k * EV_THREADS, first - 1))];
 #pragma unroll
       for (int k = 0; k < G; ++k)
-        if (j + k * EV_THREADS < in_lds) ranks[j + k * EV_THREADS] = weight_rank(w[k]);
+        if (j + k * EV_THREADS < in_lds) ranks[j + k * EV_THREADS] = j + k * EV_THREADS < first ? weight_rank(w[k]) : 0;
     }
   };
   if (in_lds > 4 * EV_THREADS) fill(std::integral_constant<int, 16>{});
   else fill(std::integral_constant<int, 2>{});
   // f(slot of the wave's first lane, the lane's rank) over the wave's run, 64 slots at a time
   auto each = [&](auto f) __attribute__((always_inline)) {
-    const int mid = min(j1, in_lds / 64 * 64);
+    const int mid = min(j1, in_lds);
     int j = j0;
-#pragma unroll 4
-    for (; j < mid; j += 64) f(j, ranks[j + lane]);
-    for (; j < j1; j += 64) {
-      const int at = min(j + lane, n - 1);
-      f(j, at < in_lds ? ranks[at] : rank_of(at));
+    for (; j + 64 * EV_AHEAD <= mid; j += 64 * EV_AHEAD) {
+      uint32_t u[EV_AHEAD];
+#pragma unroll
+      for (int k = 0; k < EV_AHEAD; ++k) u[k] = ranks[j + 64 * k + lane];
+#pragma unroll
+      for (int k = 0; k < EV_AHEAD; ++k) f(j + 64 * k, u[k]);
     }
+    for (; j < mid; j += 64) f(j, ranks[j + lane]);
+    for (; j < j1; j += 64) f(j, rank_of(j + lane));
   };
 
-  uint32_t want = (uint32_t)(budget - recent), prefix = 0;
+  uint32_t prefix = 0;
   int shift = 21;
-  if (want > 0) {
-    for (int pass = 0; pass < 3; ++pass) {
-      const int bits = pass == 2 ? 10 : 11;
-      for (int i = tid; i < EV_BINS; i += EV_THREADS) bins[i] = 0;
-      __syncthreads();
-      each([&](int j, uint32_t u) __attribute__((always_inline)) {
-        if (j + lane < min(first, j1) && (pass == 0 || (u >> (shift + bits)) == prefix))
-          atomicAdd(&bins[(u >> shift) & ((1u << bits) - 1)], 1u);
-      });
-      __syncthreads();
-      // counters from the top, two a thread: the one at which the count reaches `want`
-      const int i1 = EV_BINS - 1 - 2 * tid, i0 = i1 - 1;
-      const uint32_t c1 = bins[i1], c0 = bins[i0];
-      uint32_t inc = c1 + c0;
-      for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t x = __shfl_up(inc, o);
-        if (lane >= o) inc += x;
-      }
-      uint32_t all;
-      const uint32_t last = __shfl(inc, 63);
-      const uint32_t above = wave_scan(last, cells, all) + inc - c1 - c0;
-      if (above < want && above + c1 >= want) found[0] = (uint32_t)i1, found[1] = above;
-      if (above + c1 < want && above + c1 + c0 >= want) found[0] = (uint32_t)i0, found[1] = above + c1;
-      __syncthreads();
-      prefix = (prefix << bits) | found[0];
-      want -= found[1];  // still wanted among the keys of this prefix
-      shift = pass == 0 ? 10 : 0;
-      __syncthreads();
+  for (int pass = 0; pass < 3; ++pass) {
+    const int bits = pass == 2 ? 10 : 11;
+    for (int i = tid; i < EV_BINS; i += EV_THREADS) bins[i] = 0;
+    __syncthreads();
+    // a slot of rank 0 counts below every key, so the place looked for never lies on one
+    each([&](int, uint32_t u) __attribute__((always_inline)) {
+      if (pass == 0 || (u >> (shift + bits)) == prefix) atomicAdd(&bins[(u >> shift) & ((1u << bits) - 1)], 1u);
+    });
+    __syncthreads();
+    // counters from the top, two a thread: the one at which the count reaches `want`
+    const int i1 = EV_BINS - 1 - 2 * tid, i0 = i1 - 1;
+    const uint32_t c1 = bins[i1], c0 = bins[i0];
+    uint32_t inc = c1 + c0;
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t x = __shfl_up(inc, o);
+      if (lane >= o) inc += x;
     }
-  } else {
-    prefix = 0xffffffffu;  // nothing but the recent keys: no rank is above it, and no equal one is wanted
+    uint32_t all;
+    const uint32_t last = __shfl(inc, 63);
+    const uint32_t above = wave_scan(last, cells, all) + inc - c1 - c0;
+    if (above < want && above + c1 >= want) found[0] = (uint32_t)i1, found[1] = above;
+    if (above + c1 < want && above + c1 + c0 >= want) found[0] = (uint32_t)i0, found[1] = above + c1;
+    __syncthreads();
+    prefix = (prefix << bits) | found[0];
+    want -= found[1];  // still wanted among the keys of this prefix
+    shift = pass == 0 ? 10 : 0;
+    __syncthreads();
   }
-  // now: of the keys before the recent ones, those ranked above `prefix` are kept (none where nothing is wanted: the
-  // highest rank is), and the first `want` equal to it
-  const int o1 = min(j1, first);  // the run's end among them
-  uint32_t above = 0, equal = 0;  // by lane
-  each([&](int j, uint32_t u) __attribute__((always_inline)) {
-    const bool old = j + lane < o1;
-    above += old && u > prefix;
-    equal += old && u == prefix;
+  // now: the keys ranked above `prefix` are kept, and the first `want` equal to it
+  uint32_t above = 0, equal = 0;  // of the wave's run
+  each([&](int, uint32_t u) __attribute__((always_inline)) {
+    above += (uint32_t)__popcll(__ballot(u > prefix));
+    equal += (uint32_t)__popcll(__ballot(u == prefix));
   });
-#pragma unroll
-  for (int w = 32; w; w >>= 1) above += __shfl_xor(above, w), equal += __shfl_xor(equal, w);
   uint32_t all;
   uint32_t eq = wave_scan(equal, cells, all);  // equal ones before this wave's run, of which at most `want` are kept
-  uint32_t at = wave_scan(above + (uint32_t)(j1 - max(o1, j0)), cells, all) + min(eq, want);
-  auto lanes_below = [](uint64_t m) { return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0)); };
+  uint32_t at = wave_scan(above, cells, all) + min(eq, want);
+  auto lanes_below = [](uint64_t m) __attribute__((always_inline)) {
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+  };
   each([&](int j, uint32_t u) __attribute__((always_inline)) {
-    const bool old = j + lane < o1, recent_key = j + lane >= first && j + lane < j1;
-    bool keep = (old && u > prefix) || recent_key;
-    const uint64_t eqs = __ballot(old && u == prefix);
+    bool keep = u > prefix;
+    const uint64_t eqs = __ballot(u == prefix);
     if (eqs) {  // the same for the whole wave
       keep |= (eqs >> lane & 1) && eq + lanes_below(eqs) < want;
       eq += __popcll(eqs);
@@ -466,7 +470,7 @@ extern "C" int gwa_paged_evict(const gwa_paged_cache* cache, const int32_t* new_
   const int64_t blocks = (std::max<int64_t>(most, 1) * pieces + EC_THREADS - 1) / EC_THREADS;
   GWA_REQUIRE(groups < 65536 && blocks < (1ll << 31), "%s: %lld heads of sequences are too many", what,
               (long long)groups);
-  const int held = (int)(max_kv < EV_HELD ? max_kv : EV_HELD);
+  const int held = (int)std::min<int64_t>((max_kv + 63) / 64 * 64, EV_HELD);
   hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)groups), dim3(EV_THREADS), (size_t)held * 4,
                      (hipStream_t)stream, c, (int)budget, (int)recent, held, kept, new_len);
   const int rc = gwa_check_launch(what);
