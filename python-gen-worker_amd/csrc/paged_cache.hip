@@ -301,15 +301,16 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t mine, uint32_t* cells, ui
 // slot on, as many equal to it as are still wanted are kept. Each wave owns a run of slots, so that after one sum
 // over the waves every wave knows where its kept slots go: `kept` ascends and no order depends on timing. Bound by
 // latency and, at many keys, by the few instructions a key takes on one CU: the first EV_HELD ranks are read once, up to
-// 16 loads of a thread in flight, and held in LDS for all passes (32768 keys read again in every pass took 76 us; held in
-// registers, whose passes are unrolled code, 38 us and 13 for 640 keys). EV_AHEAD LDS reads go before what a pass does
-// with them (2 us of 30 over one at a time; 8 and 16 the same).
+// 8 loads of 4 slots a thread in flight (24.9 -> 21.5 us over 16 of one slot, at 8 caches of 32768), and held in LDS for
+// all passes (read again in every pass they took 76 us, held in registers, whose passes are unrolled code, 38 us and
+// 13 for 640 keys). EV_AHEAD LDS reads go before what a pass does with them (2 us of 30 over one at a time; 8 and 16
+// the same).
 constexpr int EV_HELD = 32768;
 constexpr int EV_AHEAD = 4;
 
 __global__ __launch_bounds__(EV_THREADS) void evict_select_kernel(PagedArgs c, int budget, int recent, int held,
                                                                   int32_t* kept, int32_t* new_len) {
-  extern __shared__ uint32_t ranks[];  // held
+  extern __shared__ __attribute__((aligned(16))) uint32_t ranks[];  // held
   __shared__ uint32_t bins[EV_BINS];
   __shared__ uint32_t cells[EV_WAVES];
   __shared__ uint32_t found[2];
@@ -337,22 +338,30 @@ __global__ __launch_bounds__(EV_THREADS) void evict_select_kernel(PagedArgs c, i
     return j < first ? u : 0;
   };
   const int in_lds = min(padded, held);
-  auto fill = [&](auto group_c) __attribute__((always_inline)) {  // a step's loads all in flight together
+  // a thread takes 4 neighbouring slots, which lie in one page (page_size >= 8), G times, all of them in flight together
+  auto fill = [&](auto group_c) __attribute__((always_inline)) {
     constexpr int G = decltype(group_c)::value;
-    for (int j = tid; j < in_lds; j += G * EV_THREADS) {
-      int page[G];
-      float w[G];
+    typedef float v4u __attribute__((ext_vector_type(4), aligned(4)));
+    for (int j = 4 * tid; j < in_lds; j += 4 * G * EV_THREADS) {
+      int from[G], page[G];
+      v4u w[G];
 #pragma unroll
-      for (int k = 0; k < G; ++k) page[k] = paged_page(c, row, min(j + k * EV_THREADS, first - 1));
+      for (int k = 0; k < G; ++k) from[k] = min(j + 4 * k * EV_THREADS, (first - 1) & ~3), page[k] = paged_page(c, row, from[k]);
 #pragma unroll
-      for (int k = 0; k < G; ++k) w[k] = c.w[paged_w_at(c, page[k], h, min(j + k * EV_THREADS, first - 1))];
+      for (int k = 0; k < G; ++k) w[k] = *(const v4u*)(c.w + paged_w_at(c, page[k], h, from[k]));
 #pragma unroll
-      for (int k = 0; k < G; ++k)
-        if (j + k * EV_THREADS < in_lds) ranks[j + k * EV_THREADS] = j + k * EV_THREADS < first ? weight_rank(w[k]) : 0;
+      for (int k = 0; k < G; ++k) {
+        const int s = j + 4 * k * EV_THREADS;
+        if (s >= in_lds) break;
+        v4i u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[i] = s + i < first ? (int)weight_rank(w[k][i]) : 0;
+        *(v4i*)(ranks + s) = u;
+      }
     }
   };
-  if (in_lds > 4 * EV_THREADS) fill(std::integral_constant<int, 16>{});
-  else fill(std::integral_constant<int, 2>{});
+  if (in_lds > 4 * EV_THREADS) fill(std::integral_constant<int, 8>{});
+  else fill(std::integral_constant<int, 1>{});
   // f(slot of the wave's first lane, the lane's rank) over the wave's run, 64 slots at a time
   auto each = [&](auto f) __attribute__((always_inline)) {
     const int mid = min(j1, in_lds);

@@ -528,6 +528,26 @@ def test_evict_keeps_the_heaviest(kv, hk, dim, page, budget, recent, dtype, weig
     assert same(k, wk) and same(v, wv) and same(w, ww)
 
 
+@pytest.mark.parametrize("n,recent", [(41, 0), (41, 3), (5003, 70)])
+def test_evict_reads_weights_of_any_stride(n, recent):
+    """Heads and pages of the weights an odd number of elements apart, from an odd one on."""
+    from gen_worker_amd.paged import paged_evict
+
+    page, budget, hk = 8, 20 + recent, 3
+    r = Ragged([0], [n], hk, hk, 64, page, BF16, seed=n, extra_pages=0)
+    pages, m = r.k.shape[0], min(n, budget)
+    count = -(-m // page)
+    grow = lambda t: torch.cat([t, torch.zeros((count,) + t.shape[1:], dtype=t.dtype, device=DEV)])  # noqa: E731
+    w = torch.full((pages + count, hk, page + 1), float("inf"), device=DEV)[:, :, 1:]
+    w.copy_(torch.rand(w.shape, generator=_gen(n), device=DEV))
+    before = w.clone()
+    new = _ints([list(range(pages, pages + count))])
+    kept, _ = paged_evict(grow(r.k), grow(r.v), w, r.table, r.kv_len, n, new, budget, recent)
+    p, s = r.places(0)
+    for h in range(hk):
+        assert kept[0, h].tolist() == _evict_reference(before[p, h, s].tolist(), n, budget, recent), h
+
+
 # ---------------------------------------------------------------------------
 # the ops, and the cache that ties them together
 # ---------------------------------------------------------------------------
