@@ -307,7 +307,7 @@ __global__ __launch_bounds__(QF_THREADS) void svdq_quant_int4_rows_kernel(
 constexpr int Q6_WAVES = 4, Q6_THREADS = 64 * Q6_WAVES, Q6_ROWS = 16 * Q6_WAVES;
 
 __device__ __forceinline__ void dma16_lds(v4i rsrc, uint32_t lds_addr, uint32_t voff, uint32_t soff) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :
                : "s"(lds_addr), "v"(voff), "s"(rsrc), "s"(soff)
                : "memory", "m0");

@@ -44,9 +44,12 @@ constexpr int kUnitE8M0 = 127;             // 2^0
 // LDS read) leaves the waits to the kernel: every LDS read of a stage buffer
 // comes after an s_waitcnt that covers this wave's copies into it and a
 // barrier that covers everyone else's. The "memory" clobber keeps the copy
-// in program order with the surrounding LDS accesses.
+// in program order with the surrounding LDS accesses. A load to LDS may issue
+// one wait state after the write of M0 at the earliest; the compiler keeps
+// that distance for its own loads, not inside an asm, so the s_nop does (all
+// asm copies are written so).
 __device__ __forceinline__ void dma16(v4i rsrc, uint32_t lds_addr, uint32_t voff, uint32_t soff) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :
                : "s"(lds_addr), "v"(voff), "s"(rsrc), "s"(soff)
                : "memory", "m0");

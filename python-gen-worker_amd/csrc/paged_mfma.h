@@ -51,11 +51,11 @@ __device__ __forceinline__ int64_t uniform64(int64_t x) {
 // (a 64-bit address: pools pass 4 GiB). As asm for dma16's reason: the waits are the kernel's, so the compiler's wait
 // counts must not include it.
 __device__ __forceinline__ void copy16(uint32_t lds_addr, const void* base, uint32_t off) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds_addr), "v"(off), "s"(base) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds_addr), "v"(off), "s"(base) : "memory", "m0");
 }
 // the same from an address of the lane's own
 __device__ __forceinline__ void copy16(uint32_t lds_addr, const void* p) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds_addr), "v"(p) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds_addr), "v"(p) : "memory", "m0");
 }
 
 __device__ __forceinline__ v4s_ lds_read_tr(const uint8_t* p) {

@@ -31,7 +31,7 @@ __device__ __forceinline__ int l_swz(int r) { return (r >> 1) & 7; }
 // Direct-to-LDS copy of 16 bytes per lane at 64-bit lane addresses: LDS [lds_addr + 16 lane, +16) <- src. Every
 // lane's source must be readable; waits are the kernel's (as for dma16).
 __device__ __forceinline__ void dma16_at(uint32_t lds_addr, const uint8_t* src) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds_addr), "v"(src) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds_addr), "v"(src) : "memory", "m0");
 }
 
 // wait until at most min(newer, most) stages of `copies` copies each are still in flight (and no LDS read)
