@@ -473,7 +473,10 @@ PyObject* rotary_embed(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// the C interface's cache of fitting tensors
+// whether a table's rows lie apart; of a single row the stride is not read
+bool rows_apart(const Tensor& t) { return t.size(0) < 2 || t.stride(0) >= t.size(1); }
+
+// the C interface's cache of fitting tensors; overlapping rows of page ids are copied in Python
 bool cache_fits(const Tensor& k, const Tensor& v, const Tensor& w, const Tensor& table, const Tensor& q_start,
                 const Tensor& kv_len, gwa_paged_cache& c) {
   const at::Device dev = k.device();
@@ -483,7 +486,7 @@ bool cache_fits(const Tensor& k, const Tensor& v, const Tensor& w, const Tensor&
       kv_len.dim() != 1 || table.dim() != 2)
     return false;
   const int64_t batch = kv_len.size(0);
-  if (!ints_on(kv_len, dev, {batch}) || !ints_on(table, dev, {batch, table.size(1)}) ||
+  if (!ints_on(kv_len, dev, {batch}) || !ints_on(table, dev, {batch, table.size(1)}) || !rows_apart(table) ||
       (q_start.defined() && !ints_on(q_start, dev, {batch + 1})))
     return false;
   if (w.defined() && (w.scalar_type() != at::kFloat || w.layout() != at::kStrided || w.device() != dev ||
@@ -603,7 +606,7 @@ PyObject* paged_evict(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     gwa_paged_cache c;
     if (budget > 0 && recent >= 0 && recent <= budget && next.dim() == 2 &&
         cache_fits(t[0], t[1], t[2], t[3], Tensor(), t[4], c) &&
-        ints_on(next, t[0].device(), {c.batch, next.size(1)})) {
+        ints_on(next, t[0].device(), {c.batch, next.size(1)}) && rows_apart(next)) {
       kept = empty_like_device({c.batch, c.kv_heads, budget}, at::kInt, next);
       len = empty_like_device({c.batch}, at::kInt, next);
       if (g_abi.paged_evict(&c, address<int32_t>(next), std::max(next.stride(0), next.size(1)), next.size(1), max_kv,

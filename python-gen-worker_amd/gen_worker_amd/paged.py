@@ -80,6 +80,14 @@ def _tables(name: str, cos: Optional[Tensor], sin: Optional[Tensor], positions: 
     return 2 * half, rows
 
 
+def _spaced(table: Tensor) -> tuple[Tensor, int]:
+    """A table of page ids and its row stride as the library takes them. Rows that overlap (``expand``: sequences that read
+    the same pages) are copied apart; of a single row the stride is not read."""
+    if table.shape[0] > 1 and table.stride(0) < table.shape[1]:
+        table = table.contiguous()
+    return table, max(table.stride(0), table.shape[1])
+
+
 def _host():
     """The native host calls, which make these calls in a few microseconds; None while the library is not loaded,
     without them, and under compilation. Theirs return None for whatever the Python way has to decide or refuse."""
@@ -234,10 +242,13 @@ def _cache_args(name: str, k_pages: Tensor, v_pages: Tensor, weights: Optional[T
                  f"weights must be float32 {[pages, heads, size]} on {dev} with unit last stride, got {weights.dtype} "
                  f"{list(weights.shape)} strides {weights.stride()} on {weights.device}")
         ws = weights.stride()
-    return nat.PagedCacheArgs(k_pages.data_ptr(), v_pages.data_ptr(), nat.ptr(weights), table.data_ptr(),
+    table, row = _spaced(table)
+    args = nat.PagedCacheArgs(k_pages.data_ptr(), v_pages.data_ptr(), nat.ptr(weights), table.data_ptr(),
                               nat.ptr(q_start), kv_len.data_ptr(), k_pages.stride(0), k_pages.stride(1),
-                              k_pages.stride(2), ws[0], ws[1], pages, max(table.stride(0), table.shape[1]),
-                              table.shape[1], batch, size, heads, dim, _DTYPES[k_pages.dtype])
+                              k_pages.stride(2), ws[0], ws[1], pages, row, table.shape[1], batch, size, heads, dim,
+                              _DTYPES[k_pages.dtype])
+    args.table_kept = table  # a copy lives until the call has been made
+    return args
 
 
 def _write_body(q: Tensor, k: Tensor, v: Tensor, cos: Optional[Tensor], sin: Optional[Tensor],
@@ -361,6 +372,8 @@ def _evict_body(k_pages: Tensor, v_pages: Tensor, weights: Tensor, table: Tensor
     dev = k_pages.device
     _require(budget > 0 and 0 <= recent <= budget, name, f"a budget of {budget} keys, {recent} of them recent")
     _ints(name, "new_table", new_table, (args.batch, new_table.shape[-1] if new_table.dim() == 2 else -1), dev)
+    _require(args.batch < 2 or new_table.stride(0) >= new_table.shape[1], name,
+             f"new_table's rows overlap (row stride {new_table.stride(0)}): sequences would be copied into one page")
     kept = torch.empty((args.batch, args.kv_heads, budget), dtype=torch.int32, device=dev)
     new_len = torch.empty(args.batch, dtype=torch.int32, device=dev)
     nat.call("gwa_paged_evict", ctypes.byref(args), new_table.data_ptr(), max(new_table.stride(0), new_table.shape[1]),

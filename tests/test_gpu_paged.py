@@ -673,3 +673,47 @@ def test_native_host_calls_and_python_bodies_agree(monkeypatch):
     (dx,) = torch.autograd.grad(paged.rotary_embed(x, cos, sin).square().sum(), x)
     # the rotation keeps lengths: d |y|^2 / dx = 2 x, to rounding of two rotations of values below 6
     assert bool(((dx - 2 * x).abs() <= 64 * E * 6).all())
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_sequences_that_share_a_row_of_the_table(native, monkeypatch):
+    """A table made with expand, all of whose rows are one (and a strided one whose rows overlap): what its contiguous copy
+    gives, bit for bit; an expanded target of an eviction is refused."""
+    from gen_worker_amd import ops
+    from gen_worker_amd.paged import PagedError, paged_attention, paged_evict, paged_write
+
+    if not native:
+        monkeypatch.setattr(ops, "_host", None)
+    r = Ragged([40], [700], 4, 2, 64, 16, BF16, seed=31)
+    for n_seq, each in ((8, 1), (3, 40)):
+        tokens = n_seq * each
+        q = torch.randn(tokens, 4, 64, generator=r.g, device=DEV).to(BF16)
+        start = torch.arange(0, tokens + 1, each, device=DEV, dtype=torch.int32)
+        lens = _ints([700 - 3 * i for i in range(n_seq)])
+        shared = r.table[:1].expand(n_seq, r.table.shape[1])
+        sliding = torch.cat([r.table[0]] * 2).as_strided((n_seq, r.table.shape[1]), (1, 1))
+        for table in (shared, sliding):
+            got = paged_attention(q, r.k, r.v, table, start, lens, each, 700)
+            want = paged_attention(q, r.k, r.v, table.contiguous(), start, lens, each, 700)
+            # (shifted rows show slots behind the history's end, which hold NaN)
+            assert all(torch.equal(a.nan_to_num(), b.nan_to_num()) for a, b in zip(got, want))
+            assert table is sliding or bool(torch.isfinite(got[0]).all())
+    # two sequences of one history; the second alone takes new tokens
+    k = torch.randn(3, 2, 64, generator=r.g, device=DEV).to(BF16)
+    q = torch.randn(3, 4, 64, generator=r.g, device=DEV).to(BF16)
+    table, pools = r.table[:1].expand(2, r.table.shape[1]), []
+    for t in (table, table.contiguous()):
+        kp, vp = r.k.clone(), r.v.clone()
+        paged_write(q, k, k, None, None, None, kp, vp, t, _ints([0, 0, 3]), _ints([600, 700]))
+        pools.append((kp, vp))
+    assert all(torch.equal(a.nan_to_num(), b.nan_to_num()) for a, b in zip(*pools))
+    p, s = r.places(0)
+    assert torch.equal(pools[0][0][p[697:], :, s[697:]], k)
+    w = torch.rand(r.w.shape, generator=r.g, device=DEV)
+    outs, new = [], _ints([[0, 1, 2], [3, 4, 5]]) + r.k.shape[0]
+    for t in (table, table.contiguous()):
+        pool = [torch.cat([x, torch.zeros_like(x[:6])]) for x in (r.k, r.v, w)]
+        outs.append([*paged_evict(*pool, t, _ints([700, 650]), 700, new, 40, 4), *pool])
+    assert all(torch.equal(a.nan_to_num(), b.nan_to_num()) for a, b in zip(*outs))
+    with pytest.raises(PagedError, match="overlap"):
+        paged_evict(*pool, table, _ints([700, 650]), 700, new[:1].expand(2, 3), 40, 4)

@@ -174,3 +174,20 @@ def test_cache_bookkeeping():
     assert c.free_pages == 6
     with pytest.raises(KeyError):
         c.length(b)
+
+
+def test_tables_whose_rows_overlap_are_copied_apart():
+    """The row stride that the library gets is one at which every row lies inside the table's own storage."""
+    p = _paged()
+    wide = torch.arange(40, dtype=torch.int32).view(5, 8)
+    for table in (wide[:1].expand(6, 8), wide.view(-1).as_strided((6, 8), (3, 1)), wide[:1, :1].expand(4, 1), wide,
+                  wide[:, 2:5], wide[:1], wide[:1].expand(1, 8), wide[:, :0], wide[:0], wide[0:1, 0:3].expand(3, 3)):
+        got, row = p._spaced(table)
+        rows, width = table.shape
+        assert row >= width and torch.equal(got, table)
+        if rows and width:
+            end = got.storage_offset() + (rows - 1) * row + width
+            assert end <= got.untyped_storage().nbytes() // 4
+            assert torch.equal(got.as_strided((rows, width), (row, 1)), table)
+    # nothing is copied that need not be
+    assert p._spaced(wide[:, 2:5])[0].data_ptr() == wide[:, 2:5].data_ptr()
