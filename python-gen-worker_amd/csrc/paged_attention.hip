@@ -602,6 +602,19 @@ __global__ __launch_bounds__(256) void paged_attn_join_parts_kernel(AttnArgs a) 
 // their join before the shares); one sequence of 701 keys, 32 heads over 8, 9 us and 3 for the join: launch and four dependent loads.
 constexpr int FW_KEYS = 32, FW_PAGES = 512;  // keys a tile; page ids staged at a time (whole tiles: page_size >= 8)
 constexpr int FW_WAVES = 4, FW_UNIT = FW_KEYS * FW_WAVES;
+// Where the segment of a run that starts at key s_lo ends, at k_hi at the latest: behind the FW_PAGES-th page from that of
+// s_lo on, which may lie inside its page (runs start at multiples of 128 keys, pages hold up to 4096). The next
+// segment starts on a page, whole tiles later.
+constexpr __host__ __device__ int segment_end(int s_lo, int k_hi, int page_shift) {
+  const int end = ((s_lo >> page_shift) + FW_PAGES) << page_shift;
+  return end < k_hi ? end : k_hi;
+}
+constexpr bool segment_fits(int s_lo, int k_hi, int page_shift) {
+  const int end = segment_end(s_lo, k_hi, page_shift);
+  return ((end - 1) >> page_shift) - (s_lo >> page_shift) < FW_PAGES && (end == k_hi || (end - s_lo) % FW_KEYS == 0);
+}
+static_assert(segment_fits(0, 1 << 30, 3) && segment_fits(128, 1 << 30, 4) && segment_fits(128, 1 << 30, 8) &&
+              segment_fits(256, 1 << 30, 9) && segment_fits(384, 131200, 8) && segment_fits(128 * 33, 1 << 30, 12));
 
 template <int D, int RB>
 struct FewShape {
@@ -677,9 +690,9 @@ __global__ __launch_bounds__(64 * FW_WAVES) void paged_attn_few_kernel(AttnArgs 
       for (int db = 0; db < S::kND; ++db) oacc[rb][db] = (v4f){};
     }
 
-    const int seg_keys = FW_PAGES << c.page_shift;  // keys whose page ids are staged at a time
-    for (int s_lo = k_lo; s_lo < k_hi; s_lo += seg_keys) {
-      const int s_hi = min(s_lo + seg_keys, k_hi), p0 = s_lo >> c.page_shift;
+    for (int s_lo = k_lo, s_hi; s_lo < k_hi; s_lo = s_hi) {  // keys whose page ids are staged at a time
+      const int p0 = s_lo >> c.page_shift;
+      s_hi = segment_end(s_lo, k_hi, c.page_shift);
       if (s_lo > k_lo) __syncthreads();  // the ids of the last segment are no longer read
       for (int i = tid; i <= ((s_hi - 1) >> c.page_shift) - p0; i += 64 * NW)
         page_ids[i] = min(max(pages[p0 + i], 0), c.pages - 1);

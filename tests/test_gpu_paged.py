@@ -717,3 +717,15 @@ def test_sequences_that_share_a_row_of_the_table(native, monkeypatch):
     assert all(torch.equal(a.nan_to_num(), b.nan_to_num()) for a, b in zip(*outs))
     with pytest.raises(PagedError, match="overlap"):
         paged_evict(*pool, table, _ints([700, 650]), 700, new[:1].expand(2, 3), 40, 4)
+
+
+@pytest.mark.parametrize("q,kv,dim,page,max_kv,gather", [
+    # two runs of one sequence, the second from key 256 of 512-slot pages on; 32 shares of 137 thousand keys, most of which
+    # start inside their page
+    ([1], [270003], 128, 512, 512, False), ([2], [270003], 64, 512, 512, True), ([1], [4400001], 64, 256, None, False)])
+def test_runs_that_start_inside_a_page_and_pass_the_staged_ids(q, kv, dim, page, max_kv, gather):
+    """More pages to a run of keys than the kernel stages at a time, from the middle of a page on."""
+    r = Ragged(q, kv, 2, 1, dim, page, BF16, seed=17)
+    w0 = r.w.clone() if gather else None
+    o, lse = r.attend(max_kv=max_kv, gather=gather)
+    r.check(o, lse, w0=w0)
