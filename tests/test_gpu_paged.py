@@ -729,3 +729,41 @@ def test_runs_that_start_inside_a_page_and_pass_the_staged_ids(q, kv, dim, page,
     w0 = r.w.clone() if gather else None
     o, lse = r.attend(max_kv=max_kv, gather=gather)
     r.check(o, lse, w0=w0)
+
+
+# one run of all of a sequence's keys (the host states one key), longer than the page ids staged at a time
+LONG_RUNS = [([1], [5003], 4, 1, 128, 8, BF16), ([6, 3], [8197, 5003], 4, 2, 64, 8, F16), ([8], [8197], 4, 2, 128, 8, BF16),
+             ([5], [16400], 6, 1, 64, 16, BF16), ([4, 0, 7], [8193, 70, 4097], 4, 1, 128, 8, F16)]
+
+
+@pytest.mark.parametrize("q,kv,heads,hk,dim,page,dtype", LONG_RUNS)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("gather", [False, True])
+def test_few_rows_over_more_pages_than_are_staged_at_once(q, kv, heads, hk, dim, page, dtype, causal, gather):
+    r = Ragged(q, kv, heads, hk, dim, page, dtype, seed=sum(kv))
+    w0 = r.w.clone() if gather else None
+    o, lse = r.attend(causal=causal, gather=gather, max_q=max(q), max_kv=1)
+    r.check(o, lse, causal, w0=w0)
+
+
+@pytest.mark.parametrize("q,kv,heads,hk,dim,page,dtype", LONG_RUNS[1:])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_nonfinite_values_behind_the_mask_of_a_late_segment(q, kv, heads, hk, dim, page, dtype, bad):
+    """NaN or infinities in the last two tokens' values, in the second or third segment of staged pages: rows that do not
+    see them are as if they were finite, rows that do are not finite in their channel and unchanged in the others."""
+    r = Ragged(q, kv, heads, hk, dim, page, dtype, seed=sum(kv) + 1)
+    o0, lse0 = r.attend(max_kv=1)
+    r.check(o0, lse0)
+    for b, n in enumerate(q):
+        if n:
+            p, s = r.places(b)
+            r.v[p[-2:], :, s[-2:], 1] = bad
+    o, lse = r.attend(max_kv=1)
+    assert torch.equal(lse, lse0)
+    for b, n in enumerate(q):
+        t0 = r.starts[b]
+        assert torch.equal(o[t0:t0 + max(n - 2, 0)], o0[t0:t0 + max(n - 2, 0)])
+        last = slice(t0 + max(n - 2, 0), t0 + n)
+        assert not bool(torch.isfinite(o[last][..., 1]).any())
+        other = torch.arange(dim, device=DEV) != 1
+        assert torch.equal(o[last][..., other], o0[last][..., other])
