@@ -474,8 +474,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_attn_tile_kernel(AttnArgs a)
       }
 
       const float l_tot = l_run + __shfl_xor(l_run, 32);
-      const float inv = m_run == -INFINITY ? 0.0f : 1.0f / l_tot;
-      const float lse2 = m_run == -INFINITY ? -INFINITY : m_run + __builtin_amdgcn_logf(l_tot);
+      const float inv = inverse_sum(l_tot), lse2 = log2_sum(m_run, l_tot);
       if (at.unit > 0 || to < units) {
         // a part: into the share's slot, the first for a tile that an earlier share began, else the second
         set_cut(a, share, at.unit > 0, to == units, (i1 - i0) * g, R.t0 + i0, h);
@@ -561,9 +560,9 @@ __global__ __launch_bounds__(256) void paged_attn_join_parts_kernel(AttnArgs a) 
   for (int k = lane; k < parts; k += 16) l += __builtin_amdgcn_exp2f(sum_of(k) - ref);
 #pragma unroll
   for (int w = 8; w; w >>= 1) l += __shfl_xor(l, w);
-  const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
+  const float inv = inverse_sum(l);
   auto out_row = [&](int r) { return (int64_t)(cut.z + (r0 + r) / g) * a.heads + cut.w * g + (r0 + r) % g; };
-  if (lane == 0 && fr < rows) a.lse[out_row(fr)] = m == -INFINITY ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+  if (lane == 0 && fr < rows) a.lse[out_row(fr)] = log2_sum(m, l) * kLn2;
   v4f o[kItems] = {};
   for (int k0 = 0; k0 < parts; k0 += kAtOnce) {
     const int n = min(kAtOnce, parts - k0);
@@ -855,8 +854,7 @@ __global__ __launch_bounds__(64 * FW_WAVES) void paged_attn_few_kernel(AttnArgs 
         l = __builtin_fmaf(stat[w][1][r], f, l);
         o += *(const v4f*)((const float*)(lds + w * S::kWave) + r * (D + 4) + d) * f;
       }
-      const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
-      const float lse2 = m == -INFINITY ? -INFINITY : m + __builtin_amdgcn_logf(l);
+      const float inv = inverse_sum(l), lse2 = log2_sum(m, l);
       const int64_t row = (int64_t)(R.t0 + i0 + r / g) * a.heads + h * g + r % g;
       if (slot < 0) {
         *(uint2*)(a.o + row * D + d) = make_uint2((uint32_t)Mfma<T>::pack(o[0] * inv, o[1] * inv),
@@ -949,10 +947,10 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) l += f[e], o += x[e] * f[e];
   }
-  const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
+  const float inv = inverse_sum(l);
   *(uint2*)(a.o + row * D + d) = make_uint2((uint32_t)Mfma<T>::pack(o[0] * inv, o[1] * inv),
                                             (uint32_t)Mfma<T>::pack(o[2] * inv, o[3] * inv));
-  if (d == 0) a.lse[row] = m == -INFINITY ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+  if (d == 0) a.lse[row] = log2_sum(m, l) * kLn2;
 }
 
 // ---------------------------------------------------------------------------

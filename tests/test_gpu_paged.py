@@ -767,3 +767,38 @@ def test_nonfinite_values_behind_the_mask_of_a_late_segment(q, kv, heads, hk, di
         assert not bool(torch.isfinite(o[last][..., 1]).any())
         other = torch.arange(dim, device=DEV) != 1
         assert torch.equal(o[last][..., other], o0[last][..., other])
+
+
+@pytest.mark.parametrize("n,L,dim", [(1, 200, 64), (1, 257, 128), (1, 700, 64), (4, 700, 128), (1, 5000, 128), (4, 5000, 64),
+                                     (70, 257, 128), (70, 700, 64), (70, 5000, 128), (300, 5000, 64), (3, 257, 48),
+                                     (3, 700, 48), (3, 5000, 48)])
+@pytest.mark.parametrize("where", ["query", "key"])
+@pytest.mark.parametrize("gather", [False, True])
+def test_nan_that_a_row_sees_is_in_its_answer(n, L, dim, where, gather):
+    """A NaN query, and a NaN last key (the last new token's own): o and lse of the rows that see it are NaN, in every
+    form (one run, splits, shares, row tiles, one wave a row); all other rows are as before, bit for bit. Every key
+    such a row sees has drawn NaN from it."""
+    heads, hk = 4, 2
+    r = Ragged([n], [L], heads, hk, dim, 16, BF16, seed=n + L)
+    w0 = r.w.clone()
+    o0, lse0 = r.attend(gather=gather)
+    clean = r.w.clone()
+    r.w.copy_(w0)
+    p, s = r.places(0)
+    hit = torch.zeros(n, heads, dtype=torch.bool, device=DEV)
+    drawn = torch.zeros(L, hk, dtype=torch.bool, device=DEV)
+    if where == "query":
+        t = n // 2
+        r.q[t, 1, 5] = float("nan")
+        hit[t, 1] = True
+        drawn[:L - n + t + 1, 0] = True
+    else:
+        r.k[p[-1], 1, s[-1], 3] = float("nan")
+        hit[n - 1, 2:] = True
+        drawn[:, 1] = True
+    o, lse = r.attend(gather=gather)
+    assert bool(torch.isnan(o[hit]).all()) and bool(torch.isnan(lse[hit]).all())
+    assert torch.equal(o[~hit], o0[~hit]) and torch.equal(lse[~hit], lse0[~hit])
+    if gather:
+        got, want = r.w[p, :, s], clean[p, :, s]
+        assert bool(torch.isnan(got[drawn]).all()) and torch.equal(got[~drawn], want[~drawn])
