@@ -618,8 +618,9 @@ int gwa_paged_write(const gwa_paged_cache* cache, const void* q, int64_t ldqt, i
  * x / (heads / kv_heads); token i of n in a sequence of L keys sees keys
  * 0 .. L - n + i with `causal`, else all L. o[t][x] = sum_j p_j v_j with
  * p = softmax(scale * q . k), lse[t][x] = log sum_j exp(scale * q . k) (natural,
- * fp32); a row that sees no key gives o = 0 and lse = -inf, rows of no
- * sequence may be left unwritten. With `gather`,
+ * fp32); a row that sees no key, or only scores of -inf, gives o = 0, lse = -inf
+ * and no weight, one that sees a NaN score NaN; rows of no sequence may be left
+ * unwritten. With `gather`,
  * w[key] += the sum of p over the sequence's new tokens and the kv head's query
  * heads, in a fixed order (sequences of one call must not share pages then).
  * fp32 scores, statistics and sums; p is rounded to the cache's dtype for the

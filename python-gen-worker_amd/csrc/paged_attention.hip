@@ -123,10 +123,10 @@ __global__ __launch_bounds__(64 * RW_WAVES) void paged_attn_rows_kernel(PagedArg
         if (lane + 64 * i < d) acc[i] = fmaf(pk, T::load(vr[lane + 64 * i]), acc[i]);
     }
   }
-  const float inv = keys > 0 ? 1.0f / l : 0.0f;
+  const float inv = inverse_sum(l);
   for (int i = 0; i < RW_MAX_D / 64; ++i)
     if (lane + 64 * i < d) o[row * d + lane + 64 * i] = (uint16_t)T::pack(acc[i] * inv, 0.0f);
-  if (lane == 0) lse[row] = keys > 0 ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+  if (lane == 0) lse[row] = log2_sum(m, l) * kLn2;
 }
 
 // w[key] += sum of 2^(s c - lse) over the rows that see the key: one lane a key, 64 keys of one kv head a wave
@@ -152,7 +152,7 @@ __global__ __launch_bounds__(64) void paged_gather_rows_kernel(PagedArgs c, cons
       for (int e = lane; e < d; e += 64) qs[e] = T::load(q[t * ldqt + x * ldqh + e]);
       __syncthreads();
       const float s = row_dot<T>(qs, key, d) * c_log2;
-      if (j <= seen) sum += __builtin_amdgcn_exp2f(s - lse[(int64_t)t * heads + x] * kLog2e);
+      if (j <= seen) sum += __builtin_amdgcn_exp2f(s - gather_lse2(lse[(int64_t)t * heads + x]));
     }
     if (j0 + lane < len) c.w[paged_w_at(c, page, h, j)] += sum;
   }
@@ -379,8 +379,8 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_attn_tile_kernel(AttnArgs a)
         const float x_max = fmaxf(m8[0], __shfl_xor(m8[0], 32)) * a.c_log2;
         const bool bump = x_max > m_run;
         const float m_new = bump ? x_max : m_run;
-        // a row that has seen no key yet subtracts 0: its scores are all -inf and its p all 0
-        const float ref = MASK && m_new == -INFINITY ? 0.0f : m_new;
+        // a row whose scores so far are all -inf (behind the mask, or by themselves) subtracts 0: its p are all 0
+        const float ref = m_new == -INFINITY ? 0.0f : m_new;
         const float alpha = __builtin_amdgcn_exp2f(m_run - ref);  // 0 on the first tile
         m_run = m_new;
         float ps[S::kNC];
@@ -762,7 +762,7 @@ __global__ __launch_bounds__(64 * FW_WAVES) void paged_attn_few_kernel(AttnArgs 
           mx = fmaxf(mx, __shfl_xor(mx, 32)) * a.c_log2;
           const bool bump = mx > m_run[rb];
           const float m_new = bump ? mx : m_run[rb];
-          const float ref = MASK && m_new == -INFINITY ? 0.0f : m_new;
+          const float ref = m_new == -INFINITY ? 0.0f : m_new;
           const float alpha = __builtin_amdgcn_exp2f(m_run[rb] - ref);
           m_run[rb] = m_new;
           float p[8];
@@ -969,7 +969,7 @@ __global__ __launch_bounds__(256) void paged_gather_scores_kernel(AttnArgs a) {
       const int lim = R.limit(r, a.causal != 0);
       if (j0 > lim) continue;
       const int64_t row = (int64_t)(R.t0 + r / g) * a.heads + h * g + r % g;
-      const float lse2 = a.lse[row] * kLog2e;
+      const float lse2 = gather_lse2(a.lse[row]);
       const float4 s = *(const float4*)(a.scores + row * a.score_stride + j0);
       const float x[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
@@ -1046,7 +1046,7 @@ __global__ __launch_bounds__(64 * GT_WAVES, 3) void paged_gather_tile_kernel(Att
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int r = 32 * x + j;  // rows past the tile's tokens: a probability of 0
-        next2[x] = r < tt * g ? lse0[(int64_t)(i + min(r / g, most)) * a.heads + r % g] * kLog2e : INFINITY;
+        next2[x] = r < tt * g ? gather_lse2(lse0[(int64_t)(i + min(r / g, most)) * a.heads + r % g]) : INFINITY;
       }
     };
     if (t_lo < t_hi) {

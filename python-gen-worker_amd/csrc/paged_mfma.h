@@ -93,10 +93,12 @@ __device__ __forceinline__ bool take_nonfinite(v4i& x) {
 }
 
 // What a row's softmax ends as, from its running maximum m (log2 domain) and sum l: the factor of its values and the log2
-// of the whole sum. A row without keys has m = -inf and l = 0: 0 and -inf. A NaN score raises no maximum but is in l,
+// of the whole sum. A row without keys, or all of whose scores are -inf, has m = -inf and l = 0: 0 and -inf. A NaN score raises no maximum but is in l,
 // so that such a row's are NaN, whether or not it has seen other scores.
 __device__ __forceinline__ float inverse_sum(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
 __device__ __forceinline__ float log2_sum(float m, float l) { return m + __builtin_amdgcn_logf(l); }
+// the lse that a row's scores are measured against for the weights it gives; a row without a sum gives none
+__device__ __forceinline__ float gather_lse2(float lse) { return lse == -INFINITY ? INFINITY : lse * kLog2e; }
 
 // Sequence b's part of a call for one kv head: its rows (new token i, query head of the group) flattened as i * group + g
 struct Rows {

@@ -345,8 +345,8 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, 
     (o [tokens, heads, head_dim] in q's type, lse fp32 [tokens, heads], the natural log of the sum of exponentials).
 
     Query head x reads kv head x // (heads / kv_heads). With ``causal`` token i of n in a sequence of L keys sees the
-    first L - n + i + 1, else all L; a row that sees none gives o = 0 and lse = -inf. ``scale`` defaults to
-    head_dim^-0.5. ``max_q`` and ``max_kv``: the batch's largest new-token count and kv_len, which choose the launch.
+    first L - n + i + 1, else all L; a row that sees none, or scores of -inf alone, gives o = 0 and lse = -inf, one that
+    sees a NaN score NaN. ``scale`` defaults to head_dim^-0.5. ``max_q`` and ``max_kv``: the batch's largest new-token count and kv_len, which choose the launch.
     ``weights`` fp32 [pages, kv_heads, page_size]: every key's slot gets, added, the probability it drew from the
     sequence's new tokens over the kv head's query heads, in an order that does not depend on timing; sequences may
     share pages only without it. head_dim: a multiple of 8 up to 256 (the matrix cores serve 64 and 128, up to 256 query

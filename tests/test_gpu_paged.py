@@ -802,3 +802,47 @@ def test_nan_that_a_row_sees_is_in_its_answer(n, L, dim, where, gather):
     if gather:
         got, want = r.w[p, :, s], clean[p, :, s]
         assert bool(torch.isnan(got[drawn]).all()) and torch.equal(got[~drawn], want[~drawn])
+
+
+MINUS_INF_FORMS = [(1, 200, 64), (1, 700, 128), (4, 700, 64), (1, 5000, 128), (4, 5000, 64), (70, 700, 128), (300, 5000, 64),
+                   (3, 700, 48)]
+
+
+@pytest.mark.parametrize("n,L,dim", MINUS_INF_FORMS)
+@pytest.mark.parametrize("gather", [False, True])
+def test_keys_whose_scores_are_minus_infinity(n, L, dim, gather):
+    """The first keys (whole tiles that every row sees) score -inf: they draw nothing, and the answer is the softmax over
+    the others. A row all of whose scores are -inf is one without keys."""
+    heads, hk, lost = 4, 2, 150
+    r = Ragged([n], [L], heads, hk, dim, 16, BF16, seed=n + L)
+    r.q[..., 0] = 1.0
+    p, s = r.places(0)
+    w0 = r.w.clone()
+    r.k[p[:lost], :, s[:lost], 0] = -math.inf
+    o, lse = r.attend(gather=gather)
+    u, dw = U[BF16], torch.zeros(L, hk, dtype=torch.float64, device=DEV)
+    dw_tol = torch.zeros_like(dw)
+    j, i = torch.arange(lost, L, device=DEV), torch.arange(n, device=DEV)
+    seen = j <= (L - n + i)[:, None]
+    for x in range(heads):
+        h = x // (heads // hk)
+        q, k, v = r.q[:, x].double(), r.k[p[lost:], h, s[lost:]].double(), r.v[p[lost:], h, s[lost:]].double()
+        z = torch.where(seen, (q @ k.t().contiguous()) * dim ** -0.5, -math.inf)
+        top = ((q.abs() @ k.abs().t().contiguous()) * dim ** -0.5).amax(-1)
+        prob, ref_lse = torch.softmax(z, -1), torch.logsumexp(z, -1)
+        ds = (dim + 4) * E * top
+        rel = 2 * ds[:, None] + 2.0 ** -20
+        ref, spread = prob @ v, prob @ v.abs()
+        assert bool(((o[:, x].double() - ref).abs() <= (u + rel) * spread + u * ref.abs() + E).all())
+        assert bool(((lse[:, x].double() - ref_lse).abs() <= ds + 4 * E * (top + ref_lse.abs()) + 2.0 ** -20).all())
+        dw[lost:, h] += prob.sum(0)
+        dw_tol[lost:, h] += (prob * rel).sum(0)
+    if gather:
+        want = w0[p, :, s].double() + dw
+        assert bool(((r.w[p, :, s].double() - want).abs() <= dw_tol + (n * heads // hk + 4) * E * want).all())
+        assert torch.equal(r.w[p[:lost], :, s[:lost]], w0[p[:lost], :, s[:lost]])
+    r.k[p, 1, s, 0] = -math.inf
+    r.w.copy_(w0)
+    o, lse = r.attend(gather=gather)
+    assert bool((o[:, 2:] == 0).all()) and bool((lse[:, 2:] == -math.inf).all()) and bool(torch.isfinite(lse[:, :2]).all())
+    assert not gather or torch.equal(r.w[p, 1, s], w0[p, 1, s])
