@@ -1234,7 +1234,8 @@ void launch_matrix(const Plan& p, AttnArgs a, int64_t max_kv, bool gather, hipSt
     hipLaunchKernelGGL((paged_gather_tile_kernel<T, D>), dim3(groups * (unsigned)(a.tiles * a.splits)),
                        dim3(64 * GT_WAVES), 0, st, a);
     if (a.splits > 1)
-      hipLaunchKernelGGL(paged_gather_join_kernel, dim3((unsigned)((max_kv + 255) / 256), groups), dim3(256), 0, st, a);
+      hipLaunchKernelGGL(paged_gather_join_kernel, dim3((unsigned)(max_kv > 0 ? (max_kv + 255) / 256 : 1), groups), dim3(256),
+                         0, st, a);
   }
 }
 

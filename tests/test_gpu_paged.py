@@ -846,3 +846,18 @@ def test_keys_whose_scores_are_minus_infinity(n, L, dim, gather):
     o, lse = r.attend(gather=gather)
     assert bool((o[:, 2:] == 0).all()) and bool((lse[:, 2:] == -math.inf).all()) and bool(torch.isfinite(lse[:, :2]).all())
     assert not gather or torch.equal(r.w[p, 1, s], w0[p, 1, s])
+
+
+@pytest.mark.parametrize("dim", [128, 48])
+def test_no_stated_keys_with_many_tokens_still_gather(dim):
+    """max_kv = 0 with chunks: keys that the host did not know of are attended and their weights gathered, and a batch
+    that has none keeps its weights."""
+    r = Ragged([300, 40], [700, 40], 8, 2, dim, 16, BF16, seed=13)
+    w0 = r.w.clone()
+    o, lse = r.attend(max_q=300, max_kv=0, gather=True)
+    r.check(o, lse, w0=w0)
+    r.kv, r.kv_len = [0, 0], _ints([0, 0])
+    r.w.copy_(w0)
+    o, lse = r.attend(max_q=300, max_kv=0, gather=True)
+    assert bool((o == 0).all()) and bool((lse == -math.inf).all())
+    assert torch.equal(r.w.nan_to_num(), w0.nan_to_num())
