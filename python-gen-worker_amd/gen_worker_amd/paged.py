@@ -24,7 +24,7 @@ from __future__ import annotations
 import ctypes
 import math
 from dataclasses import dataclass
-from typing import Optional, Sequence
+from typing import Iterator, Optional, Sequence
 
 import torch
 from torch import Tensor
@@ -457,7 +457,8 @@ class PagedCache:
 
     def twin(self) -> "PagedCache":
         """A pool of the same shape whose pages follow this cache's lists: another layer's keys and values. Write and
-        attend with this cache's batches; this cache's ``evict`` serves it too."""
+        attend with this cache's batches. Sequences are added to and cut by the first cache alone, whose ``evict`` serves
+        its twins and theirs."""
         other = PagedCache.__new__(PagedCache)
         other.page_size, other._free, other._seqs = self.page_size, self._free, self._seqs
         other.k, other.v = torch.zeros_like(self.k), torch.zeros_like(self.v)
@@ -465,6 +466,12 @@ class PagedCache:
         other._next, other._twins = -1, []
         self._twins.append(other)
         return other
+
+    def _pools(self) -> Iterator["PagedCache"]:
+        """Every pool under this cache's lists."""
+        yield self
+        for twin in self._twins:
+            yield from twin._pools()
 
     @property
     def free_pages(self) -> int:
@@ -542,10 +549,11 @@ class PagedCache:
                                scale=scale, causal=causal, weights=self.weights if gather else None)
 
     def evict(self, seqs: Sequence[int], budget: int, recent: int) -> Optional[Tensor]:
-        """Cuts those of ``seqs`` that hold more than ``budget`` keys back to it (``paged_evict``), here and in the
-        twins; their old pages are free afterwards. Returns this cache's kept slots [cut sequences, kv_heads, budget], or
+        """Cuts those of ``seqs`` that hold more than ``budget`` keys back to it (``paged_evict``), here and in all
+        twins (a twin itself refuses: it does not reach the others); their old pages are free afterwards. Returns this cache's kept slots [cut sequences, kv_heads, budget], or
         None if no sequence was longer. Needs budget / page_size free pages a cut sequence."""
         name = "PagedCache.evict"
+        _require(self._next >= 0, name, "sequences belong to the cache this is a twin of")
         _require(all(s in self._seqs for s in seqs) and len(set(seqs)) == len(seqs), name, f"sequences {list(seqs)}")
         _require(self.weights is not None, name, "the cache keeps no weights")
         _require(budget > 0 and 0 <= recent <= budget, name, f"a budget of {budget} keys, {recent} of them recent")
@@ -560,7 +568,7 @@ class PagedCache:
         flat, new = flat.view(len(cut), old_width), new.view(len(cut), width)
         kept = None
         try:
-            for cache in [self] + self._twins:
+            for cache in self._pools():
                 got = paged_evict(cache.k, cache.v, cache.weights, flat, kv_len, max(lens), new, budget, recent)[0]
                 kept = got if kept is None else kept
         except Exception:

@@ -861,3 +861,36 @@ def test_no_stated_keys_with_many_tokens_still_gather(dim):
     o, lse = r.attend(max_q=300, max_kv=0, gather=True)
     assert bool((o == 0).all()) and bool((lse == -math.inf).all())
     assert torch.equal(r.w.nan_to_num(), w0.nan_to_num())
+
+
+def test_evictions_leave_every_layer_with_its_own_keys():
+    """Three pools under one bookkeeping, the third a twin of the second: after an eviction each attends the kept keys
+    of its own, in the shared pages."""
+    from gen_worker_amd.paged import PagedCache
+
+    g = _gen(5)
+    first = PagedCache(32, 16, 1, 64, weights=True, device=DEV)
+    second = first.twin()
+    pools = [first, second, second.twin()]
+    seq = first.add()
+    first.drop(first.add())
+    batch = first.extend([seq], [90])
+    held = []
+    for pool in pools:
+        q, k, v = (torch.randn(90, 1, 64, generator=g, device=DEV).to(BF16) for _ in range(3))
+        pool.write(batch, q, k, v)
+        # gathered weights of this test's choosing: the same slots are kept in all layers
+        pool.weights[batch.table[0].long()] = torch.arange(96, device=DEV).flip(0).float().view(6, 1, 16)
+        held.append((k, v))
+    kept = first.evict([seq], 40, 8)
+    assert kept.tolist() == [[list(range(32)) + list(range(82, 90))]]
+    batch = first.extend([seq], [1])
+    for pool, (k, v) in zip(pools, held):
+        q, kn, vn = (torch.randn(1, 1, 64, generator=g, device=DEV).to(BF16) for _ in range(3))
+        o, _ = pool.attend(batch, pool.write(batch, q, kn, vn))
+        kk = torch.cat([k[kept[0, 0].long(), 0], kn[:, 0]]).double()
+        vv = torch.cat([v[kept[0, 0].long(), 0], vn[:, 0]]).double()
+        p = torch.softmax((kk @ q[0, 0].double()) / 8.0, -1)
+        ref, spread = p @ vv, p @ vv.abs()
+        # p and o each rounded once, scores of a few units off by a few 2^-24 of their terms
+        assert bool(((o[0, 0].double() - ref).abs() <= 2.0 ** -8 * (ref.abs() + spread) + 1e-4 * spread).all())

@@ -191,3 +191,31 @@ def test_tables_whose_rows_overlap_are_copied_apart():
             assert torch.equal(got.as_strided((rows, width), (row, 1)), table)
     # nothing is copied that need not be
     assert p._spaced(wide[:, 2:5])[0].data_ptr() == wide[:, 2:5].data_ptr()
+
+
+def test_evict_moves_every_pool_under_the_lists(monkeypatch):
+    """The first cache's evict cuts its twins and their twins; a twin, which does not reach the others, refuses and
+    changes nothing."""
+    p = _paged()
+    first = p.PagedCache(12, 8, 1, 64, device="cpu", weights=True)
+    twin = first.twin()
+    other, below = first.twin(), twin.twin()
+    pools = [first, twin, other, below]
+    seq = first.add()
+    first.extend([seq], [40])
+    moved = []
+
+    def evict(k, v, w, table, kv_len, max_kv, new, budget, recent):
+        moved.append((k.data_ptr(), v.data_ptr(), w.data_ptr(), table.tolist(), new.tolist()))
+        return torch.zeros(1, 1, budget, dtype=torch.int32), kv_len.clamp(max=budget)
+
+    monkeypatch.setattr(p, "paged_evict", evict)
+    pages, free = list(first._seqs[seq][0]), first.free_pages
+    for cache in pools[1:]:
+        with pytest.raises(p.PagedError, match="twin"):
+            cache.evict([seq], 16, 4)
+    assert not moved and first._seqs[seq][0] == pages and first.free_pages == free and first.length(seq) == 40
+    assert first.evict([seq], 16, 4).shape == (1, 1, 16)
+    assert {m[:3] for m in moved} == {(c.k.data_ptr(), c.v.data_ptr(), c.weights.data_ptr()) for c in pools}
+    assert len(moved) == 4 and all(m[3:] == ([pages], [first._seqs[seq][0]]) for m in moved)
+    assert first.length(seq) == 16 and not set(pages) & set(first._seqs[seq][0]) and first.free_pages == free + 3
