@@ -389,6 +389,11 @@ bool plain_args(PyObject* const* args, int n, unsigned optional, Tensor* out, bo
   return true;
 }
 
+// a tensor that a call wrote into past the dispatcher: autograd knows by the version what changed behind a graph
+void written(const Tensor& t) {
+  if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // (rotated channels, table rows) of fitting tables for `tokens` tokens
 bool tables_fit(const Tensor& cos, const Tensor& sin, const Tensor& positions, int64_t tokens, int64_t dim,
                 const at::Device& dev, int64_t& rot, int64_t& rows) {
@@ -526,6 +531,8 @@ PyObject* paged_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                               t[5].defined() ? address<int32_t>(t[5]) : nullptr, out.data_ptr(), n, h, rot, interleaved,
                               stream_of(t[6])) != GWA_OK)
           out = Tensor();
+        else
+          written(t[6]), written(t[7]), written(t[11]);
       }
     }
   }
@@ -577,6 +584,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                                 max_kv, (float)scale, causal, gather, bytes > 0 ? ws.data_ptr() : nullptr, bytes,
                                 stream_of(q)) != GWA_OK)
         o = Tensor();
+      else
+        written(t[6]);
     }
   }
   if (!o.defined()) Py_RETURN_NONE;
@@ -612,6 +621,8 @@ PyObject* paged_evict(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       if (g_abi.paged_evict(&c, address<int32_t>(next), std::max(next.stride(0), next.size(1)), next.size(1), max_kv,
                             budget, recent, address<int32_t>(kept), address<int32_t>(len), stream_of(t[0])) != GWA_OK)
         kept = Tensor();
+      else
+        written(t[0]), written(t[1]), written(t[2]);
     }
   }
   if (!kept.defined()) Py_RETURN_NONE;

@@ -109,6 +109,13 @@ def _plain(*tensors: Optional[Tensor]) -> bool:
     return True
 
 
+def _written(out, *tensors: Optional[Tensor]):
+    """``out`` of a call that wrote into these tensors past the dispatcher: as the registered op does for its
+    ``mutates_args``, their version counters are raised, by which autograd knows what changed behind a graph."""
+    torch.autograd.graph.increment_version([t for t in tensors if t is not None])
+    return out
+
+
 # ---------------------------------------------------------------------------
 # rotary positions
 # ---------------------------------------------------------------------------
@@ -299,7 +306,9 @@ def paged_write(q: Tensor, k: Tensor, v: Tensor, cos: Optional[Tensor], sin: Opt
         out = host.paged_write(*a, interleaved)
         if out is not None:
             return out
-    return _write_body(*a, interleaved) if _plain(*a) else _write_op(*a, interleaved)
+    if _plain(*a):
+        return _written(_write_body(*a, interleaved), k_pages, v_pages, weights)
+    return _write_op(*a, interleaved)
 
 
 def _attention_body(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, q_start: Tensor, kv_len: Tensor,
@@ -360,7 +369,8 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, 
         if out is not None:
             return out
     if _plain(q, k_pages, v_pages, table, q_start, kv_len, weights):
-        return _attention_body(q, k_pages, v_pages, table, q_start, kv_len, max_q, max_kv, scale, causal, weights)
+        return _written(_attention_body(q, k_pages, v_pages, table, q_start, kv_len, max_q, max_kv, scale, causal,
+                                        weights), weights)
     return _attention_op(q, k_pages, v_pages, table, q_start, kv_len, max_q, max_kv, scale, causal, weights)
 
 
@@ -408,7 +418,7 @@ def paged_evict(k_pages: Tensor, v_pages: Tensor, weights: Tensor, table: Tensor
         if out is not None:
             return out
     if _plain(*a, new_table):
-        return _evict_body(*a, max_kv, new_table, budget, recent)
+        return _written(_evict_body(*a, max_kv, new_table, budget, recent), k_pages, v_pages, weights)
     return _evict_op(*a, max_kv, new_table, budget, recent)
 
 

@@ -894,3 +894,38 @@ def test_evictions_leave_every_layer_with_its_own_keys():
         ref, spread = p @ vv, p @ vv.abs()
         # p and o each rounded once, scores of a few units off by a few 2^-24 of their terms
         assert bool(((o[0, 0].double() - ref).abs() <= 2.0 ** -8 * (ref.abs() + spread) + 1e-4 * spread).all())
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_pools_that_a_graph_saved_are_known_to_have_changed(native, monkeypatch):
+    """Every call that writes raises the version of what it wrote, as an in-place torch operation does, and of nothing
+    else; a backward pass over a pool saved before fails instead of using the new values."""
+    from gen_worker_amd import ops
+    from gen_worker_amd.paged import paged_evict, paged_write
+
+    if not native:
+        monkeypatch.setattr(ops, "_host", None)
+    r = Ragged([2], [40], 2, 1, 64, 16, BF16, seed=3)
+    new = _ints([sorted(set(range(6)) - set(r.table[0].tolist()))[:2]])
+    k = torch.randn(2, 1, 64, generator=r.g, device=DEV).to(BF16)
+    calls = [
+        (lambda: paged_write(r.q, k, k, None, None, None, r.k, r.v, r.table, r.q_start, r.kv_len), (r.k, r.v)),
+        (lambda: paged_write(r.q, k, k, None, None, None, r.k, r.v, r.table, r.q_start, r.kv_len, weights=r.w),
+         (r.k, r.v, r.w)),
+        (lambda: r.attend(), ()), (lambda: r.attend(gather=True), (r.w,)),
+        (lambda: paged_evict(r.k, r.v, r.w, r.table, r.kv_len, 40, new, 20, 4), (r.k, r.v, r.w))]
+    tensors = (r.k, r.v, r.w, r.q, k, r.table, r.q_start, r.kv_len, new)
+    for call, wrote in calls:
+        before = [t._version for t in tensors]
+        x = torch.ones((), device=DEV, requires_grad=True)
+        graphs = [(x * t).nan_to_num().sum() for t in wrote]
+        call()
+        for t, v in zip(tensors, before):
+            assert (t._version > v) == any(t is w for w in wrote)
+        for y in graphs:
+            with pytest.raises(RuntimeError, match="inplace operation"):
+                y.backward()
+    with torch.inference_mode():
+        s = Ragged([2], [40], 2, 1, 64, 16, BF16, seed=3)
+    s.attend(gather=True)   # tensors of inference mode have no version
+    paged_write(s.q, k, k, None, None, None, s.k, s.v, s.table, s.q_start, s.kv_len, weights=s.w)
