@@ -28,6 +28,7 @@ from typing import Iterator, Optional, Sequence
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _native as nat
 from . import ops
@@ -107,6 +108,16 @@ def _plain(*tensors: Optional[Tensor]) -> bool:
                               or torch._C._functorch.is_functorch_wrapped_tensor(t)):
             return False
     return True
+
+
+def _tangent(t: Optional[Tensor]) -> Optional[Tensor]:
+    """The tangent of a dual tensor (forward-mode differentiation), None of any other."""
+    return forward_ad.unpack_dual(t).tangent if t is not None and forward_ad._current_level >= 0 else None
+
+
+def _no_tangents(name: str, *tensors: Optional[Tensor]) -> None:
+    if forward_ad._current_level >= 0:   # neither the native calls nor the registered ops would notice
+        _require(all(_tangent(t) is None for t in tensors), name, "no gradient is defined for a dual tensor's tangent")
 
 
 def _written(out, *tensors: Optional[Tensor]):
@@ -208,9 +219,16 @@ def rotary_embed(x: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor
     """x [tokens, heads, head_dim] (bf16, fp16 or fp32; token and head strides free) with the first
     ``2 * cos.shape[1]`` channels of every head rotated by their token's position, the others copied. Pairs are
     (2i, 2i + 1) with ``interleaved``, else (i, i + half). ``positions``: int32 [tokens] rows of the tables (held inside
-    them), or None for 0, 1, 2, ... ``inverse`` rotates back. Computed in fp32, rounded once; differentiable in x."""
+    them), or None for 0, 1, 2, ... ``inverse`` rotates back. Computed in fp32, rounded once; differentiable in x, in
+    reverse and forward mode."""
     _require(not torch.is_grad_enabled() or not (cos is not None and cos.requires_grad or sin is not None
                                                  and sin.requires_grad), "rotary_embed", "the tables have no gradient")
+    if forward_ad._current_level >= 0:
+        _no_tangents("rotary_embed", cos, sin)
+        primal, tangent = forward_ad.unpack_dual(x)
+        if tangent is not None:   # the map is linear: a tangent turns as x does
+            return forward_ad.make_dual(*(rotary_embed(t, cos, sin, positions, interleaved=interleaved, inverse=inverse)
+                                          for t in (primal, tangent)))
     host = _host()
     if host is not None:
         y = host.rotary_embed(x, cos, sin, positions, interleaved, inverse)
@@ -301,6 +319,7 @@ def paged_write(q: Tensor, k: Tensor, v: Tensor, cos: Optional[Tensor], sin: Opt
     and keys are rotated as ``rotary_embed`` does (cos = sin = None: not at all); the new slots' gathered ``weights``
     [pages, kv_heads, page_size] start at 0. No two sequences may write one page."""
     a = (q, k, v, cos, sin, positions, k_pages, v_pages, table, q_start, kv_len, weights)
+    _no_tangents("paged_write", q, k, v, cos, sin, k_pages, v_pages, weights)
     host = _host()
     if host is not None:
         out = host.paged_write(*a, interleaved)
@@ -363,6 +382,7 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, 
     gradient is defined."""
     if scale is None:
         scale = float(q.shape[-1]) ** -0.5
+    _no_tangents("paged_attention", q, k_pages, v_pages, weights)
     host = _host()
     if host is not None:
         out = host.paged_attention(q, k_pages, v_pages, table, q_start, kv_len, weights, max_q, max_kv, scale, causal)
@@ -412,6 +432,7 @@ def paged_evict(k_pages: Tensor, v_pages: Tensor, weights: Tensor, table: Tensor
     min(budget, the largest kv_len) keys a row; ``max_kv``: the largest kv_len, which shapes the launch. Returns (kept int32
     [batch, kv_heads, budget]: the old slots, -1 past the end; the new kv_len)."""
     a = (k_pages, v_pages, weights, table, kv_len)
+    _no_tangents("paged_evict", k_pages, v_pages, weights)
     host = _host()
     if host is not None:
         out = host.paged_evict(*a, new_table, max_kv, budget, recent)

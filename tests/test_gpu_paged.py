@@ -929,3 +929,32 @@ def test_pools_that_a_graph_saved_are_known_to_have_changed(native, monkeypatch)
         s = Ragged([2], [40], 2, 1, 64, 16, BF16, seed=3)
     s.attend(gather=True)   # tensors of inference mode have no version
     paged_write(s.q, k, k, None, None, None, s.k, s.v, s.table, s.q_start, s.kv_len, weights=s.w)
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("interleaved,inverse", [(False, False), (True, True)])
+def test_rotary_forward_mode(native, interleaved, inverse, monkeypatch):
+    """The tangent turns as x does, with the tensor's own dual numbers, under torch.func.jvp and, vectorised, jacfwd."""
+    from torch.autograd import forward_ad
+
+    from gen_worker_amd import ops
+    from gen_worker_amd.paged import rotary_embed, rotary_table
+
+    if not native:
+        monkeypatch.setattr(ops, "_host", None)
+    g = _gen(4)
+    cos, sin = rotary_table(64, 32, device=DEV)
+    at = torch.randint(0, 64, (5,), generator=g, device=DEV)
+    x, v = (torch.randn(5, 2, 40, generator=g, device=DEV) for _ in range(2))
+
+    def f(t):
+        return rotary_embed(t, cos, sin, at.int(), interleaved=interleaved, inverse=inverse)
+
+    with forward_ad.dual_level():
+        y, dy = forward_ad.unpack_dual(f(forward_ad.make_dual(x, v)))
+        assert forward_ad.unpack_dual(f(x)).tangent is None
+    for got, t in ((y, x), (dy, v), *zip(torch.func.jvp(f, (x,), (v,)), (x, v))):
+        _check_turned(got, *_turn(t, cos, sin, at, interleaved, inverse))
+    # the Jacobian's columns are the rotated unit vectors: its product with v is v rotated, to fp32 sums of pairs
+    j = torch.func.jacfwd(lambda t: f(t.view(1, 1, -1).expand(5, 2, 40)))(x[0, 0])
+    assert bool(((j.double() @ v[0, 0].double()) - f(v[:1, :1].expand(5, 2, 40)).double()).abs().max() <= 16 * E * 6)

@@ -219,3 +219,28 @@ def test_evict_moves_every_pool_under_the_lists(monkeypatch):
     assert {m[:3] for m in moved} == {(c.k.data_ptr(), c.v.data_ptr(), c.weights.data_ptr()) for c in pools}
     assert len(moved) == 4 and all(m[3:] == ([pages], [first._seqs[seq][0]]) for m in moved)
     assert first.length(seq) == 16 and not set(pages) & set(first._seqs[seq][0]) and first.free_pages == free + 3
+
+
+def test_tangents_are_refused_where_no_gradient_is_defined():
+    """A dual tensor's tangent, which neither the native calls nor the registered ops would notice."""
+    from torch.autograd import forward_ad
+
+    p = _paged()
+    cos, sin = p.rotary_table(8, 8, device="cpu")
+    x = torch.zeros(4, 2, 8, dtype=BF16)
+    pages, w = torch.zeros(2, 2, 16, 8, dtype=BF16), torch.zeros(2, 2, 16)
+    one = torch.zeros(1, dtype=torch.int32)
+    table, start = torch.zeros(1, 1, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    with forward_ad.dual_level():
+        dual, dual_pages, dual_w, dual_cos = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, pages, w, cos))
+        for call in (lambda: p.rotary_embed(x, dual_cos, sin),
+                     lambda: p.paged_attention(dual, pages, pages, table, start, one, 1, 1),
+                     lambda: p.paged_attention(x, dual_pages, pages, table, start, one, 1, 1),
+                     lambda: p.paged_attention(x, pages, pages, table, start, one, 1, 1, weights=dual_w),
+                     lambda: p.paged_write(x, dual, x, cos, sin, None, pages, pages, table, start, one),
+                     lambda: p.paged_write(x, x, x, dual_cos, sin, None, pages, pages, table, start, one),
+                     lambda: p.paged_evict(pages, dual_pages, w, table, one, 1, table, 4, 1)):
+            with pytest.raises(p.PagedError, match="no gradient"):
+                call()
+        with pytest.raises(p.PagedError, match="CUDA"):   # as without a level
+            p.paged_attention(x, pages, pages, table, start, one, 1, 1)
