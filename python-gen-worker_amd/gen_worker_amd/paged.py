@@ -201,6 +201,7 @@ def _(x, cos, sin, positions, interleaved, inverse):
 
 
 def _rotary_setup(ctx, inputs, output):
+    _require(not any(ctx.needs_input_grad[1:3]), "rotary_embed", "the tables have no gradient")
     _, cos, sin, positions, ctx.interleaved, ctx.inverse = inputs
     ctx.save_for_backward(cos, sin, positions)
 

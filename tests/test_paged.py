@@ -244,3 +244,17 @@ def test_tangents_are_refused_where_no_gradient_is_defined():
                 call()
         with pytest.raises(p.PagedError, match="CUDA"):   # as without a level
             p.paged_attention(x, pages, pages, table, start, one, 1, 1)
+
+
+def test_the_registered_rotation_refuses_tables_that_ask_for_a_gradient():
+    p = _paged()
+    op = torch.ops.cozy_gen_worker.rotary_embed
+    x, cos, sin = (torch.empty(s, device="meta") for s in ((4, 2, 8), (4, 4), (4, 4)))
+    for a in ((cos.clone().requires_grad_(True), sin), (cos, sin.clone().requires_grad_(True))):
+        for x0 in (x, x.clone().requires_grad_(True)):
+            with pytest.raises(p.PagedError, match="no gradient"):
+                op(x0, *a, None, False, False)
+        with torch.no_grad():
+            assert op(x, *a, None, False, False).shape == x.shape
+    y = op(x.clone().requires_grad_(True), cos, sin, None, False, False)
+    assert y.requires_grad and not op(x, cos, sin, None, False, False).requires_grad
