@@ -199,8 +199,8 @@ bool still_bound(const BoundCall* b, PyObject* dict) {
 // its storage, or a lazy negation, whose storage holds the values before it
 constexpr c10::DispatchKeySet kNotPlain({c10::DispatchKey::Python, c10::DispatchKey::Functionalize,
                                          c10::DispatchKey::Negative, c10::DispatchKey::Conjugate,
-                                         c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
-                                         c10::DispatchKey::ZeroTensor});
+                                         c10::DispatchKey::Batched, c10::DispatchKey::FuncTorchBatched,
+                                         c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::ZeroTensor});
 bool plain_tensor(const Tensor& t) {
   return !(t.requires_grad() && at::GradMode::is_enabled()) && !t.key_set().has_any(kNotPlain);
 }
@@ -445,10 +445,18 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
+    const bool interleaved = ctx->saved_data["interleaved"].toBool(), inverse = !ctx->saved_data["inverse"].toBool();
     Tensor dx;
-    if (grads[0].defined())
-      dx = RotaryFunction::apply(grads[0], saved[0], saved[1], some(saved[2]), ctx->saved_data["interleaved"].toBool(),
-                                 !ctx->saved_data["inverse"].toBool());
+    if (!grads[0].defined()) {
+    } else if (grads[0].key_set().has_any(kNotPlain) || c10::impl::TorchDispatchModeTLS::stack_len() != 0) {
+      // a batch of gradients, a lazy negation, a wrapper: the registered op's, whose dispatch deals with them
+      static const auto op = c10::Dispatcher::singleton()
+                                 .findSchemaOrThrow("cozy_gen_worker::rotary_embed", "")
+                                 .typed<Tensor(const Tensor&, const Tensor&, const Tensor&, const OptTensor&, bool, bool)>();
+      dx = op.call(grads[0], saved[0], saved[1], some(saved[2]), interleaved, inverse);
+    } else {
+      dx = RotaryFunction::apply(grads[0], saved[0], saved[1], some(saved[2]), interleaved, inverse);
+    }
     return {dx, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };

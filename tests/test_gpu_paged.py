@@ -958,3 +958,39 @@ def test_rotary_forward_mode(native, interleaved, inverse, monkeypatch):
     # the Jacobian's columns are the rotated unit vectors: its product with v is v rotated, to fp32 sums of pairs
     j = torch.func.jacfwd(lambda t: f(t.view(1, 1, -1).expand(5, 2, 40)))(x[0, 0])
     assert bool(((j.double() @ v[0, 0].double()) - f(v[:1, :1].expand(5, 2, 40)).double()).abs().max() <= 16 * E * 6)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_rotary_gradient_of_upstream_gradients_that_are_not_plain(native, monkeypatch):
+    """A lazily negated upstream gradient, a batch of them (a vectorised Jacobian), one under a dispatch mode, and a
+    strided one: each is the plain gradient's result."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    from gen_worker_amd import ops
+    from gen_worker_amd.paged import rotary_embed, rotary_table
+
+    if not native:
+        monkeypatch.setattr(ops, "_host", None)
+
+    class Seen(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.names = getattr(self, "names", []) + [str(func)]
+            return func(*args, **(kwargs or {}))
+
+    cos, sin = rotary_table(16, 8, device=DEV)
+    g = _gen(12)
+    x = torch.randn(5, 2, 8, generator=g, device=DEV, requires_grad=True)
+    dy = torch.randn(3, 5, 2, 8, generator=g, device=DEV)
+    y = rotary_embed(x, cos, sin)
+
+    def grad(d, **kw):
+        return torch.autograd.grad(y, x, d, retain_graph=True, **kw)[0]
+
+    want = torch.stack([grad(d) for d in dy])
+    _check_turned(want[0], *_turn(dy[0], cos, sin, torch.arange(5, device=DEV), False, inverse=True))
+    assert torch.equal(grad(torch._neg_view(dy[0])), -want[0])
+    assert torch.equal(grad(dy, is_grads_batched=True), want)
+    assert torch.equal(grad(dy[1].transpose(0, 2).contiguous().transpose(0, 2)), want[1])
+    with Seen() as seen:
+        assert torch.equal(grad(dy[2]), want[2])
+    assert any("rotary_embed" in n for n in seen.names)
