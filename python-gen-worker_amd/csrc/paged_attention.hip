@@ -74,6 +74,11 @@ __device__ __forceinline__ float row_dot(const float* q, const uint16_t* key, in
   return s;
 }
 
+// The form for head sizes without a matrix kernel, right rather than fast: every row reads K and V for itself, on scalar
+// products, and a row's keys are not split. One token over 701 keys, 32 heads of 96 over 8: 232 us (floor 0.4); 32
+// sequences of up to 32768 keys 24.3 ms (241 us); 1021 and 866 tokens over 6007 and 2367 keys, 24 heads of 96 over 4: 13 ms,
+// 25 with the weights (55 us).
+//
 // 64 keys a step, one a lane: scores, the running maximum m and sum l of the softmax over all keys so far (in the
 // log2 domain, p = 2^(s c - m)), then the outputs, which lie over the lanes (channel lane + 64 i).
 template <class T>
@@ -167,6 +172,8 @@ __global__ __launch_bounds__(64) void paged_gather_rows_kernel(PagedArgs c, cons
 //   S^T = K q^T           (keys x rows: a lane holds one row, 16 keys of each 32)
 //   p   = 2^(S c - m)     (m: the row's running maximum; O and the sum l are rescaled where it moves)
 //   O^T = O^T + V^T p^T   (V^T by transposing reads, in the key order S^T leaves p in, so p stays in registers)
+// p is rounded to the cache's type, as the MFMA's operands are 16 bits wide, and summed into l before: O is off by 1.1 to
+// 1.3 times what one rounding of the output costs. m, l, S and O are fp32.
 // A tile takes two slots, each ended by a barrier: the matrix slot (O of the tile before, S of this one) and the softmax
 // slot. With 8 waves the SIMD's second wave runs one slot behind the first, so that one has the matrix cores while
 // the other has the vector unit.
@@ -174,11 +181,13 @@ __global__ __launch_bounds__(64) void paged_gather_rows_kernel(PagedArgs c, cons
 // lane's limit. There 0 * v of a hidden key must not reach O: whoever copied a part of the tile sets values that are not
 // finite to 0 and says so, and rows that do see such a key get its values added one by one at the end.
 //
-// Measured on 4096 new tokens over 16500 keys, 32 heads of 128 over 8 (981 GFLOP): 883 to 930 us, 1.05 to 1.11 PFLOP/s,
-// where an 8192^3 library product reaches 1.25. The matrix cores are busy half of the time, at a clock that falls to 1.65 to
-// 1.8 GHz; without the copies it takes 849 us (of 965 then), without the exponentials 891. Before the fixed operand order
+// Measured on 4096 new tokens over 16500 keys, 32 heads of 128 over 8 (981 GFLOP): 883 to 950 us, 1.03 to 1.11 PFLOP/s,
+// where an 8192^3 library product reaches 1.22 to 1.26. The matrix cores are busy 49 % of the time and the vector unit 51 %, at
+// a clock that falls to 1.65 to 1.8 GHz; without the copies it takes 849 us (of 965 then), without the exponentials 891. Before the fixed operand order
 // every MFMA waited for the LDS read issued just ahead of it (1057 us); both waves of a SIMD in the same phase take 1013;
-// 128-key tiles spill and take 1710. At head_dim 64 the exponentials bound it.
+// 128-key tiles spill and take 1710. Five sequences of up to 509 tokens over up to 4001 keys, 16 heads of 64: 35 us, in which
+// nothing is busy (matrix cores 11 %, vector unit 27 %, LDS 7 %): a tile has half the work between the same two barriers, and
+// 2 waves a SIMD do not cover what each waits for.
 template <int D, int BN, int NW>
 struct TileShape {
   static constexpr int kRow = 2 * D, kRun = 1024 / kRow;  // row bytes; rows a 1 KB copy covers
@@ -598,7 +607,8 @@ __global__ __launch_bounds__(256) void paged_attn_join_parts_kernel(AttnArgs a) 
 // 32768 keys: runs of 4096 keys, 866 workgroups, took 321 us, of 16384 keys, 328 workgroups, 303). Where the keys are so few
 // that runs of 256 are all there at once, a run is a split of that length, which a workgroup finds without the line.
 // Measured: the 32 sequences 276 us, 5.7 TB/s (a copy reaches 4.94; the copies alone, without the products, took 296 with
-// their join before the shares); one sequence of 701 keys, 32 heads over 8, 9 us and 3 for the join: launch and four dependent loads.
+// their join before the shares); 4 tokens each over up to 8192 keys 88 us with the join, 8 tokens 101 (floors 76 and 85); one
+// sequence of 701 keys, 32 heads over 8, 9 to 10 us and 3.9 for the join (medians): launch and four dependent loads.
 constexpr int FW_KEYS = 32, FW_PAGES = 512;  // keys a tile; page ids staged at a time (whole tiles: page_size >= 8)
 constexpr int FW_WAVES = 4, FW_UNIT = FW_KEYS * FW_WAVES;
 // Where the segment of a run that starts at key s_lo ends, at k_hi at the latest: behind the FW_PAGES-th page from that of
@@ -881,8 +891,8 @@ __global__ __launch_bounds__(64 * FW_WAVES) void paged_attn_few_kernel(AttnArgs 
     }
   } else {
     const int share = blockIdx.x % kXcds * (a.shares / kXcds) + blockIdx.x / kXcds;
-      const LineLanes lanes = line_lanes(c, a.tokens, tt, causal, 0);
-  const int64_t per_head = head_line(c, a.tokens, tt, causal, lanes), all = per_head * c.kv_heads;
+    const LineLanes lanes = line_lanes(c, a.tokens, tt, causal, 0);
+    const int64_t per_head = head_line(c, a.tokens, tt, causal, lanes), all = per_head * c.kv_heads;
     const int64_t x0 = share_start(all, share, a.shares), x1 = share_start(all, share + 1, a.shares);
     no_cuts(a, share);
     if (x0 >= x1) return;
@@ -958,7 +968,7 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a) {
 // ---------------------------------------------------------------------------
 
 // From the scores that the few-rows kernel left (a sixteenth of the keys' bytes at 4 heads of 128 to a kv head, where
-// recomputing them would read the keys again): 4 keys a thread, the rows in order. 16 sequences of up to 8192 keys: 6.4 us.
+// recomputing them would read the keys again): 4 keys a thread, the rows in order. 16 sequences of up to 8192 keys: 6.8 us.
 __global__ __launch_bounds__(256) void paged_gather_scores_kernel(AttnArgs a) {
   const PagedArgs& c = a.c;
   const int b = blockIdx.y / c.kv_heads, h = blockIdx.y % c.kv_heads, g = a.heads / c.kv_heads;
@@ -989,8 +999,9 @@ __global__ __launch_bounds__(256) void paged_gather_scores_kernel(AttnArgs a) {
 // its row's probabilities for 16 keys; the lanes of the 32 rows are joined at the end. The tokens are divided over
 // `splits` workgroups where the keys alone are too few to fill the chip: each leaves its sums in w_part
 // [split][group][score_stride], joined in order. Two sequences of 1021 and 866 tokens over 6007 and 2367 keys, 24 heads of
-// 128 over 4: 115 us, bound by the vector units beside the MFMAs, about twice what its exponentials alone would take; with
-// a division a row in the copies and a mask on every tile of such odd groups 157.
+// 128 over 4: 112 us. It waits rather than computes (vector unit busy 32 % of the time, matrix cores 17 %, LDS 11 %): a wave
+// has its scores and then their exponentials in turn, between two barriers a tile. With a division a row in the copies and a
+// mask on every tile of such odd groups 157.
 constexpr int GT_WAVES = 4, GT_ROWS = 64, GT_KEYS = 32 * GT_WAVES;
 
 template <class T, int D>
