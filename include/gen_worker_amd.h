@@ -647,6 +647,75 @@ int gwa_paged_attention(const gwa_paged_cache* cache, const void* q, int64_t ldq
 int gwa_paged_evict(const gwa_paged_cache* cache, const int32_t* new_table, int64_t new_stride, int64_t new_width,
                     int64_t max_kv, int64_t budget, int64_t recent, int32_t* kept, int32_t* new_len, void* stream);
 
+/* ---- The paged cache in 8 bits -------------------------------------------------
+ * k and v hold e4m3 codes (one byte an element: strides in bytes, multiples of 16,
+ * head_dim % 16 == 0, 16 .. 256), and every row (one slot of one kv head) has a scale
+ * byte: value = code * 2^(scale - 127), a scale of 255 is NaN. The cache's `dtype` is
+ * the type of the calls' q, k, v and o; the operators read a row's values in that type
+ * (bf16: every one exactly; fp16: what it cannot hold overflows or is rounded).
+ * A row is written with the smallest power of two, 2^-126 at least, under which none of
+ * its finite values passes 448, the largest code; a value is rounded to the nearest code
+ * (ties to even), but never past the type's largest finite one; what is not finite
+ * becomes NaN. */
+typedef struct gwa_paged_scales {
+  uint8_t* k;             /* [pages][kv_heads][page_size] at the strides below */
+  uint8_t* v;             /* at the same strides */
+  int64_t page_stride, head_stride;
+} gwa_paged_scales;
+
+/* gwa_paged_write into such a cache: k's rows are rotated in fp32 and rounded once, to
+ * their codes. */
+int gwa_paged_write_fp8(const gwa_paged_cache* cache, const gwa_paged_scales* scales, const void* q, int64_t ldqt,
+                        int64_t ldqh, const void* k, int64_t ldkt, int64_t ldkh, const void* v, int64_t ldvt,
+                        int64_t ldvh, const float* cos_t, const float* sin_t, int64_t table_rows,
+                        const int32_t* positions, void* q_out, int64_t tokens, int64_t heads, int64_t rot,
+                        int interleaved, void* stream);
+
+/* What the sequences' last rows stand for: k_out, v_out [tokens][kv_heads][head_dim]
+ * (contiguous, the cache's dtype), sequence b's rows q_start[b] .. q_start[b + 1] - 1
+ * those of its last slots, as gwa_paged_write_fp8 takes them. Rows without a slot (of no
+ * sequence, or a negative one) are not written. */
+int gwa_paged_read_fp8(const gwa_paged_cache* cache, const gwa_paged_scales* scales, void* k_out, void* v_out,
+                       int64_t tokens, void* stream);
+
+/* gwa_paged_attention over such a cache (workspace: gwa_paged_attention_workspace). */
+int gwa_paged_attention_fp8(const gwa_paged_cache* cache, const gwa_paged_scales* scales, const void* q, int64_t ldqt,
+                            int64_t ldqh, void* o, float* lse, int64_t tokens, int64_t heads, int64_t max_q,
+                            int64_t max_kv, float scale, int causal, int gather, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+
+/* gwa_paged_evict of such a cache: codes and scales are copied as they are. */
+int gwa_paged_evict_fp8(const gwa_paged_cache* cache, const gwa_paged_scales* scales, const int32_t* new_table,
+                        int64_t new_stride, int64_t new_width, int64_t max_kv, int64_t budget, int64_t recent,
+                        int32_t* kept, int32_t* new_len, void* stream);
+
+/* ---- Drawing the next tokens -----------------------------------------------------
+ * Per row of logits [rows][vocab] (row stride ld elements; dtype bf16, fp16 or fp32) a
+ * token by the row's own random number in [0, 1). With m the largest logit and weights
+ * w_i = exp((x_i - m) / temperature), tokens in falling order of x (equal ones: the
+ * lowest index first) are cut to the first top_k (0: all), then to the shortest run
+ * whose weight reaches top_p of what is left (1: all), then to those of w_i >= min_p;
+ * the first always stays. The token is the first i, in the vocabulary's order, at which
+ * the kept weights up to and with w_i pass uniform * their sum; its logprob is
+ * log(w_i / sum) (fp32). temperature 0 takes the largest (logprob 0).
+ * Weights are integers of 2^-45 of the largest (of fewer bits over 131072 tokens),
+ * formed in 64 bits, and so are sums: no order of summation changes a result.
+ * -inf and NaN are never drawn; a row that holds nothing else gives token -1 and
+ * logprob NaN. Of several +inf each has weight 1, and nothing else has any.
+ * Settings are arrays [rows] or, where the pointer is NULL, the number beside it; from
+ * an array, what is out of range counts as the nearest that is not (a NaN: 0). */
+typedef struct gwa_sampling {
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  float all_temperature;
+  int32_t all_top_k;
+  float all_top_p, all_min_p;
+} gwa_sampling;
+int gwa_sample_tokens(const void* logits, int64_t ld, int dtype, const float* uniform, const gwa_sampling* settings,
+                      int64_t* tokens, float* logprobs, int64_t rows, int64_t vocab, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

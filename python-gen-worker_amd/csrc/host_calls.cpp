@@ -48,6 +48,10 @@ struct Abi {
   decltype(&gwa_paged_attention_workspace) paged_attention_workspace;
   decltype(&gwa_paged_attention) paged_attention;
   decltype(&gwa_paged_evict) paged_evict;
+  decltype(&gwa_paged_write_fp8) paged_write_fp8;
+  decltype(&gwa_paged_read_fp8) paged_read_fp8;
+  decltype(&gwa_paged_attention_fp8) paged_attention_fp8;
+  decltype(&gwa_sample_tokens) sample_tokens;
 };
 Abi g_abi;
 bool g_bound = false;
@@ -489,12 +493,14 @@ PyObject* rotary_embed(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 // whether a table's rows lie apart; of a single row the stride is not read
 bool rows_apart(const Tensor& t) { return t.size(0) < 2 || t.stride(0) >= t.size(1); }
 
-// the C interface's cache of fitting tensors; overlapping rows of page ids are copied in Python
+// the C interface's cache of fitting tensors; overlapping rows of page ids are copied in Python. `values`: of an 8-bit
+// cache, the type of the call's q, k, v and o
 bool cache_fits(const Tensor& k, const Tensor& v, const Tensor& w, const Tensor& table, const Tensor& q_start,
-                const Tensor& kv_len, gwa_paged_cache& c) {
+                const Tensor& kv_len, gwa_paged_cache& c, std::optional<at::ScalarType> values = std::nullopt) {
   const at::Device dev = k.device();
-  if (!k.is_cuda() || k.layout() != at::kStrided || (k.scalar_type() != at::kBFloat16 && k.scalar_type() != at::kHalf) ||
-      k.dim() != 4 || k.stride(3) != 1 || v.scalar_type() != k.scalar_type() || v.device() != dev ||
+  const at::ScalarType type = values.value_or(k.scalar_type());
+  if (!k.is_cuda() || k.layout() != at::kStrided || (type != at::kBFloat16 && type != at::kHalf) ||
+      (values.has_value() && k.scalar_type() != at::kFloat8_e4m3fn) || k.dim() != 4 || k.stride(3) != 1 || v.scalar_type() != k.scalar_type() || v.device() != dev ||
       v.layout() != at::kStrided || !v.sizes().equals(k.sizes()) || !v.strides().equals(k.strides()) ||
       kv_len.dim() != 1 || table.dim() != 2)
     return false;
@@ -510,39 +516,65 @@ bool cache_fits(const Tensor& k, const Tensor& v, const Tensor& w, const Tensor&
                       q_start.defined() ? address<int32_t>(q_start) : nullptr, address<int32_t>(kv_len), k.stride(0),
                       k.stride(1), k.stride(2), w.defined() ? w.stride(0) : 0, w.defined() ? w.stride(1) : 0, k.size(0),
                       std::max(table.stride(0), table.size(1)), table.size(1), batch, (int)k.size(2), (int)k.size(1),
-                      (int)k.size(3), dt_code(k.scalar_type())};
+                      (int)k.size(3), dt_code(type)};
+  return true;
+}
+bool scales_fit(const Tensor& k, const Tensor& ks, const Tensor& vs, gwa_paged_scales& s) {
+  for (const Tensor* t : {&ks, &vs})
+    if (t->scalar_type() != at::kByte || t->layout() != at::kStrided || t->device() != k.device() ||
+        !t->sizes().equals(k.sizes().slice(0, 3)) || !t->strides().equals(ks.strides()) ||
+        (k.size(2) != 1 && t->stride(2) != 1))
+      return false;
+  s = gwa_paged_scales{address<uint8_t>(ks), address<uint8_t>(vs), ks.stride(0), ks.stride(1)};
   return true;
 }
 
-// paged_write(q, k, v, cos, sin, positions, k_pages, v_pages, table, q_start, kv_len, weights, interleaved) -> q rotated
+// q rotated of a write that fits, undefined otherwise. t: q, k, v, cos, sin, positions, k_pages, v_pages, then of an 8-bit
+// cache (E8) k_scales, v_scales, then table, q_start, kv_len, weights
+template <bool E8>
+Tensor write_call(const Tensor* t, bool interleaved) {
+  const Tensor &q = t[0], &k = t[1], &v = t[2], *rest = t + (E8 ? 10 : 8);
+  Tensor out;
+  gwa_paged_cache c;
+  gwa_paged_scales s;
+  int64_t rot, rows;
+  const at::ScalarType dt = E8 ? q.scalar_type() : t[6].scalar_type();
+  const at::Device dev = t[6].device();
+  if (q.dim() != 3 || !cache_fits(t[6], t[7], rest[3], rest[0], rest[1], rest[2], c, E8 ? std::optional(dt) : std::nullopt) ||
+      (E8 && !scales_fit(t[6], t[8], t[9], s)))
+    return out;
+  const int64_t n = q.size(0), h = q.size(1), d = c.head_dim;
+  if (!heads_on(q, dt, dev, n, h, d) || !heads_on(k, dt, dev, n, c.kv_heads, d) ||
+      !heads_on(v, dt, dev, n, c.kv_heads, d) || !tables_fit(t[3], t[4], t[5], n, d, dev, rot, rows))
+    return out;
+  out = empty_like_device({n, h, d}, dt, q);
+  auto call = [&](auto f, auto... cache) {
+    return f(cache..., q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+             v.stride(0), v.stride(1), t[3].defined() ? address<float>(t[3]) : nullptr,
+             t[4].defined() ? address<float>(t[4]) : nullptr, rows, t[5].defined() ? address<int32_t>(t[5]) : nullptr,
+             out.data_ptr(), n, h, rot, interleaved, stream_of(t[6]));
+  };
+  int rc;
+  if constexpr (E8) rc = call(g_abi.paged_write_fp8, &c, &s);
+  else rc = call(g_abi.paged_write, &c);
+  if (rc != GWA_OK) return Tensor();
+  for (const Tensor* x = t + 6; x < rest; ++x) written(*x);
+  written(rest[3]);
+  return out;
+}
+
+// paged_write(q, k, v, cos, sin, positions, k_pages, v_pages, table, q_start, kv_len, weights, interleaved) -> q rotated,
+// paged_write_fp8 with k_scales, v_scales behind v_pages
+template <bool E8>
 PyObject* paged_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  Tensor t[12];
-  if (nargs != 13 || !g_bound || !plain_args(args, 12, 1u << 3 | 1u << 4 | 1u << 5 | 1u << 11, t)) Py_RETURN_NONE;
-  const bool interleaved = PyObject_IsTrue(args[12]) == 1;
-  const Tensor &q = t[0], &k = t[1], &v = t[2];
-  Tensor out;
+  constexpr int N = E8 ? 14 : 12;
+  Tensor t[N], out;
+  if (nargs != N + 1 || !g_bound || !plain_args(args, N, 1u << 3 | 1u << 4 | 1u << 5 | 1u << (N - 1), t)) Py_RETURN_NONE;
+  const bool interleaved = PyObject_IsTrue(args[N]) == 1;
   {
     pybind11::gil_scoped_release no_gil;
-    gwa_paged_cache c;
-    int64_t rot, rows;
-    const at::ScalarType dt = t[6].scalar_type();
-    const at::Device dev = t[6].device();
-    if (q.dim() == 3 && cache_fits(t[6], t[7], t[11], t[8], t[9], t[10], c)) {
-      const int64_t n = q.size(0), h = q.size(1), d = c.head_dim;
-      if (heads_on(q, dt, dev, n, h, d) && heads_on(k, dt, dev, n, c.kv_heads, d) &&
-          heads_on(v, dt, dev, n, c.kv_heads, d) && tables_fit(t[3], t[4], t[5], n, d, dev, rot, rows)) {
-        out = empty_like_device({n, h, d}, dt, q);
-        if (g_abi.paged_write(&c, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-                              v.data_ptr(), v.stride(0), v.stride(1), t[3].defined() ? address<float>(t[3]) : nullptr,
-                              t[4].defined() ? address<float>(t[4]) : nullptr, rows,
-                              t[5].defined() ? address<int32_t>(t[5]) : nullptr, out.data_ptr(), n, h, rot, interleaved,
-                              stream_of(t[6])) != GWA_OK)
-          out = Tensor();
-        else
-          written(t[6]), written(t[7]), written(t[11]);
-      }
-    }
+    out = write_call<E8>(t, interleaved);
   }
   if (!out.defined()) Py_RETURN_NONE;
   return THPVariable_Wrap(out);
@@ -557,47 +589,127 @@ PyObject* pair(Tensor a, Tensor b) {
   return both;
 }
 
-// paged_attention(q, k_pages, v_pages, table, q_start, kv_len, weights, max_q, max_kv, scale, causal) -> (o, lse)
+// paged_attention(q, k_pages, v_pages, table, q_start, kv_len, weights, max_q, max_kv, scale, causal) -> (o, lse),
+// paged_attention_fp8 with k_scales, v_scales behind v_pages
+template <bool E8>
 PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  Tensor t[7];
-  if (nargs != 11 || !g_bound || !plain_args(args, 7, 1u << 6, t) || !PyLong_Check(args[7]) || !PyLong_Check(args[8]))
+  constexpr int N = E8 ? 9 : 7;
+  Tensor t[N];
+  if (nargs != N + 4 || !g_bound || !plain_args(args, N, 1u << (N - 1), t) || !PyLong_Check(args[N]) ||
+      !PyLong_Check(args[N + 1]))
     Py_RETURN_NONE;
-  const long long max_q = PyLong_AsLongLong(args[7]), max_kv = PyLong_AsLongLong(args[8]);
-  const double scale = PyFloat_AsDouble(args[9]);
+  const long long max_q = PyLong_AsLongLong(args[N]), max_kv = PyLong_AsLongLong(args[N + 1]);
+  const double scale = PyFloat_AsDouble(args[N + 2]);
   if (PyErr_Occurred()) {
     PyErr_Clear();
     Py_RETURN_NONE;
   }
-  const bool causal = PyObject_IsTrue(args[10]) == 1;
-  const Tensor& q = t[0];
+  const bool causal = PyObject_IsTrue(args[N + 3]) == 1;
+  const Tensor &q = t[0], *rest = t + (E8 ? 5 : 3);  // table, q_start, kv_len, weights
   Tensor o, lse;
   {
     pybind11::gil_scoped_release no_gil;
     gwa_paged_cache c;
-    if (q.dim() == 3 && q.size(1) > 0 && cache_fits(t[1], t[2], t[6], t[3], t[4], t[5], c) && c.kv_heads > 0 &&
-        q.size(1) % c.kv_heads == 0 &&
-        heads_on(q, t[1].scalar_type(), t[1].device(), q.size(0), q.size(1), c.head_dim) && q.size(0) > 0 &&
+    gwa_paged_scales s;
+    const at::ScalarType dt = E8 ? q.scalar_type() : t[1].scalar_type();
+    if (q.dim() == 3 && q.size(1) > 0 &&
+        cache_fits(t[1], t[2], rest[3], rest[0], rest[1], rest[2], c, E8 ? std::optional(dt) : std::nullopt) &&
+        (!E8 || scales_fit(t[1], t[3], t[4], s)) && c.kv_heads > 0 && q.size(1) % c.kv_heads == 0 &&
+        heads_on(q, dt, t[1].device(), q.size(0), q.size(1), c.head_dim) && q.size(0) > 0 &&
         q.stride(0) > 0 && q.stride(1) > 0 && q.stride(0) % 8 == 0 && q.stride(1) % 8 == 0 &&
         (uintptr_t)q.data_ptr() % 16 == 0) {
       const int64_t n = q.size(0), h = q.size(1);
-      const bool gather = t[6].defined();
+      const bool gather = rest[3].defined();
       o = empty_like_device({n, h, c.head_dim}, q.scalar_type(), q);
       lse = empty_like_device({n, h}, at::kFloat, q);
       const int64_t bytes = g_abi.paged_attention_workspace(c.batch, n, h, c.kv_heads, c.head_dim, max_q, max_kv,
                                                             c.table_width * c.page_size, gather);
       Tensor ws;
       if (bytes > 0) ws = empty_like_device({bytes}, at::kByte, q);
-      if (g_abi.paged_attention(&c, q.data_ptr(), q.stride(0), q.stride(1), o.data_ptr(), address<float>(lse), n, h, max_q,
-                                max_kv, (float)scale, causal, gather, bytes > 0 ? ws.data_ptr() : nullptr, bytes,
-                                stream_of(q)) != GWA_OK)
-        o = Tensor();
-      else
-        written(t[6]);
+      auto call = [&](auto f, auto... cache) {
+        return f(cache..., q.data_ptr(), q.stride(0), q.stride(1), o.data_ptr(), address<float>(lse), n, h, max_q, max_kv,
+                 (float)scale, causal, gather, bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream_of(q));
+      };
+      int rc;
+      if constexpr (E8) rc = call(g_abi.paged_attention_fp8, &c, &s);
+      else rc = call(g_abi.paged_attention, &c);
+      if (rc != GWA_OK) o = Tensor();
+      else written(rest[3]);
     }
   }
   if (!o.defined()) Py_RETURN_NONE;
   return pair(std::move(o), std::move(lse));
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_read_fp8(k_pages, v_pages, k_scales, v_scales, table, q_start, kv_len, tokens, dtype) -> (k, v)
+PyObject* paged_read_fp8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Tensor t[7];
+  if (nargs != 9 || !g_bound || !plain_args(args, 7, 0, t) || !PyLong_Check(args[7]) || !THPDtype_Check(args[8]))
+    Py_RETURN_NONE;
+  const long long tokens = PyLong_AsLongLong(args[7]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  const at::ScalarType dt = ((THPDtype*)args[8])->scalar_type;
+  Tensor k, v;
+  {
+    pybind11::gil_scoped_release no_gil;
+    gwa_paged_cache c;
+    gwa_paged_scales s;
+    if (tokens >= 0 && cache_fits(t[0], t[1], Tensor(), t[4], t[5], t[6], c, dt) && scales_fit(t[0], t[2], t[3], s)) {
+      k = empty_like_device({tokens, c.kv_heads, c.head_dim}, dt, t[0]);
+      v = empty_like_device({tokens, c.kv_heads, c.head_dim}, dt, t[0]);
+      if (g_abi.paged_read_fp8(&c, &s, k.data_ptr(), v.data_ptr(), tokens, stream_of(t[0])) != GWA_OK) k = Tensor();
+    }
+  }
+  if (!k.defined()) Py_RETURN_NONE;
+  return pair(std::move(k), std::move(v));
+  END_HANDLE_TH_ERRORS
+}
+
+// sample_tokens(logits, uniform, temperature, top_k, top_p, min_p, and a number for each of the last four that is None)
+// -> (tokens, logprobs)
+PyObject* sample_tokens(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Tensor t[6];
+  if (nargs != 10 || !g_bound || !plain_args(args, 6, 0x3cu, t) || !PyLong_Check(args[7])) Py_RETURN_NONE;
+  const double temperature = PyFloat_AsDouble(args[6]), top_p = PyFloat_AsDouble(args[8]),
+               min_p = PyFloat_AsDouble(args[9]);
+  const long long top_k = PyLong_AsLongLong(args[7]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  Tensor tokens, logprobs;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const Tensor& x = t[0];
+    bool fits = x.is_cuda() && x.layout() == at::kStrided && x.dim() == 2 && dt_code(x.scalar_type()) >= 0;
+    const int64_t rows = fits ? x.size(0) : 0, vocab = fits ? x.size(1) : 0;
+    fits = fits && vocab > 0 && (vocab == 1 || x.stride(1) == 1) && (rows < 2 || x.stride(0) >= vocab);
+    for (int i = 1; i < 6; ++i)
+      fits = fits && (!t[i].defined() || (t[i].scalar_type() == (i == 3 ? at::kInt : at::kFloat) &&
+                                          t[i].layout() == at::kStrided && t[i].device() == x.device() &&
+                                          t[i].sizes().equals({rows}) && (rows < 2 || t[i].stride(0) == 1)));
+    if (fits) {
+      const gwa_sampling s = {t[2].defined() ? address<float>(t[2]) : nullptr,
+                              t[3].defined() ? address<int32_t>(t[3]) : nullptr,
+                              t[4].defined() ? address<float>(t[4]) : nullptr,
+                              t[5].defined() ? address<float>(t[5]) : nullptr, (float)temperature, (int32_t)top_k,
+                              (float)top_p, (float)min_p};
+      tokens = empty_like_device({rows}, at::kLong, x);
+      logprobs = empty_like_device({rows}, at::kFloat, x);
+      if (g_abi.sample_tokens(x.data_ptr(), std::max(x.stride(0), vocab), dt_code(x.scalar_type()), address<float>(t[1]),
+                              &s, address<int64_t>(tokens), address<float>(logprobs), rows, vocab, stream_of(x)) != GWA_OK)
+        tokens = Tensor();
+    }
+  }
+  if (!tokens.defined()) Py_RETURN_NONE;
+  return pair(std::move(tokens), std::move(logprobs));
   END_HANDLE_TH_ERRORS
 }
 
@@ -746,6 +858,10 @@ PyObject* host_bind(PyObject*, PyObject* args) {
   GWA_BIND(paged_attention_workspace);
   GWA_BIND(paged_attention);
   GWA_BIND(paged_evict);
+  GWA_BIND(paged_write_fp8);
+  GWA_BIND(paged_read_fp8);
+  GWA_BIND(paged_attention_fp8);
+  GWA_BIND(sample_tokens);
 #undef GWA_BIND
   Py_INCREF(bodies);
   Py_INCREF(records);
@@ -765,15 +881,25 @@ PyMethodDef module_methods[] = {{"bind", host_bind, METH_VARARGS, "bind(addresse
                                  "awq_forward(x, weight, wscales, wzeros, bias, max_rows) -> output or None"},
                                 {"rotary_embed", (PyCFunction)(void (*)(void))rotary_embed, METH_FASTCALL,
                                  "rotary_embed(x, cos, sin, positions, interleaved, inverse) -> output or None"},
-                                {"paged_write", (PyCFunction)(void (*)(void))paged_write, METH_FASTCALL,
+                                {"paged_write", (PyCFunction)(void (*)(void))paged_write<false>, METH_FASTCALL,
                                  "paged_write(q, k, v, cos, sin, positions, k_pages, v_pages, table, q_start, kv_len, "
                                  "weights, interleaved) -> rotated q or None"},
-                                {"paged_attention", (PyCFunction)(void (*)(void))paged_attention, METH_FASTCALL,
+                                {"paged_attention", (PyCFunction)(void (*)(void))paged_attention<false>, METH_FASTCALL,
                                  "paged_attention(q, k_pages, v_pages, table, q_start, kv_len, weights, max_q, max_kv, "
                                  "scale, causal) -> (o, lse) or None"},
                                 {"paged_evict", (PyCFunction)(void (*)(void))paged_evict, METH_FASTCALL,
                                  "paged_evict(k_pages, v_pages, weights, table, kv_len, new_table, max_kv, budget, "
                                  "recent) -> (kept, new_len) or None"},
+                                {"paged_write_fp8", (PyCFunction)(void (*)(void))paged_write<true>, METH_FASTCALL,
+                                 "paged_write's arguments with k_scales, v_scales behind v_pages -> rotated q or None"},
+                                {"paged_read_fp8", (PyCFunction)(void (*)(void))paged_read_fp8, METH_FASTCALL,
+                                 "paged_read_fp8(k_pages, v_pages, k_scales, v_scales, table, q_start, kv_len, tokens, "
+                                 "dtype) -> (k, v) or None"},
+                                {"paged_attention_fp8", (PyCFunction)(void (*)(void))paged_attention<true>, METH_FASTCALL,
+                                 "paged_attention's arguments with k_scales, v_scales behind v_pages -> (o, lse) or None"},
+                                {"sample_tokens", (PyCFunction)(void (*)(void))sample_tokens, METH_FASTCALL,
+                                 "sample_tokens(logits, uniform, temperature, top_k, top_p, min_p, numbers of the last "
+                                 "four) -> (tokens, logprobs) or None"},
                                 {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host_calls", "Native host side of eager calls.", -1, module_methods};
 

@@ -4,125 +4,11 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "paged_common.h"
+#include "paged_rotary.h"
 
 namespace {
 
 constexpr int RT_THREADS = 256;
-
-// 8 consecutive elements of the three element types as fp32, in 16-byte pieces
-template <int DT>
-__device__ __forceinline__ void load8(const void* base, int64_t at, float (&f)[8]) {
-  if constexpr (DT == GWA_DT_F32) {
-    const float4* p = (const float4*)((const float*)base + at);
-    const float4 a = p[0], b = p[1];
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-  } else {
-    const v4i r = *(const v4i*)((const uint16_t*)base + at);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t w = (uint32_t)r[i];
-      f[2 * i] = DT == GWA_DT_BF16 ? bf16_lo(w) : f16_bits_to_f32((uint16_t)w);
-      f[2 * i + 1] = DT == GWA_DT_BF16 ? bf16_hi(w) : f16_bits_to_f32((uint16_t)(w >> 16));
-    }
-  }
-}
-template <int DT>
-__device__ __forceinline__ void store8(void* base, int64_t at, const float (&f)[8]) {
-  if constexpr (DT == GWA_DT_F32) {
-    float4* p = (float4*)((float*)base + at);
-    p[0] = make_float4(f[0], f[1], f[2], f[3]);
-    p[1] = make_float4(f[4], f[5], f[6], f[7]);
-  } else {
-    v4i r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      r[i] = (int)(DT == GWA_DT_BF16 ? Bf16::pack(f[2 * i], f[2 * i + 1]) : Fp16::pack(f[2 * i], f[2 * i + 1]));
-    *(v4i*)((uint16_t*)base + at) = r;
-  }
-}
-template <int DT>
-__device__ __forceinline__ float load1(const void* base, int64_t at) {
-  if constexpr (DT == GWA_DT_F32) return ((const float*)base)[at];
-  else return DT == GWA_DT_BF16 ? Bf16::load(((const uint16_t*)base)[at]) : Fp16::load(((const uint16_t*)base)[at]);
-}
-template <int DT>
-__device__ __forceinline__ void store1(void* base, int64_t at, float f) {
-  if constexpr (DT == GWA_DT_F32) ((float*)base)[at] = f;
-  else ((uint16_t*)base)[at] = DT == GWA_DT_BF16 ? f32_to_bf16(f) : f32_to_f16_bits(f);
-}
-
-struct Rotation {
-  const float* cos_t;
-  const float* sin_t;
-  const int32_t* positions;
-  int64_t table_rows;
-  int rot, interleaved;
-  float sign;  // -1 rotates back
-};
-
-__device__ __forceinline__ int64_t table_row(const Rotation& r, int64_t t) {
-  int64_t p = r.positions ? r.positions[t] : t;
-  p = min(max(p, (int64_t)0), r.table_rows - 1);
-  return p * (r.rot / 2);
-}
-
-// Elements a unit of work covers: 16 with VEC (8 pairs, or 16 channels past the rotated ones; both halves of the
-// half layout lie on 16-byte pieces then), else one pair / two channels. One unit reads all it writes before it
-// writes, so x and y may be the same.
-template <int DT, bool VEC>
-__device__ __forceinline__ void rotate_unit(const void* x, int64_t xo, void* y, int64_t yo, const Rotation& r,
-                                            int64_t row, int unit) {
-  const int half = r.rot / 2;
-  if constexpr (VEC) {
-    const bool tail = 16 * unit >= r.rot;
-    // first and second piece of 8: the pairs' two halves, or neighbours
-    const int c0 = tail || r.interleaved ? 16 * unit : 8 * unit;
-    const int c1 = tail || r.interleaved ? c0 + 8 : c0 + half;
-    float a[8], b[8];
-    load8<DT>(x, xo + c0, a);
-    load8<DT>(x, xo + c1, b);
-    if (!tail) {
-      float c[8], s[8];
-      load8<GWA_DT_F32>(r.cos_t, row + 8 * unit, c);
-      load8<GWA_DT_F32>(r.sin_t, row + 8 * unit, s);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s[i] *= r.sign;
-      if (r.interleaved) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float e = a[2 * i], o = a[2 * i + 1];
-          a[2 * i] = fmaf(e, c[i], -o * s[i]);
-          a[2 * i + 1] = fmaf(e, s[i], o * c[i]);
-          const float e2 = b[2 * i], o2 = b[2 * i + 1];
-          b[2 * i] = fmaf(e2, c[4 + i], -o2 * s[4 + i]);
-          b[2 * i + 1] = fmaf(e2, s[4 + i], o2 * c[4 + i]);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float e = a[i], o = b[i];
-          a[i] = fmaf(e, c[i], -o * s[i]);
-          b[i] = fmaf(e, s[i], o * c[i]);
-        }
-      }
-    }
-    store8<DT>(y, yo + c0, a);
-    store8<DT>(y, yo + c1, b);
-  } else {
-    const bool tail = 2 * unit >= r.rot;
-    const int c0 = tail || r.interleaved ? 2 * unit : unit;
-    const int c1 = tail || r.interleaved ? c0 + 1 : c0 + half;
-    float a = load1<DT>(x, xo + c0), b = load1<DT>(x, xo + c1);
-    if (!tail) {
-      const float c = r.cos_t[row + unit], s = r.sin_t[row + unit] * r.sign, e = a;
-      a = fmaf(e, c, -b * s);
-      b = fmaf(e, s, b * c);
-    }
-    store1<DT>(y, yo + c0, a);
-    store1<DT>(y, yo + c1, b);
-  }
-}
 
 // A thread a unit; the tables' rows are shared by a token's heads in L1. 16411 tokens, 24 heads of 128, half of each head
 // rotated, bf16: 41 us for 202 MB, 4.9 TB/s; fp32 91 us for 403 MB, 4.4 TB/s.
@@ -146,23 +32,12 @@ __global__ __launch_bounds__(RT_THREADS) void paged_write_kernel(PagedArgs c, co
                                                                  int64_t ldkh, const uint16_t* v, int64_t ldvt,
                                                                  int64_t ldvh, uint16_t* q_out, Rotation r, int tokens,
                                                                  int heads, int head_dim, int units) {
-  const int t = blockIdx.x, lane = threadIdx.x & 63;
-  // the token's sequence: the number of sequences that end at or before it (q_start ascends; empty ones end where
-  // they start)
-  int b = 0;
-  for (int i = 0; i < c.batch; i += 64)
-    b += __popcll(__ballot(i + lane < c.batch && c.q_start[min(i + lane, c.batch - 1) + 1] <= t));
+  const int t = blockIdx.x;
+  const TokenPlace place = token_place(c, t, tokens);
   int64_t at = -1, wat = 0;
-  if (b < c.batch) {
-    int t0, n;
-    paged_new(c, b, tokens, t0, n);
-    const int64_t place = (int64_t)c.kv_len[b] - n + (t - t0);
-    if (t >= t0 && t - t0 < n && place >= 0 && place < c.capacity) {
-      const int slot = (int)place;
-      const int page = paged_page(c, c.table + b * c.table_stride, slot);
-      at = paged_at(c, page, 0, slot);
-      wat = paged_w_at(c, page, 0, slot);
-    }
+  if (place.slot >= 0) {
+    at = paged_at(c, place.page, 0, place.slot);
+    wat = paged_w_at(c, place.page, 0, place.slot);
   }
   const int64_t row = r.rot ? table_row(r, t) : 0;
   const Rotation none = {nullptr, nullptr, nullptr, 0, 0, 0, 1.0f};
@@ -179,23 +54,6 @@ __global__ __launch_bounds__(RT_THREADS) void paged_write_kernel(PagedArgs c, co
   }
   if (at >= 0 && c.w)
     for (int h = threadIdx.x; h < hk; h += RT_THREADS) c.w[wat + h * c.w_head_stride] = 0.0f;
-}
-
-int rotation_check(const char* what, const float* cos_t, const float* sin_t, int64_t table_rows, int64_t head_dim,
-                   int64_t rot) {
-  GWA_REQUIRE(rot >= 0 && rot <= head_dim && rot % 2 == 0, "%s: %lld rotated channels of %lld (an even number expected)",
-              what, (long long)rot, (long long)head_dim);
-  GWA_REQUIRE(rot == 0 || (cos_t && sin_t && table_rows > 0 && table_rows < (1ll << 31)),
-              "%s: a table of %lld positions", what, (long long)table_rows);
-  return GWA_OK;
-}
-
-// whether every unit of 16 elements lies on 16-byte pieces of x and y and of the tables
-bool vector_units(int64_t head_dim, int64_t rot, const float* cos_t, const float* sin_t) {
-  return head_dim % 16 == 0 && rot % 16 == 0 && (rot == 0 || (GWA_ALIGNED(cos_t, 16) && GWA_ALIGNED(sin_t, 16)));
-}
-bool vector_operand(const void* p, int64_t ldt, int64_t ldh, int elem) {
-  return GWA_ALIGNED(p, 16) && ldt * elem % 16 == 0 && ldh * elem % 16 == 0;
 }
 
 }  // namespace
@@ -451,19 +309,24 @@ __global__ __launch_bounds__(EC_THREADS) void evict_copy_kernel(PagedArgs c, con
     const v4i kk = *(const v4i*)(c.k + src), vv = *(const v4i*)(c.v + src);
     *(v4i*)(c.k + dst) = kk;
     *(v4i*)(c.v + dst) = vv;
-    if (p == 0) c.w[paged_w_at(c, to, h, r)] = c.w[paged_w_at(c, from, h, j)];
+    if (p == 0) {
+      c.w[paged_w_at(c, to, h, r)] = c.w[paged_w_at(c, from, h, j)];
+      if (c.ks) {
+        c.ks[paged_s_at(c, to, h, r)] = c.ks[paged_s_at(c, from, h, j)];
+        c.vs[paged_s_at(c, to, h, r)] = c.vs[paged_s_at(c, from, h, j)];
+      }
+    }
   }
 }
 
-}  // namespace
-
-extern "C" int gwa_paged_evict(const gwa_paged_cache* cache, const int32_t* new_table, int64_t new_stride,
-                               int64_t new_width, int64_t max_kv, int64_t budget, int64_t recent, int32_t* kept,
-                               int32_t* new_len, void* stream) {
-  const char* what = "paged_evict";
+// The entry points' body; `scales`: of an 8-bit cache, whose rows the copy takes as 16-bit elements of half as many
+int evict_call(const char* what, const gwa_paged_cache* cache, const gwa_paged_scales* scales, const int32_t* new_table,
+               int64_t new_stride, int64_t new_width, int64_t max_kv, int64_t budget, int64_t recent, int32_t* kept,
+               int32_t* new_len, void* stream) {
   PagedArgs c;
-  const int bad = paged_check(what, cache, false, true, &c);
+  const int bad = paged_check(what, cache, false, true, &c, scales);
   if (bad != GWA_OK) return bad;
+  if (scales) c.page_stride /= 2, c.head_stride /= 2, c.slot_stride /= 2;
   GWA_REQUIRE(budget > 0 && budget < (1ll << 30) && recent >= 0 && recent <= budget,
               "%s: a budget of %lld keys, %lld of them recent", what, (long long)budget, (long long)recent);
   GWA_REQUIRE(max_kv >= 0 && max_kv <= c.capacity, "%s: max_kv %lld in a table of %d slots", what, (long long)max_kv,
@@ -475,7 +338,7 @@ extern "C" int gwa_paged_evict(const gwa_paged_cache* cache, const int32_t* new_
   if (c.batch == 0) return GWA_OK;
   GWA_REQUIRE(kept && new_len && (new_table || new_width == 0), "%s: null pointer", what);
   const int64_t groups = (int64_t)c.batch * c.kv_heads;
-  const int pieces = cache->head_dim / 8;
+  const int pieces = cache->head_dim / (scales ? 16 : 8);
   const int64_t blocks = (std::max<int64_t>(most, 1) * pieces + EC_THREADS - 1) / EC_THREADS;
   GWA_REQUIRE(groups < 65536 && blocks < (1ll << 31), "%s: %lld heads of sequences are too many", what,
               (long long)groups);
@@ -488,4 +351,21 @@ extern "C" int gwa_paged_evict(const gwa_paged_cache* cache, const int32_t* new_
                      (hipStream_t)stream, c, new_table, new_stride, (int)(new_width * cache->page_size), kept,
                      (int)budget, pieces);
   return gwa_check_launch(what);
+}
+
+}  // namespace
+
+extern "C" int gwa_paged_evict(const gwa_paged_cache* cache, const int32_t* new_table, int64_t new_stride,
+                               int64_t new_width, int64_t max_kv, int64_t budget, int64_t recent, int32_t* kept,
+                               int32_t* new_len, void* stream) {
+  return evict_call("paged_evict", cache, nullptr, new_table, new_stride, new_width, max_kv, budget, recent, kept, new_len,
+                    stream);
+}
+
+extern "C" int gwa_paged_evict_fp8(const gwa_paged_cache* cache, const gwa_paged_scales* scales,
+                                   const int32_t* new_table, int64_t new_stride, int64_t new_width, int64_t max_kv,
+                                   int64_t budget, int64_t recent, int32_t* kept, int32_t* new_len, void* stream) {
+  const char* what = "paged_evict_fp8";
+  GWA_REQUIRE(scales, "%s: null scales", what);
+  return evict_call(what, cache, scales, new_table, new_stride, new_width, max_kv, budget, recent, kept, new_len, stream);
 }

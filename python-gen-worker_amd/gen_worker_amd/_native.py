@@ -51,7 +51,21 @@ class PagedCacheArgs(ctypes.Structure):
                 ("batch", _i64), ("page_size", _int), ("kv_heads", _int), ("head_dim", _int), ("dtype", _int)]
 
 
+class PagedScalesArgs(ctypes.Structure):
+    """``gwa_paged_scales`` of the header."""
+
+    _fields_ = [("k", _vp), ("v", _vp), ("page_stride", _i64), ("head_stride", _i64)]
+
+
+class SamplingArgs(ctypes.Structure):
+    """``gwa_sampling`` of the header."""
+
+    _fields_ = [("temperature", _vp), ("top_k", _vp), ("top_p", _vp), ("min_p", _vp), ("all_temperature", _flt),
+                ("all_top_k", ctypes.c_int32), ("all_top_p", _flt), ("all_min_p", _flt)]
+
+
 _cache = ctypes.POINTER(PagedCacheArgs)
+_scales = ctypes.POINTER(PagedScalesArgs)
 
 # name -> argtypes (all return int status unless listed in _RESTYPES)
 _SIGNATURES: dict[str, tuple] = {
@@ -117,6 +131,13 @@ _SIGNATURES: dict[str, tuple] = {
     "gwa_paged_attention": (_cache, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _flt, _int, _int, _vp, _i64,
                             _vp),
     "gwa_paged_evict": (_cache, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp),
+    "gwa_paged_write_fp8": (_cache, _scales, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp,
+                            _i64, _i64, _i64, _int, _vp),
+    "gwa_paged_read_fp8": (_cache, _scales, _vp, _vp, _i64, _vp),
+    "gwa_paged_attention_fp8": (_cache, _scales, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _flt, _int, _int,
+                                _vp, _i64, _vp),
+    "gwa_paged_evict_fp8": (_cache, _scales, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp),
+    "gwa_sample_tokens": (_vp, _i64, _int, _vp, ctypes.POINTER(SamplingArgs), _vp, _vp, _i64, _i64, _vp),
 }
 _RESTYPES = {"gwa_build_info": ctypes.c_char_p, "gwa_last_error": ctypes.c_char_p,
              "gwa_svdq_quant_fp6_partials": ctypes.c_int64, "gwa_svdq_gemm_w4a4_fp6_next_partials": ctypes.c_int64,

@@ -30,7 +30,8 @@ ARCH = "gfx950"
 
 SOURCES = ("gwa_runtime.hip", "act_quant.hip", "w4a4_gemm.hip", "w4a4_gemm_fp6.hip", "w4a4_gemm_fp6_pipe.hip",
            "w4a4_linear.hip", "w8a8_gemm.hip", "awq_w4a16.hip", "nvfp4.hip", "dit_block.hip",
-           "w4a4_gemv.hip", "dit_attention.hip", "paged_cache.hip", "paged_attention.hip")
+           "w4a4_gemv.hip", "dit_attention.hip", "paged_cache.hip", "paged_attention.hip", "paged_attention_fp8.hip",
+           "paged_cache_fp8.hip", "sampling.hip")
 
 HIPCC_FLAGS = [
     f"--offload-arch={ARCH}",

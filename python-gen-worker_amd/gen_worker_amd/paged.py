@@ -13,9 +13,14 @@ head), a sequence in the pages its row of a table lists, and new tokens of sever
   with ``weights`` it also adds up the attention each key draws.
 * ``paged_evict``: the keys that drew least dropped, the others copied to fresh pages.
 
+The cache's values are bf16 or fp16, or 8 bits: e4m3 codes (``torch.float8_e4m3fn``) and for every row (one slot of one kv
+head) a scale byte, value = code * 2^(scale - 127), which halves what attention reads a key. ``paged_write_fp8``,
+``paged_attention_fp8`` and ``paged_evict_fp8`` are the operators on such a cache, ``paged_read_fp8`` gives its rows back as
+16-bit values (``csrc/paged_cache_fp8.hip``, ``csrc/paged_attention_fp8.hip``).
+
 ``PagedCache`` keeps the pool, the page lists and the lengths on the host and calls them. Everything runs on the current
 stream; the functions do not synchronise and may be captured in a HIP graph (outputs come from torch's allocator).
-The cache's values are bf16 or fp16; scores, softmax statistics, sums and gathered weights are fp32. CPU tensors
+Scores, softmax statistics, sums and gathered weights are fp32. CPU tensors
 are refused: there is no CPU implementation.
 """
 
@@ -33,6 +38,7 @@ from torch.autograd import forward_ad
 from . import _native as nat
 from . import ops
 
+FP8 = torch.float8_e4m3fn
 _DTYPES = {torch.bfloat16: nat.DT_BF16, torch.float16: nat.DT_F16, torch.float32: nat.DT_F32}
 
 
@@ -245,12 +251,16 @@ def rotary_embed(x: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor
 # ---------------------------------------------------------------------------
 
 def _cache_args(name: str, k_pages: Tensor, v_pages: Tensor, weights: Optional[Tensor], table: Tensor,
-                q_start: Optional[Tensor], kv_len: Tensor) -> nat.PagedCacheArgs:
+                q_start: Optional[Tensor], kv_len: Tensor, dtype: Optional[torch.dtype] = None) -> nat.PagedCacheArgs:
+    """``dtype``: of an 8-bit cache, the type of the call's values."""
     dev = k_pages.device
-    _require(k_pages.is_cuda and k_pages.dtype in (torch.bfloat16, torch.float16) and k_pages.dim() == 4
-             and k_pages.stride(3) == 1, name,
-             f"k_pages must be a bf16 or fp16 CUDA tensor [pages, kv_heads, page_size, head_dim] with unit last stride, "
-             f"got {k_pages.dtype} {list(k_pages.shape)} strides {k_pages.stride()} on {k_pages.device}")
+    held = (torch.bfloat16, torch.float16) if dtype is None else (FP8,)
+    _require(k_pages.is_cuda and k_pages.dtype in held and k_pages.dim() == 4 and k_pages.stride(3) == 1, name,
+             f"k_pages must be a {'bf16 or fp16' if dtype is None else FP8} CUDA tensor [pages, kv_heads, page_size, "
+             f"head_dim] with unit last stride, got {k_pages.dtype} {list(k_pages.shape)} strides {k_pages.stride()} on "
+             f"{k_pages.device}")
+    _require(dtype is None or dtype in (torch.bfloat16, torch.float16), name,
+             f"the values of an 8-bit cache are taken as bf16 or fp16, not {dtype}")
     _require(v_pages.dtype == k_pages.dtype and v_pages.device == dev and v_pages.shape == k_pages.shape
              and v_pages.stride() == k_pages.stride(), name,
              f"v_pages must have k_pages' type, shape and strides, got {v_pages.dtype} {list(v_pages.shape)} strides "
@@ -272,17 +282,29 @@ def _cache_args(name: str, k_pages: Tensor, v_pages: Tensor, weights: Optional[T
     args = nat.PagedCacheArgs(k_pages.data_ptr(), v_pages.data_ptr(), nat.ptr(weights), table.data_ptr(),
                               nat.ptr(q_start), kv_len.data_ptr(), k_pages.stride(0), k_pages.stride(1),
                               k_pages.stride(2), ws[0], ws[1], pages, row, table.shape[1], batch, size, heads, dim,
-                              _DTYPES[k_pages.dtype])
+                              _DTYPES[k_pages.dtype if dtype is None else dtype])
     args.table_kept = table  # a copy lives until the call has been made
     return args
 
 
+def _scale_args(name: str, k_pages: Tensor, k_scales: Tensor, v_scales: Tensor) -> nat.PagedScalesArgs:
+    shape = tuple(k_pages.shape[:3])
+    for what, t in (("k_scales", k_scales), ("v_scales", v_scales)):
+        _require(t.dtype == torch.uint8 and t.device == k_pages.device and tuple(t.shape) == shape
+                 and t.stride() == k_scales.stride() and (shape[2] == 1 or t.stride(2) == 1), name,
+                 f"{what} must be uint8 {list(shape)} on {k_pages.device} with unit last stride (v_scales at k_scales' "
+                 f"strides), got {t.dtype} {list(t.shape)} strides {t.stride()} on {t.device}")
+    return nat.PagedScalesArgs(k_scales.data_ptr(), v_scales.data_ptr(), k_scales.stride(0), k_scales.stride(1))
+
+
 def _write_body(q: Tensor, k: Tensor, v: Tensor, cos: Optional[Tensor], sin: Optional[Tensor],
                 positions: Optional[Tensor], k_pages: Tensor, v_pages: Tensor, table: Tensor, q_start: Tensor,
-                kv_len: Tensor, weights: Optional[Tensor], interleaved: bool) -> Tensor:
-    name = "paged_write"
-    args = _cache_args(name, k_pages, v_pages, weights, table, q_start, kv_len)
-    dev, dt, d = k_pages.device, k_pages.dtype, args.head_dim
+                kv_len: Tensor, weights: Optional[Tensor], interleaved: bool,
+                scales: Optional[tuple[Tensor, Tensor]] = None) -> Tensor:
+    name = "paged_write" if scales is None else "paged_write_fp8"
+    dev, dt = k_pages.device, k_pages.dtype if scales is None else q.dtype
+    args = _cache_args(name, k_pages, v_pages, weights, table, q_start, kv_len, None if scales is None else dt)
+    d = args.head_dim
     _require(q.dim() == 3, name, f"q must be [tokens, heads, {d}], got {list(q.shape)}")
     t, h = int(q.shape[0]), int(q.shape[1])
     _heads(name, "q", q, dt, dev, t, h, d)
@@ -290,9 +312,13 @@ def _write_body(q: Tensor, k: Tensor, v: Tensor, cos: Optional[Tensor], sin: Opt
     _heads(name, "v", v, dt, dev, t, args.kv_heads, d)
     rot, rows = _tables(name, cos, sin, positions, t, d, dev)
     out = torch.empty((t, h, d), dtype=dt, device=dev)
-    nat.call("gwa_paged_write", ctypes.byref(args), q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0),
-             k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), nat.ptr(cos), nat.ptr(sin), rows, nat.ptr(positions),
-             out.data_ptr(), t, h, rot, int(interleaved), nat.stream_of(k_pages))
+    rest = (q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+            v.stride(1), nat.ptr(cos), nat.ptr(sin), rows, nat.ptr(positions), out.data_ptr(), t, h, rot,
+            int(interleaved), nat.stream_of(k_pages))
+    if scales is None:
+        nat.call("gwa_paged_write", ctypes.byref(args), *rest)
+    else:
+        nat.call("gwa_paged_write_fp8", ctypes.byref(args), ctypes.byref(_scale_args(name, k_pages, *scales)), *rest)
     return out
 
 
@@ -332,14 +358,14 @@ def paged_write(q: Tensor, k: Tensor, v: Tensor, cos: Optional[Tensor], sin: Opt
 
 
 def _attention_body(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, q_start: Tensor, kv_len: Tensor,
-                    max_q: int, max_kv: int, scale: float, causal: bool,
-                    weights: Optional[Tensor]) -> tuple[Tensor, Tensor]:
-    name = "paged_attention"
-    args = _cache_args(name, k_pages, v_pages, weights, table, q_start, kv_len)
+                    max_q: int, max_kv: int, scale: float, causal: bool, weights: Optional[Tensor],
+                    scales: Optional[tuple[Tensor, Tensor]] = None) -> tuple[Tensor, Tensor]:
+    name = "paged_attention" if scales is None else "paged_attention_fp8"
+    args = _cache_args(name, k_pages, v_pages, weights, table, q_start, kv_len, None if scales is None else q.dtype)
     d, hk = args.head_dim, args.kv_heads
     _require(q.dim() == 3, name, f"q must be [tokens, heads, {d}], got {list(q.shape)}")
     t, h = int(q.shape[0]), int(q.shape[1])
-    _heads(name, "q", q, k_pages.dtype, k_pages.device, t, h, d)
+    _heads(name, "q", q, k_pages.dtype if scales is None else q.dtype, k_pages.device, t, h, d)
     _require(h > 0 and hk > 0 and h % hk == 0, name, f"{h} query heads over {hk} kv heads")
     if t and (q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16 or q.stride(0) == 0 or q.stride(1) == 0):
         q = q.contiguous() if not q.is_contiguous() else q.clone()
@@ -350,8 +376,12 @@ def _attention_body(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, 
     n = int(lib.gwa_paged_attention_workspace(args.batch, t, h, hk, d, max_q, max_kv,
                                               args.table_width * args.page_size, gather))
     ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-    nat.call("gwa_paged_attention", ctypes.byref(args), q.data_ptr(), q.stride(0), q.stride(1), o.data_ptr(),
-             lse.data_ptr(), t, h, max_q, max_kv, scale, int(causal), gather, nat.ptr(ws), n, nat.stream_of(q))
+    rest = (q.data_ptr(), q.stride(0), q.stride(1), o.data_ptr(), lse.data_ptr(), t, h, max_q, max_kv, scale,
+            int(causal), gather, nat.ptr(ws), n, nat.stream_of(q))
+    if scales is None:
+        nat.call("gwa_paged_attention", ctypes.byref(args), *rest)
+    else:
+        nat.call("gwa_paged_attention_fp8", ctypes.byref(args), ctypes.byref(_scale_args(name, k_pages, *scales)), *rest)
     return o, lse
 
 
@@ -396,10 +426,12 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, 
 
 
 def _evict_body(k_pages: Tensor, v_pages: Tensor, weights: Tensor, table: Tensor, kv_len: Tensor, max_kv: int,
-                new_table: Tensor, budget: int, recent: int) -> tuple[Tensor, Tensor]:
-    name = "paged_evict"
+                new_table: Tensor, budget: int, recent: int,
+                scales: Optional[tuple[Tensor, Tensor]] = None) -> tuple[Tensor, Tensor]:
+    name = "paged_evict" if scales is None else "paged_evict_fp8"
     _require(weights is not None, name, "weights are needed")
-    args = _cache_args(name, k_pages, v_pages, weights, table, None, kv_len)
+    args = _cache_args(name, k_pages, v_pages, weights, table, None, kv_len,
+                       None if scales is None else torch.bfloat16)   # rows are copied as they are
     dev = k_pages.device
     _require(budget > 0 and 0 <= recent <= budget, name, f"a budget of {budget} keys, {recent} of them recent")
     _ints(name, "new_table", new_table, (args.batch, new_table.shape[-1] if new_table.dim() == 2 else -1), dev)
@@ -407,8 +439,12 @@ def _evict_body(k_pages: Tensor, v_pages: Tensor, weights: Tensor, table: Tensor
              f"new_table's rows overlap (row stride {new_table.stride(0)}): sequences would be copied into one page")
     kept = torch.empty((args.batch, args.kv_heads, budget), dtype=torch.int32, device=dev)
     new_len = torch.empty(args.batch, dtype=torch.int32, device=dev)
-    nat.call("gwa_paged_evict", ctypes.byref(args), new_table.data_ptr(), max(new_table.stride(0), new_table.shape[1]),
-             new_table.shape[1], max_kv, budget, recent, kept.data_ptr(), new_len.data_ptr(), nat.stream_of(k_pages))
+    rest = (new_table.data_ptr(), max(new_table.stride(0), new_table.shape[1]), new_table.shape[1], max_kv, budget,
+            recent, kept.data_ptr(), new_len.data_ptr(), nat.stream_of(k_pages))
+    if scales is None:
+        nat.call("gwa_paged_evict", ctypes.byref(args), *rest)
+    else:
+        nat.call("gwa_paged_evict_fp8", ctypes.byref(args), ctypes.byref(_scale_args(name, k_pages, *scales)), *rest)
     return kept, new_len
 
 
@@ -445,6 +481,150 @@ def paged_evict(k_pages: Tensor, v_pages: Tensor, weights: Tensor, table: Tensor
 
 
 # ---------------------------------------------------------------------------
+# the cache in 8 bits
+# ---------------------------------------------------------------------------
+
+@torch.library.custom_op("cozy_gen_worker::paged_write_fp8",
+                         mutates_args=("k_pages", "v_pages", "k_scales", "v_scales", "weights"))
+def _write_fp8_op(q: Tensor, k: Tensor, v: Tensor, cos: Optional[Tensor], sin: Optional[Tensor],
+                  positions: Optional[Tensor], k_pages: Tensor, v_pages: Tensor, k_scales: Tensor, v_scales: Tensor,
+                  table: Tensor, q_start: Tensor, kv_len: Tensor, weights: Optional[Tensor],
+                  interleaved: bool) -> Tensor:
+    return _write_body(q, k, v, cos, sin, positions, k_pages, v_pages, table, q_start, kv_len, weights, interleaved,
+                       (k_scales, v_scales))
+
+
+@_write_fp8_op.register_fake
+def _(q, k, v, cos, sin, positions, k_pages, v_pages, k_scales, v_scales, table, q_start, kv_len, weights, interleaved):
+    return q.new_empty(q.shape)
+
+
+def paged_write_fp8(q: Tensor, k: Tensor, v: Tensor, cos: Optional[Tensor], sin: Optional[Tensor],
+                    positions: Optional[Tensor], k_pages: Tensor, v_pages: Tensor, k_scales: Tensor, v_scales: Tensor,
+                    table: Tensor, q_start: Tensor, kv_len: Tensor, *, weights: Optional[Tensor] = None,
+                    interleaved: bool = False) -> Tensor:
+    """``paged_write`` into a cache of 8 bits: k_pages and v_pages float8_e4m3fn [pages, kv_heads, page_size, head_dim]
+    (strides multiples of 16, head_dim one of 16 to 256), k_scales and v_scales uint8 [pages, kv_heads, page_size]. q, k and
+    v are bf16 or fp16; so are the rotated queries that it returns.
+
+    A row of k (rotated, in fp32) or v takes as its scale the smallest power of two, from 2^-126 on, under which none of its
+    finite values passes 448, the largest code: value = code * 2^(scale - 127). Values are rounded once, to the nearest
+    code (ties to even), and never past the largest finite value of q's type; what is not finite is stored as NaN."""
+    a = (q, k, v, cos, sin, positions, k_pages, v_pages, k_scales, v_scales, table, q_start, kv_len, weights)
+    _no_tangents("paged_write_fp8", q, k, v, cos, sin, weights)
+    host = _host()
+    if host is not None:
+        out = host.paged_write_fp8(*a, interleaved)
+        if out is not None:
+            return out
+    if _plain(*a):
+        out = _write_body(q, k, v, cos, sin, positions, k_pages, v_pages, table, q_start, kv_len, weights, interleaved,
+                          (k_scales, v_scales))
+        return _written(out, k_pages, v_pages, k_scales, v_scales, weights)
+    return _write_fp8_op(*a, interleaved)
+
+
+def _read_fp8_body(k_pages: Tensor, v_pages: Tensor, k_scales: Tensor, v_scales: Tensor, table: Tensor, q_start: Tensor,
+                   kv_len: Tensor, tokens: int, dtype: torch.dtype) -> tuple[Tensor, Tensor]:
+    name = "paged_read_fp8"
+    args = _cache_args(name, k_pages, v_pages, None, table, q_start, kv_len, dtype)
+    scales = _scale_args(name, k_pages, k_scales, v_scales)
+    _require(tokens >= 0, name, f"{tokens} tokens")
+    k = torch.empty((tokens, args.kv_heads, args.head_dim), dtype=dtype, device=k_pages.device)
+    v = torch.empty_like(k)
+    nat.call("gwa_paged_read_fp8", ctypes.byref(args), ctypes.byref(scales), k.data_ptr(), v.data_ptr(), tokens,
+             nat.stream_of(k_pages))
+    return k, v
+
+
+@torch.library.custom_op("cozy_gen_worker::paged_read_fp8", mutates_args=())
+def _read_fp8_op(k_pages: Tensor, v_pages: Tensor, k_scales: Tensor, v_scales: Tensor, table: Tensor, q_start: Tensor,
+                 kv_len: Tensor, tokens: int, dtype: torch.dtype) -> tuple[Tensor, Tensor]:
+    return _read_fp8_body(k_pages, v_pages, k_scales, v_scales, table, q_start, kv_len, tokens, dtype)
+
+
+@_read_fp8_op.register_fake
+def _(k_pages, v_pages, k_scales, v_scales, table, q_start, kv_len, tokens, dtype):
+    shape = (tokens, k_pages.shape[1], k_pages.shape[3])
+    return k_pages.new_empty(shape, dtype=dtype), k_pages.new_empty(shape, dtype=dtype)
+
+
+def paged_read_fp8(k_pages: Tensor, v_pages: Tensor, k_scales: Tensor, v_scales: Tensor, table: Tensor, q_start: Tensor,
+                   kv_len: Tensor, tokens: int, *, dtype: torch.dtype = torch.bfloat16) -> tuple[Tensor, Tensor]:
+    """What rows of an 8-bit cache stand for: (k, v) [tokens, kv_heads, head_dim] in ``dtype`` (bf16: exactly). Sequence b's
+    rows q_start[b] to q_start[b + 1] - 1 are those of its last slots, as ``paged_write_fp8`` takes them: with q_start the
+    running sums of kv_len, everything its sequences hold. ``tokens``: rows in all (q_start's last entry). Rows that belong
+    to no sequence, or to slots before a sequence's first, are not written."""
+    a = (k_pages, v_pages, k_scales, v_scales, table, q_start, kv_len)
+    host = _host()
+    if host is not None:
+        out = host.paged_read_fp8(*a, tokens, dtype)
+        if out is not None:
+            return out
+    if _plain(*a):
+        return _read_fp8_body(*a, tokens, dtype)
+    return _read_fp8_op(*a, tokens, dtype)
+
+
+@torch.library.custom_op("cozy_gen_worker::paged_attention_fp8", mutates_args=("weights",))
+def _attention_fp8_op(q: Tensor, k_pages: Tensor, v_pages: Tensor, k_scales: Tensor, v_scales: Tensor, table: Tensor,
+                      q_start: Tensor, kv_len: Tensor, max_q: int, max_kv: int, scale: float, causal: bool,
+                      weights: Optional[Tensor]) -> tuple[Tensor, Tensor]:
+    return _attention_body(q, k_pages, v_pages, table, q_start, kv_len, max_q, max_kv, scale, causal, weights,
+                           (k_scales, v_scales))
+
+
+@_attention_fp8_op.register_fake
+def _(q, k_pages, v_pages, k_scales, v_scales, table, q_start, kv_len, max_q, max_kv, scale, causal, weights):
+    return q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)
+
+
+def paged_attention_fp8(q: Tensor, k_pages: Tensor, v_pages: Tensor, k_scales: Tensor, v_scales: Tensor, table: Tensor,
+                        q_start: Tensor, kv_len: Tensor, max_q: int, max_kv: int, *, scale: Optional[float] = None,
+                        causal: bool = True, weights: Optional[Tensor] = None) -> tuple[Tensor, Tensor]:
+    """``paged_attention`` over an 8-bit cache (see ``paged_write_fp8``): keys and values are what its rows stand for, in
+    q's type (bf16 or fp16; a scale byte of 255 reads as NaN). head_dim: a multiple of 16 up to 256."""
+    if scale is None:
+        scale = float(q.shape[-1]) ** -0.5
+    _no_tangents("paged_attention_fp8", q, weights)
+    a = (q, k_pages, v_pages, k_scales, v_scales, table, q_start, kv_len)
+    host = _host()
+    if host is not None:
+        out = host.paged_attention_fp8(*a, weights, max_q, max_kv, scale, causal)
+        if out is not None:
+            return out
+    if _plain(*a, weights):
+        return _written(_attention_body(q, k_pages, v_pages, table, q_start, kv_len, max_q, max_kv, scale, causal,
+                                        weights, (k_scales, v_scales)), weights)
+    return _attention_fp8_op(*a, max_q, max_kv, scale, causal, weights)
+
+
+@torch.library.custom_op("cozy_gen_worker::paged_evict_fp8",
+                         mutates_args=("k_pages", "v_pages", "k_scales", "v_scales", "weights"))
+def _evict_fp8_op(k_pages: Tensor, v_pages: Tensor, k_scales: Tensor, v_scales: Tensor, weights: Tensor, table: Tensor,
+                  kv_len: Tensor, max_kv: int, new_table: Tensor, budget: int, recent: int) -> tuple[Tensor, Tensor]:
+    return _evict_body(k_pages, v_pages, weights, table, kv_len, max_kv, new_table, budget, recent,
+                       (k_scales, v_scales))
+
+
+@_evict_fp8_op.register_fake
+def _(k_pages, v_pages, k_scales, v_scales, weights, table, kv_len, max_kv, new_table, budget, recent):
+    b = kv_len.shape[0]
+    return kv_len.new_empty((b, k_pages.shape[1], budget)), kv_len.new_empty((b,))
+
+
+def paged_evict_fp8(k_pages: Tensor, v_pages: Tensor, k_scales: Tensor, v_scales: Tensor, weights: Tensor, table: Tensor,
+                    kv_len: Tensor, max_kv: int, new_table: Tensor, budget: int, recent: int) -> tuple[Tensor, Tensor]:
+    """``paged_evict`` of an 8-bit cache: codes and scales are copied as they are."""
+    a = (k_pages, v_pages, k_scales, v_scales, weights, table, kv_len)
+    _no_tangents("paged_evict_fp8", weights)
+    if _plain(*a, new_table):
+        return _written(_evict_body(k_pages, v_pages, weights, table, kv_len, max_kv, new_table, budget, recent,
+                                    (k_scales, v_scales)), k_pages, v_pages, k_scales, v_scales, weights)
+    return _evict_fp8_op(*a, max_kv, new_table, budget, recent)
+
+
+# ---------------------------------------------------------------------------
 # the cache and its batches
 # ---------------------------------------------------------------------------
 
@@ -463,7 +643,8 @@ class PagedBatch:
 
 
 class PagedCache:
-    """A pool of ``pages`` pages for the keys and values of one layer's kv heads, and the sequences in it.
+    """A pool of ``pages`` pages for the keys and values of one layer's kv heads, and the sequences in it. ``dtype``: bf16,
+    fp16, or ``torch.float8_e4m3fn`` for a cache in 8 bits, whose calls take queries, keys and values of either of the others.
 
     Page lists, lengths and the free list are host state; device work is enqueued on the current stream in call order, so
     use one stream for one cache (or order the streams). ``weights=True`` keeps each key's gathered attention
@@ -475,17 +656,25 @@ class PagedCache:
         name = "PagedCache"
         _require(pages > 0 and kv_heads > 0 and 8 <= page_size <= 4096 and page_size & (page_size - 1) == 0, name,
                  f"{pages} pages of {page_size} slots (a power of two, 8 to 4096), {kv_heads} kv heads")
-        _require(dtype in (torch.bfloat16, torch.float16) and head_dim % 8 == 0 and 8 <= head_dim <= 256, name,
-                 f"{dtype} heads of {head_dim} (bf16 or fp16, a multiple of 8 up to 256)")
+        unit = 16 if dtype == FP8 else 8
+        _require(dtype in (torch.bfloat16, torch.float16, FP8) and head_dim % unit == 0 and unit <= head_dim <= 256, name,
+                 f"{dtype} heads of {head_dim} (bf16 or fp16, a multiple of 8 up to 256, or {FP8}, one of 16)")
         self.page_size = page_size
         self.k = torch.zeros((pages, kv_heads, page_size, head_dim), dtype=dtype, device=device)
         self.v = torch.zeros_like(self.k)
+        self.scales = self._new_scales()
         self.weights = (torch.zeros((pages, kv_heads, page_size), dtype=torch.float32, device=device)
                         if weights else None)
         self._free = list(range(pages - 1, -1, -1))
         self._seqs: dict[int, list] = {}   # id -> [page ids, keys held, tokens seen]
         self._next = 0
         self._twins: list["PagedCache"] = []
+
+    def _new_scales(self) -> Optional[tuple[Tensor, Tensor]]:
+        """The rows' scale bytes of k and v in an 8-bit cache."""
+        if self.k.dtype != FP8:
+            return None
+        return tuple(torch.zeros(self.k.shape[:3], dtype=torch.uint8, device=self.k.device) for _ in range(2))
 
     def twin(self) -> "PagedCache":
         """A pool of the same shape whose pages follow this cache's lists: another layer's keys and values. Write and
@@ -494,6 +683,7 @@ class PagedCache:
         other = PagedCache.__new__(PagedCache)
         other.page_size, other._free, other._seqs = self.page_size, self._free, self._seqs
         other.k, other.v = torch.zeros_like(self.k), torch.zeros_like(self.v)
+        other.scales = other._new_scales()
         other.weights = None if self.weights is None else torch.zeros_like(self.weights)
         other._next, other._twins = -1, []
         self._twins.append(other)
@@ -567,18 +757,43 @@ class PagedCache:
 
     def write(self, batch: PagedBatch, q: Tensor, k: Tensor, v: Tensor, cos: Optional[Tensor] = None,
               sin: Optional[Tensor] = None, *, interleaved: bool = False) -> Tensor:
-        """``paged_write`` of the batch's tokens at its positions; the rotated queries."""
+        """``paged_write`` (``paged_write_fp8``) of the batch's tokens at its positions; the rotated queries."""
+        if self.scales is not None:
+            return paged_write_fp8(q, k, v, cos, sin, batch.positions, self.k, self.v, *self.scales, batch.table,
+                                   batch.q_start, batch.kv_len, weights=self.weights, interleaved=interleaved)
         return paged_write(q, k, v, cos, sin, batch.positions, self.k, self.v, batch.table, batch.q_start, batch.kv_len,
                            weights=self.weights, interleaved=interleaved)
 
     def attend(self, batch: PagedBatch, q: Tensor, *, scale: Optional[float] = None, causal: bool = True,
                gather: Optional[bool] = None) -> tuple[Tensor, Tensor]:
-        """``paged_attention`` of the batch's (rotated) queries: (o, lse). Weights are gathered where the cache keeps
+        """``paged_attention`` (``paged_attention_fp8``) of the batch's (rotated) queries: (o, lse). Weights are gathered where the cache keeps
         them, unless ``gather`` is False."""
         gather = self.weights is not None if gather is None else gather
         _require(not gather or self.weights is not None, "PagedCache.attend", "the cache keeps no weights")
+        weights = self.weights if gather else None
+        if self.scales is not None:
+            return paged_attention_fp8(q, self.k, self.v, *self.scales, batch.table, batch.q_start, batch.kv_len,
+                                       batch.max_q, batch.max_kv, scale=scale, causal=causal, weights=weights)
         return paged_attention(q, self.k, self.v, batch.table, batch.q_start, batch.kv_len, batch.max_q, batch.max_kv,
-                               scale=scale, causal=causal, weights=self.weights if gather else None)
+                               scale=scale, causal=causal, weights=weights)
+
+    def read(self, seqs: Sequence[int], *, dtype: Optional[torch.dtype] = None) -> list[tuple[Tensor, Tensor]]:
+        """Every sequence's keys and values as they are held, (k, v) [keys, kv_heads, head_dim] each, to move them elsewhere;
+        of an 8-bit cache (``paged_read_fp8``) in ``dtype``, bf16 by default."""
+        name = "PagedCache.read"
+        _require(len(seqs) > 0 and all(s in self._seqs for s in seqs), name, f"sequences {list(seqs)}")
+        _require(self.scales is not None or dtype in (None, self.k.dtype), name, f"a cache of {self.k.dtype}, not {dtype}")
+        lens = [self._seqs[s][1] for s in seqs]
+        table, width = self._table_rows(seqs)
+        if self.scales is not None:
+            starts = [sum(lens[:i]) for i in range(len(lens) + 1)]
+            q_start, kv_len, flat = self._device_rows([starts, lens, table])
+            k, v = paged_read_fp8(self.k, self.v, *self.scales, flat.view(len(seqs), width), q_start, kv_len, starts[-1],
+                                  dtype=torch.bfloat16 if dtype is None else dtype)
+            return list(zip(k.split(lens), v.split(lens)))
+        pages = self._device_rows([table])[0].view(len(seqs), width).long()
+        return [tuple(x[pages[i, :-(-n // self.page_size)]].transpose(1, 2).flatten(0, 1)[:n] for x in (self.k, self.v))
+                for i, n in enumerate(lens)]
 
     def evict(self, seqs: Sequence[int], budget: int, recent: int) -> Optional[Tensor]:
         """Cuts those of ``seqs`` that hold more than ``budget`` keys back to it (``paged_evict``), here and in all
@@ -601,7 +816,11 @@ class PagedCache:
         kept = None
         try:
             for cache in self._pools():
-                got = paged_evict(cache.k, cache.v, cache.weights, flat, kv_len, max(lens), new, budget, recent)[0]
+                if cache.scales is not None:
+                    got = paged_evict_fp8(cache.k, cache.v, *cache.scales, cache.weights, flat, kv_len, max(lens), new,
+                                          budget, recent)[0]
+                else:
+                    got = paged_evict(cache.k, cache.v, cache.weights, flat, kv_len, max(lens), new, budget, recent)[0]
                 kept = got if kept is None else kept
         except Exception:
             self._free.extend(fresh)   # nothing has moved: the sequences keep their pages
