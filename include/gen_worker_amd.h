@@ -703,7 +703,10 @@ int gwa_paged_evict_fp8(const gwa_paged_cache* cache, const gwa_paged_scales* sc
  * -inf and NaN are never drawn; a row that holds nothing else gives token -1 and
  * logprob NaN. Of several +inf each has weight 1, and nothing else has any.
  * Settings are arrays [rows] or, where the pointer is NULL, the number beside it; from
- * an array, what is out of range counts as the nearest that is not (a NaN: 0). */
+ * an array, what is out of range counts as the nearest that is not (a NaN: 0). A min_p
+ * below 2^-28 counts as 0.
+ * workspace: gwa_sample_tokens_workspace bytes (0 for short rows), 16-byte aligned; no
+ * state is kept in it. */
 typedef struct gwa_sampling {
   const float* temperature;
   const int32_t* top_k;
@@ -713,8 +716,10 @@ typedef struct gwa_sampling {
   int32_t all_top_k;
   float all_top_p, all_min_p;
 } gwa_sampling;
+int64_t gwa_sample_tokens_workspace(int64_t rows, int64_t vocab);
 int gwa_sample_tokens(const void* logits, int64_t ld, int dtype, const float* uniform, const gwa_sampling* settings,
-                      int64_t* tokens, float* logprobs, int64_t rows, int64_t vocab, void* stream);
+                      int64_t* tokens, float* logprobs, int64_t rows, int64_t vocab, void* workspace,
+                      int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -51,6 +51,7 @@ struct Abi {
   decltype(&gwa_paged_write_fp8) paged_write_fp8;
   decltype(&gwa_paged_read_fp8) paged_read_fp8;
   decltype(&gwa_paged_attention_fp8) paged_attention_fp8;
+  decltype(&gwa_sample_tokens_workspace) sample_tokens_workspace;
   decltype(&gwa_sample_tokens) sample_tokens;
 };
 Abi g_abi;
@@ -703,8 +704,12 @@ PyObject* sample_tokens(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                               (float)top_p, (float)min_p};
       tokens = empty_like_device({rows}, at::kLong, x);
       logprobs = empty_like_device({rows}, at::kFloat, x);
+      const int64_t bytes = g_abi.sample_tokens_workspace(rows, vocab);
+      Tensor ws;
+      if (bytes > 0) ws = empty_like_device({bytes}, at::kByte, x);
       if (g_abi.sample_tokens(x.data_ptr(), std::max(x.stride(0), vocab), dt_code(x.scalar_type()), address<float>(t[1]),
-                              &s, address<int64_t>(tokens), address<float>(logprobs), rows, vocab, stream_of(x)) != GWA_OK)
+                              &s, address<int64_t>(tokens), address<float>(logprobs), rows, vocab,
+                              bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream_of(x)) != GWA_OK)
         tokens = Tensor();
     }
   }
@@ -861,6 +866,7 @@ PyObject* host_bind(PyObject*, PyObject* args) {
   GWA_BIND(paged_write_fp8);
   GWA_BIND(paged_read_fp8);
   GWA_BIND(paged_attention_fp8);
+  GWA_BIND(sample_tokens_workspace);
   GWA_BIND(sample_tokens);
 #undef GWA_BIND
   Py_INCREF(bodies);

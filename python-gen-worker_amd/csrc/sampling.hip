@@ -5,10 +5,12 @@
 
 namespace {
 
-constexpr int SM_THREADS = 1024, SM_WAVES = SM_THREADS / 64, SM_BINS = 1024, SM_DIGITS = 2048, SM_LIST = 1024;
-constexpr int SM_AHEAD = 4;       // 16-byte loads a lane has in flight
-constexpr float SM_PER_UNIT = 32.0f;  // bins a unit of (m - x) / temperature
-constexpr int kTableBits = 5;     // of the table of 2^(j / 32)
+constexpr int SM_BINS = 384, SM_DIGITS = 2048, SM_LIST = 512, SM_FOUND = 8192;
+constexpr int SM_HELD = 8;            // logits a thread holds where a row fits a workgroup's registers
+constexpr int SM_PART = 4096, SM_PARTS = 64;  // tokens a part of a longer row at least; parts of a row at most
+constexpr int SM_AHEAD = 4;           // 16-byte loads a lane has in flight
+constexpr int SM_FEW = 128;           // collected tokens that are ranked all against all
+constexpr int kTableBits = 7;         // of the table of 2^(j / 128)
 
 struct SampleArgs {
   const void* logits;
@@ -17,7 +19,10 @@ struct SampleArgs {
   gwa_sampling s;
   int64_t* tokens;
   float* logprobs;
-  int vocab, shift;  // weights are integers of 2^-shift
+  int vocab, shift;   // weights are integers of 2^-shift
+  int parts, part;    // of a row, and the tokens of one
+  uint64_t* bins;     // [rows][parts][SM_BINS]: a part's tokens (of rows with a top_k) or their weight, by bin
+  float* most;        // [rows][parts]
 };
 
 // fp32 values as integers of the same order: -0 counts as 0, NaN below everything
@@ -52,33 +57,103 @@ struct Logits<GWA_DT_F16> {
   }
 };
 
-// A row's weights: w = exp((x - m) / temperature) as an integer of 2^-shift. With y = (x - m) log2(e) / temperature in
-// 64 bits, 2^y = 2^n 2^(j/32) 2^r, |r| <= 1/64: a table and the series of 2^r to r^5 (the rest is below 2^-48), rounded to
-// an integer by an addition of 2^52.
-struct Weigher {
-  double c;  // log2(e) / temperature
-  float m;
+// 2^(j / 128), rounded to nearest
+__device__ const double kPowers[1 << kTableBits] = {
+    0x1.0000000000000p+0, 0x1.0163da9fb3335p+0, 0x1.02c9a3e778061p+0, 0x1.04315e86e7f85p+0,
+    0x1.059b0d3158574p+0, 0x1.0706b29ddf6dep+0, 0x1.0874518759bc8p+0, 0x1.09e3ecac6f383p+0,
+    0x1.0b5586cf9890fp+0, 0x1.0cc922b7247f7p+0, 0x1.0e3ec32d3d1a2p+0, 0x1.0fb66affed31bp+0,
+    0x1.11301d0125b51p+0, 0x1.12abdc06c31ccp+0, 0x1.1429aaea92de0p+0, 0x1.15a98c8a58e51p+0,
+    0x1.172b83c7d517bp+0, 0x1.18af9388c8deap+0, 0x1.1a35beb6fcb75p+0, 0x1.1bbe084045cd4p+0,
+    0x1.1d4873168b9aap+0, 0x1.1ed5022fcd91dp+0, 0x1.2063b88628cd6p+0, 0x1.21f49917ddc96p+0,
+    0x1.2387a6e756238p+0, 0x1.251ce4fb2a63fp+0, 0x1.26b4565e27cddp+0, 0x1.284dfe1f56381p+0,
+    0x1.29e9df51fdee1p+0, 0x1.2b87fd0dad990p+0, 0x1.2d285a6e4030bp+0, 0x1.2ecafa93e2f56p+0,
+    0x1.306fe0a31b715p+0, 0x1.32170fc4cd831p+0, 0x1.33c08b26416ffp+0, 0x1.356c55f929ff1p+0,
+    0x1.371a7373aa9cbp+0, 0x1.38cae6d05d866p+0, 0x1.3a7db34e59ff7p+0, 0x1.3c32dc313a8e5p+0,
+    0x1.3dea64c123422p+0, 0x1.3fa4504ac801cp+0, 0x1.4160a21f72e2ap+0, 0x1.431f5d950a897p+0,
+    0x1.44e086061892dp+0, 0x1.46a41ed1d0057p+0, 0x1.486a2b5c13cd0p+0, 0x1.4a32af0d7d3dep+0,
+    0x1.4bfdad5362a27p+0, 0x1.4dcb299fddd0dp+0, 0x1.4f9b2769d2ca7p+0, 0x1.516daa2cf6642p+0,
+    0x1.5342b569d4f82p+0, 0x1.551a4ca5d920fp+0, 0x1.56f4736b527dap+0, 0x1.58d12d497c7fdp+0,
+    0x1.5ab07dd485429p+0, 0x1.5c9268a5946b7p+0, 0x1.5e76f15ad2148p+0, 0x1.605e1b976dc09p+0,
+    0x1.6247eb03a5585p+0, 0x1.6434634ccc320p+0, 0x1.6623882552225p+0, 0x1.68155d44ca973p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.6c012750bdabfp+0, 0x1.6dfb23c651a2fp+0, 0x1.6ff7df9519484p+0,
+    0x1.71f75e8ec5f74p+0, 0x1.73f9a48a58174p+0, 0x1.75feb564267c9p+0, 0x1.780694fde5d3fp+0,
+    0x1.7a11473eb0187p+0, 0x1.7c1ed0130c132p+0, 0x1.7e2f336cf4e62p+0, 0x1.80427543e1a12p+0,
+    0x1.82589994cce13p+0, 0x1.8471a4623c7adp+0, 0x1.868d99b4492edp+0, 0x1.88ac7d98a6699p+0,
+    0x1.8ace5422aa0dbp+0, 0x1.8cf3216b5448cp+0, 0x1.8f1ae99157736p+0, 0x1.9145b0b91ffc6p+0,
+    0x1.93737b0cdc5e5p+0, 0x1.95a44cbc8520fp+0, 0x1.97d829fde4e50p+0, 0x1.9a0f170ca07bap+0,
+    0x1.9c49182a3f090p+0, 0x1.9e86319e32323p+0, 0x1.a0c667b5de565p+0, 0x1.a309bec4a2d33p+0,
+    0x1.a5503b23e255dp+0, 0x1.a799e1330b358p+0, 0x1.a9e6b5579fdbfp+0, 0x1.ac36bbfd3f37ap+0,
+    0x1.ae89f995ad3adp+0, 0x1.b0e07298db666p+0, 0x1.b33a2b84f15fbp+0, 0x1.b59728de5593ap+0,
+    0x1.b7f76f2fb5e47p+0, 0x1.ba5b030a1064ap+0, 0x1.bcc1e904bc1d2p+0, 0x1.bf2c25bd71e09p+0,
+    0x1.c199bdd85529cp+0, 0x1.c40ab5fffd07ap+0, 0x1.c67f12e57d14bp+0, 0x1.c8f6d9406e7b5p+0,
+    0x1.cb720dcef9069p+0, 0x1.cdf0b555dc3fap+0, 0x1.d072d4a07897cp+0, 0x1.d2f87080d89f2p+0,
+    0x1.d5818dcfba487p+0, 0x1.d80e316c98398p+0, 0x1.da9e603db3285p+0, 0x1.dd321f301b460p+0,
+    0x1.dfc97337b9b5fp+0, 0x1.e264614f5a129p+0, 0x1.e502ee78b3ff6p+0, 0x1.e7a51fbc74c83p+0,
+    0x1.ea4afa2a490dap+0, 0x1.ecf482d8e67f1p+0, 0x1.efa1bee615a27p+0, 0x1.f252b376bba97p+0,
+    0x1.f50765b6e4540p+0, 0x1.f7bfdad9cbe14p+0, 0x1.fa7c1819e90d8p+0, 0x1.fd3c22b8f71f1p+0};
+__device__ __forceinline__ void fill_table(double* table) {
+  for (int i = threadIdx.x; i < (1 << kTableBits); i += blockDim.x) table[i] = kPowers[i];
+}
+
+// A row's tokens by their weight exp((x - m) / temperature) = 2^y, y = (x - m) log2(e) / temperature in 64 bits. The weight
+// is an integer of 2^-shift: 2^y = 2^n 2^(j/128) 2^r, |r| <= 1/256, by a table and the series of 2^r to r^4 (the rest is
+// below 2^-49), rounded by an addition of 2^52. Bins are an eighth of a unit of y wide; the last is for what weighs
+// nothing: y < -47, -inf and NaN. Bins and their halves (`inside`) fall as x grows, never the other way. A token's weight and
+// bin have to be the same wherever they are formed, so the compiler may not choose where products and sums are fused.
+// m = +inf is held as 1e300: +inf is then at y = 0, all else far below.
+struct Scale {
+  double c, m;
   int shift;
   const double* table;
-  __device__ __forceinline__ uint64_t operator()(float x) const {
-    const double y = ((double)x - (double)m) * c;
-    uint64_t w = 0;
-    if (y >= -47.0) {  // not for -inf and NaN
-      constexpr double kMagic = 6755399441055744.0 / (1 << kTableBits);  // 1.5 * 2^52: its last bit is 1 / 32
-      const double t = y + kMagic;
-      const int k = (int)(uint32_t)__builtin_bit_cast(uint64_t, t);
-      const double r = y - (t - kMagic);
-      // ln(2)^i / i!
-      double p = 1.3333558146428441e-3;
-      p = __builtin_fma(p, r, 9.6181291076284772e-3);
-      p = __builtin_fma(p, r, 5.5504108664821580e-2);
-      p = __builtin_fma(p, r, 2.4022650695910072e-1);
-      p = __builtin_fma(p, r, 6.9314718055994531e-1);
-      p = __builtin_fma(p, r, 1.0);
-      p = __builtin_amdgcn_ldexp(p * table[k & ((1 << kTableBits) - 1)], shift + (k >> kTableBits));
-      w = __builtin_bit_cast(uint64_t, p + 4503599627370496.0) & 0xfffffffffffffull;
-    }
-    return x == m ? 1ull << shift : w;
+  static constexpr double kMagic = 6755399441055744.0 / (1 << kTableBits);  // 1.5 * 2^52: its last bit is 1 / 128
+  static constexpr int kPerBin = 4;  // log2 of 1 / 128 in a bin
+  __device__ __forceinline__ bool weighs(float x, double& y) const {
+#pragma clang fp contract(off)
+    y = ((double)x - m) * c;
+    return y >= -47.0;
+  }
+  static __device__ __forceinline__ int steps_of(double& y, double& r) {
+#pragma clang fp contract(off)
+    y = fmin(y, 0.0);
+    const double t = y + kMagic;
+    r = y - (t - kMagic);
+    return (int)(uint32_t)__builtin_bit_cast(uint64_t, t);
+  }
+  __device__ __forceinline__ uint64_t of_steps(int k, double r) const {
+#pragma clang fp contract(off)
+    // ln(2)^i / i!
+    double p = 9.6181291076284772e-3;
+    p = __builtin_fma(p, r, 5.5504108664821580e-2);
+    p = __builtin_fma(p, r, 2.4022650695910072e-1);
+    p = __builtin_fma(p, r, 6.9314718055994531e-1);
+    p = __builtin_fma(p, r, 1.0);
+    p = __builtin_amdgcn_ldexp(p * table[k & ((1 << kTableBits) - 1)], shift + (k >> kTableBits));
+    return __builtin_bit_cast(uint64_t, p + 4503599627370496.0) & 0xfffffffffffffull;
+  }
+  static __device__ __forceinline__ int bin_of_steps(int k) { return -k >> kPerBin; }
+  __device__ __forceinline__ uint64_t weight(float x) const {
+    double y, r;
+    if (!weighs(x, y)) return 0;
+    const int k = steps_of(y, r);
+    return of_steps(k, r);
+  }
+  __device__ __forceinline__ int bin(float x) const {
+    double y, r;
+    return weighs(x, y) ? bin_of_steps(steps_of(y, r)) : SM_BINS - 1;
+  }
+  // a bin's tokens once more into SM_BINS: by how far -8 y lies past the bin's start, bin - 1 / 32
+  __device__ __forceinline__ int inside(float x, int bin) const {
+#pragma clang fp contract(off)
+    double y;
+    if (!weighs(x, y)) return SM_BINS - 1;
+    const double f = (fmin(y, 0.0) * -8.0 - ((double)bin - 0.03125)) * (double)SM_BINS;
+    return min(max((int)f, 0), SM_BINS - 1);
+  }
+  // a range of logits that holds all of bins from to .. (and some more), in fp32
+  __device__ __forceinline__ void range(int from, int to, float& lo, float& hi) const {
+    const double a = m - ((double)(to + 1) * 0.125 + 0.01) / c, b = m - ((double)from * 0.125 - 0.02) / c;
+    lo = (float)(a - fabs(a) * 1e-6 - 1e-37);
+    hi = from == 0 ? INFINITY : (float)(b + fabs(b) * 1e-6 + 1e-37);
   }
 };
 
@@ -95,314 +170,717 @@ __device__ __forceinline__ uint64_t wave_sum64(uint64_t x) {
   return x;
 }
 
-struct SampleLds {
-  double table[1 << kTableBits];
-  uint64_t mass[SM_DIGITS];
-  uint32_t count[SM_DIGITS];
-  uint64_t list_w[SM_LIST];
-  uint32_t list_key[SM_LIST];
-  uint64_t cells[2][SM_WAVES];
-  uint64_t found[4];
-  uint32_t n;
-};
 
-// Sums of a and b over the threads before this one, in the threads' order, and over all
-__device__ __forceinline__ void block_scan(SampleLds& l, uint64_t a, uint64_t b, uint64_t& a_before, uint64_t& b_before,
-                                           uint64_t& a_all, uint64_t& b_all) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint64_t x = a, y = b;
+// Below this a min_p keeps all: there weights of a few units of 2^-shift (38 at least) would be compared, whose rounding
+// tells the least kept one apart from its neighbours no better than a bin does.
+constexpr float kLeastMinP = 0x1p-28f;
+
+// One row's settings and how its cuts are found: kCount: the first top_k by the numbers of tokens in the bins; kMass: what
+// there are of top_p and min_p by the weights in them; kWhole: by passes over the whole row
+enum Way { kGreedy, kCount, kMass, kWhole };
+struct Settings {
+  float temperature, top_p, min_p;
+  int top_k;  // 0: all
+  Way way;
+};
+__device__ __forceinline__ float held_in(float x, float lo, float hi) { return fminf(fmaxf(x, lo), hi); }
+__device__ __forceinline__ Settings settings_of(const SampleArgs& a, int64_t row) {
+  Settings s;
+  s.temperature = a.s.temperature ? a.s.temperature[row] : a.s.all_temperature;
+  if (s.temperature > 3.0e38f) s.temperature = 3.0e38f;  // (not a NaN)
+  s.top_k = a.s.top_k ? a.s.top_k[row] : a.s.all_top_k;
+  s.top_p = held_in(a.s.top_p ? a.s.top_p[row] : a.s.all_top_p, 0.0f, 1.0f);
+  s.min_p = held_in(a.s.min_p ? a.s.min_p[row] : a.s.all_min_p, 0.0f, 1.0f);
+  if (s.top_k <= 0 || s.top_k >= a.vocab) s.top_k = 0;
+  if (s.min_p < kLeastMinP) s.min_p = 0.0f;
+  s.way = !(s.temperature > 0.0f) ? kGreedy : s.top_k == 0 ? kMass : s.top_k <= SM_FOUND / 4 ? kCount : kWhole;
+  return s;
+}
+
+__device__ __forceinline__ Scale scale_of(const SampleArgs& a, const Settings& s, float m, const double* table) {
+  return {1.4426950408889634 / (double)s.temperature, m == INFINITY ? 1e300 : (double)m, a.shift, table};
+}
+
+// f(index, logit) over tokens [lo, hi) of the row at base, by threads `id` of n, in 16-byte pieces where they are whole
+template <int DT, class F>
+__device__ __forceinline__ void each_token(const uint8_t* base, int lo, int hi, int id, int n, F f) {
+  using L = Logits<DT>;
+  const uint8_t* p = base + (int64_t)lo * L::kBytes;
+  const int head = min((int)((16 - ((uintptr_t)p & 15)) & 15) / L::kBytes, hi - lo);
+  if (id < head) f(lo + id, L::at(p, id));
+  const int v0 = lo + head, vecs = (hi - v0) / L::kVec;
+  const v4i* body = (const v4i*)(base + (int64_t)v0 * L::kBytes);
+  for (int v = id; v < vecs; v += n * SM_AHEAD) {
+    v4i x[SM_AHEAD];
 #pragma unroll
-  for (int w = 1; w < 64; w <<= 1) {
-    const uint64_t p = shfl64_up(x, w), q = shfl64_up(y, w);
-    if (lane >= w) x += p, y += q;
+    for (int u = 0; u < SM_AHEAD; ++u) x[u] = body[min(v + n * u, vecs - 1)];
+#pragma unroll
+    for (int u = 0; u < SM_AHEAD; ++u)
+      if (v + n * u < vecs) {
+#pragma unroll
+        for (int e = 0; e < L::kVec; ++e) f(v0 + (v + n * u) * L::kVec + e, L::of(x[u], e));
+      }
   }
-  __syncthreads();
-  if (lane == 63) l.cells[0][wave] = x, l.cells[1][wave] = y;
-  __syncthreads();
-  a_before = x - a, b_before = y - b, a_all = b_all = 0;
-  for (int i = 0; i < SM_WAVES; ++i) {
-    if (i < wave) a_before += l.cells[0][i], b_before += l.cells[1][i];
-    a_all += l.cells[0][i], b_all += l.cells[1][i];
-  }
+  const int tail = v0 + vecs * L::kVec + id;
+  if (tail < hi) f(tail, L::at(base, tail));
 }
 
 // What a cut keeps: the tokens ordered above `key`, and of those equal to it the first `ties` by index. `equal`: how many
-// those are, `above`: the weight of the ones before them (where weights were asked for).
+// those are.
 struct Cut {
-  uint32_t key;
-  uint32_t ties, equal;
-  uint64_t above;
+  uint32_t key, ties, equal;
 };
 
-// One workgroup a row, several passes over its logits (from the caches after the first): the largest; for a cut a histogram
-// of the tokens by their distance from it, then the tokens of the one bin that the cut falls into, ranked by counting; the
-// kept weights of 16 parts of the vocabulary; and the tokens of the part that the random number falls into.
-template <int DT>
-__global__ __launch_bounds__(SM_THREADS) void sample_rows_kernel(SampleArgs a) {
-  using L = Logits<DT>;
-  __shared__ SampleLds l;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t row = blockIdx.x;
-  const uint8_t* base = (const uint8_t*)a.logits + row * a.ld * L::kBytes;
-  const int vocab = a.vocab;
-  auto held = [](float x, float lo, float hi) { return fminf(fmaxf(x, lo), hi); };
-  const float temperature = a.s.temperature ? a.s.temperature[row] : a.s.all_temperature;
-  const int top_k = a.s.top_k ? a.s.top_k[row] : a.s.all_top_k;
-  const float top_p = held(a.s.top_p ? a.s.top_p[row] : a.s.all_top_p, 0.0f, 1.0f);
-  const float min_p = held(a.s.min_p ? a.s.min_p[row] : a.s.all_min_p, 0.0f, 1.0f);
+// A workgroup of NW waves on one row
+template <int NW>
+struct Drawer {
+  static constexpr int NT = 64 * NW;
+  struct Lds {
+    double table[1 << kTableBits];
+    uint64_t mass[SM_DIGITS];
+    uint32_t count[SM_DIGITS];
+    uint64_t list_w[SM_LIST];
+    uint32_t list_key[SM_LIST];
+    uint64_t cells[2][NW];
+    uint64_t found[4];
+    uint32_t n;
+  };
+  Lds& l;
+  const SampleArgs& a;
+  const Settings& s;
+  int64_t row;
+  Scale scale;
+  float m;
+  double low;  // the least weight that min_p keeps
 
-  // The waves' parts of the row, [part(i), part(i + 1)): tokens before the first 16-byte boundary, whole 16-byte pieces,
-  // and the rest, so that loads are wide whatever the row's alignment is
-  const int head = min((int)((16 - ((uintptr_t)base & 15)) & 15) / L::kBytes, vocab);
-  const int vecs = (vocab - head) / L::kVec;
-  const int per = (vecs + SM_WAVES - 1) / SM_WAVES;
-  auto vec_of = [&](int w) { return min(w * per, vecs); };
-  auto part = [&](int w) { return w == 0 ? 0 : w == SM_WAVES ? vocab : head + vec_of(w) * L::kVec; };
-  const v4i* body = (const v4i*)(base + head * L::kBytes);
-  // f(index, logit) over this wave's part
-  auto each = [&](auto f) __attribute__((always_inline)) {
-    if (wave == 0 && lane < head) f(lane, L::at(base, lane));
-    const int v1 = vec_of(wave + 1);
-    for (int v = vec_of(wave) + lane; v < v1; v += 64 * SM_AHEAD) {
-      v4i x[SM_AHEAD];
+  __device__ __forceinline__ Drawer(Lds& l, const SampleArgs& a, const Settings& s, int64_t row, float m)
+      : l(l), a(a), s(s), row(row), scale(scale_of(a, s, m, l.table)), m(m),
+        low((double)s.min_p * (double)(1ull << a.shift)) {}
+  __device__ __forceinline__ uint64_t weight(float x) const { return scale.weight(x); }
+
+  // Sums of x and y over the threads before this one, in the threads' order, and over all
+  __device__ __forceinline__ void scan(uint64_t x, uint64_t y, uint64_t& x_before, uint64_t& y_before, uint64_t& x_all,
+                                       uint64_t& y_all) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint64_t p = x, q = y;
 #pragma unroll
-      for (int u = 0; u < SM_AHEAD; ++u) x[u] = body[min(v + 64 * u, v1 - 1)];
-#pragma unroll
-      for (int u = 0; u < SM_AHEAD; ++u)
-        if (v + 64 * u < v1) {
-#pragma unroll
-          for (int e = 0; e < L::kVec; ++e) f(head + (v + 64 * u) * L::kVec + e, L::of(x[u], e));
-        }
+    for (int w = 1; w < 64; w <<= 1) {
+      const uint64_t u = shfl64_up(p, w), v = shfl64_up(q, w);
+      if (lane >= w) p += u, q += v;
     }
-    const int tail = head + vecs * L::kVec + lane;
-    if (wave == SM_WAVES - 1 && tail < vocab) f(tail, L::at(base, tail));
-  };
-
-  if (tid < (1 << kTableBits)) l.table[tid] = exp2((double)tid / (1 << kTableBits));
-  float m = -INFINITY;
-  each([&](int, float x) __attribute__((always_inline)) { m = fmaxf(m, x); });
+    __syncthreads();
+    if (lane == 63) l.cells[0][wave] = p, l.cells[1][wave] = q;
+    __syncthreads();
+    // the waves' sums, one a lane
+    const uint64_t cx = lane < NW ? l.cells[0][lane] : 0, cy = lane < NW ? l.cells[1][lane] : 0;
+    uint64_t sx = cx, sy = cy;
 #pragma unroll
-  for (int w = 32; w; w >>= 1) m = fmaxf(m, __shfl_xor(m, w));
-  if (lane == 0) l.cells[0][wave] = __float_as_uint(m);
-  __syncthreads();
-  for (int i = 0; i < SM_WAVES; ++i) m = fmaxf(m, __uint_as_float((uint32_t)l.cells[0][i]));
-  if (m == -INFINITY) {
-    if (tid == 0) a.tokens[row] = -1, a.logprobs[row] = NAN;
-    return;
+    for (int w = 1; w < NW; w <<= 1) {
+      const uint64_t u = shfl64_up(sx, w), v = shfl64_up(sy, w);
+      if (lane >= w) sx += u, sy += v;
+    }
+    x_before = p - x + shfl64(sx - cx, wave), y_before = q - y + shfl64(sy - cy, wave);
+    x_all = shfl64(sx, NW - 1), y_all = shfl64(sy, NW - 1);
   }
-  if (!(temperature > 0.0f)) {
-    if (tid == 0) l.n = 0xffffffffu;
-    __syncthreads();
-    uint32_t first = 0xffffffffu;
-    each([&](int i, float x) __attribute__((always_inline)) { first = x == m ? min(first, (uint32_t)i) : first; });
-    if (first != 0xffffffffu) atomicMin(&l.n, first);
-    __syncthreads();
-    if (tid == 0) a.tokens[row] = l.n, a.logprobs[row] = 0.0f;
-    return;
-  }
-  const Weigher weight = {1.4426950408889634 / (double)temperature, m, a.shift, l.table};
-  const float per_unit = SM_PER_UNIT / temperature;
-  // bins of falling logits; the last takes all from SM_BINS - 1 on, whose weights are 0
-  auto bin_of = [&](float x) __attribute__((always_inline)) {
-    const float d = (m - x) * per_unit;
-    return x == m ? 0 : d < (float)(SM_BINS - 1) ? (int)d : SM_BINS - 1;
-  };
 
-  // The cut at the want-th token (MASS: at which the weight reaches `target`) among those ordered at or above `least`
-  auto cut_at = [&](auto mass_c, uint32_t least, uint64_t want, auto target_of) __attribute__((always_inline)) {
-    constexpr bool MASS = decltype(mass_c)::value;
+  // Where a sum over bins of counts n and weights w (SM_BINS / NT bins or fewer a thread, from bin `first` on) reaches what
+  // is wanted: MASS: the weight `target`, else the number `want`, both counted from n0, w0 on
+  struct Place {
+    int bin;
+    uint32_t inside;
+    uint64_t before, above;  // tokens, and weight, ahead of it
+  };
+  template <bool MASS, int PER, class Target>
+  __device__ __forceinline__ Place reach(const uint64_t (&n)[PER], const uint64_t (&w)[PER], int first, uint64_t n0,
+                                         uint64_t w0, uint64_t want, Target target_of) {
+    uint64_t sn = 0, sw = 0, nb, wb, na, wa;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) sn += n[i], sw += w[i];
+    scan(sn, sw, nb, wb, na, wa);
+    nb += n0, wb += w0;
+    const double target = MASS ? target_of(wa) : 0.0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const bool here = MASS ? (double)wb < target && (double)(wb + w[i]) >= target : nb < want && nb + n[i] >= want;
+      if (here) l.found[0] = first + i, l.found[1] = nb, l.found[2] = wb, l.found[3] = n[i];
+      nb += n[i], wb += w[i];
+    }
     __syncthreads();
-    l.count[tid] = 0, l.mass[tid] = 0;
-    if (tid == 0) l.n = 0;
+    const Place p = {(int)l.found[0], (uint32_t)l.found[3], l.found[1], l.found[2]};
+    __syncthreads();
+    return p;
+  }
+
+  // the ties that are kept of `equal` weights w each behind a weight of `from`: as few as reach the target
+  static __device__ __forceinline__ uint32_t ties_to(double target, uint64_t from, uint64_t w, uint32_t equal) {
+    uint32_t e = w ? (uint32_t)fmin(fmax(ceil((target - (double)from) / (double)w), 1.0), (double)equal) : 1;
+    while (e > 1 && (double)(from + (e - 1) * w) >= target) --e;
+    while (e < equal && (double)(from + e * w) < target) ++e;
+    return e;
+  }
+
+  // a histogram by bin_of(x) of the tokens that `each` passes on and `take` accepts, and the place in it
+  static constexpr int kPer = (SM_BINS + NT - 1) / NT;
+  template <bool MASS, class Each, class Take, class Of, class Target>
+  __device__ __forceinline__ Place locate(Each each, Take take, Of bin_of, uint64_t n0, uint64_t w0, uint64_t want,
+                                          Target target_of) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < SM_BINS; i += NT) l.count[i] = 0, l.mass[i] = 0;
     __syncthreads();
     each([&](int, float x) __attribute__((always_inline)) {
-      const int b = bin_of(x);
-      if (b < SM_BINS - 1 && (!MASS || order_of(x) >= least)) {
-        atomicAdd(&l.count[b], 1u);
-        if (MASS) atomicAdd((unsigned long long*)&l.mass[b], (unsigned long long)weight(x));
+      if (take(x)) {
+        const int b = bin_of(x);
+        if (b >= 0) {
+          atomicAdd(&l.count[b], 1u);
+          if (MASS) atomicAdd((unsigned long long*)&l.mass[b], (unsigned long long)weight(x));
+        }
       }
     });
     __syncthreads();
-    uint64_t n = l.count[tid], w = l.mass[tid], n_before, w_before, n_all, w_all;
-    block_scan(l, n, w, n_before, w_before, n_all, w_all);
-    const double target = MASS ? target_of(w_all) : 0.0;
-    if (!MASS && tid == SM_BINS - 1) n = vocab - n_all;  // the last bin's
-    const bool here = MASS ? (double)w_before < target && (double)(w_before + w) >= target
-                           : n_before < want && n_before + n >= want;
-    if (here) l.found[0] = tid, l.found[1] = n_before, l.found[2] = w_before, l.found[3] = n;
-    __syncthreads();
-    const int bin = (int)l.found[0];
-    uint64_t before = l.found[1], above = l.found[2];
-    const uint32_t inside = (uint32_t)l.found[3];
-    __syncthreads();
-    Cut cut;
-    // the ties that are kept of `equal` weights w each behind a weight of `above`: as few as reach the target
-    auto ties_to = [&](uint64_t from, uint64_t w, uint32_t equal) __attribute__((always_inline)) {
-      uint32_t e = w ? (uint32_t)fmin(fmax(ceil((target - (double)from) / (double)w), 1.0), (double)equal) : 1;
-      while (e > 1 && (double)(from + (e - 1) * w) >= target) --e;
-      while (e < equal && (double)(from + e * w) < target) ++e;
-      return e;
-    };
-    if (inside <= SM_LIST) {
+    uint64_t n[kPer], w[kPer];
+    const int first = kPer * threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const bool in = first + i < SM_BINS;
+      n[i] = in ? l.count[first + i] : 0, w[i] = in ? l.mass[first + i] : 0;
+    }
+    return reach<MASS>(n, w, first, n0, w0, want, target_of);
+  }
+
+  // The cut inside bin `p.bin`, from the tokens that `each` passes on and `take` accepts, which hold all of the bin's
+  template <bool MASS, class Each, class Take>
+  __device__ __forceinline__ Cut resolve(Each each, Take take, Place p, uint64_t want, double target) {
+    const int bin = p.bin;
+    auto in_bin = [&](float x) __attribute__((always_inline)) { return take(x) && scale.bin(x) == bin; };
+    int sub = -1;
+    if (p.inside > 32) {  // once more into bins
+      p = locate<MASS>(each, in_bin, [&](float x) { return scale.inside(x, bin); }, p.before, p.above, want,
+                       [&](uint64_t) { return target; });
+      sub = p.bin;
+    }
+    auto here = [&](float x) __attribute__((always_inline)) { return in_bin(x) && (sub < 0 || scale.inside(x, bin) == sub); };
+    if (p.inside <= SM_LIST) {  // ranked by counting
+      if (threadIdx.x == 0) l.n = 0;
+      __syncthreads();
       each([&](int, float x) __attribute__((always_inline)) {
-        if (bin_of(x) == bin && (!MASS || order_of(x) >= least)) {
+        if (here(x)) {
           const uint32_t i = atomicAdd(&l.n, 1u);
           l.list_key[i] = order_of(x);
           if (MASS) l.list_w[i] = weight(x);
         }
       });
       __syncthreads();
-      if (tid < (int)inside) {
-        const uint32_t key = l.list_key[tid];
+      for (int j = threadIdx.x; j < (int)p.inside; j += NT) {
+        const uint32_t key = l.list_key[j];
         uint32_t over = 0, equal = 0;
-        uint64_t heavier = 0;
-        for (uint32_t i = 0; i < inside; ++i) {
+        uint64_t from = p.above;
+        for (uint32_t i = 0; i < p.inside; ++i) {
           const uint32_t k = l.list_key[i];
           over += k > key, equal += k == key;
-          if (MASS) heavier += k > key ? l.list_w[i] : 0;
+          if (MASS) from += k > key ? l.list_w[i] : 0;
         }
-        const uint64_t from = above + heavier;
-        const uint64_t mine = MASS ? l.list_w[tid] : 0;
+        const uint64_t mine = MASS ? l.list_w[j] : 0;
         const bool at = MASS ? (double)from < target && (double)(from + equal * mine) >= target
-                             : before + over < want && before + over + equal >= want;
+                             : p.before + over < want && p.before + over + equal >= want;
         if (at) {  // equal ones all write the same
-          l.found[0] = key, l.found[1] = equal, l.found[2] = from;
-          l.found[3] = MASS ? ties_to(from, mine, equal) : want - before - over;
+          l.found[0] = key, l.found[1] = equal;
+          l.found[2] = MASS ? ties_to(target, from, mine, equal) : want - p.before - over;
         }
       }
       __syncthreads();
-      cut = {(uint32_t)l.found[0], (uint32_t)l.found[3], (uint32_t)l.found[1], l.found[2]};
-    } else {
-      // digit by digit of the ordered values: 11 + 11 + 10 bits
-      uint32_t prefix = 0, in_digit = 0;
-      uint64_t digit_w = 0;
-      int shift = 21;
-      for (int pass = 0; pass < 3; ++pass) {
-        const int bits = pass == 2 ? 10 : 11;
-        for (int i = tid; i < SM_DIGITS; i += SM_THREADS) l.count[i] = 0, l.mass[i] = 0;
-        __syncthreads();
-        each([&](int, float x) __attribute__((always_inline)) {
-          const uint32_t key = order_of(x);
-          if (bin_of(x) == bin && (!MASS || key >= least) && (pass == 0 || key >> (shift + bits) == prefix)) {
-            const uint32_t d = key >> shift & ((1u << bits) - 1);
-            atomicAdd(&l.count[d], 1u);
-            if (MASS) atomicAdd((unsigned long long*)&l.mass[d], (unsigned long long)weight(x));
-          }
-        });
-        __syncthreads();
-        // digits from the top, two a thread
-        const int d1 = SM_DIGITS - 1 - 2 * tid, d0 = d1 - 1;
-        const uint32_t n1 = l.count[d1], n0 = l.count[d0];
-        const uint64_t w1 = l.mass[d1], w0 = l.mass[d0];
-        uint64_t n_up, w_up, na, wa;
-        block_scan(l, n1 + n0, w1 + w0, n_up, w_up, na, wa);
-        n_up += before, w_up += above;
-        auto check = [&](int d, uint64_t nb, uint64_t wb, uint32_t n, uint64_t w) __attribute__((always_inline)) {
-          const bool at = MASS ? (double)wb < target && (double)(wb + w) >= target : nb < want && nb + n >= want;
-          if (at) l.found[0] = (uint64_t)d << 32 | n, l.found[1] = nb, l.found[2] = wb, l.found[3] = w;
-        };
-        check(d1, n_up, w_up, n1, w1);
-        check(d0, n_up + n1, w_up + w1, n0, w0);
-        __syncthreads();
-        prefix = prefix << bits | (uint32_t)(l.found[0] >> 32);
-        in_digit = (uint32_t)l.found[0];
-        before = l.found[1], above = l.found[2], digit_w = l.found[3];
-        shift = pass == 0 ? 10 : 0;
-        __syncthreads();
-      }
-      cut = {prefix, MASS ? ties_to(above, digit_w / in_digit, in_digit) : (uint32_t)(want - before), in_digit, above};
+      const Cut c = {(uint32_t)l.found[0], (uint32_t)l.found[2], (uint32_t)l.found[1]};
+      __syncthreads();
+      return c;
     }
-    __syncthreads();
-    return cut;
-  };
-
-  Cut cut = {0, (uint32_t)vocab, (uint32_t)vocab, 0};
-  uint32_t least = 0, dropped = 0;  // of the tokens at `least`, the last `dropped` are not among the first top_k
-  if (top_k > 0 && top_k < vocab) {
-    cut = cut_at(std::false_type{}, 0, (uint64_t)top_k, [](uint64_t) { return 0.0; });
-    least = cut.key, dropped = cut.equal - cut.ties;
+    // digit by digit of the ordered values: 11 + 11 + 10 bits
+    uint32_t prefix = 0;
+    int shift = 21;
+    uint64_t digit_w = 0;
+    for (int pass = 0; pass < 3; ++pass) {
+      const int bits = pass == 2 ? 10 : 11;
+      for (int i = threadIdx.x; i < SM_DIGITS; i += NT) l.count[i] = 0, l.mass[i] = 0;
+      __syncthreads();
+      each([&](int, float x) __attribute__((always_inline)) {
+        const uint32_t key = order_of(x);
+        if (here(x) && (pass == 0 || key >> (shift + bits) == prefix)) {
+          const uint32_t d = SM_DIGITS - 1 - (key >> shift & ((1u << bits) - 1));  // falling
+          atomicAdd(&l.count[d], 1u);
+          if (MASS) atomicAdd((unsigned long long*)&l.mass[d], (unsigned long long)weight(x));
+        }
+      });
+      __syncthreads();
+      constexpr int PER = SM_DIGITS / NT;
+      uint64_t n[PER], w[PER];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) n[i] = l.count[PER * threadIdx.x + i], w[i] = l.mass[PER * threadIdx.x + i];
+      p = reach<MASS>(n, w, PER * threadIdx.x, p.before, p.above, want, [&](uint64_t) { return target; });
+      digit_w = l.mass[p.bin];
+      prefix = prefix << bits | (uint32_t)(SM_DIGITS - 1 - p.bin);
+      shift = pass == 0 ? 10 : 0;
+      __syncthreads();
+    }
+    return {prefix, MASS ? ties_to(target, p.above, digit_w / p.inside, p.inside) : (uint32_t)(want - p.before), p.inside};
   }
-  auto value_of = [](uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); };
-  if (top_p < 1.0f) {
-    const uint64_t off = dropped ? dropped * weight(value_of(least)) : 0;
-    cut = cut_at(std::true_type{}, least, 0, [&](uint64_t all) {
-      return fmax((double)top_p * (double)(all - off), 0.5);  // the first token reaches 0.5 alone
-    });
+
+  static __device__ __forceinline__ float value_of(uint32_t key) {
+    return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+  }
+  __device__ __forceinline__ double target_of(uint64_t all) const {
+    return fmax((double)s.top_p * (double)all, 0.5);  // the first token reaches 0.5 alone
   }
 
-  // the kept weights of the waves' parts, and the ties in them
-  const double low = (double)min_p * (double)(1ull << a.shift);
-  auto kept = [&](float x) __attribute__((always_inline)) {
+  // top_k's cut among the tokens of `each`
+  template <class Each>
+  __device__ __forceinline__ Cut cut_by_count(Each each) {
+    auto any = [](float) { return true; };
+    const Place p = locate<false>(each, any, [&](float x) { return scale.bin(x); }, 0, 0, (uint64_t)s.top_k,
+                                  [](uint64_t) { return 0.0; });
+    return resolve<false>(each, any, p, (uint64_t)s.top_k, 0.0);
+  }
+  // top_p's among those that `top` (of top_k, or of all) keeps
+  template <class Each>
+  __device__ __forceinline__ Cut cut_by_mass(Each each, const Cut& top) {
+    auto take = [&](float x) __attribute__((always_inline)) { return order_of(x) >= top.key; };
+    const uint32_t dropped = top.equal - top.ties;
+    const uint64_t off = dropped ? dropped * weight(value_of(top.key)) : 0;
+    double target = 0.0;
+    const Place p = locate<true>(each, take, [&](float x) { return scale.bin(x); }, 0, 0, 0,
+                                 [&](uint64_t all) { return target = target_of(all - off); });
+    return resolve<true>(each, take, p, 0, target);
+  }
+
+  __device__ __forceinline__ uint64_t kept(float x) const {
     const uint64_t w = weight(x);
     return (double)w >= low ? w : 0;
-  };
-  const uint64_t tie_w = cut.key ? kept(value_of(cut.key)) : 0;
-  uint64_t sum = 0, ties = 0;
-  each([&](int, float x) __attribute__((always_inline)) {
-    const uint32_t key = order_of(x);
-    if (key > cut.key) sum += kept(x);
-    ties += key == cut.key;
-  });
-  sum = wave_sum64(sum), ties = wave_sum64(ties);
-  __syncthreads();
-  if (lane == 0) l.cells[0][wave] = sum, l.cells[1][wave] = ties;
-  __syncthreads();
-  uint64_t total = 0, n_ties = 0;
-  auto ties_in = [&](uint64_t upto, uint64_t n) {  // those kept of n ties behind `upto` others
-    return upto >= cut.ties ? 0 : min(n, (uint64_t)cut.ties - upto);
-  };
-  for (int i = 0; i < SM_WAVES; ++i) {
-    total += l.cells[0][i] + ties_in(n_ties, l.cells[1][i]) * tie_w;
-    n_ties += l.cells[1][i];
+  }
+  __device__ __forceinline__ uint64_t tie_weight(const Cut& cut) const { return cut.key ? kept(value_of(cut.key)) : 0; }
+  static __device__ __forceinline__ uint64_t ties_in(const Cut& cut, uint64_t before, uint64_t n) {  // kept, of n behind `before`
+    return before >= cut.ties ? 0 : min(n, (uint64_t)cut.ties - before);
   }
   // cum > u total: for integers, cum > floor(u total)
-  const uint64_t r = min((uint64_t)((double)held(a.uniform[row], 0.0f, 1.0f) * (double)total), total - 1);
-  uint64_t cum = 0, upto = 0;
-  int at = 0;
-  for (; at < SM_WAVES - 1; ++at) {
-    const uint64_t next = cum + l.cells[0][at] + ties_in(upto, l.cells[1][at]) * tie_w;
-    if (next > r) break;
-    cum = next, upto += l.cells[1][at];
+  __device__ __forceinline__ uint64_t drawn(uint64_t total) const {
+    return min((uint64_t)((double)held_in(a.uniform[row], 0.0f, 1.0f) * (double)total), total - 1);
   }
-  // that part's tokens, neighbouring ones a thread
-  const int p0 = part(at), len = part(at + 1) - p0, each_n = (len + SM_THREADS - 1) / SM_THREADS;
-  const int i0 = min(tid * each_n, len), i1 = min(i0 + each_n, len);
-  sum = ties = 0;
-  for (int i = i0; i < i1; ++i) {
-    const float x = L::at(base, p0 + i);
-    const uint32_t key = order_of(x);
-    if (key > cut.key) sum += kept(x);
-    ties += key == cut.key;
+
+  __device__ __forceinline__ void draw(int index, float x, uint64_t total) const {
+    a.tokens[row] = index;
+    const double y = x == m ? 0.0 : ((double)x - (double)m) / (double)s.temperature;
+    a.logprobs[row] = (float)(y - log((double)total / (double)(1ull << a.shift)));
   }
-  uint64_t sum_before, ties_before, sa, ta;
-  block_scan(l, sum, ties, sum_before, ties_before, sa, ta);
-  upto += ties_before;
-  // kept ties before this thread's tokens, less those before the part
-  const uint64_t first_tie = upto - ties_before;
-  uint64_t c = cum + sum_before + ties_in(first_tie, ties_before) * tie_w;
-  if (c <= r && c + sum + ties_in(upto, ties) * tie_w > r) {
-    for (int i = i0; i < i1; ++i) {
-      const float x = L::at(base, p0 + i);
+  // The token at which the kept weights, `cum` of them and `upto` ties before this thread's tokens, pass r: f(i) is the
+  // thread's i-th of n neighbouring tokens from `index` on
+  template <class F>
+  __device__ __forceinline__ void pick(const Cut& cut, uint64_t tie_w, uint64_t cum, uint64_t upto, uint64_t r, uint64_t total,
+                                       int index, int n, F f) {
+    for (int i = 0; i < n; ++i) {
+      const float x = f(i);
       const uint32_t key = order_of(x);
-      uint64_t w = 0;
-      if (key > cut.key) w = kept(x);
-      else if (key == cut.key) w = upto++ < cut.ties ? tie_w : 0;
-      c += w;
-      if (c > r) {
-        a.tokens[row] = p0 + i;
-        const double y = x == m ? 0.0 : ((double)x - (double)m) / (double)temperature;
-        a.logprobs[row] = (float)(y - log((double)total / (double)(1ull << a.shift)));
+      if (key > cut.key) cum += kept(x);
+      else if (key == cut.key) cum += upto++ < cut.ties ? tie_w : 0;
+      if (cum > r) {
+        draw(index + i, x, total);
         break;
       }
     }
+  }
+};
+
+__device__ __forceinline__ const uint8_t* row_at(const SampleArgs& a, int64_t row, int bytes) {
+  return (const uint8_t*)a.logits + row * a.ld * bytes;
+}
+__device__ __forceinline__ float wave_max(float m) {
+#pragma unroll
+  for (int w = 32; w; w >>= 1) m = fmaxf(m, __shfl_xor(m, w));
+  return m;
+}
+
+// Rows that fit a workgroup's registers: SM_HELD neighbouring tokens a thread, read once.
+template <int DT, int NW>
+__global__ __launch_bounds__(64 * NW) void sample_held_kernel(SampleArgs a) {
+  using D = Drawer<NW>;
+  using L = Logits<DT>;
+  __shared__ typename D::Lds l;
+  __shared__ uint32_t least;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t row = blockIdx.x;
+  const uint8_t* base = row_at(a, row, L::kBytes);
+  const Settings s = settings_of(a, row);
+  const int i0 = SM_HELD * tid, n = min(max(a.vocab - i0, 0), SM_HELD);
+  float x[SM_HELD];
+  if (n == SM_HELD && ((uintptr_t)base & 15) == 0) {
+#pragma unroll
+    for (int v = 0; v < SM_HELD / L::kVec; ++v) {
+      const v4i w = ((const v4i*)(base + (int64_t)i0 * L::kBytes))[v];
+#pragma unroll
+      for (int e = 0; e < L::kVec; ++e) x[v * L::kVec + e] = L::of(w, e);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < SM_HELD; ++i) x[i] = i < n ? L::at(base, i0 + i) : NAN;
+  }
+  fill_table(l.table);
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < SM_HELD; ++i) m = fmaxf(m, x[i]);
+  m = wave_max(m);
+  if (lane == 0) l.cells[0][wave] = __float_as_uint(m);
+  if (tid == 0) least = 0xffffffffu;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < NW; ++i) m = fmaxf(m, __uint_as_float((uint32_t)l.cells[0][i]));
+  if (m == -INFINITY) {
+    if (tid == 0) a.tokens[row] = -1, a.logprobs[row] = NAN;
+    return;
+  }
+  if (s.way == kGreedy) {
+    uint32_t first = 0xffffffffu;
+#pragma unroll
+    for (int i = SM_HELD - 1; i >= 0; --i) first = x[i] == m ? (uint32_t)(i0 + i) : first;
+    if (first != 0xffffffffu) atomicMin(&least, first);
+    __syncthreads();
+    if (tid == 0) a.tokens[row] = least, a.logprobs[row] = 0.0f;
+    return;
+  }
+  D d(l, a, s, row, m);
+  auto each = [&](auto f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < SM_HELD; ++i)
+      if (i < n) f(i0 + i, x[i]);
+  };
+  Cut cut = {0, (uint32_t)a.vocab, (uint32_t)a.vocab};
+  if (s.top_k) cut = d.cut_by_count(each);
+  if (s.top_p < 1.0f) cut = d.cut_by_mass(each, cut);
+  const uint64_t tie_w = d.tie_weight(cut);
+  uint64_t sum = 0, ties = 0, sum_before, ties_before, sum_all, ties_all;
+  each([&](int, float x) __attribute__((always_inline)) {
+    const uint32_t key = order_of(x);
+    if (key > cut.key) sum += d.kept(x);
+    ties += key == cut.key;
+  });
+  d.scan(sum, ties, sum_before, ties_before, sum_all, ties_all);
+  const uint64_t total = sum_all + D::ties_in(cut, 0, ties_all) * tie_w, r = d.drawn(total);
+  const uint64_t cum = sum_before + D::ties_in(cut, 0, ties_before) * tie_w;
+  if (cum <= r && cum + sum + D::ties_in(cut, ties_before, ties) * tie_w > r) {
+    d.pick(cut, tie_w, cum, ties_before, r, total, i0, n, [&](int i) __attribute__((always_inline)) {
+      float y = x[0];
+#pragma unroll
+      for (int e = 1; e < SM_HELD; ++e) y = i == e ? x[e] : y;
+      return y;
+    });
+  }
+}
+
+// Longer rows, first: the largest logit of every part
+template <int DT>
+__global__ __launch_bounds__(256) void sample_max_kernel(SampleArgs a) {
+  __shared__ float cells[4];
+  const int64_t row = blockIdx.x / a.parts;
+  const int g = blockIdx.x - (int)row * a.parts, lo = g * a.part, hi = min(lo + a.part, a.vocab);
+  float m = -INFINITY;
+  each_token<DT>(row_at(a, row, Logits<DT>::kBytes), lo, hi, threadIdx.x, 256,
+                 [&](int, float x) __attribute__((always_inline)) { m = fmaxf(m, x); });
+  m = wave_max(m);
+  if ((threadIdx.x & 63) == 0) cells[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) a.most[blockIdx.x] = fmaxf(fmaxf(cells[0], cells[1]), fmaxf(cells[2], cells[3]));
+}
+__device__ __forceinline__ float row_max(const SampleArgs& a, int64_t row) {
+  const int lane = threadIdx.x & 63;
+  return wave_max(lane < a.parts ? a.most[row * a.parts + lane] : -INFINITY);  // SM_PARTS at most
+}
+
+// second: every part's histogram, of tokens or of their weight
+template <int DT>
+__global__ __launch_bounds__(256) void sample_bins_kernel(SampleArgs a) {
+  __shared__ uint64_t bin[SM_BINS];
+  __shared__ double table[1 << kTableBits];
+  const int tid = threadIdx.x;
+  const int64_t row = blockIdx.x / a.parts;
+  const int g = blockIdx.x - (int)row * a.parts, lo = g * a.part, hi = min(lo + a.part, a.vocab);
+  const Settings s = settings_of(a, row);
+  if (s.way == kGreedy || s.way == kWhole) return;
+  const float m = row_max(a, row);
+  if (m == -INFINITY) return;
+  fill_table(table);
+  for (int i = tid; i < SM_BINS; i += 256) bin[i] = 0;
+  __syncthreads();
+  const Scale scale = scale_of(a, s, m, table);
+  const uint8_t* base = row_at(a, row, Logits<DT>::kBytes);
+  if (s.way == kCount) {
+    each_token<DT>(base, lo, hi, tid, 256, [&](int, float x) __attribute__((always_inline)) {
+      double y, r;
+      if (scale.weighs(x, y)) atomicAdd((uint32_t*)&bin[Scale::bin_of_steps(Scale::steps_of(y, r))], 1u);
+    });
+  } else {
+    each_token<DT>(base, lo, hi, tid, 256, [&](int, float x) __attribute__((always_inline)) {
+      double y, r;
+      if (scale.weighs(x, y)) {
+        const int k = Scale::steps_of(y, r);
+        atomicAdd((unsigned long long*)&bin[Scale::bin_of_steps(k)], (unsigned long long)scale.of_steps(k, r));
+      }
+    });
+  }
+  __syncthreads();
+  uint64_t* out = a.bins + (int64_t)blockIdx.x * SM_BINS;
+  for (int i = tid; i < SM_BINS; i += 256) out[i] = bin[i];
+}
+
+// third: a workgroup a row. From the parts' histograms the bin that the cut falls into; the tokens that may be kept (kCount)
+// or that lie where the cuts fall (kMass) are collected in one pass of comparisons and the cut found among them; the kept
+// weight of every part; and the tokens of the part that the random number falls into. Where the collected ones are too
+// many (thousands of nearly equal logits, a very large top_k) all is done by passes over the row.
+template <int DT>
+__global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
+  constexpr int NW = 16, NT = 1024;
+  using D = Drawer<NW>;
+  using L = Logits<DT>;
+  __shared__ typename D::Lds l;
+  __shared__ float found_x[SM_FOUND];
+  __shared__ int found_i[SM_FOUND];
+  __shared__ ulonglong2 few[SM_FEW];
+  __shared__ uint64_t part_w[SM_PARTS];
+  __shared__ uint32_t part_ties[SM_PARTS], n_found;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t row = blockIdx.x;
+  const uint8_t* base = row_at(a, row, L::kBytes);
+  const Settings s = settings_of(a, row);
+  const float m = row_max(a, row);
+  if (m == -INFINITY) {
+    if (tid == 0) a.tokens[row] = -1, a.logprobs[row] = NAN;
+    return;
+  }
+  if (s.way == kGreedy) {
+    // the first part that holds the largest
+    const uint64_t with = __ballot(lane < a.parts && a.most[row * a.parts + min(lane, a.parts - 1)] == m);
+    const int g = __ffsll((unsigned long long)with) - 1, lo = g * a.part, hi = min(lo + a.part, a.vocab);
+    if (tid == 0) n_found = 0xffffffffu;
+    __syncthreads();
+    uint32_t first = 0xffffffffu;
+    each_token<DT>(base, lo, hi, tid, NT,
+                   [&](int i, float x) __attribute__((always_inline)) { first = x == m ? min(first, (uint32_t)i) : first; });
+    if (first != 0xffffffffu) atomicMin(&n_found, first);
+    __syncthreads();
+    if (tid == 0) a.tokens[row] = n_found, a.logprobs[row] = 0.0f;
+    return;
+  }
+  fill_table(l.table);
+  if (tid < SM_PARTS) part_w[tid] = 0, part_ties[tid] = 0;
+  if (tid == 0) n_found = 0;
+  D d(l, a, s, row, m);
+  const uint64_t* bins = a.bins + row * a.parts * SM_BINS;
+  Cut cut = {0, (uint32_t)a.vocab, (uint32_t)a.vocab};
+  bool whole = s.way == kWhole;
+  int from = 0, to = SM_BINS - 1;  // bins whose tokens are collected
+  typename D::Place p = {SM_BINS, 0, 0, 0};
+  double target = 0.0;
+  if (!whole) {
+    // the row's histogram: two threads a bin, each half of the parts, joined in LDS
+    uint64_t mine = 0;
+    const int b = tid & 511;
+    if (b < SM_BINS)
+      for (int g = tid / 512; g < a.parts; g += 2) mine += bins[g * SM_BINS + b];
+    if (tid >= 512 && b < SM_BINS) l.mass[b] = mine;
+    __syncthreads();
+    uint64_t n[1] = {0}, w[1] = {0};
+    if (tid < SM_BINS) (s.way == kCount ? n[0] : w[0]) = mine + l.mass[tid];
+    if (s.way == kCount) {
+      if (tid == 0) l.found[0] = SM_BINS;  // where fewer tokens weigh anything: all of them are kept
+      p = d.template reach<false>(n, w, tid, 0, 0, (uint64_t)s.top_k, [](uint64_t) { return 0.0; });
+      to = min(p.bin, SM_BINS - 2);
+      whole = p.bin < SM_BINS && p.before + p.inside > SM_FOUND;
+    } else {
+      from = SM_BINS, to = SM_BINS - 2;  // the last bin's weights are 0
+      if (s.top_p < 1.0f) {
+        p = d.template reach<true>(n, w, tid, 0, 0, 0, [&](uint64_t all) { return target = d.target_of(all); });
+        from = to = p.bin;
+      }
+      if (s.min_p > 0.0f) {
+        // the bin of the least weight that stays (-8 y + 1 / 32 of it; fp32 finds it to 2^-12), and the one beside it where
+        // their border is near
+        const float at = -log2f(s.min_p) * 8.0f + 0.03125f;
+        from = min(from, (int)fminf(fmaxf(at - 0.01f, 0.0f), (float)SM_BINS));
+        to = min(to, (int)fminf(at + 0.01f, (float)SM_BINS));
+      }
+    }
+  }
+  if (!whole && from < SM_BINS) {
+    float lo, hi;
+    d.scale.range(from, to, lo, hi);
+    each_token<DT>(base, 0, a.vocab, tid, NT, [&](int i, float x) __attribute__((always_inline)) {
+      if (x >= lo && x <= hi) {
+        const int b = d.scale.bin(x);
+        if (b >= from && b <= to) {
+          const uint32_t at = atomicAdd(&n_found, 1u);
+          if (at < SM_FOUND) found_x[at] = x, found_i[at] = i;
+        }
+      }
+    });
+    __syncthreads();
+    whole = n_found > SM_FOUND;
+  }
+  __syncthreads();
+  const int n = (int)n_found;
+  if (!whole && s.way == kCount && n <= SM_FEW) {
+    // each against all. `order`: larger for what comes first (equal logits: the lowest index)
+    const bool mine = tid < n;
+    uint64_t w = 0, order = 0, ahead = 0;
+    int rank = 0;
+    if (mine) {
+      w = d.weight(found_x[tid]);
+      order = (uint64_t)order_of(found_x[tid]) << 32 | (uint32_t)~found_i[tid];
+      few[tid] = make_ulonglong2(w, order);
+    }
+    __syncthreads();
+    if (mine) {
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const ulonglong2 o = few[i];
+        rank += o.y > order, ahead += o.y > order ? o.x : 0;
+      }
+    }
+    const bool among = mine && rank < s.top_k;
+    if (tid < SM_FEW) {
+      const uint64_t sum = wave_sum64(among ? w : 0);
+      if (lane == 0) l.cells[0][wave] = sum;
+    }
+    __syncthreads();
+    // of the run that reaches top_p of the sum, what lies ahead of a token does not
+    const bool stays = among && (s.top_p >= 1.0f || (double)ahead < d.target_of(l.cells[0][0] + l.cells[0][1])) &&
+                       (double)w >= d.low;
+    if (mine) few[tid].x = stays ? w : 0;
+    __syncthreads();
+    if (stays) {
+      uint64_t total = 0, cum = 0;
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const ulonglong2 o = few[i];
+        total += o.x, cum += (uint32_t)o.y > (uint32_t)order ? o.x : 0;
+      }
+      const uint64_t r = d.drawn(total);
+      if (cum <= r && cum + w > r) d.draw(found_i[tid], found_x[tid], total);
+    }
+    return;
+  }
+  auto each_found = [&](auto f) __attribute__((always_inline)) {
+    for (int i = tid; i < n; i += NT) f(i, found_x[i]);
+  };
+  auto each = [&](auto f) __attribute__((always_inline)) { each_token<DT>(base, 0, a.vocab, tid, NT, f); };
+  if (whole) {
+    if (s.top_k) cut = d.cut_by_count(each);
+    if (s.top_p < 1.0f) cut = d.cut_by_mass(each, cut);
+  } else if (s.way == kCount) {
+    auto any = [](float) { return true; };
+    if (p.bin < SM_BINS) cut = d.template resolve<false>(each_found, any, p, (uint64_t)s.top_k, 0.0);
+    if (s.top_p < 1.0f) cut = d.cut_by_mass(each_found, cut);
+  } else if (p.bin <= to) {
+    auto any = [](float) { return true; };
+    p.inside = 0xffffffffu;  // not counted: found on the way
+    cut = d.template resolve<true>(each_found, any, p, 0, target);
+  }
+  const uint64_t tie_w = d.tie_weight(cut);
+
+  // the parts' kept weights and their ties
+  if (whole || s.way == kCount || from < SM_BINS) {
+    auto add = [&](int g, float x) __attribute__((always_inline)) {
+      const uint32_t key = order_of(x);
+      if (key > cut.key) {
+        const uint64_t w = d.kept(x);
+        if (w) atomicAdd((unsigned long long*)&part_w[g], (unsigned long long)w);
+      } else if (key == cut.key) {
+        atomicAdd(&part_ties[g], 1u);
+      }
+    };
+    if (whole) {
+      for (int g = wave; g < a.parts; g += NW) {
+        uint64_t sum = 0;
+        uint32_t ties = 0;
+        each_token<DT>(base, g * a.part, min((g + 1) * a.part, a.vocab), lane, 64,
+                       [&](int, float x) __attribute__((always_inline)) {
+                         const uint32_t key = order_of(x);
+                         if (key > cut.key) sum += d.kept(x);
+                         ties += key == cut.key;
+                       });
+        sum = wave_sum64(sum);
+        const uint64_t t = wave_sum64(ties);
+        if (lane == 0) part_w[g] = sum, part_ties[g] = (uint32_t)t;
+      }
+    } else {
+      for (int i = tid; i < n; i += NT) add(found_i[i] / a.part, found_x[i]);
+    }
+  }
+  if (!whole && s.way == kMass) {  // what lies ahead of the collected bins is kept whole
+    __syncthreads();
+    for (int g = wave; g < a.parts; g += NW) {
+      uint64_t sum = 0;
+      for (int b = lane; b < min(from, SM_BINS); b += 64) sum += bins[g * SM_BINS + b];
+      sum = wave_sum64(sum);
+      if (lane == 0) part_w[g] += sum;
+    }
+  }
+  __syncthreads();
+  // the parts, one a lane of every wave: the weight and the ties before each; the first at whose end the kept weights pass r
+  const uint64_t pw = part_w[lane], pt = part_ties[lane];
+  uint64_t pw_end = pw, pt_end = pt;
+#pragma unroll
+  for (int w = 1; w < 64; w <<= 1) {
+    const uint64_t u = shfl64_up(pw_end, w), v = shfl64_up(pt_end, w);
+    if (lane >= w) pw_end += u, pt_end += v;
+  }
+  const uint64_t end = pw_end + D::ties_in(cut, 0, pt_end) * tie_w, total = shfl64(end, 63), r = d.drawn(total);
+  const int at = __ffsll((unsigned long long)__ballot(end > r)) - 1;
+  uint64_t upto = shfl64(pt_end - pt, at), cum = shfl64(pw_end - pw, at) + D::ties_in(cut, 0, upto) * tie_w;
+  // that part's tokens, neighbouring ones a thread
+  const int p0 = at * a.part, len = min(a.part, a.vocab - p0), run = (len + NT - 1) / NT;
+  const int i0 = min(tid * run, len), i1 = min(i0 + run, len);
+  uint64_t sum = 0, ties = 0, sum_before, ties_before, sum_all, ties_all;
+  for (int i = i0; i < i1; ++i) {
+    const float x = L::at(base, p0 + i);
+    const uint32_t key = order_of(x);
+    if (key > cut.key) sum += d.kept(x);
+    ties += key == cut.key;
+  }
+  d.scan(sum, ties, sum_before, ties_before, sum_all, ties_all);
+  cum += sum_before + D::ties_in(cut, upto, ties_before) * tie_w;
+  upto += ties_before;
+  if (cum <= r && cum + sum + D::ties_in(cut, upto, ties) * tie_w > r)
+    d.pick(cut, tie_w, cum, upto, r, total, p0 + i0, i1 - i0,
+           [&](int i) __attribute__((always_inline)) { return L::at(base, p0 + i0 + i); });
+}
+
+// tokens a part of a row of `vocab`, of `rows`: SM_PART, more where that gives more than SM_PARTS parts, or more workgroups
+// than keep the chip busy (a part costs 4 KB of bins)
+int part_of(int64_t rows, int64_t vocab) {
+  int64_t part = SM_PART;
+  while (part * SM_PARTS < vocab || (part < 4 * SM_PART && rows * (vocab / part) > 2048)) part *= 2;
+  return (int)part;
+}
+bool row_is_held(int64_t vocab) { return vocab <= 1024 * SM_HELD; }
+
+template <int DT>
+void launch_sample(const SampleArgs& a, int64_t rows, hipStream_t st) {
+  const dim3 grid((unsigned)rows), parts((unsigned)(rows * a.parts));
+  if (a.vocab <= 256 * SM_HELD) {
+    hipLaunchKernelGGL((sample_held_kernel<DT, 4>), grid, dim3(256), 0, st, a);
+  } else if (row_is_held(a.vocab)) {
+    hipLaunchKernelGGL((sample_held_kernel<DT, 16>), grid, dim3(1024), 0, st, a);
+  } else {
+    hipLaunchKernelGGL((sample_max_kernel<DT>), parts, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((sample_bins_kernel<DT>), parts, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((sample_draw_kernel<DT>), grid, dim3(1024), 0, st, a);
   }
 }
 
 }  // namespace
 
+extern "C" int64_t gwa_sample_tokens_workspace(int64_t rows, int64_t vocab) {
+  if (rows <= 0 || vocab <= 0 || vocab > (1 << 24) || row_is_held(vocab)) return 0;
+  const int64_t part = part_of(rows, vocab);
+  return rows * ((vocab + part - 1) / part) * (SM_BINS * 8 + 4);
+}
+
 extern "C" int gwa_sample_tokens(const void* logits, int64_t ld, int dtype, const float* uniform,
                                  const gwa_sampling* settings, int64_t* tokens, float* logprobs, int64_t rows,
-                                 int64_t vocab, void* stream) {
+                                 int64_t vocab, void* workspace, int64_t workspace_bytes, void* stream) {
   const char* what = "sample_tokens";
   GWA_REQUIRE(settings, "%s: null settings", what);
   GWA_REQUIRE(dtype >= GWA_DT_BF16 && dtype <= GWA_DT_F32, "%s: dtype %d", what, dtype);
@@ -424,10 +902,18 @@ extern "C" int gwa_sample_tokens(const void* logits, int64_t ld, int dtype, cons
               "%s: misaligned pointer", what);
   int bits = 0;  // sums of `vocab` weights stay below 2^62
   while ((1ll << bits) < vocab) ++bits;
-  const SampleArgs a = {logits, ld, uniform, s, tokens, logprobs, (int)vocab, bits <= 17 ? 45 : 62 - bits};
-  const dim3 grid((unsigned)rows), block(SM_THREADS);
-  if (dtype == GWA_DT_BF16) hipLaunchKernelGGL((sample_rows_kernel<GWA_DT_BF16>), grid, block, 0, (hipStream_t)stream, a);
-  else if (dtype == GWA_DT_F16) hipLaunchKernelGGL((sample_rows_kernel<GWA_DT_F16>), grid, block, 0, (hipStream_t)stream, a);
-  else hipLaunchKernelGGL((sample_rows_kernel<GWA_DT_F32>), grid, block, 0, (hipStream_t)stream, a);
+  const int64_t need = gwa_sample_tokens_workspace(rows, vocab), part = part_of(rows, vocab);
+  const int64_t parts = (vocab + part - 1) / part;
+  GWA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && GWA_ALIGNED(workspace, 16)),
+              "%s: a workspace of %lld bytes, %lld are needed (16-byte aligned)", what, (long long)workspace_bytes,
+              (long long)need);
+  GWA_REQUIRE(rows * parts < (1ll << 31), "%s: %lld rows of %lld tokens are too many", what, (long long)rows,
+              (long long)vocab);
+  uint64_t* bins = (uint64_t*)workspace;
+  const SampleArgs a = {logits, ld, uniform, s, tokens, logprobs, (int)vocab, bits <= 17 ? 45 : 62 - bits, (int)parts,
+                        (int)part, bins, need ? (float*)(bins + rows * parts * SM_BINS) : nullptr};
+  if (dtype == GWA_DT_BF16) launch_sample<GWA_DT_BF16>(a, rows, (hipStream_t)stream);
+  else if (dtype == GWA_DT_F16) launch_sample<GWA_DT_F16>(a, rows, (hipStream_t)stream);
+  else launch_sample<GWA_DT_F32>(a, rows, (hipStream_t)stream);
   return gwa_check_launch(what);
 }

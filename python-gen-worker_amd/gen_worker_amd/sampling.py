@@ -56,9 +56,11 @@ def _sample_body(logits: Tensor, uniform: Tensor, temperature: Optional[Tensor],
     logprobs = torch.empty(rows, dtype=torch.float32, device=dev)
     settings = nat.SamplingArgs(nat.ptr(temperature), nat.ptr(top_k), nat.ptr(top_p), nat.ptr(min_p), all_temperature,
                                 all_top_k, all_top_p, all_min_p)
+    n = int(nat.load().gwa_sample_tokens_workspace(rows, vocab))
+    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     nat.call("gwa_sample_tokens", logits.data_ptr(), max(logits.stride(0), vocab), _DTYPES[logits.dtype],
-             uniform.data_ptr(), ctypes.byref(settings), tokens.data_ptr(), logprobs.data_ptr(), rows, vocab,
-             nat.stream_of(logits))
+             uniform.data_ptr(), ctypes.byref(settings), tokens.data_ptr(), logprobs.data_ptr(), rows, vocab, nat.ptr(ws),
+             n, nat.stream_of(logits))
     return tokens, logprobs
 
 

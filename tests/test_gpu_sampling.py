@@ -74,10 +74,12 @@ def check(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
 
 SETTINGS = [dict(), dict(temperature=0.0), dict(temperature=0.7), dict(temperature=40.0), dict(top_k=1), dict(top_k=7),
             dict(top_k=50, top_p=0.9), dict(top_p=0.5), dict(top_p=0.999), dict(top_p=0.0), dict(min_p=0.1),
-            dict(min_p=1.0), dict(temperature=1.5, top_k=300, top_p=0.95, min_p=0.02), dict(top_k=10 ** 6, top_p=0.3)]
+            dict(min_p=1.0), dict(min_p=1e-3), dict(min_p=0.3, top_p=0.7), dict(min_p=1e-6, temperature=2.0),
+            dict(top_k=100, top_p=0.8), dict(top_k=600, min_p=0.01), dict(temperature=1.5, top_k=300, top_p=0.95, min_p=0.02), dict(top_k=10 ** 6, top_p=0.3)]
 
 
-@pytest.mark.parametrize("rows,vocab", [(3, 1), (5, 2), (4, 7), (9, 64), (6, 257), (5, 2048), (3, 5003), (2, 70001)])
+@pytest.mark.parametrize("rows,vocab", [(3, 1), (5, 2), (4, 7), (9, 64), (6, 257), (5, 2048), (5, 2049), (3, 5003),
+                                        (3, 8192), (3, 8193), (2, 12289), (2, 70001), (40, 20011), (1, 300007)])
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 def test_tokens_by_the_definition(rows, vocab, dtype):
     """bf16 rows of tens of thousands hold many equal logits: cuts fall among them."""
@@ -211,6 +213,35 @@ def test_draws_follow_the_weights():
     share = torch.where(keep, w, 0.0) / torch.where(keep, w, 0.0).sum()
     assert bool(((torch.bincount(tokens, minlength=40).double() - n * share).abs() <= 1.0).all())
     assert bool((lp.double() - torch.log(share[tokens])).abs().max() < 1e-6)
+
+
+@pytest.mark.parametrize("vocab", [700, 20011])
+def test_fewer_drawable_tokens_than_top_k(vocab):
+    """A mask that leaves a few tokens (of 64, of 200, of 3000), under a larger top_k: its cut drops none of them."""
+    g = _gen(vocab)
+    logits = torch.full((6, vocab), -math.inf, device=DEV)
+    for r, n in enumerate((1, 3, 64, 200, 500, 3000)):
+        at = torch.randperm(vocab, generator=g, device=DEV)[:n]
+        logits[r, at] = torch.randn(len(at), generator=g, device=DEV) * 2
+    logits[3, logits[3] == -math.inf] = torch.finfo(F32).min
+    for k in (1, 70, 250, 1500):
+        for s in (dict(), dict(top_p=0.8), dict(min_p=0.2)):
+            check(logits, torch.rand(6, generator=g, device=DEV), top_k=k, **s)
+
+
+@pytest.mark.parametrize("min_p", [2.0 ** -30, 2.0 ** -28, 2.0 ** -27, 1e-7, 2.0 ** -10])
+def test_least_min_p(min_p):
+    """Weights down to nothing on either side of a tiny min_p; below 2^-28 all are kept."""
+    from gen_worker_amd.sampling import sample_tokens
+
+    x = -torch.arange(20000, device=DEV).float()[None] * (32.0 / 20000)
+    u = torch.tensor([1.0], device=DEV)
+    token, _ = sample_tokens(x, u, min_p=min_p)
+    # of all, those of weight 2^-46 or more are drawn: the others' integers of 2^-45 are 0 (31.88 units below the largest)
+    least = min_p if min_p >= 2.0 ** -28 else 2.0 ** -46
+    want = int((torch.exp(x.double()) >= least).sum()) - 1
+    # the last kept token, to the one whose weight is on the border to fp32 rounding of its logit
+    assert abs(int(token) - want) <= 1
 
 
 def test_another_stream_and_a_graph():

@@ -26,14 +26,14 @@ class TestEntryPoint:
     """The C entry point refuses before any launch."""
 
     def call(self, logits=4096, ld=100, dtype=2, uniform=4096, tokens=4096, logprobs=4096, rows=2, vocab=100, settings=True,
-             **change):
+             workspace=None, nbytes=0, **change):
         from gen_worker_amd import _native as nat
 
         v = dict(all_temperature=1.0, all_top_k=0, all_top_p=1.0, all_min_p=0.0)
         v.update(change)
         s = ctypes.byref(nat.SamplingArgs(**v)) if settings else None
         lib = nat.load()
-        rc = lib.gwa_sample_tokens(logits, ld, dtype, uniform, s, tokens, logprobs, rows, vocab, None)
+        rc = lib.gwa_sample_tokens(logits, ld, dtype, uniform, s, tokens, logprobs, rows, vocab, workspace, nbytes, None)
         return rc, lib.gwa_last_error().decode()
 
     @pytest.mark.parametrize("change,match", [
@@ -44,10 +44,20 @@ class TestEntryPoint:
         (dict(temperature=4098), "misaligned"), (dict(all_temperature=-1.0), "temperature"),
         (dict(all_temperature=math.nan), "temperature"), (dict(all_temperature=math.inf), "temperature"),
         (dict(all_top_k=-1), "top_k"), (dict(all_top_p=1.5), "top_p"), (dict(all_top_p=math.nan), "top_p"),
-        (dict(all_min_p=-0.1), "min_p")])
+        (dict(all_min_p=-0.1), "min_p"), (dict(vocab=50000, ld=50000), "workspace"),
+        (dict(vocab=50000, ld=50000, workspace=4096, nbytes=1000), "workspace"),
+        (dict(vocab=50000, ld=50000, workspace=4104, nbytes=1 << 30), "workspace"),
+        (dict(rows=2 ** 30, vocab=50000, ld=50000, workspace=4096, nbytes=1 << 60), "too many")])
     def test_refuses(self, change, match):
         rc, said = self.call(**change)
         assert rc == 1 and match in said, said
 
     def test_no_rows_need_no_device(self):
         assert self.call(rows=0, logits=None)[0] == 0
+
+    def test_workspace(self):
+        from gen_worker_amd import _native as nat
+
+        of = nat.load().gwa_sample_tokens_workspace
+        assert of(5, 8192) == of(0, 10 ** 6) == of(3, 0) == of(-1, 50000) == 0
+        assert 0 < of(1, 8193) < of(2, 8193) < of(2, 2 ** 24) < 2 ** 20
