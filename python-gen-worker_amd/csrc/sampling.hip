@@ -10,7 +10,7 @@ constexpr int SM_HELD = 8;            // logits a thread holds where a row fits 
 constexpr int SM_PART = 4096, SM_PARTS = 64;  // tokens a part of a longer row at least; parts of a row at most
 constexpr int SM_AHEAD = 4;           // 16-byte loads a lane has in flight
 constexpr int SM_FEW = 128;           // collected tokens that are ranked all against all
-constexpr int kTableBits = 7;         // of the table of 2^(j / 128)
+constexpr int kTableBits = 9;         // of the table of 2^(j / 512)
 
 struct SampleArgs {
   const void* logits;
@@ -57,56 +57,38 @@ struct Logits<GWA_DT_F16> {
   }
 };
 
-// 2^(j / 128), rounded to nearest
-__device__ const double kPowers[1 << kTableBits] = {
-    0x1.0000000000000p+0, 0x1.0163da9fb3335p+0, 0x1.02c9a3e778061p+0, 0x1.04315e86e7f85p+0,
-    0x1.059b0d3158574p+0, 0x1.0706b29ddf6dep+0, 0x1.0874518759bc8p+0, 0x1.09e3ecac6f383p+0,
-    0x1.0b5586cf9890fp+0, 0x1.0cc922b7247f7p+0, 0x1.0e3ec32d3d1a2p+0, 0x1.0fb66affed31bp+0,
-    0x1.11301d0125b51p+0, 0x1.12abdc06c31ccp+0, 0x1.1429aaea92de0p+0, 0x1.15a98c8a58e51p+0,
-    0x1.172b83c7d517bp+0, 0x1.18af9388c8deap+0, 0x1.1a35beb6fcb75p+0, 0x1.1bbe084045cd4p+0,
-    0x1.1d4873168b9aap+0, 0x1.1ed5022fcd91dp+0, 0x1.2063b88628cd6p+0, 0x1.21f49917ddc96p+0,
-    0x1.2387a6e756238p+0, 0x1.251ce4fb2a63fp+0, 0x1.26b4565e27cddp+0, 0x1.284dfe1f56381p+0,
-    0x1.29e9df51fdee1p+0, 0x1.2b87fd0dad990p+0, 0x1.2d285a6e4030bp+0, 0x1.2ecafa93e2f56p+0,
-    0x1.306fe0a31b715p+0, 0x1.32170fc4cd831p+0, 0x1.33c08b26416ffp+0, 0x1.356c55f929ff1p+0,
-    0x1.371a7373aa9cbp+0, 0x1.38cae6d05d866p+0, 0x1.3a7db34e59ff7p+0, 0x1.3c32dc313a8e5p+0,
-    0x1.3dea64c123422p+0, 0x1.3fa4504ac801cp+0, 0x1.4160a21f72e2ap+0, 0x1.431f5d950a897p+0,
-    0x1.44e086061892dp+0, 0x1.46a41ed1d0057p+0, 0x1.486a2b5c13cd0p+0, 0x1.4a32af0d7d3dep+0,
-    0x1.4bfdad5362a27p+0, 0x1.4dcb299fddd0dp+0, 0x1.4f9b2769d2ca7p+0, 0x1.516daa2cf6642p+0,
-    0x1.5342b569d4f82p+0, 0x1.551a4ca5d920fp+0, 0x1.56f4736b527dap+0, 0x1.58d12d497c7fdp+0,
-    0x1.5ab07dd485429p+0, 0x1.5c9268a5946b7p+0, 0x1.5e76f15ad2148p+0, 0x1.605e1b976dc09p+0,
-    0x1.6247eb03a5585p+0, 0x1.6434634ccc320p+0, 0x1.6623882552225p+0, 0x1.68155d44ca973p+0,
-    0x1.6a09e667f3bcdp+0, 0x1.6c012750bdabfp+0, 0x1.6dfb23c651a2fp+0, 0x1.6ff7df9519484p+0,
-    0x1.71f75e8ec5f74p+0, 0x1.73f9a48a58174p+0, 0x1.75feb564267c9p+0, 0x1.780694fde5d3fp+0,
-    0x1.7a11473eb0187p+0, 0x1.7c1ed0130c132p+0, 0x1.7e2f336cf4e62p+0, 0x1.80427543e1a12p+0,
-    0x1.82589994cce13p+0, 0x1.8471a4623c7adp+0, 0x1.868d99b4492edp+0, 0x1.88ac7d98a6699p+0,
-    0x1.8ace5422aa0dbp+0, 0x1.8cf3216b5448cp+0, 0x1.8f1ae99157736p+0, 0x1.9145b0b91ffc6p+0,
-    0x1.93737b0cdc5e5p+0, 0x1.95a44cbc8520fp+0, 0x1.97d829fde4e50p+0, 0x1.9a0f170ca07bap+0,
-    0x1.9c49182a3f090p+0, 0x1.9e86319e32323p+0, 0x1.a0c667b5de565p+0, 0x1.a309bec4a2d33p+0,
-    0x1.a5503b23e255dp+0, 0x1.a799e1330b358p+0, 0x1.a9e6b5579fdbfp+0, 0x1.ac36bbfd3f37ap+0,
-    0x1.ae89f995ad3adp+0, 0x1.b0e07298db666p+0, 0x1.b33a2b84f15fbp+0, 0x1.b59728de5593ap+0,
-    0x1.b7f76f2fb5e47p+0, 0x1.ba5b030a1064ap+0, 0x1.bcc1e904bc1d2p+0, 0x1.bf2c25bd71e09p+0,
-    0x1.c199bdd85529cp+0, 0x1.c40ab5fffd07ap+0, 0x1.c67f12e57d14bp+0, 0x1.c8f6d9406e7b5p+0,
-    0x1.cb720dcef9069p+0, 0x1.cdf0b555dc3fap+0, 0x1.d072d4a07897cp+0, 0x1.d2f87080d89f2p+0,
-    0x1.d5818dcfba487p+0, 0x1.d80e316c98398p+0, 0x1.da9e603db3285p+0, 0x1.dd321f301b460p+0,
-    0x1.dfc97337b9b5fp+0, 0x1.e264614f5a129p+0, 0x1.e502ee78b3ff6p+0, 0x1.e7a51fbc74c83p+0,
-    0x1.ea4afa2a490dap+0, 0x1.ecf482d8e67f1p+0, 0x1.efa1bee615a27p+0, 0x1.f252b376bba97p+0,
-    0x1.f50765b6e4540p+0, 0x1.f7bfdad9cbe14p+0, 0x1.fa7c1819e90d8p+0, 0x1.fd3c22b8f71f1p+0};
-__device__ __forceinline__ void fill_table(double* table) {
-  for (int i = threadIdx.x; i < (1 << kTableBits); i += blockDim.x) table[i] = kPowers[i];
+// 2^(j / 16) and 2^(j / 512), rounded to nearest
+__device__ const double kPowers16[16] = {
+    0x1.0000000000000p+0, 0x1.0b5586cf9890fp+0, 0x1.172b83c7d517bp+0, 0x1.2387a6e756238p+0,
+    0x1.306fe0a31b715p+0, 0x1.3dea64c123422p+0, 0x1.4bfdad5362a27p+0, 0x1.5ab07dd485429p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.7a11473eb0187p+0, 0x1.8ace5422aa0dbp+0, 0x1.9c49182a3f090p+0,
+    0x1.ae89f995ad3adp+0, 0x1.c199bdd85529cp+0, 0x1.d5818dcfba487p+0, 0x1.ea4afa2a490dap+0};
+__device__ const double kPowers512[32] = {
+    0x1.0000000000000p+0, 0x1.0058c86da1c0ap+0, 0x1.00b1afa5abcbfp+0, 0x1.010ab5b2cbd11p+0,
+    0x1.0163da9fb3335p+0, 0x1.01bd1e77170b4p+0, 0x1.02168143b0281p+0, 0x1.027003103b10ep+0,
+    0x1.02c9a3e778061p+0, 0x1.032363d42b027p+0, 0x1.037d42e11bbccp+0, 0x1.03d7411915a8ap+0,
+    0x1.04315e86e7f85p+0, 0x1.048b9b35659d8p+0, 0x1.04e5f72f654b1p+0, 0x1.0540727fc1762p+0,
+    0x1.059b0d3158574p+0, 0x1.05f5c74f0bec2p+0, 0x1.0650a0e3c1f89p+0, 0x1.06ab99fa6407cp+0,
+    0x1.0706b29ddf6dep+0, 0x1.0761ead925493p+0, 0x1.07bd42b72a836p+0, 0x1.0818ba42e7d30p+0,
+    0x1.0874518759bc8p+0, 0x1.08d0088f8093fp+0, 0x1.092bdf66607e0p+0, 0x1.0987d61701716p+0,
+    0x1.09e3ecac6f383p+0, 0x1.0a402331b9715p+0, 0x1.0a9c79b1f3919p+0, 0x1.0af8f03834e52p+0};
+// 2^shift 2^(j / 512)
+__device__ __forceinline__ void fill_table(double* table, int shift) {
+  for (int i = threadIdx.x; i < (1 << kTableBits); i += blockDim.x)
+    table[i] = __builtin_amdgcn_ldexp(kPowers16[i >> 5] * kPowers512[i & 31], shift);
 }
 
 // A row's tokens by their weight exp((x - m) / temperature) = 2^y, y = (x - m) log2(e) / temperature in 64 bits. The weight
-// is an integer of 2^-shift: 2^y = 2^n 2^(j/128) 2^r, |r| <= 1/256, by a table and the series of 2^r to r^4 (the rest is
-// below 2^-49), rounded by an addition of 2^52. Bins are an eighth of a unit of y wide; the last is for what weighs
+// is an integer of 2^-shift: 2^y = 2^n 2^(j/512) 2^r, |r| <= 1/1024, by a table (which holds the 2^shift) and the series of
+// 2^r to r^3 (the rest is below 2^-46), rounded by an addition of 2^52. Bins are an eighth of a unit of y wide; the last is for what weighs
 // nothing: y < -47, -inf and NaN. Bins and their halves (`inside`) fall as x grows, never the other way. A token's weight and
 // bin have to be the same wherever they are formed, so the compiler may not choose where products and sums are fused.
 // m = +inf is held as 1e300: +inf is then at y = 0, all else far below.
 struct Scale {
   double c, m;
-  int shift;
   const double* table;
-  static constexpr double kMagic = 6755399441055744.0 / (1 << kTableBits);  // 1.5 * 2^52: its last bit is 1 / 128
-  static constexpr int kPerBin = 4;  // log2 of 1 / 128 in a bin
+  static constexpr double kMagic = 6755399441055744.0 / (1 << kTableBits);  // 1.5 * 2^52: its last bit is 1 / 512
+  static constexpr int kPerBin = 6;  // log2 of the 1 / 512 in a bin
   __device__ __forceinline__ bool weighs(float x, double& y) const {
 #pragma clang fp contract(off)
     y = ((double)x - m) * c;
@@ -122,12 +104,14 @@ struct Scale {
   __device__ __forceinline__ uint64_t of_steps(int k, double r) const {
 #pragma clang fp contract(off)
     // ln(2)^i / i!
-    double p = 9.6181291076284772e-3;
-    p = __builtin_fma(p, r, 5.5504108664821580e-2);
+    double p = 5.5504108664821580e-2;
     p = __builtin_fma(p, r, 2.4022650695910072e-1);
     p = __builtin_fma(p, r, 6.9314718055994531e-1);
     p = __builtin_fma(p, r, 1.0);
-    p = __builtin_amdgcn_ldexp(p * table[k & ((1 << kTableBits) - 1)], shift + (k >> kTableBits));
+    // times 2^(k >> 9), in the exponent: the product lies in 2^shift [0.99, 2), n is -48 at least and shift 38
+    const uint64_t u = __builtin_bit_cast(uint64_t, p * table[k & ((1 << kTableBits) - 1)]);
+    const uint32_t hi = (uint32_t)(u >> 32) + ((uint32_t)(k & ~((1 << kTableBits) - 1)) << (20 - kTableBits));
+    p = __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)u);
     return __builtin_bit_cast(uint64_t, p + 4503599627370496.0) & 0xfffffffffffffull;
   }
   static __device__ __forceinline__ int bin_of_steps(int k) { return -k >> kPerBin; }
@@ -141,12 +125,12 @@ struct Scale {
     double y, r;
     return weighs(x, y) ? bin_of_steps(steps_of(y, r)) : SM_BINS - 1;
   }
-  // a bin's tokens once more into SM_BINS: by how far -8 y lies past the bin's start, bin - 1 / 32
+  // a bin's tokens once more into SM_BINS: by how far -8 y lies past the bin's start, bin - 1 / 128
   __device__ __forceinline__ int inside(float x, int bin) const {
 #pragma clang fp contract(off)
     double y;
     if (!weighs(x, y)) return SM_BINS - 1;
-    const double f = (fmin(y, 0.0) * -8.0 - ((double)bin - 0.03125)) * (double)SM_BINS;
+    const double f = (fmin(y, 0.0) * -8.0 - ((double)bin - 0.0078125)) * (double)SM_BINS;
     return min(max((int)f, 0), SM_BINS - 1);
   }
   // a range of logits that holds all of bins from to .. (and some more), in fp32
@@ -198,31 +182,51 @@ __device__ __forceinline__ Settings settings_of(const SampleArgs& a, int64_t row
 }
 
 __device__ __forceinline__ Scale scale_of(const SampleArgs& a, const Settings& s, float m, const double* table) {
-  return {1.4426950408889634 / (double)s.temperature, m == INFINITY ? 1e300 : (double)m, a.shift, table};
+  return {1.4426950408889634 / (double)s.temperature, m == INFINITY ? 1e300 : (double)m, table};
 }
 
-// f(index, logit) over tokens [lo, hi) of the row at base, by threads `id` of n, in 16-byte pieces where they are whole
+// f(N, index of the first, N neighbouring logits) over tokens [lo, hi) of the row at base, by threads `id` of n, in 16-byte
+// pieces where they are whole
 template <int DT, class F>
-__device__ __forceinline__ void each_token(const uint8_t* base, int lo, int hi, int id, int n, F f) {
+__device__ __forceinline__ void each_vector(const uint8_t* base, int lo, int hi, int id, int n, F f) {
   using L = Logits<DT>;
+  constexpr std::integral_constant<int, 1> one;
+  constexpr std::integral_constant<int, L::kVec> many;
   const uint8_t* p = base + (int64_t)lo * L::kBytes;
   const int head = min((int)((16 - ((uintptr_t)p & 15)) & 15) / L::kBytes, hi - lo);
-  if (id < head) f(lo + id, L::at(p, id));
+  if (id < head) {
+    const float x[1] = {L::at(p, id)};
+    f(one, lo + id, x);
+  }
   const int v0 = lo + head, vecs = (hi - v0) / L::kVec;
   const v4i* body = (const v4i*)(base + (int64_t)v0 * L::kBytes);
   for (int v = id; v < vecs; v += n * SM_AHEAD) {
-    v4i x[SM_AHEAD];
+    v4i w[SM_AHEAD];
 #pragma unroll
-    for (int u = 0; u < SM_AHEAD; ++u) x[u] = body[min(v + n * u, vecs - 1)];
+    for (int u = 0; u < SM_AHEAD; ++u) w[u] = body[min(v + n * u, vecs - 1)];
 #pragma unroll
     for (int u = 0; u < SM_AHEAD; ++u)
       if (v + n * u < vecs) {
+        float x[L::kVec];
 #pragma unroll
-        for (int e = 0; e < L::kVec; ++e) f(v0 + (v + n * u) * L::kVec + e, L::of(x[u], e));
+        for (int e = 0; e < L::kVec; ++e) x[e] = L::of(w[u], e);
+        f(many, v0 + (v + n * u) * L::kVec, x);
       }
   }
   const int tail = v0 + vecs * L::kVec + id;
-  if (tail < hi) f(tail, L::at(base, tail));
+  if (tail < hi) {
+    const float x[1] = {L::at(base, tail)};
+    f(one, tail, x);
+  }
+}
+
+// the same with f(index, logit)
+template <int DT, class F>
+__device__ __forceinline__ void each_token(const uint8_t* base, int lo, int hi, int id, int n, F f) {
+  each_vector<DT>(base, lo, hi, id, n, [&](auto n_c, int i, const float (&x)[decltype(n_c)::value]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < decltype(n_c)::value; ++e) f(i + e, x[e]);
+  });
 }
 
 // What a cut keeps: the tokens ordered above `key`, and of those equal to it the first `ties` by index. `equal`: how many
@@ -327,12 +331,12 @@ struct Drawer {
     __syncthreads();
     for (int i = threadIdx.x; i < SM_BINS; i += NT) l.count[i] = 0, l.mass[i] = 0;
     __syncthreads();
-    each([&](int, float x) __attribute__((always_inline)) {
+    each([&](int, float x, auto weight) __attribute__((always_inline)) {
       if (take(x)) {
         const int b = bin_of(x);
         if (b >= 0) {
           atomicAdd(&l.count[b], 1u);
-          if (MASS) atomicAdd((unsigned long long*)&l.mass[b], (unsigned long long)weight(x));
+          if (MASS) atomicAdd((unsigned long long*)&l.mass[b], (unsigned long long)weight());
         }
       }
     });
@@ -362,11 +366,11 @@ struct Drawer {
     if (p.inside <= SM_LIST) {  // ranked by counting
       if (threadIdx.x == 0) l.n = 0;
       __syncthreads();
-      each([&](int, float x) __attribute__((always_inline)) {
+      each([&](int, float x, auto weight) __attribute__((always_inline)) {
         if (here(x)) {
           const uint32_t i = atomicAdd(&l.n, 1u);
           l.list_key[i] = order_of(x);
-          if (MASS) l.list_w[i] = weight(x);
+          if (MASS) l.list_w[i] = weight();
         }
       });
       __syncthreads();
@@ -400,12 +404,12 @@ struct Drawer {
       const int bits = pass == 2 ? 10 : 11;
       for (int i = threadIdx.x; i < SM_DIGITS; i += NT) l.count[i] = 0, l.mass[i] = 0;
       __syncthreads();
-      each([&](int, float x) __attribute__((always_inline)) {
+      each([&](int, float x, auto weight) __attribute__((always_inline)) {
         const uint32_t key = order_of(x);
         if (here(x) && (pass == 0 || key >> (shift + bits) == prefix)) {
           const uint32_t d = SM_DIGITS - 1 - (key >> shift & ((1u << bits) - 1));  // falling
           atomicAdd(&l.count[d], 1u);
-          if (MASS) atomicAdd((unsigned long long*)&l.mass[d], (unsigned long long)weight(x));
+          if (MASS) atomicAdd((unsigned long long*)&l.mass[d], (unsigned long long)weight());
         }
       });
       __syncthreads();
@@ -449,11 +453,8 @@ struct Drawer {
     return resolve<true>(each, take, p, 0, target);
   }
 
-  __device__ __forceinline__ uint64_t kept(float x) const {
-    const uint64_t w = weight(x);
-    return (double)w >= low ? w : 0;
-  }
-  __device__ __forceinline__ uint64_t tie_weight(const Cut& cut) const { return cut.key ? kept(value_of(cut.key)) : 0; }
+  __device__ __forceinline__ uint64_t kept(uint64_t w) const { return (double)w >= low ? w : 0; }
+  __device__ __forceinline__ uint64_t tie_weight(const Cut& cut) const { return cut.key ? kept(weight(value_of(cut.key))) : 0; }
   static __device__ __forceinline__ uint64_t ties_in(const Cut& cut, uint64_t before, uint64_t n) {  // kept, of n behind `before`
     return before >= cut.ties ? 0 : min(n, (uint64_t)cut.ties - before);
   }
@@ -473,9 +474,10 @@ struct Drawer {
   __device__ __forceinline__ void pick(const Cut& cut, uint64_t tie_w, uint64_t cum, uint64_t upto, uint64_t r, uint64_t total,
                                        int index, int n, F f) {
     for (int i = 0; i < n; ++i) {
-      const float x = f(i);
+      uint64_t w;
+      const float x = f(i, w);
       const uint32_t key = order_of(x);
-      if (key > cut.key) cum += kept(x);
+      if (key > cut.key) cum += kept(w);
       else if (key == cut.key) cum += upto++ < cut.ties ? tie_w : 0;
       if (cum > r) {
         draw(index + i, x, total);
@@ -518,7 +520,7 @@ __global__ __launch_bounds__(64 * NW) void sample_held_kernel(SampleArgs a) {
 #pragma unroll
     for (int i = 0; i < SM_HELD; ++i) x[i] = i < n ? L::at(base, i0 + i) : NAN;
   }
-  fill_table(l.table);
+  fill_table(l.table, a.shift);
   float m = -INFINITY;
 #pragma unroll
   for (int i = 0; i < SM_HELD; ++i) m = fmaxf(m, x[i]);
@@ -542,29 +544,33 @@ __global__ __launch_bounds__(64 * NW) void sample_held_kernel(SampleArgs a) {
     return;
   }
   D d(l, a, s, row, m);
+  uint64_t w[SM_HELD];
+#pragma unroll
+  for (int i = 0; i < SM_HELD; ++i) w[i] = d.weight(x[i]);
   auto each = [&](auto f) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < SM_HELD; ++i)
-      if (i < n) f(i0 + i, x[i]);
+      if (i < n) f(i0 + i, x[i], [&]() { return w[i]; });
   };
   Cut cut = {0, (uint32_t)a.vocab, (uint32_t)a.vocab};
   if (s.top_k) cut = d.cut_by_count(each);
   if (s.top_p < 1.0f) cut = d.cut_by_mass(each, cut);
   const uint64_t tie_w = d.tie_weight(cut);
   uint64_t sum = 0, ties = 0, sum_before, ties_before, sum_all, ties_all;
-  each([&](int, float x) __attribute__((always_inline)) {
+  each([&](int, float x, auto weight) __attribute__((always_inline)) {
     const uint32_t key = order_of(x);
-    if (key > cut.key) sum += d.kept(x);
+    if (key > cut.key) sum += d.kept(weight());
     ties += key == cut.key;
   });
   d.scan(sum, ties, sum_before, ties_before, sum_all, ties_all);
   const uint64_t total = sum_all + D::ties_in(cut, 0, ties_all) * tie_w, r = d.drawn(total);
   const uint64_t cum = sum_before + D::ties_in(cut, 0, ties_before) * tie_w;
   if (cum <= r && cum + sum + D::ties_in(cut, ties_before, ties) * tie_w > r) {
-    d.pick(cut, tie_w, cum, ties_before, r, total, i0, n, [&](int i) __attribute__((always_inline)) {
+    d.pick(cut, tie_w, cum, ties_before, r, total, i0, n, [&](int i, uint64_t& wi) __attribute__((always_inline)) {
       float y = x[0];
+      wi = w[0];
 #pragma unroll
-      for (int e = 1; e < SM_HELD; ++e) y = i == e ? x[e] : y;
+      for (int e = 1; e < SM_HELD; ++e) y = i == e ? x[e] : y, wi = i == e ? w[e] : wi;
       return y;
     });
   }
@@ -601,7 +607,7 @@ __global__ __launch_bounds__(256) void sample_bins_kernel(SampleArgs a) {
   if (s.way == kGreedy || s.way == kWhole) return;
   const float m = row_max(a, row);
   if (m == -INFINITY) return;
-  fill_table(table);
+  fill_table(table, a.shift);
   for (int i = tid; i < SM_BINS; i += 256) bin[i] = 0;
   __syncthreads();
   const Scale scale = scale_of(a, s, m, table);
@@ -635,11 +641,15 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
   using D = Drawer<NW>;
   using L = Logits<DT>;
   __shared__ typename D::Lds l;
+  constexpr int SEG = SM_FOUND / NW;  // a wave's own part of the collected tokens
   __shared__ float found_x[SM_FOUND];
   __shared__ int found_i[SM_FOUND];
+  __shared__ int found_n[NW];
   __shared__ ulonglong2 few[SM_FEW];
+  __shared__ float few_x[SM_FEW];
+  __shared__ int few_i[SM_FEW];
   __shared__ uint64_t part_w[SM_PARTS];
-  __shared__ uint32_t part_ties[SM_PARTS], n_found;
+  __shared__ uint32_t part_ties[SM_PARTS], least;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x;
   const uint8_t* base = row_at(a, row, L::kBytes);
@@ -653,19 +663,18 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
     // the first part that holds the largest
     const uint64_t with = __ballot(lane < a.parts && a.most[row * a.parts + min(lane, a.parts - 1)] == m);
     const int g = __ffsll((unsigned long long)with) - 1, lo = g * a.part, hi = min(lo + a.part, a.vocab);
-    if (tid == 0) n_found = 0xffffffffu;
+    if (tid == 0) least = 0xffffffffu;
     __syncthreads();
     uint32_t first = 0xffffffffu;
     each_token<DT>(base, lo, hi, tid, NT,
                    [&](int i, float x) __attribute__((always_inline)) { first = x == m ? min(first, (uint32_t)i) : first; });
-    if (first != 0xffffffffu) atomicMin(&n_found, first);
+    if (first != 0xffffffffu) atomicMin(&least, first);
     __syncthreads();
-    if (tid == 0) a.tokens[row] = n_found, a.logprobs[row] = 0.0f;
+    if (tid == 0) a.tokens[row] = least, a.logprobs[row] = 0.0f;
     return;
   }
-  fill_table(l.table);
+  fill_table(l.table, a.shift);
   if (tid < SM_PARTS) part_w[tid] = 0, part_ties[tid] = 0;
-  if (tid == 0) n_found = 0;
   D d(l, a, s, row, m);
   const uint64_t* bins = a.bins + row * a.parts * SM_BINS;
   Cut cut = {0, (uint32_t)a.vocab, (uint32_t)a.vocab};
@@ -695,39 +704,77 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
         from = to = p.bin;
       }
       if (s.min_p > 0.0f) {
-        // the bin of the least weight that stays (-8 y + 1 / 32 of it; fp32 finds it to 2^-12), and the one beside it where
+        // the bin of the least weight that stays (-8 y + 1 / 128 of it; fp32 finds it to 2^-12), and the one beside it where
         // their border is near
-        const float at = -log2f(s.min_p) * 8.0f + 0.03125f;
+        const float at = -log2f(s.min_p) * 8.0f + 0.0078125f;
         from = min(from, (int)fminf(fmaxf(at - 0.01f, 0.0f), (float)SM_BINS));
         to = min(to, (int)fminf(at + 0.01f, (float)SM_BINS));
       }
     }
   }
+  float* const my_x = found_x + wave * SEG;
+  int* const my_i = found_i + wave * SEG;
+  int mine_n = 0;
   if (!whole && from < SM_BINS) {
+    // by comparisons in fp32, of a range that holds the bins; then what is not of them goes
     float lo, hi;
     d.scale.range(from, to, lo, hi);
-    each_token<DT>(base, 0, a.vocab, tid, NT, [&](int i, float x) __attribute__((always_inline)) {
-      if (x >= lo && x <= hi) {
-        const int b = d.scale.bin(x);
-        if (b >= from && b <= to) {
-          const uint32_t at = atomicAdd(&n_found, 1u);
-          if (at < SM_FOUND) found_x[at] = x, found_i[at] = i;
-        }
+    auto below = [](uint64_t m) __attribute__((always_inline)) {
+      return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+    };
+    // the lane's N neighbouring tokens from i on
+    auto take = [&](auto n_c, int i, const float (&x)[decltype(n_c)::value]) __attribute__((always_inline)) {
+      constexpr int N = decltype(n_c)::value;
+      uint64_t hits[N], any = 0;
+#pragma unroll
+      for (int e = 0; e < N; ++e) any |= hits[e] = __ballot(__builtin_amdgcn_fmed3f(x[e], lo, hi) == x[e]);
+      if (any == 0) return;
+      // the first lane takes part whenever any of its wave does, so its count is the wave's
+      int at = __builtin_amdgcn_readfirstlane(mine_n);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int to = at + below(hits[e]);
+        if ((hits[e] >> lane & 1) && to < SEG) my_x[to] = x[e], my_i[to] = i + e;
+        at += __popcll(hits[e]);
       }
-    });
-    __syncthreads();
-    whole = n_found > SM_FOUND;
+      mine_n = at;
+    };
+    each_vector<DT>(base, 0, a.vocab, tid, NT, take);
+    mine_n = __shfl(mine_n, 0);
+    whole = mine_n > SEG;
+    int left = 0;
+    for (int i = 0; i < min(mine_n, SEG); i += 64) {
+      const bool in = i + lane < min(mine_n, SEG);
+      const float x = in ? my_x[i + lane] : NAN;
+      const int index = in ? my_i[i + lane] : 0, b = d.scale.bin(x);
+      const bool stays = in && b >= from && b <= to;
+      const uint64_t those = __ballot(stays);
+      if (stays) my_x[left + below(those)] = x, my_i[left + below(those)] = index;
+      left += __popcll(those);
+    }
+    mine_n = left;
   }
+  if (lane == 0) found_n[wave] = whole ? -1 : mine_n;
   __syncthreads();
-  const int n = (int)n_found;
+  const int of_wave = found_n[lane & (NW - 1)];
+  whole = __ballot(of_wave < 0) != 0;
+  int upto_wave = lane < NW ? of_wave : 0;
+#pragma unroll
+  for (int w = 1; w < NW; w <<= 1) {
+    const int u = __shfl_up(upto_wave, w);
+    if (lane >= w) upto_wave += u;
+  }
+  const int n = __shfl(upto_wave, NW - 1), my_first = __shfl(upto_wave, wave) - mine_n;
   if (!whole && s.way == kCount && n <= SM_FEW) {
     // each against all. `order`: larger for what comes first (equal logits: the lowest index)
     const bool mine = tid < n;
     uint64_t w = 0, order = 0, ahead = 0;
     int rank = 0;
+    for (int i = lane; i < mine_n; i += 64) few_x[my_first + i] = my_x[i], few_i[my_first + i] = my_i[i];
+    __syncthreads();
     if (mine) {
-      w = d.weight(found_x[tid]);
-      order = (uint64_t)order_of(found_x[tid]) << 32 | (uint32_t)~found_i[tid];
+      w = d.weight(few_x[tid]);
+      order = (uint64_t)order_of(few_x[tid]) << 32 | (uint32_t)~few_i[tid];
       few[tid] = make_ulonglong2(w, order);
     }
     __syncthreads();
@@ -757,14 +804,17 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
         total += o.x, cum += (uint32_t)o.y > (uint32_t)order ? o.x : 0;
       }
       const uint64_t r = d.drawn(total);
-      if (cum <= r && cum + w > r) d.draw(found_i[tid], found_x[tid], total);
+      if (cum <= r && cum + w > r) d.draw(few_i[tid], few_x[tid], total);
     }
     return;
   }
   auto each_found = [&](auto f) __attribute__((always_inline)) {
-    for (int i = tid; i < n; i += NT) f(i, found_x[i]);
+    for (int i = lane; i < mine_n; i += 64) f(my_i[i], my_x[i], [&]() { return d.weight(my_x[i]); });
   };
-  auto each = [&](auto f) __attribute__((always_inline)) { each_token<DT>(base, 0, a.vocab, tid, NT, f); };
+  auto each = [&](auto f) __attribute__((always_inline)) {
+    each_token<DT>(base, 0, a.vocab, tid, NT,
+                   [&](int i, float x) __attribute__((always_inline)) { f(i, x, [&]() { return d.weight(x); }); });
+  };
   if (whole) {
     if (s.top_k) cut = d.cut_by_count(each);
     if (s.top_p < 1.0f) cut = d.cut_by_mass(each, cut);
@@ -784,7 +834,7 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
     auto add = [&](int g, float x) __attribute__((always_inline)) {
       const uint32_t key = order_of(x);
       if (key > cut.key) {
-        const uint64_t w = d.kept(x);
+        const uint64_t w = d.kept(d.weight(x));
         if (w) atomicAdd((unsigned long long*)&part_w[g], (unsigned long long)w);
       } else if (key == cut.key) {
         atomicAdd(&part_ties[g], 1u);
@@ -797,7 +847,7 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
         each_token<DT>(base, g * a.part, min((g + 1) * a.part, a.vocab), lane, 64,
                        [&](int, float x) __attribute__((always_inline)) {
                          const uint32_t key = order_of(x);
-                         if (key > cut.key) sum += d.kept(x);
+                         if (key > cut.key) sum += d.kept(d.weight(x));
                          ties += key == cut.key;
                        });
         sum = wave_sum64(sum);
@@ -805,7 +855,7 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
         if (lane == 0) part_w[g] = sum, part_ties[g] = (uint32_t)t;
       }
     } else {
-      for (int i = tid; i < n; i += NT) add(found_i[i] / a.part, found_x[i]);
+      for (int i = lane; i < mine_n; i += 64) add(my_i[i] / a.part, my_x[i]);
     }
   }
   if (!whole && s.way == kMass) {  // what lies ahead of the collected bins is kept whole
@@ -836,7 +886,7 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
   for (int i = i0; i < i1; ++i) {
     const float x = L::at(base, p0 + i);
     const uint32_t key = order_of(x);
-    if (key > cut.key) sum += d.kept(x);
+    if (key > cut.key) sum += d.kept(d.weight(x));
     ties += key == cut.key;
   }
   d.scan(sum, ties, sum_before, ties_before, sum_all, ties_all);
@@ -844,7 +894,11 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
   upto += ties_before;
   if (cum <= r && cum + sum + D::ties_in(cut, upto, ties) * tie_w > r)
     d.pick(cut, tie_w, cum, upto, r, total, p0 + i0, i1 - i0,
-           [&](int i) __attribute__((always_inline)) { return L::at(base, p0 + i0 + i); });
+           [&](int i, uint64_t& w) __attribute__((always_inline)) {
+             const float x = L::at(base, p0 + i0 + i);
+             w = d.weight(x);
+             return x;
+           });
 }
 
 // tokens a part of a row of `vocab`, of `rows`: SM_PART, more where that gives more than SM_PARTS parts, or more workgroups
