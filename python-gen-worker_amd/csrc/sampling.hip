@@ -21,7 +21,7 @@ struct SampleArgs {
   float* logprobs;
   int vocab, shift;   // weights are integers of 2^-shift
   int parts, part;    // of a row, and the tokens of one
-  uint64_t* bins;     // [rows][parts][SM_BINS]: a part's tokens (of rows with a top_k) or their weight, by bin
+  uint64_t* bins;     // [rows][parts][SM_BINS]: a part's tokens (of rows with a top_k) or their weight, up to and with each bin
   float* most;        // [rows][parts]
 };
 
@@ -141,19 +141,34 @@ struct Scale {
   }
 };
 
-__device__ __forceinline__ uint64_t shfl64(uint64_t x, int lane) {
-  const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)x, lane), hi = (uint32_t)__shfl((int)(x >> 32), lane);
-  return (uint64_t)hi << 32 | lo;
+__device__ __forceinline__ uint64_t two_words(uint32_t lo, uint32_t hi) { return (uint64_t)hi << 32 | lo; }
+// lane `lane`'s x (the same lane for the wave)
+__device__ __forceinline__ uint64_t lane64(uint64_t x, int lane) {
+  return two_words((uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, lane),
+                   (uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane));
 }
-__device__ __forceinline__ uint64_t shfl64_up(uint64_t x, int by) {
-  const uint32_t lo = (uint32_t)__shfl_up((int)(uint32_t)x, by), hi = (uint32_t)__shfl_up((int)(x >> 32), by);
-  return (uint64_t)hi << 32 | lo;
+// x of another lane by a data-parallel move, 0 where there is none
+template <int MOVE, int ROWS>
+__device__ __forceinline__ uint64_t moved64(uint64_t x) {
+  return two_words((uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, MOVE, ROWS, 0xf, false),
+                   (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(x >> 32), MOVE, ROWS, 0xf, false));
 }
-__device__ __forceinline__ uint64_t wave_sum64(uint64_t x) {
-  for (int w = 32; w; w >>= 1) x += shfl64(x, (threadIdx.x & 63) ^ w);
+// Sums up to and with each lane: within rows of 16 lanes (shifts by 1, 2, 4, 8), then over the wave (lane 15 of a row to the
+// next, lane 31 to the upper half). All lanes take part.
+__device__ __forceinline__ uint64_t row_scan64(uint64_t x) {
+  x += moved64<0x111, 0xf>(x);
+  x += moved64<0x112, 0xf>(x);
+  x += moved64<0x114, 0xf>(x);
+  x += moved64<0x118, 0xf>(x);
   return x;
 }
-
+__device__ __forceinline__ uint64_t wave_scan64(uint64_t x) {
+  x = row_scan64(x);
+  x += moved64<0x142, 0xa>(x);
+  x += moved64<0x143, 0xc>(x);
+  return x;
+}
+__device__ __forceinline__ uint64_t wave_sum64(uint64_t x) { return lane64(wave_scan64(x), 63); }
 
 // Below this a min_p keeps all: there weights of a few units of 2^-shift (38 at least) would be compared, whose rounding
 // tells the least kept one apart from its neighbours no better than a bin does.
@@ -265,26 +280,16 @@ struct Drawer {
   // Sums of x and y over the threads before this one, in the threads' order, and over all
   __device__ __forceinline__ void scan(uint64_t x, uint64_t y, uint64_t& x_before, uint64_t& y_before, uint64_t& x_all,
                                        uint64_t& y_all) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint64_t p = x, q = y;
-#pragma unroll
-    for (int w = 1; w < 64; w <<= 1) {
-      const uint64_t u = shfl64_up(p, w), v = shfl64_up(q, w);
-      if (lane >= w) p += u, q += v;
-    }
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint64_t p = wave_scan64(x), q = wave_scan64(y);
     __syncthreads();
     if (lane == 63) l.cells[0][wave] = p, l.cells[1][wave] = q;
     __syncthreads();
-    // the waves' sums, one a lane
+    // the waves' sums, one a lane (16 at most)
     const uint64_t cx = lane < NW ? l.cells[0][lane] : 0, cy = lane < NW ? l.cells[1][lane] : 0;
-    uint64_t sx = cx, sy = cy;
-#pragma unroll
-    for (int w = 1; w < NW; w <<= 1) {
-      const uint64_t u = shfl64_up(sx, w), v = shfl64_up(sy, w);
-      if (lane >= w) sx += u, sy += v;
-    }
-    x_before = p - x + shfl64(sx - cx, wave), y_before = q - y + shfl64(sy - cy, wave);
-    x_all = shfl64(sx, NW - 1), y_all = shfl64(sy, NW - 1);
+    const uint64_t sx = row_scan64(cx), sy = row_scan64(cy);
+    x_before = p - x + lane64(sx - cx, wave), y_before = q - y + lane64(sy - cy, wave);
+    x_all = lane64(sx, NW - 1), y_all = lane64(sy, NW - 1);
   }
 
   // Where a sum over bins of counts n and weights w (SM_BINS / NT bins or fewer a thread, from bin `first` on) reaches what
@@ -595,7 +600,7 @@ __device__ __forceinline__ float row_max(const SampleArgs& a, int64_t row) {
   return wave_max(lane < a.parts ? a.most[row * a.parts + lane] : -INFINITY);  // SM_PARTS at most
 }
 
-// second: every part's histogram, of tokens or of their weight
+// second: every part's histogram, of tokens or of their weight, as sums up to each bin
 template <int DT>
 __global__ __launch_bounds__(256) void sample_bins_kernel(SampleArgs a) {
   __shared__ uint64_t bin[SM_BINS];
@@ -627,8 +632,16 @@ __global__ __launch_bounds__(256) void sample_bins_kernel(SampleArgs a) {
     });
   }
   __syncthreads();
-  uint64_t* out = a.bins + (int64_t)blockIdx.x * SM_BINS;
-  for (int i = tid; i < SM_BINS; i += 256) out[i] = bin[i];
+  if (tid < 64) {
+    constexpr int PER = SM_BINS / 64;
+    uint64_t* out = a.bins + (int64_t)blockIdx.x * SM_BINS + PER * tid;
+    uint64_t upto[PER], sum = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) upto[i] = sum += bin[PER * tid + i];
+    const uint64_t before = wave_scan64(sum) - sum;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) out[i] = before + upto[i];
+  }
 }
 
 // third: a workgroup a row. From the parts' histograms the bin that the cut falls into; the tokens that may be kept (kCount)
@@ -682,25 +695,35 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
   int from = 0, to = SM_BINS - 1;  // bins whose tokens are collected
   typename D::Place p = {SM_BINS, 0, 0, 0};
   double target = 0.0;
+  uint64_t ahead_of = 0, part_ahead = 0;
   if (!whole) {
-    // the row's histogram: two threads a bin, each half of the parts, joined in LDS
+    // the row's sums up to each bin: two threads a bin, each half of the parts, joined in LDS
     uint64_t mine = 0;
     const int b = tid & 511;
-    if (b < SM_BINS)
+    if (b < SM_BINS) {
+#pragma unroll 8
       for (int g = tid / 512; g < a.parts; g += 2) mine += bins[g * SM_BINS + b];
+    }
     if (tid >= 512 && b < SM_BINS) l.mass[b] = mine;
+    if (tid == 0) l.found[0] = SM_BINS;
     __syncthreads();
-    uint64_t n[1] = {0}, w[1] = {0};
-    if (tid < SM_BINS) (s.way == kCount ? n[0] : w[0]) = mine + l.mass[tid];
+    if (tid < SM_BINS) l.mass[tid] = mine += l.mass[tid];
+    __syncthreads();
+    const uint64_t before = tid > 0 && tid < SM_BINS ? l.mass[tid - 1] : 0;
+    if (s.way == kMass) target = d.target_of(l.mass[SM_BINS - 1]);
+    if (tid < SM_BINS && (s.way == kCount ? before < (uint64_t)s.top_k && mine >= (uint64_t)s.top_k
+                                          : (double)before < target && (double)mine >= target))
+      l.found[0] = tid, l.found[1] = before, l.found[2] = mine - before;
+    __syncthreads();
     if (s.way == kCount) {
-      if (tid == 0) l.found[0] = SM_BINS;  // where fewer tokens weigh anything: all of them are kept
-      p = d.template reach<false>(n, w, tid, 0, 0, (uint64_t)s.top_k, [](uint64_t) { return 0.0; });
+      // where fewer tokens weigh anything all of them are kept
+      p = {(int)l.found[0], (uint32_t)l.found[2], l.found[1], 0};
       to = min(p.bin, SM_BINS - 2);
       whole = p.bin < SM_BINS && p.before + p.inside > SM_FOUND;
     } else {
       from = SM_BINS, to = SM_BINS - 2;  // the last bin's weights are 0
       if (s.top_p < 1.0f) {
-        p = d.template reach<true>(n, w, tid, 0, 0, 0, [&](uint64_t all) { return target = d.target_of(all); });
+        p = {(int)l.found[0], 0xffffffffu, 0, l.found[1]};  // its tokens are counted on the way
         from = to = p.bin;
       }
       if (s.min_p > 0.0f) {
@@ -709,6 +732,11 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
         const float at = -log2f(s.min_p) * 8.0f + 0.0078125f;
         from = min(from, (int)fminf(fmaxf(at - 0.01f, 0.0f), (float)SM_BINS));
         to = min(to, (int)fminf(at + 0.01f, (float)SM_BINS));
+      }
+      // what lies ahead of the collected bins is kept whole: in the row, and in the lane's part
+      if (from > 0) {
+        ahead_of = l.mass[from - 1];
+        if (lane < a.parts) part_ahead = bins[lane * SM_BINS + from - 1];
       }
     }
   }
@@ -765,11 +793,13 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
     if (lane >= w) upto_wave += u;
   }
   const int n = __shfl(upto_wave, NW - 1), my_first = __shfl(upto_wave, wave) - mine_n;
-  if (!whole && s.way == kCount && n <= SM_FEW) {
+  const bool cuts = s.way == kCount || p.bin <= to;  // whether what is collected is cut by its order
+  const bool few_found = !whole && cuts && n <= SM_FEW;
+  if (few_found) {
     // each against all. `order`: larger for what comes first (equal logits: the lowest index)
     const bool mine = tid < n;
-    uint64_t w = 0, order = 0, ahead = 0;
-    int rank = 0;
+    uint64_t w = 0, order = 0, ahead = ahead_of;
+    uint32_t rank = 0, equal = 0;
     for (int i = lane; i < mine_n; i += 64) few_x[my_first + i] = my_x[i], few_i[my_first + i] = my_i[i];
     __syncthreads();
     if (mine) {
@@ -782,31 +812,37 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
 #pragma unroll 4
       for (int i = 0; i < n; ++i) {
         const ulonglong2 o = few[i];
-        rank += o.y > order, ahead += o.y > order ? o.x : 0;
+        const bool first = o.y > order;
+        rank += first, ahead += first ? o.x : 0, equal += first && (o.y ^ order) >> 32 == 0;
       }
     }
-    const bool among = mine && rank < s.top_k;
-    if (tid < SM_FEW) {
-      const uint64_t sum = wave_sum64(among ? w : 0);
-      if (lane == 0) l.cells[0][wave] = sum;
-    }
-    __syncthreads();
-    // of the run that reaches top_p of the sum, what lies ahead of a token does not
-    const bool stays = among && (s.top_p >= 1.0f || (double)ahead < d.target_of(l.cells[0][0] + l.cells[0][1])) &&
-                       (double)w >= d.low;
-    if (mine) few[tid].x = stays ? w : 0;
-    __syncthreads();
-    if (stays) {
-      uint64_t total = 0, cum = 0;
+    if (s.way == kCount) {
+      const bool among = mine && rank < (uint32_t)s.top_k;
+      if (tid < SM_FEW) {
+        const uint64_t sum = wave_sum64(among ? w : 0);
+        if (lane == 0) l.cells[0][wave] = sum;
+      }
+      __syncthreads();
+      // of the run that reaches top_p of the sum, what lies ahead of a token does not
+      const bool stays = among && (s.top_p >= 1.0f || (double)ahead < d.target_of(l.cells[0][0] + l.cells[0][1])) &&
+                         (double)w >= d.low;
+      if (mine) few[tid].x = stays ? w : 0;
+      __syncthreads();
+      if (stays) {
+        uint64_t total = 0, cum = 0;
 #pragma unroll 4
-      for (int i = 0; i < n; ++i) {
-        const ulonglong2 o = few[i];
-        total += o.x, cum += (uint32_t)o.y > (uint32_t)order ? o.x : 0;
+        for (int i = 0; i < n; ++i) {
+          const ulonglong2 o = few[i];
+          total += o.x, cum += (uint32_t)o.y > (uint32_t)order ? o.x : 0;
+        }
+        const uint64_t r = d.drawn(total);
+        if (cum <= r && cum + w > r) d.draw(few_i[tid], few_x[tid], total);
       }
-      const uint64_t r = d.drawn(total);
-      if (cum <= r && cum + w > r) d.draw(few_i[tid], few_x[tid], total);
+      return;
     }
-    return;
+    if (mine && (double)ahead < target && (double)(ahead + w) >= target) l.found[0] = order >> 32, l.found[1] = equal + 1;
+    __syncthreads();
+    cut = {(uint32_t)l.found[0], (uint32_t)l.found[1], (uint32_t)l.found[1]};
   }
   auto each_found = [&](auto f) __attribute__((always_inline)) {
     for (int i = lane; i < mine_n; i += 64) f(my_i[i], my_x[i], [&]() { return d.weight(my_x[i]); });
@@ -822,9 +858,8 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
     auto any = [](float) { return true; };
     if (p.bin < SM_BINS) cut = d.template resolve<false>(each_found, any, p, (uint64_t)s.top_k, 0.0);
     if (s.top_p < 1.0f) cut = d.cut_by_mass(each_found, cut);
-  } else if (p.bin <= to) {
+  } else if (cuts && !few_found) {
     auto any = [](float) { return true; };
-    p.inside = 0xffffffffu;  // not counted: found on the way
     cut = d.template resolve<true>(each_found, any, p, 0, target);
   }
   const uint64_t tie_w = d.tie_weight(cut);
@@ -858,54 +893,50 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
       for (int i = lane; i < mine_n; i += 64) add(my_i[i] / a.part, my_x[i]);
     }
   }
-  if (!whole && s.way == kMass) {  // what lies ahead of the collected bins is kept whole
-    __syncthreads();
-    for (int g = wave; g < a.parts; g += NW) {
-      uint64_t sum = 0;
-      for (int b = lane; b < min(from, SM_BINS); b += 64) sum += bins[g * SM_BINS + b];
-      sum = wave_sum64(sum);
-      if (lane == 0) part_w[g] += sum;
-    }
-  }
   __syncthreads();
   // the parts, one a lane of every wave: the weight and the ties before each; the first at whose end the kept weights pass r
-  const uint64_t pw = part_w[lane], pt = part_ties[lane];
-  uint64_t pw_end = pw, pt_end = pt;
-#pragma unroll
-  for (int w = 1; w < 64; w <<= 1) {
-    const uint64_t u = shfl64_up(pw_end, w), v = shfl64_up(pt_end, w);
-    if (lane >= w) pw_end += u, pt_end += v;
-  }
-  const uint64_t end = pw_end + D::ties_in(cut, 0, pt_end) * tie_w, total = shfl64(end, 63), r = d.drawn(total);
+  const uint64_t pw = part_w[lane] + (whole ? 0 : part_ahead), pt = part_ties[lane];
+  const uint64_t pw_end = wave_scan64(pw), pt_end = wave_scan64(pt);
+  const uint64_t end = pw_end + D::ties_in(cut, 0, pt_end) * tie_w, total = lane64(end, 63), r = d.drawn(total);
   const int at = __ffsll((unsigned long long)__ballot(end > r)) - 1;
-  uint64_t upto = shfl64(pt_end - pt, at), cum = shfl64(pw_end - pw, at) + D::ties_in(cut, 0, upto) * tie_w;
-  // that part's tokens, neighbouring ones a thread
-  const int p0 = at * a.part, len = min(a.part, a.vocab - p0), run = (len + NT - 1) / NT;
-  const int i0 = min(tid * run, len), i1 = min(i0 + run, len);
-  uint64_t sum = 0, ties = 0, sum_before, ties_before, sum_all, ties_all;
-  for (int i = i0; i < i1; ++i) {
-    const float x = L::at(base, p0 + i);
-    const uint32_t key = order_of(x);
-    if (key > cut.key) sum += d.kept(d.weight(x));
-    ties += key == cut.key;
+  uint64_t upto = lane64(pt_end - pt, at), cum = lane64(pw_end - pw, at) + D::ties_in(cut, 0, upto) * tie_w;
+  // that part's tokens, PER neighbouring ones a thread at a time
+  constexpr int PER = SM_PART / NT;
+  const int end_at = min((at + 1) * a.part, a.vocab);
+  for (int p0 = at * a.part; p0 < end_at; p0 += NT * PER) {
+    const int i0 = p0 + PER * tid, n_here = min(max(end_at - i0, 0), PER);
+    float x[PER];
+    uint64_t w[PER], sum = 0, ties = 0, sum_before, ties_before, sum_all, ties_all;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) x[i] = i < n_here ? L::at(base, i0 + i) : NAN;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const uint32_t key = order_of(x[i]);
+      w[i] = d.weight(x[i]);
+      if (key > cut.key) sum += d.kept(w[i]);
+      ties += i < n_here && key == cut.key;
+    }
+    d.scan(sum, ties, sum_before, ties_before, sum_all, ties_all);
+    const uint64_t first = cum + sum_before + D::ties_in(cut, upto, ties_before) * tie_w;
+    if (first <= r && first + sum + D::ties_in(cut, upto + ties_before, ties) * tie_w > r)
+      d.pick(cut, tie_w, first, upto + ties_before, r, total, i0, n_here, [&](int i, uint64_t& wi) __attribute__((always_inline)) {
+        float y = x[0];
+        wi = w[0];
+#pragma unroll
+        for (int e = 1; e < PER; ++e) y = i == e ? x[e] : y, wi = i == e ? w[e] : wi;
+        return y;
+      });
+    cum += sum_all + D::ties_in(cut, upto, ties_all) * tie_w;
+    upto += ties_all;
+    if (cum > r) break;
   }
-  d.scan(sum, ties, sum_before, ties_before, sum_all, ties_all);
-  cum += sum_before + D::ties_in(cut, upto, ties_before) * tie_w;
-  upto += ties_before;
-  if (cum <= r && cum + sum + D::ties_in(cut, upto, ties) * tie_w > r)
-    d.pick(cut, tie_w, cum, upto, r, total, p0 + i0, i1 - i0,
-           [&](int i, uint64_t& w) __attribute__((always_inline)) {
-             const float x = L::at(base, p0 + i0 + i);
-             w = d.weight(x);
-             return x;
-           });
 }
 
 // tokens a part of a row of `vocab`, of `rows`: SM_PART, more where that gives more than SM_PARTS parts, or more workgroups
 // than keep the chip busy (a part costs 4 KB of bins)
 int part_of(int64_t rows, int64_t vocab) {
   int64_t part = SM_PART;
-  while (part * SM_PARTS < vocab || (part < 4 * SM_PART && rows * (vocab / part) > 2048)) part *= 2;
+  while (part * SM_PARTS < vocab || (part < 2 * SM_PART && rows * (vocab / part) > 4096)) part *= 2;
   return (int)part;
 }
 bool row_is_held(int64_t vocab) { return vocab <= 1024 * SM_HELD; }
