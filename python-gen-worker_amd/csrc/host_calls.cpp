@@ -50,6 +50,7 @@ struct Abi {
   decltype(&gwa_paged_evict) paged_evict;
   decltype(&gwa_paged_write_fp8) paged_write_fp8;
   decltype(&gwa_paged_read_fp8) paged_read_fp8;
+  decltype(&gwa_paged_attention_fp8_workspace) paged_attention_fp8_workspace;
   decltype(&gwa_paged_attention_fp8) paged_attention_fp8;
   decltype(&gwa_sample_tokens_workspace) sample_tokens_workspace;
   decltype(&gwa_sample_tokens) sample_tokens;
@@ -624,8 +625,9 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       const bool gather = rest[3].defined();
       o = empty_like_device({n, h, c.head_dim}, q.scalar_type(), q);
       lse = empty_like_device({n, h}, at::kFloat, q);
-      const int64_t bytes = g_abi.paged_attention_workspace(c.batch, n, h, c.kv_heads, c.head_dim, max_q, max_kv,
-                                                            c.table_width * c.page_size, gather);
+      const auto bytes_of = E8 ? g_abi.paged_attention_fp8_workspace : g_abi.paged_attention_workspace;
+      const int64_t bytes = bytes_of(c.batch, n, h, c.kv_heads, c.head_dim, max_q, max_kv, c.table_width * c.page_size,
+                                     gather);
       Tensor ws;
       if (bytes > 0) ws = empty_like_device({bytes}, at::kByte, q);
       auto call = [&](auto f, auto... cache) {
@@ -865,6 +867,7 @@ PyObject* host_bind(PyObject*, PyObject* args) {
   GWA_BIND(paged_evict);
   GWA_BIND(paged_write_fp8);
   GWA_BIND(paged_read_fp8);
+  GWA_BIND(paged_attention_fp8_workspace);
   GWA_BIND(paged_attention_fp8);
   GWA_BIND(sample_tokens_workspace);
   GWA_BIND(sample_tokens);

@@ -705,10 +705,11 @@ struct FewRaw {
   uint32_t ks[2], vs[kV];
 };
 
-template <class T, int D, int RB, bool SHARES, bool E8>
-__global__ __launch_bounds__(64 * FW_WAVES) void paged_attn_few_kernel(AttnArgs a) {
+template <class T, int D, int RB, bool SHARES, bool E8, int NW = FW_WAVES>
+__global__ __launch_bounds__(64 * NW, E8 ? 2 : 1) void paged_attn_few_kernel(AttnArgs a) {
   using S = FewShape<D, RB, E8>;
-  constexpr int NW = FW_WAVES, BM = 16 * RB;
+  constexpr int BM = 16 * RB;
+  static_assert(!SHARES || NW == FW_WAVES);
   __shared__ __attribute__((aligned(1024))) uint8_t lds[NW * S::kWave];
   __shared__ float stat[NW][2][BM];  // m and l by wave
   __shared__ int page_ids[FW_PAGES];
@@ -901,27 +902,41 @@ __global__ __launch_bounds__(64 * FW_WAVES) void paged_attn_few_kernel(AttnArgs 
             for (int db = 0; db < S::kND; ++db) oacc[rb][db] *= alpha;
           }
         }
+        if constexpr (E8) {  // all reads ahead of the products: one at a time each waits for its own
+          v4i vop[S::kND];
 #pragma unroll
-        for (int db = 0; db < S::kND; ++db) {
-          const v4s_ lo = lds_read_tr(kb + vro[db]), hi = lds_read_tr(kb + vro[db] + 16 * S::kRow);
-          const v4i vop = two_halves(lo, hi);
+          for (int db = 0; db < S::kND; ++db) vop[db] = two_halves(lds_read_tr(kb + vro[db]), lds_read_tr(kb + vro[db] + 16 * S::kRow));
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int rb = 0; rb < RB; ++rb) oacc[rb][db] = Mfma<T>::tall(vop, pop[rb], oacc[rb][db]);
+          for (int db = 0; db < S::kND; ++db)
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) oacc[rb][db] = Mfma<T>::tall(vop[db], pop[rb], oacc[rb][db]);
+        } else {
+#pragma unroll
+          for (int db = 0; db < S::kND; ++db) {
+            const v4s_ lo = lds_read_tr(kb + vro[db]), hi = lds_read_tr(kb + vro[db] + 16 * S::kRow);
+            const v4i vop = two_halves(lo, hi);
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) oacc[rb][db] = Mfma<T>::tall(vop, pop[rb], oacc[rb][db]);
+          }
         }
       };
       if constexpr (E8) {
-        // tiles wave, wave + NW, ...: two in flight, in registers of their own
+        // tiles wave, wave + NW, ...: two in flight, in registers of their own. The loads go out whether or not there is such
+        // a tile (past the end they repeat the last key), so that how many are outstanding is known wherever one is waited
+        // for: with conditions around them every wait is for all
         FewRaw<D> w0, w1;
         auto tile = [&](int t, FewRaw<D>& w) __attribute__((always_inline)) {
           if (whole(t)) step(t, w, std::false_type{});
           else step(t, w, std::true_type{});
-          if (t + 2 * NW < ntiles) load(t + 2 * NW, w);
+          load(t + 2 * NW, w);
         };
-        if (wave < ntiles) load(wave, w0);
-        if (wave + NW < ntiles) load(wave + NW, w1);
+        load(wave, w0);
+        load(wave + NW, w1);
         for (int t = wave; t < ntiles; t += 2 * NW) {
           tile(t, w0);
-          if (t + NW < ntiles) tile(t + NW, w1);
+          if (t + NW >= ntiles) break;
+          tile(t + NW, w1);
         }
       } else {
         // tiles wave, wave + NW, ...: the next one's copies go out before this one's are waited for
@@ -1276,12 +1291,14 @@ constexpr int64_t kScoreBytes = 256ll << 20;  // most workspace spent on kept sc
 
 struct Plan {
   bool matrix, few, keep_scores;
+  bool wide;          // few rows: a workgroup of 8 waves
   int64_t tile_rows;  // rows a workgroup: 16 or 32 (few), 128 or 256
   int splits, split_keys, shares, tiles;
   int row_splits, key_tiles;  // of the recomputing gather
   int64_t score_stride, gathered, part_floats, bytes;
 };
 
+template <bool E8>
 Plan plan_of(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t d, int64_t max_q, int64_t max_kv,
              int64_t capacity, bool gather) {
   Plan p = {};
@@ -1295,7 +1312,9 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int
   p.tile_rows = p.few ? (rows <= 16 ? 16 : 32) : rows <= 128 ? 128 : 256;
   if (p.few) p.keep_scores = gather && tokens * heads * ((capacity + 3) / 4 * 4) * 4 <= kScoreBytes;
   // few splits only: their join reads them in turn (72 of 2 sequences of 18361 keys: 39 us in all, as shares 19)
-  if (p.few && groups * ((max_kv + 255) / 256) <= kCus && max_kv <= 8 * 256) {
+  if (E8 && p.few && p.tile_rows == 16 && max_kv <= 1024 && groups <= kCus) {
+    p.wide = true;
+  } else if (p.few && groups * ((max_kv + 255) / 256) <= kCus && max_kv <= 8 * 256) {
     p.split_keys = 256;
     p.splits = (int)((max_kv + 255) / 256);
     if (p.splits > 1) p.part_floats = p.splits * tokens * heads * (d + 1);
@@ -1304,7 +1323,7 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int
     // heads over 2, cut into 64 parts a tile take 26 us, into 32 23, into 8 32; the join reads every part
     const int64_t tt = p.tile_rows / group, tiles = ((max_q < 1 ? 1 : max_q) + tt - 1) / tt;
     const int64_t row_tiles = kv_heads * std::min(batch * tiles, tokens / tt + batch), units = (max_kv + 63) / 64;
-    p.shares = p.tile_rows == 128 ? 2 * kCus : kCus;
+    p.shares = p.tile_rows == 128 || (E8 && p.tile_rows == 16) ? 2 * kCus : kCus;
     // Many rows: a workgroup a row tile where that takes no longer. 64 keys take it about 2 us, and it goes through
     // whole rounds of workgroups; shares always end together, but take 8 us to find and to join and 6 % more for
     // their cut tiles (4096 tokens over 16500 keys, 32 heads over 8, 512 tiles: 894 us against 965; 150 tokens over 152
@@ -1339,7 +1358,8 @@ void launch_matrix(const Plan& p, AttnArgs a, int64_t max_kv, bool gather, hipSt
   const unsigned groups = (unsigned)(a.c.batch * a.c.kv_heads);
   if (p.few && p.shares == 0) {
     const dim3 grid(groups * (unsigned)p.splits), block(64 * FW_WAVES);
-    if (p.tile_rows == 16) hipLaunchKernelGGL((paged_attn_few_kernel<T, D, 1, false, E8>), grid, block, 0, st, a);
+    if (E8 && p.wide) hipLaunchKernelGGL((paged_attn_few_kernel<T, D, 1, false, E8, E8 ? 8 : FW_WAVES>), grid, dim3(512), 0, st, a);
+    else if (p.tile_rows == 16) hipLaunchKernelGGL((paged_attn_few_kernel<T, D, 1, false, E8>), grid, block, 0, st, a);
     else hipLaunchKernelGGL((paged_attn_few_kernel<T, D, 2, false, E8>), grid, block, 0, st, a);
     if (p.splits > 1)
       hipLaunchKernelGGL((paged_attn_join_kernel<T, D>), dim3((unsigned)(((int64_t)a.tokens * a.heads * D + 1023) / 1024)),
@@ -1384,7 +1404,14 @@ void launch_matrix(const Plan& p, AttnArgs a, int64_t max_kv, bool gather, hipSt
   }
 }
 
-// The entry points' body; `scales`: of an 8-bit cache
+// The entry points' bodies; `scales`: of an 8-bit cache
+template <bool E8>
+int64_t workspace_of(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_q,
+                     int64_t max_kv, int64_t capacity, int gather) {
+  if (batch < 0 || tokens < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || max_q < 0 || max_kv < 0) return 0;
+  return plan_of<E8>(batch, tokens, heads, kv_heads, head_dim, max_q, max_kv, capacity, gather != 0).bytes;
+}
+
 template <bool E8>
 int attention_call(const char* what, const gwa_paged_cache* cache, const gwa_paged_scales* scales, const void* q,
                    int64_t ldqt, int64_t ldqh, void* o, float* lse, int64_t tokens, int64_t heads, int64_t max_q,
@@ -1412,7 +1439,7 @@ int attention_call(const char* what, const gwa_paged_cache* cache, const gwa_pag
               "%s: q and o must be 16-byte aligned", what);
   hipStream_t st = (hipStream_t)stream;
   const float c_log2 = scale * kLog2e;
-  const Plan p = plan_of(c.batch, tokens, heads, c.kv_heads, d, max_q, max_kv, c.capacity, gather != 0);
+  const Plan p = plan_of<E8>(c.batch, tokens, heads, c.kv_heads, d, max_q, max_kv, c.capacity, gather != 0);
   if (p.matrix && c.batch > 0) {
     GWA_REQUIRE(rows * p.splits < (1ll << 31) && groups * (p.key_tiles + 1) * (p.row_splits + 1) < (1ll << 31),
                 "%s: %lld rows over %lld sequences' heads are too many", what, (long long)rows, (long long)groups);

@@ -4,8 +4,7 @@
 extern "C" int64_t gwa_paged_attention_workspace(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
                                                  int64_t head_dim, int64_t max_q, int64_t max_kv, int64_t capacity,
                                                  int gather) {
-  if (batch < 0 || tokens < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || max_q < 0 || max_kv < 0) return 0;
-  return plan_of(batch, tokens, heads, kv_heads, head_dim, max_q, max_kv, capacity, gather != 0).bytes;
+  return workspace_of<false>(batch, tokens, heads, kv_heads, head_dim, max_q, max_kv, capacity, gather);
 }
 
 extern "C" int gwa_paged_attention(const gwa_paged_cache* cache, const void* q, int64_t ldqt, int64_t ldqh, void* o,

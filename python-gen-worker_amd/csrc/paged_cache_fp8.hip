@@ -19,16 +19,9 @@ __device__ __forceinline__ RowScale row_scale(uint32_t amax) {
   const int b = max((int)(amax >> 23) - 8 + ((amax & 0x7fffffu) > 0x600000u), 1);
   return {(uint32_t)b, __uint_as_float((uint32_t)(254 - b) << 23), b >= kTop ? 240.0f : 448.0f};
 }
-// fp32 bits of |x|, 0 for what is not finite
-__device__ __forceinline__ uint32_t finite_bits(float x) {
-  const uint32_t u = __float_as_uint(x) & 0x7fffffffu;
-  return u < 0x7f800000u ? u : 0;
-}
-// x scaled, for the conversion (which rounds to nearest, ties to even, and takes NaN to NaN)
-__device__ __forceinline__ float scaled(float x, const RowScale& s) {
-  const float y = fminf(fmaxf(x * s.inverse, -s.most), s.most);
-  return fabsf(x) < INFINITY ? y : NAN;
-}
+// x under its row's scale, for the conversion, which rounds to nearest (ties to even) and takes infinities and NaN to NaN.
+// No finite value of the row passes 448.
+__device__ __forceinline__ float scaled(float x, const RowScale& s) { return x * s.inverse; }
 __device__ __forceinline__ uint2 codes8(const float (&x)[8], const RowScale& s) {
   uint32_t w[2];
 #pragma unroll
@@ -38,10 +31,35 @@ __device__ __forceinline__ uint2 codes8(const float (&x)[8], const RowScale& s) 
   }
   return make_uint2(w[0], w[1]);
 }
+// x, if finite, held to the largest code of a row whose codes end below 448
+__device__ __forceinline__ float held_to(float x, const RowScale& s) {
+  const float top = s.most / s.inverse;
+  return fabsf(x) < INFINITY ? fminf(fmaxf(x, -top), top) : x;
+}
+// the larger of `most` and |x|, NaN and (with FINITE) infinities left out
+template <bool FINITE>
+__device__ __forceinline__ float larger(float most, float x) {
+  return FINITE && fabsf(x) == INFINITY ? most : fmaxf(most, fabsf(x));
+}
+
+// x's maximum over groups of n neighbouring lanes, n a power of two up to 64
+__device__ __forceinline__ float group_max(float x, int n) {
+  auto moved = [](float v, auto move_c) __attribute__((always_inline)) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), decltype(move_c)::value, 0xf, 0xf, true));
+  };
+  if (n > 1) x = fmaxf(x, moved(x, std::integral_constant<int, 0xb1>{}));   // the neighbour's, within four
+  if (n > 2) x = fmaxf(x, moved(x, std::integral_constant<int, 0x4e>{}));   // the other pair's
+  if (n > 4) x = fmaxf(x, moved(x, std::integral_constant<int, 0x141>{}));  // eight lanes mirrored
+  if (n > 8) x = fmaxf(x, moved(x, std::integral_constant<int, 0x140>{}));  // sixteen
+  if (n > 16) x = fmaxf(x, __shfl_xor(x, 16)), x = fmaxf(x, __shfl_xor(x, 32));
+  return x;
+}
 
 // One workgroup a token: its query heads into q_out, its key and value heads into the slot, each row by a group of lanes
 // (`lanes`, a power of two: the units of 16 channels of a row, or with odd sizes and places a wave, a lane two pairs at
-// most), which find the row's largest value between them; a row is read once and held in registers meanwhile.
+// most), which find the row's largest value between them; a row is read once and held in registers meanwhile. The first
+// rows' loads go out before the three dependent ones that find the slot. Every XCD has a run of neighbouring tokens, whose
+// codes and scale bytes share lines in its L2.
 template <int DT, bool VEC>
 __global__ __launch_bounds__(W8_THREADS) void paged_write_fp8_kernel(PagedArgs c, const uint16_t* q, int64_t ldqt,
                                                                      int64_t ldqh, const uint16_t* k, int64_t ldkt,
@@ -49,38 +67,62 @@ __global__ __launch_bounds__(W8_THREADS) void paged_write_fp8_kernel(PagedArgs c
                                                                      int64_t ldvh, uint16_t* q_out, Rotation r, int tokens,
                                                                      int heads, int head_dim, int lanes) {
   constexpr int N = VEC ? 8 : 1, kHeld = VEC ? 1 : 2;
-  const int t = blockIdx.x;
-  const TokenPlace place = token_place(c, t, tokens);
+  const int t = blockIdx.x % kXcds * (gridDim.x / kXcds) + blockIdx.x / kXcds;
+  if (t >= tokens) return;
   const int64_t row = r.rot ? table_row(r, t) : 0;
   const Rotation none = {nullptr, nullptr, nullptr, 0, 0, 0, 1.0f};
-  const int hk = c.kv_heads, rows = heads + (place.slot >= 0 ? 2 * hk : 0), units = head_dim / (2 * N);
+  const int hk = c.kv_heads, rows = heads + 2 * hk, units = head_dim / (2 * N);
   const int u0 = threadIdx.x & (lanes - 1), step = W8_THREADS / lanes;
-  for (int h = threadIdx.x / lanes; h < rows; h += step) {
-    const bool is_k = h >= heads && h < heads + hk;
+  TokenPlace place = {0, -1};
+  for (int h0 = 0; h0 < rows; h0 += step) {
+    const int h = h0 + threadIdx.x / lanes;
+    const bool is_q = h < heads, is_k = !is_q && h < heads + hk, is_v = !is_q && !is_k && h < rows;
     const int kh = is_k ? h - heads : h - heads - hk;
-    if (h < heads) {
-      for (int u = u0; u < units; u += lanes)
-        rotate_unit<DT, VEC>(q, t * ldqt + h * ldqh, q_out, ((int64_t)t * heads + h) * head_dim, r, row, u);
-      continue;
-    }
     float a[kHeld][N], b[kHeld][N];
     int c0[kHeld], c1[kHeld];
-    uint32_t amax = 0;
+    auto each = [&](auto f) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-      const int u = u0 + i * lanes;
-      if (u >= units) continue;
-      rotated_unit<DT, VEC>(is_k ? k : v, is_k ? t * ldkt + kh * ldkh : t * ldvt + kh * ldvh, is_k ? r : none,
-                            is_k ? row : 0, u, c0[i], c1[i], a[i], b[i]);
-#pragma unroll
-      for (int e = 0; e < N; ++e) amax = max(amax, max(finite_bits(a[i][e]), finite_bits(b[i][e])));
+      for (int i = 0; i < kHeld; ++i)
+        if (u0 + i * lanes < units && h < rows) f(i);
+    };
+    const uint16_t* from = is_q ? q + t * ldqt + h * ldqh : is_k ? k + t * ldkt + kh * ldkh : v + t * ldvt + kh * ldvh;
+    each([&](int i) __attribute__((always_inline)) {
+      rotated_unit<DT, VEC>(from, 0, is_v ? none : r, is_v ? 0 : row, u0 + i * lanes, c0[i], c1[i], a[i], b[i]);
+    });
+    if (h0 == 0) place = token_place(c, t, tokens);
+    if (is_q) {
+      uint16_t* out = q_out + ((int64_t)t * heads + h) * head_dim;
+      each([&](int i) __attribute__((always_inline)) {
+        if constexpr (VEC) {
+          store8<DT>(out, c0[i], a[i]);
+          store8<DT>(out, c1[i], b[i]);
+        } else {
+          store1<DT>(out, c0[i], a[i][0]);
+          store1<DT>(out, c1[i], b[i][0]);
+        }
+      });
     }
-    for (int w = lanes / 2; w; w >>= 1) amax = max(amax, (uint32_t)__shfl_xor((int)amax, w));
-    const RowScale s = row_scale<DT>(amax);
-    uint8_t* out = (uint8_t*)(is_k ? c.k : c.v) + paged_at(c, place.page, kh, place.slot);
+    auto row_max = [&](auto finite_c) __attribute__((always_inline)) {
+      float most = 0.0f;
+      each([&](int i) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-      if (u0 + i * lanes >= units) continue;
+        for (int e = 0; e < N; ++e)
+          most = larger<decltype(finite_c)::value>(larger<decltype(finite_c)::value>(most, a[i][e]), b[i][e]);
+      });
+      return group_max(most, lanes);
+    };
+    float most = row_max(std::false_type{});
+    // (all lanes take part in both; what is not a row's has 0)
+    if (__ballot(most == INFINITY)) most = row_max(std::true_type{});
+    if (place.slot < 0 || !(is_k || is_v)) continue;
+    const RowScale s = row_scale<DT>(__float_as_uint(most));
+    if (s.most < 448.0f)  // a row at the top of the type's range
+      each([&](int i) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) a[i][e] = held_to(a[i][e], s), b[i][e] = held_to(b[i][e], s);
+      });
+    uint8_t* out = (uint8_t*)(is_k ? c.k : c.v) + paged_at(c, place.page, kh, place.slot);
+    each([&](int i) __attribute__((always_inline)) {
       if constexpr (VEC) {
         *(uint2*)(out + c0[i]) = codes8(a[i], s);
         *(uint2*)(out + c1[i]) = codes8(b[i], s);
@@ -89,7 +131,7 @@ __global__ __launch_bounds__(W8_THREADS) void paged_write_fp8_kernel(PagedArgs c
         out[c0[i]] = (uint8_t)pair;
         out[c1[i]] = (uint8_t)(pair >> 8);
       }
-    }
+    });
     if (u0 == 0) {
       (is_k ? c.ks : c.vs)[paged_s_at(c, place.page, kh, place.slot)] = (uint8_t)s.byte;
       if (is_k && c.w) c.w[paged_w_at(c, place.page, kh, place.slot)] = 0.0f;
@@ -159,7 +201,7 @@ extern "C" int gwa_paged_write_fp8(const gwa_paged_cache* cache, const gwa_paged
   if (vec)
     for (lanes = 1; lanes < d / 16; lanes *= 2) {}
 #define GWA_WRITE8(DT, VEC)                                                                                        \
-  hipLaunchKernelGGL((paged_write_fp8_kernel<DT, VEC>), dim3((unsigned)tokens), dim3(W8_THREADS), 0,               \
+  hipLaunchKernelGGL((paged_write_fp8_kernel<DT, VEC>), dim3((unsigned)((tokens + kXcds - 1) / kXcds * kXcds)), dim3(W8_THREADS), 0, \
                      (hipStream_t)stream, c, (const uint16_t*)q, ldqt, ldqh, (const uint16_t*)k, ldkt, ldkh,       \
                      (const uint16_t*)v, ldvt, ldvh, (uint16_t*)q_out, r, (int)tokens, (int)heads, (int)d, lanes)
   if (cache->dtype == GWA_DT_BF16) { if (vec) GWA_WRITE8(GWA_DT_BF16, true); else GWA_WRITE8(GWA_DT_BF16, false); }

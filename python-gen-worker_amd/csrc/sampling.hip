@@ -9,7 +9,7 @@ constexpr int SM_BINS = 384, SM_DIGITS = 2048, SM_LIST = 512, SM_FOUND = 8192;
 constexpr int SM_HELD = 8;            // logits a thread holds where a row fits a workgroup's registers
 constexpr int SM_PART = 4096, SM_PARTS = 64;  // tokens a part of a longer row at least; parts of a row at most
 constexpr int SM_AHEAD = 4;           // 16-byte loads a lane has in flight
-constexpr int SM_FEW = 128;           // collected tokens that are ranked all against all
+constexpr int SM_FEW = 256;           // collected tokens that are ranked all against all
 constexpr int kTableBits = 9;         // of the table of 2^(j / 512)
 
 struct SampleArgs {
@@ -658,7 +658,9 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
   __shared__ float found_x[SM_FOUND];
   __shared__ int found_i[SM_FOUND];
   __shared__ int found_n[NW];
-  __shared__ ulonglong2 few[SM_FEW];
+  __shared__ ulonglong2 few[SM_FEW];  // weight, and order
+  __shared__ uint64_t few_sum[2][SM_FEW];
+  __shared__ uint32_t few_rank[SM_FEW], few_equal[SM_FEW];
   __shared__ float few_x[SM_FEW];
   __shared__ int few_i[SM_FEW];
   __shared__ uint64_t part_w[SM_PARTS];
@@ -796,26 +798,37 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
   const bool cuts = s.way == kCount || p.bin <= to;  // whether what is collected is cut by its order
   const bool few_found = !whole && cuts && n <= SM_FEW;
   if (few_found) {
-    // each against all. `order`: larger for what comes first (equal logits: the lowest index)
+    // each against all, by four threads a token. `order`: larger for what comes first (equal logits: the lowest index)
+    constexpr int SHARE = NT / SM_FEW;
+    const int j = tid & (SM_FEW - 1), i0 = tid / SM_FEW;
     const bool mine = tid < n;
-    uint64_t w = 0, order = 0, ahead = ahead_of;
-    uint32_t rank = 0, equal = 0;
     for (int i = lane; i < mine_n; i += 64) few_x[my_first + i] = my_x[i], few_i[my_first + i] = my_i[i];
+    if (tid < SM_FEW) few_sum[0][tid] = few_sum[1][tid] = 0, few_rank[tid] = few_equal[tid] = 0;
     __syncthreads();
+    uint64_t w = 0, order = 0;
     if (mine) {
       w = d.weight(few_x[tid]);
       order = (uint64_t)order_of(few_x[tid]) << 32 | (uint32_t)~few_i[tid];
       few[tid] = make_ulonglong2(w, order);
     }
     __syncthreads();
-    if (mine) {
+    if (j < n) {
+      const uint64_t my_order = few[j].y;
+      uint64_t ahead = 0;
+      uint32_t rank = 0, equal = 0;
 #pragma unroll 4
-      for (int i = 0; i < n; ++i) {
+      for (int i = i0; i < n; i += SHARE) {
         const ulonglong2 o = few[i];
-        const bool first = o.y > order;
-        rank += first, ahead += first ? o.x : 0, equal += first && (o.y ^ order) >> 32 == 0;
+        const bool first = o.y > my_order;
+        rank += first, ahead += first ? o.x : 0, equal += first && (o.y ^ my_order) >> 32 == 0;
       }
+      atomicAdd(&few_rank[j], rank);
+      atomicAdd(&few_equal[j], equal);
+      atomicAdd((unsigned long long*)&few_sum[0][j], (unsigned long long)ahead);
     }
+    __syncthreads();
+    const uint32_t rank = mine ? few_rank[tid] : 0, equal = mine ? few_equal[tid] : 0;
+    const uint64_t ahead = ahead_of + (mine ? few_sum[0][tid] : 0);
     if (s.way == kCount) {
       const bool among = mine && rank < (uint32_t)s.top_k;
       if (tid < SM_FEW) {
@@ -823,19 +836,33 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
         if (lane == 0) l.cells[0][wave] = sum;
       }
       __syncthreads();
+      uint64_t all = 0;
+#pragma unroll
+      for (int i = 0; i < SM_FEW / 64; ++i) all += l.cells[0][i];
       // of the run that reaches top_p of the sum, what lies ahead of a token does not
-      const bool stays = among && (s.top_p >= 1.0f || (double)ahead < d.target_of(l.cells[0][0] + l.cells[0][1])) &&
-                         (double)w >= d.low;
+      const bool stays = among && (s.top_p >= 1.0f || (double)ahead < d.target_of(all)) && (double)w >= d.low;
       if (mine) few[tid].x = stays ? w : 0;
+      if (tid < SM_FEW) {
+        const uint64_t sum = wave_sum64(stays ? w : 0);
+        if (lane == 0) l.cells[1][wave] = sum;
+      }
+      __syncthreads();
+      if (j < n && few[j].x) {
+        const uint32_t my_place = (uint32_t)few[j].y;  // larger for lower indices
+        uint64_t cum = 0;
+#pragma unroll 4
+        for (int i = i0; i < n; i += SHARE) {
+          const ulonglong2 o = few[i];
+          cum += (uint32_t)o.y > my_place ? o.x : 0;
+        }
+        atomicAdd((unsigned long long*)&few_sum[1][j], (unsigned long long)cum);
+      }
       __syncthreads();
       if (stays) {
-        uint64_t total = 0, cum = 0;
-#pragma unroll 4
-        for (int i = 0; i < n; ++i) {
-          const ulonglong2 o = few[i];
-          total += o.x, cum += (uint32_t)o.y > (uint32_t)order ? o.x : 0;
-        }
-        const uint64_t r = d.drawn(total);
+        uint64_t total = 0;
+#pragma unroll
+        for (int i = 0; i < SM_FEW / 64; ++i) total += l.cells[1][i];
+        const uint64_t r = d.drawn(total), cum = few_sum[1][tid];
         if (cum <= r && cum + w > r) d.draw(few_i[tid], few_x[tid], total);
       }
       return;

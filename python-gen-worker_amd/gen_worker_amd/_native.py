@@ -134,6 +134,7 @@ _SIGNATURES: dict[str, tuple] = {
     "gwa_paged_write_fp8": (_cache, _scales, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp,
                             _i64, _i64, _i64, _int, _vp),
     "gwa_paged_read_fp8": (_cache, _scales, _vp, _vp, _i64, _vp),
+    "gwa_paged_attention_fp8_workspace": (_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int),
     "gwa_paged_attention_fp8": (_cache, _scales, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _flt, _int, _int,
                                 _vp, _i64, _vp),
     "gwa_paged_evict_fp8": (_cache, _scales, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp),
@@ -146,7 +147,8 @@ _RESTYPES = {"gwa_build_info": ctypes.c_char_p, "gwa_last_error": ctypes.c_char_
              "gwa_svdq_w4a4_linear_fp6_noalloc_scratch_bytes": ctypes.c_int64,
              "gwa_svdq_quant_fp6_la_workspace": ctypes.c_int64,
              "gwa_svdq_w4a4_linear_gemv_workspace": ctypes.c_int64,
-             "gwa_paged_attention_workspace": ctypes.c_int64, "gwa_sample_tokens_workspace": ctypes.c_int64}
+             "gwa_paged_attention_workspace": ctypes.c_int64,
+             "gwa_paged_attention_fp8_workspace": ctypes.c_int64, "gwa_sample_tokens_workspace": ctypes.c_int64}
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 

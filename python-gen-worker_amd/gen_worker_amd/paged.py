@@ -373,8 +373,8 @@ def _attention_body(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, 
     lse = torch.empty((t, h), dtype=torch.float32, device=q.device)
     lib = nat.load()
     gather = int(weights is not None)
-    n = int(lib.gwa_paged_attention_workspace(args.batch, t, h, hk, d, max_q, max_kv,
-                                              args.table_width * args.page_size, gather))
+    bytes_of = lib.gwa_paged_attention_workspace if scales is None else lib.gwa_paged_attention_fp8_workspace
+    n = int(bytes_of(args.batch, t, h, hk, d, max_q, max_kv, args.table_width * args.page_size, gather))
     ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
     rest = (q.data_ptr(), q.stride(0), q.stride(1), o.data_ptr(), lse.data_ptr(), t, h, max_q, max_kv, scale,
             int(causal), gather, nat.ptr(ws), n, nat.stream_of(q))
