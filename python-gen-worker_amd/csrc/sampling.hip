@@ -762,11 +762,12 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
       // the first lane takes part whenever any of its wave does, so its count is the wave's
       int at = __builtin_amdgcn_readfirstlane(mine_n);
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const int to = at + below(hits[e]);
-        if ((hits[e] >> lane & 1) && to < SEG) my_x[to] = x[e], my_i[to] = i + e;
-        at += __popcll(hits[e]);
-      }
+      for (int e = 0; e < N; ++e)
+        if (hits[e]) {  // the same for the wave
+          const int to = at + below(hits[e]);
+          if (__builtin_amdgcn_fmed3f(x[e], lo, hi) == x[e] && to < SEG) my_x[to] = x[e], my_i[to] = i + e;
+          at += __popcll(hits[e]);
+        }
       mine_n = at;
     };
     each_vector<DT>(base, 0, a.vocab, tid, NT, take);
