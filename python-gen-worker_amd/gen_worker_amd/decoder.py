@@ -1,11 +1,12 @@
 """A small decoder on the quantized linears and the paged cache: how the pieces of ``paged`` run together.
 
-Random weights, pre-norm blocks (RMSNorm, rotary attention whose query heads share key/value heads, GELU MLP), greedy
-answers. Every linear comes from ``flux_dit.linear_factory``, so the same model runs W4A4 or bf16. Prompts of any
+Random weights, pre-norm blocks (RMSNorm, rotary attention whose query heads share key/value heads, GELU MLP), answers
+greedy or drawn (``sampling``). Every linear comes from ``flux_dit.linear_factory``, so the same model runs W4A4 or bf16. Prompts of any
 lengths go in together, in chunks; then every step takes one token of each sequence. With a ``budget`` each layer's keys
-are cut back to the most attended whenever a sequence has outgrown it by a page:
+are cut back to the most attended whenever a sequence has outgrown it by a page; the caches hold bf16 or 8 bits:
 
     python -m gen_worker_amd.decoder --kind w4a4 --prompts 300,17,120 --tokens 64 --budget 128
+    python -m gen_worker_amd.decoder --cache fp8 --temperature 0.8 --top-p 0.95 --seed 3
 """
 
 from __future__ import annotations
@@ -19,7 +20,8 @@ import torch
 from torch import Tensor, nn
 
 from .flux_dit import _rms, linear_factory
-from .paged import PagedBatch, PagedCache, PagedError, rotary_table
+from .paged import FP8, PagedBatch, PagedCache, PagedError, rotary_table
+from .sampling import sample_tokens, settings
 
 
 @dataclass
@@ -80,10 +82,11 @@ class PagedDecoder(nn.Module):
         self.register_buffer("cos", cos)
         self.register_buffer("sin", sin)
 
-    def caches(self, pages: int, page_size: int = 16, weights: bool = False) -> list[PagedCache]:
+    def caches(self, pages: int, page_size: int = 16, weights: bool = False,
+               dtype: torch.dtype = torch.bfloat16) -> list[PagedCache]:
         """A pool for each layer under one bookkeeping (the first's)."""
-        first = PagedCache(pages, page_size, self.cfg.kv_heads, self.cfg.head_dim, device=self.embed.device,
-                           weights=weights)
+        first = PagedCache(pages, page_size, self.cfg.kv_heads, self.cfg.head_dim, dtype=dtype,
+                           device=self.embed.device, weights=weights)
         return [first] + [first.twin() for _ in range(self.cfg.layers - 1)]
 
     @torch.no_grad()
@@ -98,19 +101,31 @@ class PagedDecoder(nn.Module):
 
     @torch.no_grad()
     def generate(self, prompts: Sequence[Sequence[int]], new_tokens: int, *, budget: Optional[int] = None,
-                 recent: int = 16, chunk: int = 512, page_size: int = 16) -> list[list[int]]:
-        """Greedy answers of ``new_tokens`` tokens to each prompt, all in one batch. ``budget``: keys a layer keeps of a
-        sequence, the last ``recent`` among them."""
+                 recent: int = 16, chunk: int = 512, page_size: int = 16, dtype: torch.dtype = torch.bfloat16,
+                 temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0,
+                 seed: int = 0) -> list[list[int]]:
+        """Answers of ``new_tokens`` tokens to each prompt, all in one batch: greedy, or with a ``temperature`` drawn
+        (``sample_tokens``) by random numbers of the ``seed``. ``budget``: keys a layer keeps of a sequence, the last
+        ``recent`` among them. ``dtype``: of the caches (``torch.float8_e4m3fn``: 8 bits)."""
         if not prompts or not all(len(p) for p in prompts) or new_tokens < 1:
             raise PagedError("generate: every prompt needs a token, and the answer one")
         if max(len(p) for p in prompts) + new_tokens > self.cfg.positions:
             raise PagedError(f"generate: more than {self.cfg.positions} positions")
+        settings(temperature, top_k, top_p, min_p)   # refused before anything runs
         held = [len(p) + new_tokens for p in prompts]
         if budget is not None:
             held = [min(n, budget + page_size + max(chunk, 1)) for n in held]
         pages = sum(-(-n // page_size) + 1 for n in held) + (len(prompts) * -(-(budget or 0) // page_size))
-        caches = self.caches(pages, page_size, weights=budget is not None)
+        caches = self.caches(pages, page_size, weights=budget is not None, dtype=dtype)
         first, dev = caches[0], self.embed.device
+        numbers = torch.Generator(device=dev).manual_seed(seed)
+
+        def next_tokens(logits: Tensor) -> Tensor:
+            if temperature == 0.0:
+                return logits.argmax(-1)
+            uniform = torch.rand(len(logits), generator=numbers, device=dev)
+            return sample_tokens(logits, uniform, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)[0]
+
         seqs = [first.add() for _ in prompts]
         logits = torch.empty(len(prompts), self.cfg.vocab, device=dev)
         done = 0
@@ -122,10 +137,10 @@ class PagedDecoder(nn.Module):
             logits[torch.tensor(here, device=dev)] = self(packed, batch, caches)
             self._cut(first, seqs, budget, recent, page_size)
             done += chunk
-        answer = [logits.argmax(-1)]
+        answer = [next_tokens(logits)]
         for _ in range(new_tokens - 1):
             batch = first.extend(seqs, [1] * len(seqs))
-            answer.append(self(answer[-1], batch, caches).argmax(-1))
+            answer.append(next_tokens(self(answer[-1], batch, caches)))
             self._cut(first, seqs, budget, recent, page_size)
         return torch.stack(answer, 1).tolist()
 
@@ -144,6 +159,12 @@ def main() -> None:
     ap.add_argument("--tokens", type=int, default=64)
     ap.add_argument("--budget", type=int, default=None, help="keys a layer keeps of a sequence")
     ap.add_argument("--layers", type=int, default=4)
+    ap.add_argument("--cache", choices=("bf16", "fp8"), default="bf16", help="what the key/value caches hold")
+    ap.add_argument("--temperature", type=float, default=0.0, help="of the drawn tokens; 0: greedy")
+    ap.add_argument("--top-k", type=int, default=0)
+    ap.add_argument("--top-p", type=float, default=1.0)
+    ap.add_argument("--min-p", type=float, default=0.0)
+    ap.add_argument("--seed", type=int, default=0, help="of the random numbers")
     a = ap.parse_args()
     model = PagedDecoder(DecoderConfig(layers=a.layers), a.kind)
     g = torch.Generator().manual_seed(1)
@@ -151,7 +172,8 @@ def main() -> None:
     for run in ("warm-up", "timed"):
         torch.cuda.synchronize()
         t = time.perf_counter()
-        answers = model.generate(prompts, a.tokens, budget=a.budget)
+        answers = model.generate(prompts, a.tokens, budget=a.budget, dtype=FP8 if a.cache == "fp8" else torch.bfloat16,
+                                 temperature=a.temperature, top_k=a.top_k, top_p=a.top_p, min_p=a.min_p, seed=a.seed)
         torch.cuda.synchronize()
         t = time.perf_counter() - t
     for p, x in zip(prompts, answers):

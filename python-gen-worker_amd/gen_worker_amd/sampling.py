@@ -82,9 +82,17 @@ def _setting(value, plain, what: str, low, high):
     """(tensor, 0) or (None, number) of a setting."""
     if isinstance(value, Tensor):
         return value, plain
-    _require(isinstance(value, (int, float)) and not isinstance(value, bool) and low <= value <= high,
+    kinds = int if isinstance(plain, int) else (int, float)
+    _require(isinstance(value, kinds) and not isinstance(value, bool) and low <= value <= high,
              f"{what} must be {low} to {high} or a tensor, got {value!r}")
     return None, type(plain)(value)
+
+
+def settings(temperature, top_k, top_p, min_p) -> tuple[tuple, tuple]:
+    """``sample_tokens``' settings, checked: (tensors, None for numbers; numbers, a default for tensors)."""
+    pairs = (_setting(temperature, 1.0, "temperature", 0.0, 3.0e38), _setting(top_k, 0, "top_k", 0, (1 << 31) - 1),
+             _setting(top_p, 1.0, "top_p", 0.0, 1.0), _setting(min_p, 0.0, "min_p", 0.0, 1.0))
+    return tuple(t for t, _ in pairs), tuple(n for _, n in pairs)
 
 
 def sample_tokens(logits: Tensor, uniform: Tensor, *, temperature: Union[float, Tensor] = 1.0,
@@ -102,16 +110,13 @@ def sample_tokens(logits: Tensor, uniform: Tensor, *, temperature: Union[float, 
     range count as the nearest in it (a NaN as 0). Settings are fp32. -inf and NaN are never drawn; a row with nothing else
     gives token -1 and logprob NaN. Weights and sums are integers in 64 bits: the result does not depend on how the work is
     split. No gradient is defined."""
-    t, all_t = _setting(temperature, 1.0, "temperature", 0.0, 3.0e38)
-    k, all_k = _setting(top_k, 0, "top_k", 0, (1 << 31) - 1)
-    p, all_p = _setting(top_p, 1.0, "top_p", 0.0, 1.0)
-    m, all_m = _setting(min_p, 0.0, "min_p", 0.0, 1.0)
-    a = (logits, uniform, t, k, p, m)
+    each, numbers = settings(temperature, top_k, top_p, min_p)
+    a = (logits, uniform, *each)
     host = paged._host()
     if host is not None:
-        out = host.sample_tokens(*a, all_t, all_k, all_p, all_m)
+        out = host.sample_tokens(*a, *numbers)
         if out is not None:
             return out
     if paged._plain(*a):
-        return _sample_body(*a, all_t, all_k, all_p, all_m)
-    return _sample_op(*a, all_t, all_k, all_p, all_m)
+        return _sample_body(*a, *numbers)
+    return _sample_op(*a, *numbers)
