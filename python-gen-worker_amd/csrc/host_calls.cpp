@@ -10,6 +10,7 @@
 // layer 20.6 -> 12.9, the quantize / GEMM operator pair at 1024 x 9216 x 3072 87.6 -> 67.1.
 #include <ATen/ATen.h>
 #include <ATen/hip/EmptyTensor.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -550,6 +551,7 @@ Tensor write_call(const Tensor* t, bool interleaved) {
       !heads_on(v, dt, dev, n, c.kv_heads, d) || !tables_fit(t[3], t[4], t[5], n, d, dev, rot, rows))
     return out;
   out = empty_like_device({n, h, d}, dt, q);
+  const c10::OptionalDeviceGuard guard(E8 ? std::optional(dev) : std::nullopt);
   auto call = [&](auto f, auto... cache) {
     return f(cache..., q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
              v.stride(0), v.stride(1), t[3].defined() ? address<float>(t[3]) : nullptr,
@@ -625,6 +627,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       const bool gather = rest[3].defined();
       o = empty_like_device({n, h, c.head_dim}, q.scalar_type(), q);
       lse = empty_like_device({n, h}, at::kFloat, q);
+      const c10::OptionalDeviceGuard guard(E8 ? std::optional(q.device()) : std::nullopt);
       const auto bytes_of = E8 ? g_abi.paged_attention_fp8_workspace : g_abi.paged_attention_workspace;
       const int64_t bytes = bytes_of(c.batch, n, h, c.kv_heads, c.head_dim, max_q, max_kv, c.table_width * c.page_size,
                                      gather);
@@ -664,6 +667,7 @@ PyObject* paged_read_fp8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     gwa_paged_cache c;
     gwa_paged_scales s;
     if (tokens >= 0 && cache_fits(t[0], t[1], Tensor(), t[4], t[5], t[6], c, dt) && scales_fit(t[0], t[2], t[3], s)) {
+      const c10::DeviceGuard guard(t[0].device());
       k = empty_like_device({tokens, c.kv_heads, c.head_dim}, dt, t[0]);
       v = empty_like_device({tokens, c.kv_heads, c.head_dim}, dt, t[0]);
       if (g_abi.paged_read_fp8(&c, &s, k.data_ptr(), v.data_ptr(), tokens, stream_of(t[0])) != GWA_OK) k = Tensor();
@@ -699,6 +703,7 @@ PyObject* sample_tokens(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                                           t[i].layout() == at::kStrided && t[i].device() == x.device() &&
                                           t[i].sizes().equals({rows}) && (rows < 2 || t[i].stride(0) == 1)));
     if (fits) {
+      const c10::DeviceGuard guard(x.device());
       const gwa_sampling s = {t[2].defined() ? address<float>(t[2]) : nullptr,
                               t[3].defined() ? address<int32_t>(t[3]) : nullptr,
                               t[4].defined() ? address<float>(t[4]) : nullptr,

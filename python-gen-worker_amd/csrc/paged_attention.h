@@ -697,19 +697,19 @@ struct FewShape {
 };
 // A lane's part of a tile of an 8-bit cache, in registers from its loads to its use: of keys i16 and 16 + i16 the D / 4 codes
 // from channel D / 4 q4 on, which are the lane's operands as they lie (the queries' chunks follow that order); of the
-// values 16 codes of every (1024 / D)th row, which go through LDS to be read across keys.
+// values 16 codes of every (1024 / D)th row, which go through LDS to be read across keys. A lane loads one scale byte and gets
+// those it needs from others.
 template <int D>
 struct FewRaw {
   static constexpr int kK = D / 64, kV = D / 32, kRows = 1024 / D;
   v4i k[2][kK], v[kV];
-  uint32_t ks[2], vs[kV];
+  uint32_t scale;  // of the key `lane`, in the upper half of its value 32 lanes below
 };
 
-template <class T, int D, int RB, bool SHARES, bool E8, int NW = FW_WAVES>
-__global__ __launch_bounds__(64 * NW, E8 ? 2 : 1) void paged_attn_few_kernel(AttnArgs a) {
+template <class T, int D, int RB, bool SHARES, bool E8>
+__global__ __launch_bounds__(64 * FW_WAVES, E8 ? 2 : 1) void paged_attn_few_kernel(AttnArgs a) {
   using S = FewShape<D, RB, E8>;
-  constexpr int BM = 16 * RB;
-  static_assert(!SHARES || NW == FW_WAVES);
+  constexpr int NW = FW_WAVES, BM = 16 * RB;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[NW * S::kWave];
   __shared__ float stat[NW][2][BM];  // m and l by wave
   __shared__ int page_ids[FW_PAGES];
@@ -797,41 +797,47 @@ __global__ __launch_bounds__(64 * NW, E8 ? 2 : 1) void paged_attn_few_kernel(Att
           copy16(st + S::kTile + u * 1024, vbase + off, vlane[u]);
         }
       };
-      // E8: the loads of a tile; rows past the last key repeat it
+      // E8: the loads of a tile, by runs of 8 rows, which lie in one page: their places are the wave's. Runs wholly past the
+      // last key repeat that key's.
       auto load = [&](int t, FewRaw<D>& w) __attribute__((always_inline)) {
-        const int k0 = s_lo + t * FW_KEYS;
-        auto row_at = [&](int key, int64_t& scale) __attribute__((always_inline)) {
-          const int page = page_ids[(key >> c.page_shift) - p0];
-          scale = page * c.s_page_stride + h * c.s_head_stride + (key & slot_mask);
-          return (uint64_t)(uint32_t)page * page_bytes + (key & slot_mask) * slot_bytes;
-        };
-        int64_t scale;
+        int64_t at[4], sat[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int key = min(s_lo + t * FW_KEYS + 8 * r, (s_hi - 1) & ~7), page = uniform(page_ids[(key >> c.page_shift) - p0]);
+          at[r] = (int64_t)((uint64_t)(uint32_t)page * page_bytes + (key & slot_mask) * slot_bytes);
+          sat[r] = page * c.s_page_stride + h * c.s_head_stride + (key & slot_mask);
+        }
+        const uint32_t k_lane = (i16 & 7) * slot_bytes + D / 4 * q4, v_lane = (lane / (D / 16) & 7) * slot_bytes + 16 * (lane % (D / 16));
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const uint8_t* p = kbase + row_at(min(k0 + 16 * x + i16, s_hi - 1), scale) + D / 4 * q4;
+          const uint8_t* p = kbase + (i16 < 8 ? at[2 * x] : at[2 * x + 1]) + k_lane;
 #pragma unroll
           for (int i = 0; i < FewRaw<D>::kK; ++i) w.k[x][i] = *(const v4i*)(p + 16 * i);
-          w.ks[x] = c.ks[scale];
         }
 #pragma unroll
-        for (int u = 0; u < FewRaw<D>::kV; ++u) {
-          const int row = FewRaw<D>::kRows * u + lane / (D / 16);
-          w.v[u] = *(const v4i*)(vbase + row_at(min(k0 + row, s_hi - 1), scale) + 16 * (lane % (D / 16)));
-          w.vs[u] = c.vs[scale];
-        }
+        for (int u = 0; u < FewRaw<D>::kV; ++u)
+          w.v[u] = *(const v4i*)(vbase + (D == 128 ? at[u] : lane < 32 ? at[2 * u] : at[2 * u + 1]) + v_lane);
+        const int run = lane >> 3 & 3;
+        w.scale = (lane < 32 ? c.ks : c.vs)[(run < 2 ? run == 0 ? sat[0] : sat[1] : run == 2 ? sat[2] : sat[3]) + (lane & 7)];
       };
       auto step = [&](int t, const FewRaw<D>& w, auto mask_c) __attribute__((always_inline)) {
         constexpr bool MASK = decltype(mask_c)::value;
         uint8_t* kb = E8 ? mine : mine + ((t / NW) & 1) * 2 * S::kTile;
         const int k0 = s_lo + t * FW_KEYS;
         v4i pop[RB];
+        float ks[2], vs[FewRaw<D>::kV];
         if constexpr (E8) {
+#pragma unroll
+          for (int u = 0; u < FewRaw<D>::kV; ++u)
+            vs[u] = scale_of((uint32_t)__shfl((int)w.scale, 32 + FewRaw<D>::kRows * u + lane / (D / 16)));
+          ks[0] = scale_of((uint32_t)__shfl((int)w.scale, i16)), ks[1] = scale_of((uint32_t)__shfl((int)w.scale, 16 + i16));
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int u = 0; u < FewRaw<D>::kV; ++u) {
             const int row = FewRaw<D>::kRows * u + lane / (D / 16);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              v4i x = widen8<T>(w.v[u][2 * e], w.v[u][2 * e + 1], scale_of(w.vs[u]));
+              v4i x = widen8<T>(w.v[u][2 * e], w.v[u][2 * e + 1], vs[u]);
               if (MASK) {
                 if (k0 + row >= s_hi) x = (v4i){};  // whatever a page holds past the end
                 else if (take_nonfinite<T>(x)) aside = true;
@@ -857,7 +863,7 @@ __global__ __launch_bounds__(64 * NW, E8 ? 2 : 1) void paged_attn_few_kernel(Att
           for (int x = 0; x < 2; ++x) {
             v4i kop;
             if constexpr (E8) {
-              kop = widen8<T>(w.k[x][cd / 2][2 * (cd & 1)], w.k[x][cd / 2][2 * (cd & 1) + 1], scale_of(w.ks[x]));
+              kop = widen8<T>(w.k[x][cd / 2][2 * (cd & 1)], w.k[x][cd / 2][2 * (cd & 1) + 1], ks[x]);
             } else {
               kop = *(const v4i*)(kb + 16 * x * S::kRow + (kro ^ (uint32_t)(64 * cd)));
             }
@@ -1291,7 +1297,6 @@ constexpr int64_t kScoreBytes = 256ll << 20;  // most workspace spent on kept sc
 
 struct Plan {
   bool matrix, few, keep_scores;
-  bool wide;          // few rows: a workgroup of 8 waves
   int64_t tile_rows;  // rows a workgroup: 16 or 32 (few), 128 or 256
   int splits, split_keys, shares, tiles;
   int row_splits, key_tiles;  // of the recomputing gather
@@ -1312,9 +1317,7 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int
   p.tile_rows = p.few ? (rows <= 16 ? 16 : 32) : rows <= 128 ? 128 : 256;
   if (p.few) p.keep_scores = gather && tokens * heads * ((capacity + 3) / 4 * 4) * 4 <= kScoreBytes;
   // few splits only: their join reads them in turn (72 of 2 sequences of 18361 keys: 39 us in all, as shares 19)
-  if (E8 && p.few && p.tile_rows == 16 && max_kv <= 1024 && groups <= kCus) {
-    p.wide = true;
-  } else if (p.few && groups * ((max_kv + 255) / 256) <= kCus && max_kv <= 8 * 256) {
+  if (p.few && groups * ((max_kv + 255) / 256) <= kCus && max_kv <= 8 * 256) {
     p.split_keys = 256;
     p.splits = (int)((max_kv + 255) / 256);
     if (p.splits > 1) p.part_floats = p.splits * tokens * heads * (d + 1);
@@ -1358,8 +1361,7 @@ void launch_matrix(const Plan& p, AttnArgs a, int64_t max_kv, bool gather, hipSt
   const unsigned groups = (unsigned)(a.c.batch * a.c.kv_heads);
   if (p.few && p.shares == 0) {
     const dim3 grid(groups * (unsigned)p.splits), block(64 * FW_WAVES);
-    if (E8 && p.wide) hipLaunchKernelGGL((paged_attn_few_kernel<T, D, 1, false, E8, E8 ? 8 : FW_WAVES>), grid, dim3(512), 0, st, a);
-    else if (p.tile_rows == 16) hipLaunchKernelGGL((paged_attn_few_kernel<T, D, 1, false, E8>), grid, block, 0, st, a);
+    if (p.tile_rows == 16) hipLaunchKernelGGL((paged_attn_few_kernel<T, D, 1, false, E8>), grid, block, 0, st, a);
     else hipLaunchKernelGGL((paged_attn_few_kernel<T, D, 2, false, E8>), grid, block, 0, st, a);
     if (p.splits > 1)
       hipLaunchKernelGGL((paged_attn_join_kernel<T, D>), dim3((unsigned)(((int64_t)a.tokens * a.heads * D + 1023) / 1024)),

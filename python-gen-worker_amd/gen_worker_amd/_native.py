@@ -11,6 +11,7 @@ in the reference).
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -250,6 +251,13 @@ def build_info() -> str:
 def ptr(t) -> Optional[int]:
     """Device pointer of a tensor (None for None)."""
     return None if t is None else t.data_ptr()
+
+
+def on_device_of(t):
+    """A context in which launches go to ``t``'s device, whichever is current outside it."""
+    import torch
+
+    return (contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device))
 
 
 def stream_of(t) -> int:

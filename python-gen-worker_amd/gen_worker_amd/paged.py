@@ -318,7 +318,8 @@ def _write_body(q: Tensor, k: Tensor, v: Tensor, cos: Optional[Tensor], sin: Opt
     if scales is None:
         nat.call("gwa_paged_write", ctypes.byref(args), *rest)
     else:
-        nat.call("gwa_paged_write_fp8", ctypes.byref(args), ctypes.byref(_scale_args(name, k_pages, *scales)), *rest)
+        with nat.on_device_of(k_pages):
+            nat.call("gwa_paged_write_fp8", ctypes.byref(args), ctypes.byref(_scale_args(name, k_pages, *scales)), *rest)
     return out
 
 
@@ -381,7 +382,9 @@ def _attention_body(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, 
     if scales is None:
         nat.call("gwa_paged_attention", ctypes.byref(args), *rest)
     else:
-        nat.call("gwa_paged_attention_fp8", ctypes.byref(args), ctypes.byref(_scale_args(name, k_pages, *scales)), *rest)
+        with nat.on_device_of(q):
+            nat.call("gwa_paged_attention_fp8", ctypes.byref(args), ctypes.byref(_scale_args(name, k_pages, *scales)),
+                     *rest)
     return o, lse
 
 
@@ -444,7 +447,8 @@ def _evict_body(k_pages: Tensor, v_pages: Tensor, weights: Tensor, table: Tensor
     if scales is None:
         nat.call("gwa_paged_evict", ctypes.byref(args), *rest)
     else:
-        nat.call("gwa_paged_evict_fp8", ctypes.byref(args), ctypes.byref(_scale_args(name, k_pages, *scales)), *rest)
+        with nat.on_device_of(k_pages):
+            nat.call("gwa_paged_evict_fp8", ctypes.byref(args), ctypes.byref(_scale_args(name, k_pages, *scales)), *rest)
     return kept, new_len
 
 
@@ -532,8 +536,9 @@ def _read_fp8_body(k_pages: Tensor, v_pages: Tensor, k_scales: Tensor, v_scales:
     _require(tokens >= 0, name, f"{tokens} tokens")
     k = torch.empty((tokens, args.kv_heads, args.head_dim), dtype=dtype, device=k_pages.device)
     v = torch.empty_like(k)
-    nat.call("gwa_paged_read_fp8", ctypes.byref(args), ctypes.byref(scales), k.data_ptr(), v.data_ptr(), tokens,
-             nat.stream_of(k_pages))
+    with nat.on_device_of(k_pages):
+        nat.call("gwa_paged_read_fp8", ctypes.byref(args), ctypes.byref(scales), k.data_ptr(), v.data_ptr(), tokens,
+                 nat.stream_of(k_pages))
     return k, v
 
 

@@ -54,13 +54,14 @@ def _sample_body(logits: Tensor, uniform: Tensor, temperature: Optional[Tensor],
         logits = logits.contiguous()
     tokens = torch.empty(rows, dtype=torch.int64, device=dev)
     logprobs = torch.empty(rows, dtype=torch.float32, device=dev)
-    settings = nat.SamplingArgs(nat.ptr(temperature), nat.ptr(top_k), nat.ptr(top_p), nat.ptr(min_p), all_temperature,
-                                all_top_k, all_top_p, all_min_p)
+    args = nat.SamplingArgs(nat.ptr(temperature), nat.ptr(top_k), nat.ptr(top_p), nat.ptr(min_p), all_temperature, all_top_k,
+                            all_top_p, all_min_p)
     n = int(nat.load().gwa_sample_tokens_workspace(rows, vocab))
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    nat.call("gwa_sample_tokens", logits.data_ptr(), max(logits.stride(0), vocab), _DTYPES[logits.dtype],
-             uniform.data_ptr(), ctypes.byref(settings), tokens.data_ptr(), logprobs.data_ptr(), rows, vocab, nat.ptr(ws),
-             n, nat.stream_of(logits))
+    with nat.on_device_of(logits):
+        nat.call("gwa_sample_tokens", logits.data_ptr(), max(logits.stride(0), vocab), _DTYPES[logits.dtype],
+                 uniform.data_ptr(), ctypes.byref(args), tokens.data_ptr(), logprobs.data_ptr(), rows, vocab, nat.ptr(ws),
+                 n, nat.stream_of(logits))
     return tokens, logprobs
 
 
@@ -112,6 +113,7 @@ def sample_tokens(logits: Tensor, uniform: Tensor, *, temperature: Union[float, 
     split. No gradient is defined."""
     each, numbers = settings(temperature, top_k, top_p, min_p)
     a = (logits, uniform, *each)
+    _require(all(paged._tangent(x) is None for x in a), "no gradient is defined for a dual tensor's tangent")
     host = paged._host()
     if host is not None:
         out = host.sample_tokens(*a, *numbers)

@@ -592,6 +592,10 @@ def test_native_host_calls_ops_and_python_bodies_agree(monkeypatch):
             with pytest.raises(ValueError):
                 bad()
 
+    # (opcheck's schema test multiplies its arguments, which torch does not do in float8)
+    for op, args in ((library.paged_attention_fp8, (r.q, *r.pool(), r.table, r.q_start, r.kv_len, 3, 700, 0.125, True, None)),
+                     (library.paged_read_fp8, (*r.pool(), r.table, r.q_start, r.kv_len, r.tokens, F16))):
+        torch.library.opcheck(op, args, test_utils=("test_faketensor",))
     with_host = everything()
     refused()
     by_ops = everything(through_ops=True)
@@ -640,3 +644,22 @@ def test_nothing_to_do():
     assert o.shape == (0, 4, 64) and lse.shape == (0, 4)
     for n, t in r.pools.items():
         assert torch.equal(t.view(torch.uint8), before[n].view(torch.uint8))
+
+
+def test_tangents_are_refused():
+    """No call here has a forward-mode rule."""
+    import torch.autograd.forward_ad as fwad
+
+    from gen_worker_amd.paged import PagedError, paged_write_fp8
+    from gen_worker_amd.sampling import SamplingError, sample_tokens
+
+    r = Ragged8([3], [50], 4, 2, 64, 16, BF16, seed=3)
+    with fwad.dual_level():
+        q = fwad.make_dual(r.q, torch.ones_like(r.q))
+        with pytest.raises(PagedError, match="tangent"):
+            r.attend(q=q)
+        with pytest.raises(PagedError, match="tangent"):
+            paged_write_fp8(q, r.q[:, :2], r.q[:, :2], None, None, None, *r.pool(), r.table, r.q_start, r.kv_len)
+        x = torch.randn(2, 9, device=DEV)
+        with pytest.raises(SamplingError, match="tangent"):
+            sample_tokens(fwad.make_dual(x, x), torch.rand(2, device=DEV))
