@@ -192,7 +192,7 @@ __device__ __forceinline__ Settings settings_of(const SampleArgs& a, int64_t row
   s.min_p = held_in(a.s.min_p ? a.s.min_p[row] : a.s.all_min_p, 0.0f, 1.0f);
   if (s.top_k <= 0 || s.top_k >= a.vocab) s.top_k = 0;
   if (s.min_p < kLeastMinP) s.min_p = 0.0f;
-  s.way = !(s.temperature > 0.0f) ? kGreedy : s.top_k == 0 ? kMass : s.top_k <= SM_FOUND / 4 ? kCount : kWhole;
+  s.way = !(s.temperature > 0.0f) ? kGreedy : s.top_k == 0 ? kMass : s.top_k <= SM_FOUND / 2 ? kCount : kWhole;
   return s;
 }
 
@@ -799,9 +799,10 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
   const bool cuts = s.way == kCount || p.bin <= to;  // whether what is collected is cut by its order
   const bool few_found = !whole && cuts && n <= SM_FEW;
   if (few_found) {
-    // each against all, by four threads a token. `order`: larger for what comes first (equal logits: the lowest index)
-    constexpr int SHARE = NT / SM_FEW;
-    const int j = tid & (SM_FEW - 1), i0 = tid / SM_FEW;
+    // each against all, by as many threads a token as there are (four at least). `order`: larger for what comes first (equal
+    // logits: the lowest index)
+    const int bits = n <= 64 ? 6 : 32 - __clz(n - 1), share = NT >> bits;
+    const int j = tid & ((1 << bits) - 1), i0 = tid >> bits;
     const bool mine = tid < n;
     for (int i = lane; i < mine_n; i += 64) few_x[my_first + i] = my_x[i], few_i[my_first + i] = my_i[i];
     if (tid < SM_FEW) few_sum[0][tid] = few_sum[1][tid] = 0, few_rank[tid] = few_equal[tid] = 0;
@@ -818,7 +819,7 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
       uint64_t ahead = 0;
       uint32_t rank = 0, equal = 0;
 #pragma unroll 4
-      for (int i = i0; i < n; i += SHARE) {
+      for (int i = i0; i < n; i += share) {
         const ulonglong2 o = few[i];
         const bool first = o.y > my_order;
         rank += first, ahead += first ? o.x : 0, equal += first && (o.y ^ my_order) >> 32 == 0;
@@ -852,7 +853,7 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
         const uint32_t my_place = (uint32_t)few[j].y;  // larger for lower indices
         uint64_t cum = 0;
 #pragma unroll 4
-        for (int i = i0; i < n; i += SHARE) {
+        for (int i = i0; i < n; i += share) {
           const ulonglong2 o = few[i];
           cum += (uint32_t)o.y > my_place ? o.x : 0;
         }
