@@ -5,7 +5,7 @@
 
 namespace {
 
-constexpr int SM_BINS = 384, SM_DIGITS = 2048, SM_LIST = 512, SM_FOUND = 8192;
+constexpr int SM_BINS = 384, SM_DIGITS = 2048, SM_FOUND = 8192;
 constexpr int SM_HELD = 8;            // logits a thread holds where a row fits a workgroup's registers
 constexpr int SM_PART = 4096, SM_PARTS = 64;  // tokens a part of a longer row at least; parts of a row at most
 constexpr int SM_AHEAD = 4;           // 16-byte loads a lane has in flight
@@ -170,6 +170,60 @@ __device__ __forceinline__ uint64_t wave_scan64(uint64_t x) {
 }
 __device__ __forceinline__ uint64_t wave_sum64(uint64_t x) { return lane64(wave_scan64(x), 63); }
 
+// x of lane ^ X
+template <int X>
+__device__ __forceinline__ uint32_t beside32(uint32_t x) {
+  if constexpr (X == 4) return beside32<3>(beside32<7>(x));
+  else if constexpr (X >= 16) return (uint32_t)__shfl_xor((int)x, X);
+  else {
+    // within fours; eights and sixteens mirrored; sixteens turned by 8
+    constexpr int kMove = X == 1 ? 0xb1 : X == 2 ? 0x4e : X == 3 ? 0x1b : X == 7 ? 0x141 : X == 15 ? 0x140 : 0x128;
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, kMove, 0xf, 0xf, true);
+  }
+}
+// A step of sorting: the larger of a pair to the lower place, the one without the bit LOW
+template <int X, int LOW>
+__device__ __forceinline__ uint32_t stepped32(uint32_t x) {
+  const uint32_t o = beside32<X>(x);
+  return threadIdx.x & LOW ? min(x, o) : max(x, o);
+}
+template <int S>
+__device__ __forceinline__ uint32_t settled32(uint32_t x) {
+  x = stepped32<S, S>(x);
+  if constexpr (S > 1) x = settled32<S / 2>(x);
+  return x;
+}
+// Falling over the first 2^bits threads of a workgroup of NT (bits at least 6; all threads call it, with 0 behind what is
+// sorted): runs of twice the length from two, the one against the other reversed, then halved; between waves by LDS, two
+// buffers in turn, so that one barrier a step is enough. cells[1] may hold the threads' own values.
+template <int NT>
+__device__ __forceinline__ uint32_t sorted32(uint32_t x, int bits, uint32_t (&cells)[2][NT]) {
+  const int tid = threadIdx.x;
+  const bool in = tid < 1 << bits;  // the same for the wave
+  if (in) {
+    x = stepped32<1, 1>(x);
+    x = settled32<1>(stepped32<3, 2>(x));
+    x = settled32<2>(stepped32<7, 4>(x));
+    x = settled32<4>(stepped32<15, 8>(x));
+    x = settled32<8>(stepped32<31, 16>(x));
+    x = settled32<16>(stepped32<63, 32>(x));
+  }
+  int turn = 0;
+  for (int size = 128; size <= 1 << bits; size *= 2) {
+    for (int low = size / 2, other = size - 1; low >= 64; other = low /= 2) {
+      if (in) cells[turn][tid] = x;
+      __syncthreads();
+      if (in) {
+        const uint32_t o = cells[turn][tid ^ other];
+        x = tid & low ? min(x, o) : max(x, o);
+      }
+      turn ^= 1;
+    }
+    if (in) x = settled32<32>(x);
+  }
+  return x;
+}
+
 // Below this a min_p keeps all: there weights of a few units of 2^-shift (38 at least) would be compared, whose rounding
 // tells the least kept one apart from its neighbours no better than a bin does.
 constexpr float kLeastMinP = 0x1p-28f;
@@ -258,8 +312,7 @@ struct Drawer {
     double table[1 << kTableBits];
     uint64_t mass[SM_DIGITS];
     uint32_t count[SM_DIGITS];
-    uint64_t list_w[SM_LIST];
-    uint32_t list_key[SM_LIST];
+    uint32_t list[2][NT];
     uint64_t cells[2][NW];
     uint64_t found[4];
     uint32_t n;
@@ -356,50 +409,48 @@ struct Drawer {
     return reach<MASS>(n, w, first, n0, w0, want, target_of);
   }
 
-  // The cut inside bin `p.bin`, from the tokens that `each` passes on and `take` accepts, which hold all of the bin's
+  // The cut inside bin `p.bin` of p.inside tokens (or fewer), from the tokens that `each` passes on and `take` accepts, which hold all of the bin's
   template <bool MASS, class Each, class Take>
   __device__ __forceinline__ Cut resolve(Each each, Take take, Place p, uint64_t want, double target) {
     const int bin = p.bin;
     auto in_bin = [&](float x) __attribute__((always_inline)) { return take(x) && scale.bin(x) == bin; };
     int sub = -1;
-    if (p.inside > 32) {  // once more into bins
+    if (p.inside > NT) {  // once more into bins
       p = locate<MASS>(each, in_bin, [&](float x) { return scale.inside(x, bin); }, p.before, p.above, want,
                        [&](uint64_t) { return target; });
       sub = p.bin;
     }
     auto here = [&](float x) __attribute__((always_inline)) { return in_bin(x) && (sub < 0 || scale.inside(x, bin) == sub); };
-    if (p.inside <= SM_LIST) {  // ranked by counting
-      if (threadIdx.x == 0) l.n = 0;
+    if (p.inside <= NT) {  // sorted, one a thread
+      const int tid = threadIdx.x;
+      if (tid == 0) l.n = 0;
       __syncthreads();
-      each([&](int, float x, auto weight) __attribute__((always_inline)) {
-        if (here(x)) {
-          const uint32_t i = atomicAdd(&l.n, 1u);
-          l.list_key[i] = order_of(x);
-          if (MASS) l.list_w[i] = weight();
-        }
+      each([&](int, float x, auto) __attribute__((always_inline)) {
+        if (here(x)) l.list[1][atomicAdd(&l.n, 1u)] = order_of(x);
       });
       __syncthreads();
-      for (int j = threadIdx.x; j < (int)p.inside; j += NT) {
-        const uint32_t key = l.list_key[j];
-        uint32_t over = 0, equal = 0;
-        uint64_t from = p.above;
-        for (uint32_t i = 0; i < p.inside; ++i) {
-          const uint32_t k = l.list_key[i];
-          over += k > key, equal += k == key;
-          if (MASS) from += k > key ? l.list_w[i] : 0;
-        }
-        const uint64_t mine = MASS ? l.list_w[j] : 0;
-        const bool at = MASS ? (double)from < target && (double)(from + equal * mine) >= target
-                             : p.before + over < want && p.before + over + equal >= want;
-        if (at) {  // equal ones all write the same
-          l.found[0] = key, l.found[1] = equal;
-          l.found[2] = MASS ? ties_to(target, from, mine, equal) : want - p.before - over;
-        }
+      const int n = (int)l.n;
+      const uint32_t key = sorted32<NT>(tid < n ? l.list[1][tid] : 0, n <= 64 ? 6 : 32 - __clz(n - 1), l.list);
+      const uint64_t w = MASS && tid < n ? weight(value_of(key)) : 0;
+      uint64_t before = 0, unused, all, none;
+      if (MASS) scan(w, 0, before, unused, all, none);
+      else __syncthreads();
+      if (tid < n) l.list[0][tid] = key;
+      __syncthreads();
+      before += p.above;
+      if (tid < n && (MASS ? (double)before < target && (double)(before + w) >= target : p.before + tid + 1 == want))
+        l.found[0] = key, l.found[1] = tid;
+      __syncthreads();
+      // the first place of that value, and the one behind its last
+      const uint32_t at = (uint32_t)l.found[0], place = (uint32_t)l.found[1];
+      if (tid < n && key == at) {
+        if (tid == 0 || l.list[0][tid - 1] != at) l.found[2] = tid;
+        if (tid == n - 1 || l.list[0][tid + 1] != at) l.found[3] = tid + 1;
       }
       __syncthreads();
-      const Cut c = {(uint32_t)l.found[0], (uint32_t)l.found[2], (uint32_t)l.found[1]};
+      const uint32_t first = (uint32_t)l.found[2], behind = (uint32_t)l.found[3];
       __syncthreads();
-      return c;
+      return {at, place + 1 - first, behind - first};
     }
     // digit by digit of the ordered values: 11 + 11 + 10 bits
     uint32_t prefix = 0;
@@ -725,7 +776,7 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
     } else {
       from = SM_BINS, to = SM_BINS - 2;  // the last bin's weights are 0
       if (s.top_p < 1.0f) {
-        p = {(int)l.found[0], 0xffffffffu, 0, l.found[1]};  // its tokens are counted on the way
+        p = {(int)l.found[0], 0, 0, l.found[1]};  // its tokens are counted below
         from = to = p.bin;
       }
       if (s.min_p > 0.0f) {
@@ -797,6 +848,7 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
   }
   const int n = __shfl(upto_wave, NW - 1), my_first = __shfl(upto_wave, wave) - mine_n;
   const bool cuts = s.way == kCount || p.bin <= to;  // whether what is collected is cut by its order
+  if (s.way == kMass) p.inside = (uint32_t)n;
   const bool few_found = !whole && cuts && n <= SM_FEW;
   if (few_found) {
     // each against all, by as many threads a token as there are (four at least). `order`: larger for what comes first (equal
