@@ -4,7 +4,7 @@
 
 namespace {
 
-constexpr int W8_THREADS = 256;
+constexpr int W8_THREADS = 512, R8_THREADS = 256;  // of a workgroup at most; of one that reads
 
 // A row's scale byte b from its largest finite magnitude (fp32 bits), 2^(127 - b), and the largest code magnitude. 448 * 2^e
 // >= amax holds from e = floor(log2 amax) - 8 on, or one more where amax's fraction passes that of 448 = 1.75 * 2^8. At
@@ -70,9 +70,8 @@ __global__ __launch_bounds__(W8_THREADS) void paged_write_fp8_kernel(PagedArgs c
   const int t = blockIdx.x % kXcds * (gridDim.x / kXcds) + blockIdx.x / kXcds;
   if (t >= tokens) return;
   const int64_t row = r.rot ? table_row(r, t) : 0;
-  const Rotation none = {nullptr, nullptr, nullptr, 0, 0, 0, 1.0f};
   const int hk = c.kv_heads, rows = heads + 2 * hk, units = head_dim / (2 * N);
-  const int u0 = threadIdx.x & (lanes - 1), step = W8_THREADS / lanes;
+  const int u0 = threadIdx.x & (lanes - 1), step = blockDim.x / lanes;
   TokenPlace place = {0, -1};
   for (int h0 = 0; h0 < rows; h0 += step) {
     const int h = h0 + threadIdx.x / lanes;
@@ -85,9 +84,11 @@ __global__ __launch_bounds__(W8_THREADS) void paged_write_fp8_kernel(PagedArgs c
       for (int i = 0; i < kHeld; ++i)
         if (u0 + i * lanes < units && h < rows) f(i);
     };
-    const uint16_t* from = is_q ? q + t * ldqt + h * ldqh : is_k ? k + t * ldkt + kh * ldkh : v + t * ldvt + kh * ldvh;
+    const uint16_t* from = (is_q ? q + t * ldqt : is_k ? k + t * ldkt : v + t * ldvt) +
+                           (is_q ? h : kh) * (is_q ? ldqh : is_k ? ldkh : ldvh);
+    const Rotation turn = {r.cos_t, r.sin_t, r.positions, r.table_rows, is_v ? 0 : r.rot, r.interleaved, 1.0f};
     each([&](int i) __attribute__((always_inline)) {
-      rotated_unit<DT, VEC>(from, 0, is_v ? none : r, is_v ? 0 : row, u0 + i * lanes, c0[i], c1[i], a[i], b[i]);
+      rotated_unit<DT, VEC>(from, 0, turn, row, u0 + i * lanes, c0[i], c1[i], a[i], b[i]);
     });
     if (h0 == 0) place = token_place(c, t, tokens);
     if (is_q) {
@@ -142,9 +143,9 @@ __global__ __launch_bounds__(W8_THREADS) void paged_write_fp8_kernel(PagedArgs c
 // A thread the same 16 channels of a key's and its value's row; a token's place is found by the thread, in a few dependent
 // loads that neighbours share.
 template <class T>
-__global__ __launch_bounds__(W8_THREADS) void paged_read_fp8_kernel(PagedArgs c, uint16_t* k_out, uint16_t* v_out,
+__global__ __launch_bounds__(R8_THREADS) void paged_read_fp8_kernel(PagedArgs c, uint16_t* k_out, uint16_t* v_out,
                                                                     int tokens, int pieces) {
-  const int64_t i = (int64_t)blockIdx.x * W8_THREADS + threadIdx.x;
+  const int64_t i = (int64_t)blockIdx.x * R8_THREADS + threadIdx.x;
   const uint32_t per = (uint32_t)c.kv_heads * (uint32_t)pieces;
   const int64_t t64 = i / per;
   if (t64 >= tokens) return;
@@ -200,10 +201,15 @@ extern "C" int gwa_paged_write_fp8(const gwa_paged_cache* cache, const gwa_paged
   int lanes = 64;
   if (vec)
     for (lanes = 1; lanes < d / 16; lanes *= 2) {}
+  // whole waves, as many as a token's rows need, in as few turns as W8_THREADS allows
+  const int64_t needed = (heads + 2 * c.kv_heads) * lanes, turns = (needed + W8_THREADS - 1) / W8_THREADS;
+  const dim3 grid((unsigned)((tokens + kXcds - 1) / kXcds * kXcds));
+  const dim3 block((unsigned)(((needed + turns - 1) / turns + 63) / 64 * 64));
+  GWA_REQUIRE((int64_t)grid.x * block.x < (1ll << 32), "%s: %lld tokens are too many", what, (long long)tokens);
 #define GWA_WRITE8(DT, VEC)                                                                                        \
-  hipLaunchKernelGGL((paged_write_fp8_kernel<DT, VEC>), dim3((unsigned)((tokens + kXcds - 1) / kXcds * kXcds)), dim3(W8_THREADS), 0, \
-                     (hipStream_t)stream, c, (const uint16_t*)q, ldqt, ldqh, (const uint16_t*)k, ldkt, ldkh,       \
-                     (const uint16_t*)v, ldvt, ldvh, (uint16_t*)q_out, r, (int)tokens, (int)heads, (int)d, lanes)
+  hipLaunchKernelGGL((paged_write_fp8_kernel<DT, VEC>), grid, block, 0, (hipStream_t)stream, c, (const uint16_t*)q, \
+                     ldqt, ldqh, (const uint16_t*)k, ldkt, ldkh, (const uint16_t*)v, ldvt, ldvh, (uint16_t*)q_out, r, \
+                     (int)tokens, (int)heads, (int)d, lanes)
   if (cache->dtype == GWA_DT_BF16) { if (vec) GWA_WRITE8(GWA_DT_BF16, true); else GWA_WRITE8(GWA_DT_BF16, false); }
   else { if (vec) GWA_WRITE8(GWA_DT_F16, true); else GWA_WRITE8(GWA_DT_F16, false); }
 #undef GWA_WRITE8
@@ -222,9 +228,9 @@ extern "C" int gwa_paged_read_fp8(const gwa_paged_cache* cache, const gwa_paged_
   GWA_REQUIRE(k_out && v_out && GWA_ALIGNED(k_out, 16) && GWA_ALIGNED(v_out, 16),
               "%s: the outputs must be there, 16-byte aligned", what);
   const int pieces = cache->head_dim / 16;
-  const int64_t blocks = (tokens * c.kv_heads * pieces + W8_THREADS - 1) / W8_THREADS;
-  GWA_REQUIRE(blocks < (1ll << 31), "%s: %lld tokens are too many", what, (long long)tokens);
-  const dim3 grid((unsigned)blocks), block(W8_THREADS);
+  const int64_t blocks = (tokens * c.kv_heads * pieces + R8_THREADS - 1) / R8_THREADS;
+  GWA_REQUIRE(blocks * R8_THREADS < (1ll << 32), "%s: %lld tokens are too many", what, (long long)tokens);
+  const dim3 grid((unsigned)blocks), block(R8_THREADS);
   if (cache->dtype == GWA_DT_BF16)
     hipLaunchKernelGGL((paged_read_fp8_kernel<Bf16>), grid, block, 0, (hipStream_t)stream, c, (uint16_t*)k_out,
                        (uint16_t*)v_out, (int)tokens, pieces);

@@ -1073,7 +1073,7 @@ extern "C" int gwa_sample_tokens(const void* logits, int64_t ld, int dtype, cons
   GWA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && GWA_ALIGNED(workspace, 16)),
               "%s: a workspace of %lld bytes, %lld are needed (16-byte aligned)", what, (long long)workspace_bytes,
               (long long)need);
-  GWA_REQUIRE(rows * parts < (1ll << 31), "%s: %lld rows of %lld tokens are too many", what, (long long)rows,
+  GWA_REQUIRE(rows * max((int64_t)1024, 256 * parts) < (1ll << 32), "%s: %lld rows of %lld tokens are too many", what, (long long)rows,
               (long long)vocab);
   uint64_t* bins = (uint64_t*)workspace;
   const SampleArgs a = {logits, ld, uniform, s, tokens, logprobs, (int)vocab, bits <= 17 ? 45 : 62 - bits, (int)parts,

@@ -83,6 +83,8 @@ class TestEntryPoints:
         self.refused("gwa_paged_attention_fp8", None, s, *self.ATTEND, match="null cache")
         self.refused("gwa_paged_write_fp8", c, None, *self.WRITE, 2, 1, 64, 0, None, match="null scales")
         self.refused("gwa_paged_write_fp8", c, s, *self.WRITE, -1, 1, 64, 0, None, match="tokens")
+        self.refused("gwa_paged_write_fp8", c, s, *self.WRITE, 2 ** 31 - 1, 1, 64, 0, None, match="too many")
+        self.refused("gwa_paged_read_fp8", c, s, 4096, 4096, 2 ** 31 - 1, None, match="too many")
         self.refused("gwa_paged_write_fp8", c, s, *self.WRITE, 2, 1, 66, 0, None, match="rotated channels")
         self.refused("gwa_paged_write_fp8", c, s, *self.WRITE[:-1], 4097, 2, 1, 64, 0, None, match="misaligned")
         self.refused("gwa_paged_write_fp8", c, s, *self.WRITE[:3], None, *self.WRITE[4:], 2, 1, 64, 0, None,

@@ -47,7 +47,9 @@ class TestEntryPoint:
         (dict(all_min_p=-0.1), "min_p"), (dict(vocab=50000, ld=50000), "workspace"),
         (dict(vocab=50000, ld=50000, workspace=4096, nbytes=1000), "workspace"),
         (dict(vocab=50000, ld=50000, workspace=4104, nbytes=1 << 30), "workspace"),
-        (dict(rows=2 ** 30, vocab=50000, ld=50000, workspace=4096, nbytes=1 << 60), "too many")])
+        (dict(rows=2 ** 30, vocab=50000, ld=50000, workspace=4096, nbytes=1 << 60), "too many"),
+        (dict(rows=2 ** 22), "too many"),
+        (dict(rows=2 ** 22 - 1, vocab=50000, ld=50000, workspace=4096, nbytes=1 << 60), "too many")])
     def test_refuses(self, change, match):
         rc, said = self.call(**change)
         assert rc == 1 and match in said, said
