@@ -33,7 +33,7 @@ __global__ __launch_bounds__(RT_THREADS) void paged_write_kernel(PagedArgs c, co
                                                                  int64_t ldvh, uint16_t* q_out, Rotation r, int tokens,
                                                                  int heads, int head_dim, int units) {
   const int t = blockIdx.x;
-  const TokenPlace place = token_place(c, t, tokens);
+  const TokenPlace place = token_place(c, token_sequence(c, t), t, tokens);
   int64_t at = -1, wat = 0;
   if (place.slot >= 0) {
     at = paged_at(c, place.page, 0, place.slot);

@@ -65,18 +65,20 @@ __global__ __launch_bounds__(W8_THREADS) void paged_write_fp8_kernel(PagedArgs c
                                                                      int64_t ldqh, const uint16_t* k, int64_t ldkt,
                                                                      int64_t ldkh, const uint16_t* v, int64_t ldvt,
                                                                      int64_t ldvh, uint16_t* q_out, Rotation r, int tokens,
-                                                                     int heads, int head_dim, int lanes) {
+                                                                     int heads, int head_dim, int lane_bits) {
   constexpr int N = VEC ? 8 : 1, kHeld = VEC ? 1 : 2;
   const int t = blockIdx.x % kXcds * (gridDim.x / kXcds) + blockIdx.x / kXcds;
   if (t >= tokens) return;
   const int64_t row = r.rot ? table_row(r, t) : 0;
+  const TokenPlace place = token_place(c, token_sequence(c, t), t, tokens);
   const int hk = c.kv_heads, rows = heads + 2 * hk, units = head_dim / (2 * N);
-  const int u0 = threadIdx.x & (lanes - 1), step = blockDim.x / lanes;
-  TokenPlace place = {0, -1};
+  const int lanes = 1 << lane_bits, u0 = threadIdx.x & (lanes - 1), step = blockDim.x >> lane_bits;
   for (int h0 = 0; h0 < rows; h0 += step) {
-    const int h = h0 + threadIdx.x / lanes;
+    const int h = h0 + (threadIdx.x >> lane_bits);
     const bool is_q = h < heads, is_k = !is_q && h < heads + hk, is_v = !is_q && !is_k && h < rows;
     const int kh = is_k ? h - heads : h - heads - hk;
+    const uint16_t* from = is_q ? q + t * ldqt + h * ldqh : is_k ? k + t * ldkt + kh * ldkh : v + t * ldvt + kh * ldvh;
+    const Rotation turn = {r.cos_t, r.sin_t, nullptr, 0, is_v ? 0 : r.rot, r.interleaved, 1.0f};
     float a[kHeld][N], b[kHeld][N];
     int c0[kHeld], c1[kHeld];
     auto each = [&](auto f) __attribute__((always_inline)) {
@@ -84,13 +86,9 @@ __global__ __launch_bounds__(W8_THREADS) void paged_write_fp8_kernel(PagedArgs c
       for (int i = 0; i < kHeld; ++i)
         if (u0 + i * lanes < units && h < rows) f(i);
     };
-    const uint16_t* from = (is_q ? q + t * ldqt : is_k ? k + t * ldkt : v + t * ldvt) +
-                           (is_q ? h : kh) * (is_q ? ldqh : is_k ? ldkh : ldvh);
-    const Rotation turn = {r.cos_t, r.sin_t, r.positions, r.table_rows, is_v ? 0 : r.rot, r.interleaved, 1.0f};
     each([&](int i) __attribute__((always_inline)) {
       rotated_unit<DT, VEC>(from, 0, turn, row, u0 + i * lanes, c0[i], c1[i], a[i], b[i]);
     });
-    if (h0 == 0) place = token_place(c, t, tokens);
     if (is_q) {
       uint16_t* out = q_out + ((int64_t)t * heads + h) * head_dim;
       each([&](int i) __attribute__((always_inline)) {
@@ -198,18 +196,18 @@ extern "C" int gwa_paged_write_fp8(const gwa_paged_cache* cache, const gwa_paged
   const Rotation r = {cos_t, sin_t, positions, table_rows, (int)rot, interleaved != 0, 1.0f};
   const bool vec = vector_units(d, rot, cos_t, sin_t) && vector_operand(q, ldqt, ldqh, 2) &&
                    vector_operand(k, ldkt, ldkh, 2) && vector_operand(v, ldvt, ldvh, 2) && GWA_ALIGNED(q_out, 16);
-  int lanes = 64;
+  int lane_bits = 6;
   if (vec)
-    for (lanes = 1; lanes < d / 16; lanes *= 2) {}
+    for (lane_bits = 0; 1 << lane_bits < d / 16; ++lane_bits) {}
   // whole waves, as many as a token's rows need, in as few turns as W8_THREADS allows
-  const int64_t needed = (heads + 2 * c.kv_heads) * lanes, turns = (needed + W8_THREADS - 1) / W8_THREADS;
+  const int64_t needed = (heads + 2 * c.kv_heads) << lane_bits, turns = (needed + W8_THREADS - 1) / W8_THREADS;
   const dim3 grid((unsigned)((tokens + kXcds - 1) / kXcds * kXcds));
   const dim3 block((unsigned)(((needed + turns - 1) / turns + 63) / 64 * 64));
   GWA_REQUIRE((int64_t)grid.x * block.x < (1ll << 32), "%s: %lld tokens are too many", what, (long long)tokens);
 #define GWA_WRITE8(DT, VEC)                                                                                        \
   hipLaunchKernelGGL((paged_write_fp8_kernel<DT, VEC>), grid, block, 0, (hipStream_t)stream, c, (const uint16_t*)q, \
                      ldqt, ldqh, (const uint16_t*)k, ldkt, ldkh, (const uint16_t*)v, ldvt, ldvh, (uint16_t*)q_out, r, \
-                     (int)tokens, (int)heads, (int)d, lanes)
+                     (int)tokens, (int)heads, (int)d, lane_bits)
   if (cache->dtype == GWA_DT_BF16) { if (vec) GWA_WRITE8(GWA_DT_BF16, true); else GWA_WRITE8(GWA_DT_BF16, false); }
   else { if (vec) GWA_WRITE8(GWA_DT_F16, true); else GWA_WRITE8(GWA_DT_F16, false); }
 #undef GWA_WRITE8

@@ -7,19 +7,22 @@ namespace {
 
 // 8 consecutive elements of the three element types as fp32, in 16-byte pieces
 template <int DT>
+__device__ __forceinline__ void unpack8(const v4i& r, float (&f)[8]) {  // of the two 16-bit types
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = (uint32_t)r[i];
+    f[2 * i] = DT == GWA_DT_BF16 ? bf16_lo(w) : f16_bits_to_f32((uint16_t)w);
+    f[2 * i + 1] = DT == GWA_DT_BF16 ? bf16_hi(w) : f16_bits_to_f32((uint16_t)(w >> 16));
+  }
+}
+template <int DT>
 __device__ __forceinline__ void load8(const void* base, int64_t at, float (&f)[8]) {
   if constexpr (DT == GWA_DT_F32) {
     const float4* p = (const float4*)((const float*)base + at);
     const float4 a = p[0], b = p[1];
     f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
   } else {
-    const v4i r = *(const v4i*)((const uint16_t*)base + at);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t w = (uint32_t)r[i];
-      f[2 * i] = DT == GWA_DT_BF16 ? bf16_lo(w) : f16_bits_to_f32((uint16_t)w);
-      f[2 * i + 1] = DT == GWA_DT_BF16 ? bf16_hi(w) : f16_bits_to_f32((uint16_t)(w >> 16));
-    }
+    unpack8<DT>(*(const v4i*)((const uint16_t*)base + at), f);
   }
 }
 template <int DT>
@@ -63,53 +66,74 @@ __device__ __forceinline__ int64_t table_row(const Rotation& r, int64_t t) {
 }
 
 // Elements a unit of work covers: 16 with VEC (8 pairs, or 16 channels past the rotated ones; both halves of the
-// half layout lie on 16-byte pieces then), else one pair / two channels: its rotated values, and the channels c0 and c1
-// where each part of it begins.
+// half layout lie on 16-byte pieces then), else one pair / two channels: the channels c0 and c1 where each part of it
+// begins, and whether it lies past the rotated ones.
+template <bool VEC>
+__device__ __forceinline__ bool unit_channels(const Rotation& r, int unit, int& c0, int& c1) {
+  constexpr int N = VEC ? 8 : 1;
+  const bool tail = 2 * N * unit >= r.rot;
+  // first and second piece: the pairs' two halves, or neighbours
+  c0 = tail || r.interleaved ? 2 * N * unit : N * unit;
+  c1 = tail || r.interleaved ? c0 + N : c0 + r.rot / 2;
+  return tail;
+}
+// a unit's pairs turned by their cosines and sines
+template <int N>
+__device__ __forceinline__ void turn_unit(const Rotation& r, float (&a)[N], float (&b)[N], const float (&c)[N],
+                                          float (&s)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) s[i] *= r.sign;
+  if (N > 1 && r.interleaved) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const float e = a[2 * i], o = a[2 * i + 1];
+      a[2 * i] = fmaf(e, c[i], -o * s[i]);
+      a[2 * i + 1] = fmaf(e, s[i], o * c[i]);
+      const float e2 = b[2 * i], o2 = b[2 * i + 1];
+      b[2 * i] = fmaf(e2, c[N / 2 + i], -o2 * s[N / 2 + i]);
+      b[2 * i + 1] = fmaf(e2, s[N / 2 + i], o2 * c[N / 2 + i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float e = a[i], o = b[i];
+      a[i] = fmaf(e, c[i], -o * s[i]);
+      b[i] = fmaf(e, s[i], o * c[i]);
+    }
+  }
+}
+// A unit's rotated values
 template <int DT, bool VEC>
 __device__ __forceinline__ void rotated_unit(const void* x, int64_t xo, const Rotation& r, int64_t row, int unit, int& c0,
                                              int& c1, float (&a)[VEC ? 8 : 1], float (&b)[VEC ? 8 : 1]) {
-  const int half = r.rot / 2;
+  const bool tail = unit_channels<VEC>(r, unit, c0, c1);
   if constexpr (VEC) {
-    const bool tail = 16 * unit >= r.rot;
-    // first and second piece of 8: the pairs' two halves, or neighbours
-    c0 = tail || r.interleaved ? 16 * unit : 8 * unit;
-    c1 = tail || r.interleaved ? c0 + 8 : c0 + half;
-    load8<DT>(x, xo + c0, a);
-    load8<DT>(x, xo + c1, b);
-    if (!tail) {
-      float c[8], s[8];
-      load8<GWA_DT_F32>(r.cos_t, row + 8 * unit, c);
-      load8<GWA_DT_F32>(r.sin_t, row + 8 * unit, s);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s[i] *= r.sign;
-      if (r.interleaved) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float e = a[2 * i], o = a[2 * i + 1];
-          a[2 * i] = fmaf(e, c[i], -o * s[i]);
-          a[2 * i + 1] = fmaf(e, s[i], o * c[i]);
-          const float e2 = b[2 * i], o2 = b[2 * i + 1];
-          b[2 * i] = fmaf(e2, c[4 + i], -o2 * s[4 + i]);
-          b[2 * i + 1] = fmaf(e2, s[4 + i], o2 * c[4 + i]);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float e = a[i], o = b[i];
-          a[i] = fmaf(e, c[i], -o * s[i]);
-          b[i] = fmaf(e, s[i], o * c[i]);
-        }
+    if constexpr (DT == GWA_DT_F32) {
+      load8<DT>(x, xo + c0, a);
+      load8<DT>(x, xo + c1, b);
+      if (!tail) {
+        float c[8], s[8];
+        load8<GWA_DT_F32>(r.cos_t, row + 8 * unit, c);
+        load8<GWA_DT_F32>(r.sin_t, row + 8 * unit, s);
+        turn_unit<8>(r, a, b, c, s);
       }
+    } else {
+      const v4i xa = *(const v4i*)((const uint16_t*)x + xo + c0), xb = *(const v4i*)((const uint16_t*)x + xo + c1);
+      float c[8], s[8];
+      if (!tail) {
+        load8<GWA_DT_F32>(r.cos_t, row + 8 * unit, c);
+        load8<GWA_DT_F32>(r.sin_t, row + 8 * unit, s);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      unpack8<DT>(xa, a);
+      unpack8<DT>(xb, b);
+      if (!tail) turn_unit<8>(r, a, b, c, s);
     }
   } else {
-    const bool tail = 2 * unit >= r.rot;
-    c0 = tail || r.interleaved ? 2 * unit : unit;
-    c1 = tail || r.interleaved ? c0 + 1 : c0 + half;
     a[0] = load1<DT>(x, xo + c0), b[0] = load1<DT>(x, xo + c1);
     if (!tail) {
-      const float c = r.cos_t[row + unit], s = r.sin_t[row + unit] * r.sign, e = a[0];
-      a[0] = fmaf(e, c, -b[0] * s);
-      b[0] = fmaf(e, s, b[0] * c);
+      float c[1] = {r.cos_t[row + unit]}, s[1] = {r.sin_t[row + unit]};
+      turn_unit<1>(r, a, b, c, s);
     }
   }
 }
@@ -129,17 +153,21 @@ __device__ __forceinline__ void rotate_unit(const void* x, int64_t xo, void* y, 
   }
 }
 
-// A new token's sequence's page and slot for it; slot -1: none (a token of no sequence, a slot before the first or past
-// the table). The whole wave calls it, for one token.
-struct TokenPlace {
-  int page, slot;
-};
-__device__ __forceinline__ TokenPlace token_place(const PagedArgs& c, int t, int tokens) {
+// The sequence of a new token: how many end at or before it (q_start ascends; empty ones end where they start). The whole
+// wave calls it, for one token.
+__device__ __forceinline__ int token_sequence(const PagedArgs& c, int t) {
   const int lane = threadIdx.x & 63;
-  // the number of sequences that end at or before it (q_start ascends; empty ones end where they start)
   int b = 0;
   for (int i = 0; i < c.batch; i += 64)
     b += __popcll(__ballot(i + lane < c.batch && c.q_start[min(i + lane, c.batch - 1) + 1] <= t));
+  return b;
+}
+// The page and slot of a new token of sequence b; slot -1: none (a token of no sequence, a slot before the first or past the
+// table)
+struct TokenPlace {
+  int page, slot;
+};
+__device__ __forceinline__ TokenPlace token_place(const PagedArgs& c, int b, int t, int tokens) {
   TokenPlace p = {0, -1};
   if (b < c.batch) {
     int t0, n;
