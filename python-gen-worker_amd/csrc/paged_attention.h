@@ -194,9 +194,11 @@ __global__ __launch_bounds__(64) void paged_gather_rows_kernel(PagedArgs c, cons
 // where an 8192^3 library product reaches 1.22 to 1.26. The matrix cores are busy 49 % of the time and the vector unit 51 %, at
 // a clock that falls to 1.65 to 1.8 GHz; without the copies it takes 849 us (of 965 then), without the exponentials 891. Before the fixed operand order
 // every MFMA waited for the LDS read issued just ahead of it (1057 us); both waves of a SIMD in the same phase take 1013;
-// 128-key tiles spill and take 1710. Five sequences of up to 509 tokens over up to 4001 keys, 16 heads of 64: 35 us, in which
-// nothing is busy (matrix cores 11 %, vector unit 27 %, LDS 7 %): a tile has half the work between the same two barriers, and
-// 2 waves a SIMD do not cover what each waits for.
+// 128-key tiles spill and take 1710. Of an 8-bit cache (E8) the rows pass through registers, where they become 16-bit values
+// on their way to LDS, a tile ahead: one conversion for two values, again for each row tile; 2048 tokens over 16500 keys
+// (525 GFLOP) take 550 to 605 us where a 16-bit cache takes 515 to 540. Five sequences of up to 509 tokens over up to 4001
+// keys, 16 heads of 64: 35 us, in which nothing is busy (matrix cores 11 %, vector unit 27 %, LDS 7 %): a tile has half the work between the same two barriers, and
+// 2 waves a SIMD do not cover what each waits for (38 us of an 8-bit cache).
 template <int D, int BN, int NW>
 struct TileShape {
   static constexpr int kRow = 2 * D, kRun = 1024 / kRow;  // row bytes; rows a 1 KB copy covers
@@ -669,6 +671,11 @@ __global__ __launch_bounds__(256) void paged_attn_join_parts_kernel(AttnArgs a) 
 // Measured: the 32 sequences 276 us, 5.7 TB/s (a copy reaches 4.94; the copies alone, without the products, took 296 with
 // their join before the shares); 4 tokens each over up to 8192 keys 88 us with the join, 8 tokens 101 (floors 76 and 85); one
 // sequence of 701 keys, 32 heads over 8, 9 to 10 us and 3.9 for the join (medians): launch and four dependent loads.
+// Of an 8-bit cache (E8) two tiles are in flight in registers, K's codes as the operands need them and V's on to LDS as
+// 16-bit values. The 32 sequences of up to 32768 keys: 162 us, 4.9 TB/s (169 to 170 a call with the join); the same loads
+// without any work on them 153. One scale byte a lane, given out by lane moves, and places found by the wave: 179 us of a
+// call with every lane loading its rows' own. The sequence of 701 keys: 9.2 us and 3.8; a workgroup of 8 waves for all its
+// keys, with no join: 11.6 to 12.5, so there is none.
 constexpr int FW_KEYS = 32, FW_PAGES = 512;  // keys a tile; page ids staged at a time (whole tiles: page_size >= 8)
 constexpr int FW_WAVES = 4, FW_UNIT = FW_KEYS * FW_WAVES;
 // Where the segment of a run that starts at key s_lo ends, at k_hi at the latest: behind the FW_PAGES-th page from that of
@@ -803,11 +810,13 @@ __global__ __launch_bounds__(64 * FW_WAVES, E8 ? 2 : 1) void paged_attn_few_kern
         int64_t at[4], sat[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int key = min(s_lo + t * FW_KEYS + 8 * r, (s_hi - 1) & ~7), page = uniform(page_ids[(key >> c.page_shift) - p0]);
+          const int key = min(s_lo + t * FW_KEYS + 8 * r, (s_hi - 1) & ~7);
+          const int page = uniform(page_ids[(key >> c.page_shift) - p0]);
           at[r] = (int64_t)((uint64_t)(uint32_t)page * page_bytes + (key & slot_mask) * slot_bytes);
           sat[r] = page * c.s_page_stride + h * c.s_head_stride + (key & slot_mask);
         }
-        const uint32_t k_lane = (i16 & 7) * slot_bytes + D / 4 * q4, v_lane = (lane / (D / 16) & 7) * slot_bytes + 16 * (lane % (D / 16));
+        const uint32_t k_lane = (i16 & 7) * slot_bytes + D / 4 * q4;
+        const uint32_t v_lane = (lane / (D / 16) & 7) * slot_bytes + 16 * (lane % (D / 16));
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const uint8_t* p = kbase + (i16 < 8 ? at[2 * x] : at[2 * x + 1]) + k_lane;
@@ -911,7 +920,8 @@ __global__ __launch_bounds__(64 * FW_WAVES, E8 ? 2 : 1) void paged_attn_few_kern
         if constexpr (E8) {  // all reads ahead of the products: one at a time each waits for its own
           v4i vop[S::kND];
 #pragma unroll
-          for (int db = 0; db < S::kND; ++db) vop[db] = two_halves(lds_read_tr(kb + vro[db]), lds_read_tr(kb + vro[db] + 16 * S::kRow));
+          for (int db = 0; db < S::kND; ++db)
+            vop[db] = two_halves(lds_read_tr(kb + vro[db]), lds_read_tr(kb + vro[db] + 16 * S::kRow));
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int db = 0; db < S::kND; ++db)
@@ -1326,6 +1336,8 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int
     // heads over 2, cut into 64 parts a tile take 26 us, into 32 23, into 8 32; the join reads every part
     const int64_t tt = p.tile_rows / group, tiles = ((max_q < 1 ? 1 : max_q) + tt - 1) / tt;
     const int64_t row_tiles = kv_heads * std::min(batch * tiles, tokens / tt + batch), units = (max_kv + 63) / 64;
+    // (two workgroups a CU where they fit; 8-bit rows leave fewer bytes in flight a wave: 16 rows over up to 32768 keys of 32
+    // sequences take 170 us with two and 178 with one)
     p.shares = p.tile_rows == 128 || (E8 && p.tile_rows == 16) ? 2 * kCus : kCus;
     // Many rows: a workgroup a row tile where that takes no longer. 64 keys take it about 2 us, and it goes through
     // whole rounds of workgroups; shares always end together, but take 8 us to find and to join and 6 % more for

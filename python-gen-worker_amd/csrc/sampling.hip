@@ -10,6 +10,8 @@ constexpr int SM_HELD = 8;            // logits a thread holds where a row fits 
 constexpr int SM_PART = 4096, SM_PARTS = 64;  // tokens a part of a longer row at least; parts of a row at most
 constexpr int SM_AHEAD = 4;           // 16-byte loads a lane has in flight
 constexpr int SM_FEW = 256;           // collected tokens that are ranked all against all
+// Measured, bf16 logits: 64 rows of 131072, a top_k of 50: 27 us with SM_FEW at 256, 35 where none are ranked so; up to 512 at
+// 512 the squares cost more than sorting does (rows of 300 to 470 collected tokens: 61 against 51).
 constexpr int kTableBits = 9;         // of the table of 2^(j / 512)
 
 struct SampleArgs {
@@ -80,8 +82,8 @@ __device__ __forceinline__ void fill_table(double* table, int shift) {
 
 // A row's tokens by their weight exp((x - m) / temperature) = 2^y, y = (x - m) log2(e) / temperature in 64 bits. The weight
 // is an integer of 2^-shift: 2^y = 2^n 2^(j/512) 2^r, |r| <= 1/1024, by a table (which holds the 2^shift) and the series of
-// 2^r to r^3 (the rest is below 2^-46), rounded by an addition of 2^52. Bins are an eighth of a unit of y wide; the last is for what weighs
-// nothing: y < -47, -inf and NaN. Bins and their halves (`inside`) fall as x grows, never the other way. A token's weight and
+// 2^r to r^3 (the rest is below 2^-46), rounded by an addition of 2^52. Bins are an eighth of a unit of y wide; the last is
+// for what weighs nothing: y < -47, -inf and NaN. Bins and their halves (`inside`) fall as x grows, never the other way. A token's weight and
 // bin have to be the same wherever they are formed, so the compiler may not choose where products and sums are fused.
 // m = +inf is held as 1e300: +inf is then at y = 0, all else far below.
 struct Scale {
@@ -229,7 +231,9 @@ __device__ __forceinline__ uint32_t sorted32(uint32_t x, int bits, uint32_t (&ce
 constexpr float kLeastMinP = 0x1p-28f;
 
 // One row's settings and how its cuts are found: kCount: the first top_k by the numbers of tokens in the bins; kMass: what
-// there are of top_p and min_p by the weights in them; kWhole: by passes over the whole row
+// there are of top_p and min_p by the weights in them; kWhole: by passes over the whole row. 64 rows of 131072 by kCount: 34 us
+// for a top_k of 200 and 46 for 4000; by kWhole 73 and 101. Past half of SM_FOUND a wave's own part of the collected tokens
+// would often be too short.
 enum Way { kGreedy, kCount, kMass, kWhole };
 struct Settings {
   float temperature, top_p, min_p;
@@ -409,7 +413,8 @@ struct Drawer {
     return reach<MASS>(n, w, first, n0, w0, want, target_of);
   }
 
-  // The cut inside bin `p.bin` of p.inside tokens (or fewer), from the tokens that `each` passes on and `take` accepts, which hold all of the bin's
+  // The cut inside bin `p.bin` of p.inside tokens (or fewer), from the tokens that `each` passes on and `take` accepts, which
+  // hold all of the bin's
   template <bool MASS, class Each, class Take>
   __device__ __forceinline__ Cut resolve(Each each, Take take, Place p, uint64_t want, double target) {
     const int bin = p.bin;
@@ -552,7 +557,9 @@ __device__ __forceinline__ float wave_max(float m) {
   return m;
 }
 
-// Rows that fit a workgroup's registers: SM_HELD neighbouring tokens a thread, read once.
+// Rows that fit a workgroup's registers: SM_HELD neighbouring tokens a thread, read once. Bound by its chain of barriers and
+// scans: one row of 2048 with a top_p 9.7 us (a top_k as well 12), 1024 such rows 22. With 16 waves for such a row as well: 13
+// and 41; rows of 8192 by the three kernels below: 64 of them 20 us instead of 15, 1024 62 instead of 55.
 template <int DT, int NW>
 __global__ __launch_bounds__(64 * NW) void sample_held_kernel(SampleArgs a) {
   using D = Drawer<NW>;
@@ -632,7 +639,7 @@ __global__ __launch_bounds__(64 * NW) void sample_held_kernel(SampleArgs a) {
   }
 }
 
-// Longer rows, first: the largest logit of every part
+// Longer rows, first: the largest logit of every part. Bound by memory: 256 rows of 131072, fp32: 23 us, 5.8 TB/s.
 template <int DT>
 __global__ __launch_bounds__(256) void sample_max_kernel(SampleArgs a) {
   __shared__ float cells[4];
@@ -651,7 +658,8 @@ __device__ __forceinline__ float row_max(const SampleArgs& a, int64_t row) {
   return wave_max(lane < a.parts ? a.most[row * a.parts + lane] : -INFINITY);  // SM_PARTS at most
 }
 
-// second: every part's histogram, of tokens or of their weight, as sums up to each bin
+// second: every part's histogram, of tokens or of their weight, as sums up to each bin. Bound by the weights' arithmetic in
+// 64 bits (the logits come from the last-level cache): 256 rows of 131072 37 us, 3.6 TB/s; 64 of bf16 10 us.
 template <int DT>
 __global__ __launch_bounds__(256) void sample_bins_kernel(SampleArgs a) {
   __shared__ uint64_t bin[SM_BINS];
@@ -699,6 +707,9 @@ __global__ __launch_bounds__(256) void sample_bins_kernel(SampleArgs a) {
 // or that lie where the cuts fall (kMass) are collected in one pass of comparisons and the cut found among them; the kept
 // weight of every part; and the tokens of the part that the random number falls into. Where the collected ones are too
 // many (thousands of nearly equal logits, a very large top_k) all is done by passes over the row.
+// 256 rows of 131072, fp32, a top_p: 42 us, of which 20 read the row once more (6.7 TB/s), 7 find the cut among some 800
+// tokens, 6 the drawn token in its part; 64 rows of bf16, each with settings of its own: 27, the slowest row's. Bound by
+// what one workgroup does in turn.
 template <int DT>
 __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
   constexpr int NW = 16, NT = 1024;
@@ -1014,7 +1025,8 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
 }
 
 // tokens a part of a row of `vocab`, of `rows`: SM_PART, more where that gives more than SM_PARTS parts, or more workgroups
-// than keep the chip busy (a part costs 4 KB of bins)
+// than keep the chip busy (a part costs 3 KB of bins, written and read): 256 rows of 131072 with a top_k of 40 take 49 us with
+// parts of 8192 and 55 with 4096; 64 rows 38 with either, 33 against 28 (top_k) with 2048.
 int part_of(int64_t rows, int64_t vocab) {
   int64_t part = SM_PART;
   while (part * SM_PARTS < vocab || (part < 2 * SM_PART && rows * (vocab / part) > 4096)) part *= 2;
@@ -1073,8 +1085,8 @@ extern "C" int gwa_sample_tokens(const void* logits, int64_t ld, int dtype, cons
   GWA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && GWA_ALIGNED(workspace, 16)),
               "%s: a workspace of %lld bytes, %lld are needed (16-byte aligned)", what, (long long)workspace_bytes,
               (long long)need);
-  GWA_REQUIRE(rows * max((int64_t)1024, 256 * parts) < (1ll << 32), "%s: %lld rows of %lld tokens are too many", what, (long long)rows,
-              (long long)vocab);
+  GWA_REQUIRE(rows * max((int64_t)1024, 256 * parts) < (1ll << 32), "%s: %lld rows of %lld tokens are too many", what,
+              (long long)rows, (long long)vocab);
   uint64_t* bins = (uint64_t*)workspace;
   const SampleArgs a = {logits, ld, uniform, s, tokens, logprobs, (int)vocab, bits <= 17 ? 45 : 62 - bits, (int)parts,
                         (int)part, bins, need ? (float*)(bins + rows * parts * SM_BINS) : nullptr};

@@ -1,9 +1,10 @@
 """A small decoder on the quantized linears and the paged cache: how the pieces of ``paged`` run together.
 
 Random weights, pre-norm blocks (RMSNorm, rotary attention whose query heads share key/value heads, GELU MLP), answers
-greedy or drawn (``sampling``). Every linear comes from ``flux_dit.linear_factory``, so the same model runs W4A4 or bf16. Prompts of any
-lengths go in together, in chunks; then every step takes one token of each sequence. With a ``budget`` each layer's keys
-are cut back to the most attended whenever a sequence has outgrown it by a page; the caches hold bf16 or 8 bits:
+greedy or drawn (``sampling``). Every linear comes from ``flux_dit.linear_factory``, so the same model runs W4A4 or bf16.
+Prompts of any lengths go in together, in chunks; then every step takes one token of each sequence. With a ``budget`` each
+layer's keys are cut back to the most attended whenever a sequence has outgrown it by a page; the caches hold bf16 or 8
+bits:
 
     python -m gen_worker_amd.decoder --kind w4a4 --prompts 300,17,120 --tokens 64 --budget 128
     python -m gen_worker_amd.decoder --cache fp8 --temperature 0.8 --top-p 0.95 --seed 3

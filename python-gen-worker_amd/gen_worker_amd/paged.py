@@ -771,8 +771,8 @@ class PagedCache:
 
     def attend(self, batch: PagedBatch, q: Tensor, *, scale: Optional[float] = None, causal: bool = True,
                gather: Optional[bool] = None) -> tuple[Tensor, Tensor]:
-        """``paged_attention`` (``paged_attention_fp8``) of the batch's (rotated) queries: (o, lse). Weights are gathered where the cache keeps
-        them, unless ``gather`` is False."""
+        """``paged_attention`` (``paged_attention_fp8``) of the batch's (rotated) queries: (o, lse). Weights are gathered
+        where the cache keeps them, unless ``gather`` is False."""
         gather = self.weights is not None if gather is None else gather
         _require(not gather or self.weights is not None, "PagedCache.attend", "the cache keeps no weights")
         weights = self.weights if gather else None
