@@ -147,6 +147,7 @@ def test_read_leaves_rows_without_a_slot(monkeypatch):
     ([33, 2], [100, 2], 4, 4, 80, 20, 32, False, BF16),
     ([9, 4], [30, 4], 3, 1, 96, 96, 16, False, F16),
     ([3, 1], [3, 70], 20, 1, 256, 64, 64, True, BF16),
+    ([2, 3], [2, 70], 60, 2, 256, 256, 16, False, BF16),
     ([7], [9], 2, 2, 16, 6, 8, False, F16),
     ([6], [6], 2, 1, 64, 0, 16, False, F16)])
 @pytest.mark.parametrize("odd", [False, True])
@@ -366,6 +367,38 @@ def test_a_pool_past_32_bits():
         r.pools = {"k": k, "v": v, "ks": ks, "vs": vs}
         got = r.attend()
         assert torch.equal(got[0], o) and torch.equal(got[1], lse)
+
+
+def test_operands_past_32_bits():
+    """New rows whose offsets pass 2^31 elements, and rows read back past them."""
+    from gen_worker_amd.paged import paged_read_fp8, paged_write_fp8
+
+    stride, n, dim = 2 ** 31 + 128, 2, 64
+    pool = torch.empty(stride + n * 3 * dim, dtype=BF16, device=DEV)
+    x = pool.as_strided((2, 3 * n, dim), (stride, dim, 1))
+    x.copy_(torch.randn(2, 3 * n, dim, generator=_gen(9), device=DEV))
+    q, k, v = x[:, :n], x[:, n:2 * n], x[:, 2 * n:]
+    got = []
+    for a in ((q, k, v), tuple(t.contiguous() for t in (q, k, v))):
+        codes = [torch.zeros(1, n, 8, dim, dtype=torch.uint8, device=DEV).view(FP8) for _ in range(2)]
+        scales = [torch.zeros(1, n, 8, dtype=torch.uint8, device=DEV) for _ in range(2)]
+        out = paged_write_fp8(*a, None, None, None, *codes, *scales, _ints([[0]]), _ints([0, 2]), _ints([2]))
+        got.append([out] + [t.view(torch.uint8) for t in codes + scales])
+    assert all(torch.equal(a, b) for a, b in zip(*got)) and torch.equal(got[0][0], q)
+    del pool, x
+    # many sequences that hold the same row: 2^31 elements and more of it
+    rows = 2 ** 31 // (n * dim) + 1000
+    batch = 60000
+    each = rows // batch + 1
+    width = -(-each // 8)
+    codes = [t.view(FP8) for t in got[0][1:3]]
+    table = torch.zeros(batch, width, dtype=torch.int32, device=DEV)
+    q_start = (torch.arange(batch + 1, device=DEV) * each).int()
+    kv_len = torch.full((batch,), each, dtype=torch.int32, device=DEV)
+    k, v = paged_read_fp8(*codes, *got[0][3:], table, q_start, kv_len, batch * each)
+    assert k.numel() > 2 ** 31
+    first = paged_read_fp8(*codes, *got[0][3:], table[:1], q_start[:2], kv_len[:1], each)
+    assert torch.equal(k[-each:], first[0]) and torch.equal(v[-each:], first[1])
 
 
 def test_large_scores_and_small_rows():

@@ -100,6 +100,53 @@ def test_rows_of_one_bin_and_of_many(spread, dtype):
         check(logits, torch.rand(3, generator=g, device=DEV), **s)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("spread", [1.0, 4.0])
+def test_cuts_of_every_length(spread, dtype):
+    """A few collected tokens, hundreds, thousands, and more than are collected; bf16: ties on every border."""
+    g = _gen(21)
+    logits = (torch.randn(2, 50021, generator=g, device=DEV) * spread).to(dtype)
+    for k in (2, 63, 64, 65, 255, 256, 257, 511, 513, 1000, 1024, 1025, 2048, 4096, 4097):
+        for more in (dict(), dict(top_p=0.9), dict(min_p=0.02)):
+            check(logits, torch.rand(2, generator=g, device=DEV), top_k=k, **more)
+    for p in (0.01, 0.2, 0.6, 0.97, 0.9999):
+        for t in (0.6, 1.0, 3.0):
+            check(logits, torch.rand(2, generator=g, device=DEV), temperature=t, top_p=p)
+
+
+def test_rows_past_32_bits():
+    """Rows whose offset passes 2^31 elements and 2^32 bytes."""
+    from gen_worker_amd.sampling import sample_tokens
+
+    for vocab in (2000, 40001):
+        pool = torch.empty(2 ** 31 + 64 + vocab, dtype=BF16, device=DEV)
+        logits = pool.as_strided((2, vocab), (2 ** 31 + 64, 1))
+        logits.copy_(torch.randn(2, vocab, generator=_gen(vocab), device=DEV) * 3)
+        u = torch.rand(2, generator=_gen(3), device=DEV)
+        for s in (dict(), dict(temperature=0.0), dict(top_k=50, top_p=0.9)):
+            got, want = sample_tokens(logits, u, **s), sample_tokens(logits.contiguous(), u, **s)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+            check(logits.contiguous(), u, **s)
+
+
+def test_two_streams_at_once():
+    from gen_worker_amd.sampling import sample_tokens
+
+    g = _gen(13)
+    logits = [torch.randn(32, 60000, generator=g, device=DEV) * 3 for _ in range(2)]
+    u = torch.rand(32, generator=g, device=DEV)
+    want = [sample_tokens(x, u, top_p=0.95) for x in logits]
+    streams = [torch.cuda.Stream() for _ in logits]
+    torch.cuda.synchronize()
+    got = [[] for _ in logits]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(sample_tokens(logits[i], u, top_p=0.95))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for i, w in enumerate(want) for x in got[i] for a, b in zip(x, w))
+
+
 def test_equal_weights_split_the_unit_interval():
     """Of n equal tokens number i is drawn from u = i / n on: exactly, borders included; cuts keep the lowest indices."""
     from gen_worker_amd.sampling import sample_tokens
