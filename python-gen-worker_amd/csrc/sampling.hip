@@ -236,7 +236,7 @@ constexpr float kLeastMinP = 0x1p-28f;
 // would often be too short.
 enum Way { kGreedy, kCount, kMass, kWhole };
 struct Settings {
-  float temperature, top_p, min_p;
+  float temperature, top_p, min_p, uniform;
   int top_k;  // 0: all
   Way way;
 };
@@ -248,6 +248,7 @@ __device__ __forceinline__ Settings settings_of(const SampleArgs& a, int64_t row
   s.top_k = a.s.top_k ? a.s.top_k[row] : a.s.all_top_k;
   s.top_p = held_in(a.s.top_p ? a.s.top_p[row] : a.s.all_top_p, 0.0f, 1.0f);
   s.min_p = held_in(a.s.min_p ? a.s.min_p[row] : a.s.all_min_p, 0.0f, 1.0f);
+  s.uniform = held_in(a.uniform[row], 0.0f, 1.0f);
   if (s.top_k <= 0 || s.top_k >= a.vocab) s.top_k = 0;
   if (s.min_p < kLeastMinP) s.min_p = 0.0f;
   s.way = !(s.temperature > 0.0f) ? kGreedy : s.top_k == 0 ? kMass : s.top_k <= SM_FOUND / 2 ? kCount : kWhole;
@@ -334,6 +335,17 @@ struct Drawer {
         low((double)s.min_p * (double)(1ull << a.shift)) {}
   __device__ __forceinline__ uint64_t weight(float x) const { return scale.weight(x); }
 
+  // The sum of x over the threads before this one, in the threads' order, and over all
+  __device__ __forceinline__ void scan(uint64_t x, uint64_t& before, uint64_t& all) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint64_t p = wave_scan64(x);
+    __syncthreads();
+    if (lane == 63) l.cells[0][wave] = p;
+    __syncthreads();
+    // the waves' sums, one a lane (16 at most)
+    const uint64_t c = lane < NW ? l.cells[0][lane] : 0, upto = row_scan64(c);
+    before = p - x + lane64(upto - c, wave), all = lane64(upto, NW - 1);
+  }
   // Sums of x and y over the threads before this one, in the threads' order, and over all
   __device__ __forceinline__ void scan(uint64_t x, uint64_t y, uint64_t& x_before, uint64_t& y_before, uint64_t& x_all,
                                        uint64_t& y_all) {
@@ -342,7 +354,6 @@ struct Drawer {
     __syncthreads();
     if (lane == 63) l.cells[0][wave] = p, l.cells[1][wave] = q;
     __syncthreads();
-    // the waves' sums, one a lane (16 at most)
     const uint64_t cx = lane < NW ? l.cells[0][lane] : 0, cy = lane < NW ? l.cells[1][lane] : 0;
     const uint64_t sx = row_scan64(cx), sy = row_scan64(cy);
     x_before = p - x + lane64(sx - cx, wave), y_before = q - y + lane64(sy - cy, wave);
@@ -354,25 +365,27 @@ struct Drawer {
   struct Place {
     int bin;
     uint32_t inside;
-    uint64_t before, above;  // tokens, and weight, ahead of it
+    uint64_t before, above;  // tokens, or weight, ahead of it
   };
   template <bool MASS, int PER, class Target>
   __device__ __forceinline__ Place reach(const uint64_t (&n)[PER], const uint64_t (&w)[PER], int first, uint64_t n0,
                                          uint64_t w0, uint64_t want, Target target_of) {
-    uint64_t sn = 0, sw = 0, nb, wb, na, wa;
+    uint64_t sum = 0, upto, all;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) sn += n[i], sw += w[i];
-    scan(sn, sw, nb, wb, na, wa);
-    nb += n0, wb += w0;
-    const double target = MASS ? target_of(wa) : 0.0;
+    for (int i = 0; i < PER; ++i) sum += MASS ? w[i] : n[i];
+    scan(sum, upto, all);
+    upto += MASS ? w0 : n0;
+    const double target = MASS ? target_of(all) : 0.0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const bool here = MASS ? (double)wb < target && (double)(wb + w[i]) >= target : nb < want && nb + n[i] >= want;
-      if (here) l.found[0] = first + i, l.found[1] = nb, l.found[2] = wb, l.found[3] = n[i];
-      nb += n[i], wb += w[i];
+      const uint64_t before = upto;
+      upto += MASS ? w[i] : n[i];
+      if (MASS ? (double)before < target && (double)upto >= target : before < want && upto >= want)
+        l.found[0] = first + i, l.found[1] = before, l.found[2] = n[i];
     }
     __syncthreads();
-    const Place p = {(int)l.found[0], (uint32_t)l.found[3], l.found[1], l.found[2]};
+    const uint64_t before = l.found[1];
+    const Place p = {(int)l.found[0], (uint32_t)l.found[2], MASS ? 0 : before, MASS ? before : 0};
     __syncthreads();
     return p;
   }
@@ -437,8 +450,8 @@ struct Drawer {
       const int n = (int)l.n;
       const uint32_t key = sorted32<NT>(tid < n ? l.list[1][tid] : 0, n <= 64 ? 6 : 32 - __clz(n - 1), l.list);
       const uint64_t w = MASS && tid < n ? weight(value_of(key)) : 0;
-      uint64_t before = 0, unused, all, none;
-      if (MASS) scan(w, 0, before, unused, all, none);
+      uint64_t before = 0, all;
+      if (MASS) scan(w, before, all);
       else __syncthreads();
       if (tid < n) l.list[0][tid] = key;
       __syncthreads();
@@ -521,7 +534,7 @@ struct Drawer {
   }
   // cum > u total: for integers, cum > floor(u total)
   __device__ __forceinline__ uint64_t drawn(uint64_t total) const {
-    return min((uint64_t)((double)held_in(a.uniform[row], 0.0f, 1.0f) * (double)total), total - 1);
+    return min((uint64_t)((double)s.uniform * (double)total), total - 1);
   }
 
   __device__ __forceinline__ void draw(int index, float x, uint64_t total) const {
