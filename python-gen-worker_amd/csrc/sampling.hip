@@ -117,11 +117,17 @@ struct Scale {
     return __builtin_bit_cast(uint64_t, p + 4503599627370496.0) & 0xfffffffffffffull;
   }
   static __device__ __forceinline__ int bin_of_steps(int k) { return -k >> kPerBin; }
-  __device__ __forceinline__ uint64_t weight(float x) const {
+  __device__ __forceinline__ uint64_t weight(float x, int& bin) const {
     double y, r;
+    bin = SM_BINS - 1;
     if (!weighs(x, y)) return 0;
     const int k = steps_of(y, r);
+    bin = bin_of_steps(k);
     return of_steps(k, r);
+  }
+  __device__ __forceinline__ uint64_t weight(float x) const {
+    int bin;
+    return weight(x, bin);
   }
   __device__ __forceinline__ int bin(float x) const {
     double y, r;
@@ -141,6 +147,20 @@ struct Scale {
     lo = (float)(a - fabs(a) * 1e-6 - 1e-37);
     hi = from == 0 ? INFINITY : (float)(b + fabs(b) * 1e-6 + 1e-37);
   }
+};
+
+// A token's weight and bin: as they were formed, or to be formed
+struct Formed {
+  uint64_t w;
+  int b;
+  __device__ __forceinline__ uint64_t weight() const { return w; }
+  __device__ __forceinline__ int bin() const { return b; }
+};
+struct Unformed {
+  const Scale& scale;
+  float x;
+  __device__ __forceinline__ uint64_t weight() const { return scale.weight(x); }
+  __device__ __forceinline__ int bin() const { return scale.bin(x); }
 };
 
 __device__ __forceinline__ uint64_t two_words(uint32_t lo, uint32_t hi) { return (uint64_t)hi << 32 | lo; }
@@ -398,7 +418,8 @@ struct Drawer {
     return e;
   }
 
-  // a histogram by bin_of(x) of the tokens that `each` passes on and `take` accepts, and the place in it
+  // a histogram by bin_of of the tokens that `each` passes on (their index, logit, and weight and bin) and `take` accepts,
+  // and the place in it
   static constexpr int kPer = (SM_BINS + NT - 1) / NT;
   template <bool MASS, class Each, class Take, class Of, class Target>
   __device__ __forceinline__ Place locate(Each each, Take take, Of bin_of, uint64_t n0, uint64_t w0, uint64_t want,
@@ -406,13 +427,11 @@ struct Drawer {
     __syncthreads();
     for (int i = threadIdx.x; i < SM_BINS; i += NT) l.count[i] = 0, l.mass[i] = 0;
     __syncthreads();
-    each([&](int, float x, auto weight) __attribute__((always_inline)) {
-      if (take(x)) {
-        const int b = bin_of(x);
-        if (b >= 0) {
-          atomicAdd(&l.count[b], 1u);
-          if (MASS) atomicAdd((unsigned long long*)&l.mass[b], (unsigned long long)weight());
-        }
+    each([&](int, float x, auto of) __attribute__((always_inline)) {
+      if (take(x, of)) {
+        const int b = bin_of(x, of);
+        atomicAdd(&l.count[b], 1u);
+        if (MASS) atomicAdd((unsigned long long*)&l.mass[b], (unsigned long long)of.weight());
       }
     });
     __syncthreads();
@@ -431,20 +450,22 @@ struct Drawer {
   template <bool MASS, class Each, class Take>
   __device__ __forceinline__ Cut resolve(Each each, Take take, Place p, uint64_t want, double target) {
     const int bin = p.bin;
-    auto in_bin = [&](float x) __attribute__((always_inline)) { return take(x) && scale.bin(x) == bin; };
+    auto in_bin = [&](float x, auto of) __attribute__((always_inline)) { return take(x, of) && of.bin() == bin; };
     int sub = -1;
     if (p.inside > NT) {  // once more into bins
-      p = locate<MASS>(each, in_bin, [&](float x) { return scale.inside(x, bin); }, p.before, p.above, want,
+      p = locate<MASS>(each, in_bin, [&](float x, auto) { return scale.inside(x, bin); }, p.before, p.above, want,
                        [&](uint64_t) { return target; });
       sub = p.bin;
     }
-    auto here = [&](float x) __attribute__((always_inline)) { return in_bin(x) && (sub < 0 || scale.inside(x, bin) == sub); };
+    auto here = [&](float x, auto of) __attribute__((always_inline)) {
+      return in_bin(x, of) && (sub < 0 || scale.inside(x, bin) == sub);
+    };
     if (p.inside <= NT) {  // sorted, one a thread
       const int tid = threadIdx.x;
       if (tid == 0) l.n = 0;
       __syncthreads();
-      each([&](int, float x, auto) __attribute__((always_inline)) {
-        if (here(x)) l.list[1][atomicAdd(&l.n, 1u)] = order_of(x);
+      each([&](int, float x, auto of) __attribute__((always_inline)) {
+        if (here(x, of)) l.list[1][atomicAdd(&l.n, 1u)] = order_of(x);
       });
       __syncthreads();
       const int n = (int)l.n;
@@ -478,12 +499,12 @@ struct Drawer {
       const int bits = pass == 2 ? 10 : 11;
       for (int i = threadIdx.x; i < SM_DIGITS; i += NT) l.count[i] = 0, l.mass[i] = 0;
       __syncthreads();
-      each([&](int, float x, auto weight) __attribute__((always_inline)) {
+      each([&](int, float x, auto of) __attribute__((always_inline)) {
         const uint32_t key = order_of(x);
-        if (here(x) && (pass == 0 || key >> (shift + bits) == prefix)) {
+        if (here(x, of) && (pass == 0 || key >> (shift + bits) == prefix)) {
           const uint32_t d = SM_DIGITS - 1 - (key >> shift & ((1u << bits) - 1));  // falling
           atomicAdd(&l.count[d], 1u);
-          if (MASS) atomicAdd((unsigned long long*)&l.mass[d], (unsigned long long)weight());
+          if (MASS) atomicAdd((unsigned long long*)&l.mass[d], (unsigned long long)of.weight());
         }
       });
       __syncthreads();
@@ -510,19 +531,19 @@ struct Drawer {
   // top_k's cut among the tokens of `each`
   template <class Each>
   __device__ __forceinline__ Cut cut_by_count(Each each) {
-    auto any = [](float) { return true; };
-    const Place p = locate<false>(each, any, [&](float x) { return scale.bin(x); }, 0, 0, (uint64_t)s.top_k,
+    auto any = [](float, auto) { return true; };
+    const Place p = locate<false>(each, any, [&](float, auto of) { return of.bin(); }, 0, 0, (uint64_t)s.top_k,
                                   [](uint64_t) { return 0.0; });
     return resolve<false>(each, any, p, (uint64_t)s.top_k, 0.0);
   }
   // top_p's among those that `top` (of top_k, or of all) keeps
   template <class Each>
   __device__ __forceinline__ Cut cut_by_mass(Each each, const Cut& top) {
-    auto take = [&](float x) __attribute__((always_inline)) { return order_of(x) >= top.key; };
+    auto take = [&](float x, auto) __attribute__((always_inline)) { return order_of(x) >= top.key; };
     const uint32_t dropped = top.equal - top.ties;
     const uint64_t off = dropped ? dropped * weight(value_of(top.key)) : 0;
     double target = 0.0;
-    const Place p = locate<true>(each, take, [&](float x) { return scale.bin(x); }, 0, 0, 0,
+    const Place p = locate<true>(each, take, [&](float, auto of) { return of.bin(); }, 0, 0, 0,
                                  [&](uint64_t all) { return target = target_of(all - off); });
     return resolve<true>(each, take, p, 0, target);
   }
@@ -542,22 +563,21 @@ struct Drawer {
     const double y = x == m ? 0.0 : ((double)x - (double)m) / (double)s.temperature;
     a.logprobs[row] = (float)(y - log((double)total / (double)(1ull << a.shift)));
   }
-  // The token at which the kept weights, `cum` of them and `upto` ties before this thread's tokens, pass r: f(i) is the
-  // thread's i-th of n neighbouring tokens from `index` on
-  template <class F>
+  // The token at which the kept weights, `cum` of them and `upto` ties before this thread's tokens, pass r: one of its n
+  // neighbouring ones from `index` on
+  template <int N>
   __device__ __forceinline__ void pick(const Cut& cut, uint64_t tie_w, uint64_t cum, uint64_t upto, uint64_t r, uint64_t total,
-                                       int index, int n, F f) {
-    for (int i = 0; i < n; ++i) {
-      uint64_t w;
-      const float x = f(i, w);
-      const uint32_t key = order_of(x);
-      if (key > cut.key) cum += kept(w);
-      else if (key == cut.key) cum += upto++ < cut.ties ? tie_w : 0;
-      if (cum > r) {
-        draw(index + i, x, total);
-        break;
-      }
+                                       int index, int n, const float (&x)[N], const uint64_t (&w)[N]) const {
+    int at = -1;
+    float x_at = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t key = order_of(x[i]);
+      if (i < n && key > cut.key) cum += kept(w[i]);
+      else if (i < n && key == cut.key) cum += upto++ < cut.ties ? tie_w : 0;
+      if (at < 0 && cum > r) at = i, x_at = x[i];
     }
+    draw(index + at, x_at, total);
   }
 };
 
@@ -621,34 +641,29 @@ __global__ __launch_bounds__(64 * NW) void sample_held_kernel(SampleArgs a) {
   }
   D d(l, a, s, row, m);
   uint64_t w[SM_HELD];
+  int bin[SM_HELD];
 #pragma unroll
-  for (int i = 0; i < SM_HELD; ++i) w[i] = d.weight(x[i]);
+  for (int i = 0; i < SM_HELD; ++i) w[i] = d.scale.weight(x[i], bin[i]);
   auto each = [&](auto f) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < SM_HELD; ++i)
-      if (i < n) f(i0 + i, x[i], [&]() { return w[i]; });
+      if (i < n) f(i0 + i, x[i], Formed{w[i], bin[i]});
   };
   Cut cut = {0, (uint32_t)a.vocab, (uint32_t)a.vocab};
   if (s.top_k) cut = d.cut_by_count(each);
   if (s.top_p < 1.0f) cut = d.cut_by_mass(each, cut);
   const uint64_t tie_w = d.tie_weight(cut);
   uint64_t sum = 0, ties = 0, sum_before, ties_before, sum_all, ties_all;
-  each([&](int, float x, auto weight) __attribute__((always_inline)) {
+  each([&](int, float x, auto of) __attribute__((always_inline)) {
     const uint32_t key = order_of(x);
-    if (key > cut.key) sum += d.kept(weight());
+    if (key > cut.key) sum += d.kept(of.weight());
     ties += key == cut.key;
   });
   d.scan(sum, ties, sum_before, ties_before, sum_all, ties_all);
   const uint64_t total = sum_all + D::ties_in(cut, 0, ties_all) * tie_w, r = d.drawn(total);
   const uint64_t cum = sum_before + D::ties_in(cut, 0, ties_before) * tie_w;
   if (cum <= r && cum + sum + D::ties_in(cut, ties_before, ties) * tie_w > r) {
-    d.pick(cut, tie_w, cum, ties_before, r, total, i0, n, [&](int i, uint64_t& wi) __attribute__((always_inline)) {
-      float y = x[0];
-      wi = w[0];
-#pragma unroll
-      for (int e = 1; e < SM_HELD; ++e) y = i == e ? x[e] : y, wi = i == e ? w[e] : wi;
-      return y;
-    });
+    d.pick(cut, tie_w, cum, ties_before, r, total, i0, n, x, w);
   }
 }
 
@@ -950,21 +965,21 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
     cut = {(uint32_t)l.found[0], (uint32_t)l.found[1], (uint32_t)l.found[1]};
   }
   auto each_found = [&](auto f) __attribute__((always_inline)) {
-    for (int i = lane; i < mine_n; i += 64) f(my_i[i], my_x[i], [&]() { return d.weight(my_x[i]); });
+    for (int i = lane; i < mine_n; i += 64) f(my_i[i], my_x[i], Unformed{d.scale, my_x[i]});
   };
   auto each = [&](auto f) __attribute__((always_inline)) {
     each_token<DT>(base, 0, a.vocab, tid, NT,
-                   [&](int i, float x) __attribute__((always_inline)) { f(i, x, [&]() { return d.weight(x); }); });
+                   [&](int i, float x) __attribute__((always_inline)) { f(i, x, Unformed{d.scale, x}); });
   };
   if (whole) {
     if (s.top_k) cut = d.cut_by_count(each);
     if (s.top_p < 1.0f) cut = d.cut_by_mass(each, cut);
   } else if (s.way == kCount) {
-    auto any = [](float) { return true; };
+    auto any = [](float, auto) { return true; };
     if (p.bin < SM_BINS) cut = d.template resolve<false>(each_found, any, p, (uint64_t)s.top_k, 0.0);
     if (s.top_p < 1.0f) cut = d.cut_by_mass(each_found, cut);
   } else if (cuts && !few_found) {
-    auto any = [](float) { return true; };
+    auto any = [](float, auto) { return true; };
     cut = d.template resolve<true>(each_found, any, p, 0, target);
   }
   const uint64_t tie_w = d.tie_weight(cut);
@@ -1024,13 +1039,7 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
     d.scan(sum, ties, sum_before, ties_before, sum_all, ties_all);
     const uint64_t first = cum + sum_before + D::ties_in(cut, upto, ties_before) * tie_w;
     if (first <= r && first + sum + D::ties_in(cut, upto + ties_before, ties) * tie_w > r)
-      d.pick(cut, tie_w, first, upto + ties_before, r, total, i0, n_here, [&](int i, uint64_t& wi) __attribute__((always_inline)) {
-        float y = x[0];
-        wi = w[0];
-#pragma unroll
-        for (int e = 1; e < PER; ++e) y = i == e ? x[e] : y, wi = i == e ? w[e] : wi;
-        return y;
-      });
+      d.pick(cut, tie_w, first, upto + ties_before, r, total, i0, n_here, x, w);
     cum += sum_all + D::ties_in(cut, upto, ties_all) * tie_w;
     upto += ties_all;
     if (cum > r) break;
