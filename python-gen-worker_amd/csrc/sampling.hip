@@ -608,8 +608,8 @@ __device__ __forceinline__ float wave_max(float m) {
 }
 
 // Rows that fit a workgroup's registers: SM_HELD neighbouring tokens a thread, read once. Bound by its chain of barriers and
-// scans: one row of 2048 with a top_p 9.7 us (a top_k as well 12), 1024 such rows 22. With 16 waves for such a row as well: 13
-// and 41; rows of 8192 by the three kernels below: 64 of them 20 us instead of 15, 1024 62 instead of 55.
+// scans: one row of 2048 with a top_p 8.8 us, 1024 such rows 20. With 16 waves for such rows as well, 41 (one of them with a
+// top_k too: 13 where four waves take 11.5); rows of 8192 by the three kernels below: 64 of them 20 us instead of 15, 1024 62 instead of 55.
 template <int DT, int NW>
 __global__ __launch_bounds__(64 * NW) void sample_held_kernel(SampleArgs a) {
   using D = Drawer<NW>;
@@ -694,7 +694,7 @@ __device__ __forceinline__ float row_max(const SampleArgs& a, int64_t row) {
 }
 
 // second: every part's histogram, of tokens or of their weight, as sums up to each bin. Bound by the weights' arithmetic in
-// 64 bits (the logits come from the last-level cache): 256 rows of 131072 37 us, 3.6 TB/s; 64 of bf16 10 us.
+// 64 bits, 33 vector instructions a logit (the logits come from the last-level cache): 256 rows of 131072 37 us, 3.6 TB/s; 64 of bf16 10 us.
 template <int DT>
 __global__ __launch_bounds__(256) void sample_bins_kernel(SampleArgs a) {
   __shared__ uint64_t bin[SM_BINS];
@@ -742,8 +742,8 @@ __global__ __launch_bounds__(256) void sample_bins_kernel(SampleArgs a) {
 // or that lie where the cuts fall (kMass) are collected in one pass of comparisons and the cut found among them; the kept
 // weight of every part; and the tokens of the part that the random number falls into. Where the collected ones are too
 // many (thousands of nearly equal logits, a very large top_k) all is done by passes over the row.
-// 256 rows of 131072, fp32, a top_p: 42 us, of which 20 read the row once more (6.7 TB/s), 7 find the cut among some 800
-// tokens, 6 the drawn token in its part; 64 rows of bf16, each with settings of its own: 27, the slowest row's. Bound by
+// 256 rows of 131072, fp32, a top_p: 41 us, of which 20 read the row once more (6.7 TB/s), 7 find the cut among some 800
+// tokens, 5 the drawn token in its part; 64 rows of bf16, each with settings of its own: 27, the slowest row's. Bound by
 // what one workgroup does in turn.
 template <int DT>
 __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
