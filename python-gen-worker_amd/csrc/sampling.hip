@@ -465,10 +465,13 @@ struct Drawer {
       if (tid == 0) l.n = 0;
       __syncthreads();
       each([&](int, float x, auto of) __attribute__((always_inline)) {
-        if (here(x, of)) l.list[1][atomicAdd(&l.n, 1u)] = order_of(x);
+        if (here(x, of)) {
+          const uint32_t i = atomicAdd(&l.n, 1u);
+          if (i < NT) l.list[1][i] = order_of(x);  // (more only of logits that are written meanwhile)
+        }
       });
       __syncthreads();
-      const int n = (int)l.n;
+      const int n = min((int)l.n, NT);
       const uint32_t key = sorted32<NT>(tid < n ? l.list[1][tid] : 0, n <= 64 ? 6 : 32 - __clz(n - 1), l.list);
       const uint64_t w = MASS && tid < n ? weight(value_of(key)) : 0;
       uint64_t before = 0, all;
@@ -518,7 +521,8 @@ struct Drawer {
       shift = pass == 0 ? 10 : 0;
       __syncthreads();
     }
-    return {prefix, MASS ? ties_to(target, p.above, digit_w / p.inside, p.inside) : (uint32_t)(want - p.before), p.inside};
+    const uint32_t equal = min(max(p.inside, 1u), (uint32_t)a.vocab);
+    return {prefix, MASS ? ties_to(target, p.above, digit_w / equal, equal) : (uint32_t)(want - p.before), equal};
   }
 
   static __device__ __forceinline__ float value_of(uint32_t key) {
@@ -1025,7 +1029,7 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
   const uint64_t pw = part_w[lane] + (whole ? 0 : part_ahead), pt = part_ties[lane];
   const uint64_t pw_end = wave_scan64(pw), pt_end = wave_scan64(pt);
   const uint64_t end = pw_end + D::ties_in(cut, 0, pt_end) * tie_w, total = lane64(end, 63), r = d.drawn(total);
-  const int at = __ffsll((unsigned long long)__ballot(end > r)) - 1;
+  const int at = max(__ffsll((unsigned long long)__ballot(end > r)) - 1, 0);
   uint64_t upto = lane64(pt_end - pt, at), cum = lane64(pw_end - pw, at) + D::ties_in(cut, 0, upto) * tie_w;
   // that part's tokens, PER neighbouring ones a thread at a time
   const int end_at = min((at + 1) * a.part, a.vocab);
