@@ -503,8 +503,9 @@ bool cache_fits(const Tensor& k, const Tensor& v, const Tensor& w, const Tensor&
   const at::Device dev = k.device();
   const at::ScalarType type = values.value_or(k.scalar_type());
   if (!k.is_cuda() || k.layout() != at::kStrided || (type != at::kBFloat16 && type != at::kHalf) ||
-      (values.has_value() && k.scalar_type() != at::kFloat8_e4m3fn) || k.dim() != 4 || k.stride(3) != 1 || v.scalar_type() != k.scalar_type() || v.device() != dev ||
-      v.layout() != at::kStrided || !v.sizes().equals(k.sizes()) || !v.strides().equals(k.strides()) ||
+      (values.has_value() && k.scalar_type() != at::kFloat8_e4m3fn) || k.dim() != 4 || k.stride(3) != 1 ||
+      v.scalar_type() != k.scalar_type() || v.device() != dev || v.layout() != at::kStrided ||
+      !v.sizes().equals(k.sizes()) || !v.strides().equals(k.strides()) ||
       kv_len.dim() != 1 || table.dim() != 2)
     return false;
   const int64_t batch = kv_len.size(0);

@@ -112,6 +112,8 @@ class PagedDecoder(nn.Module):
             raise PagedError("generate: every prompt needs a token, and the answer one")
         if max(len(p) for p in prompts) + new_tokens > self.cfg.positions:
             raise PagedError(f"generate: more than {self.cfg.positions} positions")
+        if any(isinstance(x, Tensor) for x in (temperature, top_k, top_p, min_p)):
+            raise PagedError("generate: temperature, top_k, top_p and min_p are numbers, the same for every prompt")
         settings(temperature, top_k, top_p, min_p)   # refused before anything runs
         held = [len(p) + new_tokens for p in prompts]
         if budget is not None:

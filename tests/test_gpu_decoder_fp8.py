@@ -98,12 +98,16 @@ def test_drawn_answers(dtype):
 
 def test_drawing_refuses():
     from gen_worker_amd.decoder import PagedDecoder
+    from gen_worker_amd.paged import PagedError
     from gen_worker_amd.sampling import SamplingError
 
     model = PagedDecoder(_config(layers=1), "bf16")
     for bad in (dict(temperature=-1.0), dict(temperature=1.0, top_p=1.5), dict(temperature=1.0, top_k=-2), dict(top_k=2.5)):
         with pytest.raises(SamplingError):
             model.generate([[1]], 1, **bad)
+    for bad in (dict(temperature=torch.ones(2, device="cuda")), dict(temperature=1.0, top_p=torch.ones(2))):
+        with pytest.raises(PagedError, match="numbers"):
+            model.generate([[1], [2]], 1, **bad)
 
 
 def test_the_command_runs(monkeypatch, capsys):
