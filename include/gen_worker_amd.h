@@ -655,8 +655,8 @@ int gwa_paged_evict(const gwa_paged_cache* cache, const int32_t* new_table, int6
  * (bf16: every one exactly; fp16: what it cannot hold overflows or is rounded).
  * A row is written with the smallest power of two, 2^-126 at least, under which none of
  * its finite values passes 448, the largest code; a value is rounded to the nearest code
- * (ties to even), but never past the type's largest finite one; what is not finite
- * becomes NaN. */
+ * (ties to even), but never past the type's largest finite one, and a key that its
+ * rotation takes past that one counts as it; what is not finite becomes NaN. */
 typedef struct gwa_paged_scales {
   uint8_t* k;             /* [pages][kv_heads][page_size] at the strides below */
   uint8_t* v;             /* at the same strides */

@@ -8,7 +8,8 @@ constexpr int W8_THREADS = 512, R8_THREADS = 256;  // of a workgroup at most; of
 
 // A row's scale byte b from its largest finite magnitude (fp32 bits), 2^(127 - b), and the largest code magnitude. 448 * 2^e
 // >= amax holds from e = floor(log2 amax) - 8 on, or one more where amax's fraction passes that of 448 = 1.75 * 2^8. At
-// the type's last binade 256 * 2^e would be infinite: there codes end at 240.
+// the type's last binade 256 * 2^e would be infinite: there codes end at 240. A rotation may take a key past the type's
+// range, by tables longer than 1; it counts as the type's largest value then, whose byte is kTop.
 struct RowScale {
   uint32_t byte;
   float inverse, most;
@@ -16,11 +17,11 @@ struct RowScale {
 template <int DT>
 __device__ __forceinline__ RowScale row_scale(uint32_t amax) {
   constexpr int kTop = DT == GWA_DT_BF16 ? 247 : 135;
-  const int b = max((int)(amax >> 23) - 8 + ((amax & 0x7fffffu) > 0x600000u), 1);
-  return {(uint32_t)b, __uint_as_float((uint32_t)(254 - b) << 23), b >= kTop ? 240.0f : 448.0f};
+  const int b = min(max((int)(amax >> 23) - 8 + ((amax & 0x7fffffu) > 0x600000u), 1), kTop);
+  return {(uint32_t)b, __uint_as_float((uint32_t)(254 - b) << 23), b == kTop ? 240.0f : 448.0f};
 }
 // x under its row's scale, for the conversion, which rounds to nearest (ties to even) and takes infinities and NaN to NaN.
-// No finite value of the row passes 448.
+// No finite value of the row passes 448 (held_to).
 __device__ __forceinline__ float scaled(float x, const RowScale& s) { return x * s.inverse; }
 __device__ __forceinline__ uint2 codes8(const float (&x)[8], const RowScale& s) {
   uint32_t w[2];

@@ -513,7 +513,8 @@ def paged_write_fp8(q: Tensor, k: Tensor, v: Tensor, cos: Optional[Tensor], sin:
 
     A row of k (rotated, in fp32) or v takes as its scale the smallest power of two, from 2^-126 on, under which none of its
     finite values passes 448, the largest code: value = code * 2^(scale - 127). Values are rounded once, to the nearest
-    code (ties to even), and never past the largest finite value of q's type; what is not finite is stored as NaN."""
+    code (ties to even), and never past the largest finite value of q's type, as which a key counts that its rotation takes past
+    it; what is not finite is stored as NaN."""
     a = (q, k, v, cos, sin, positions, k_pages, v_pages, k_scales, v_scales, table, q_start, kv_len, weights)
     _no_tangents("paged_write_fp8", q, k, v, cos, sin, weights)
     host = _host()
