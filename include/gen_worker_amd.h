@@ -652,7 +652,8 @@ int gwa_paged_evict(const gwa_paged_cache* cache, const int32_t* new_table, int6
  * head_dim % 16 == 0, 16 .. 256), and every row (one slot of one kv head) has a scale
  * byte: value = code * 2^(scale - 127), a scale of 255 is NaN. The cache's `dtype` is
  * the type of the calls' q, k, v and o; the operators read a row's values in that type
- * (bf16: every one exactly; fp16: what it cannot hold overflows or is rounded).
+ * (bf16: exactly under the bytes 3 to 246; past them, and in fp16, what the type cannot
+ * hold is rounded, or infinite).
  * A row is written with the smallest power of two, 2^-126 at least, under which none of
  * its finite values passes 448, the largest code; a value is rounded to the nearest code
  * (ties to even), but never past the type's largest finite one, and a key that its

@@ -56,8 +56,8 @@ __device__ __forceinline__ int64_t paged_s_at(const PagedArgs& c, int page, int 
 }
 
 // Eight e4m3 codes under a row's scale as eight values of T, by the conversions that take a scale: its exponent field is
-// the scale byte, value = code * 2^(byte - 127) (byte 255: NaN). Exact in bf16, whose range holds every such value that a
-// bf16 row was quantised to; in fp16 rounded where it is subnormal.
+// the scale byte, value = code * 2^(byte - 127) (byte 255: NaN). Exact in bf16 under the bytes 3 (its least code stands for
+// 2^-133) to 246; past them, and in fp16, rounded where the type's subnormals do not hold the value, or infinite.
 __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
 template <class T>
 __device__ __forceinline__ v4i widen8(uint32_t lo, uint32_t hi, float s) {

@@ -557,9 +557,10 @@ def _(k_pages, v_pages, k_scales, v_scales, table, q_start, kv_len, tokens, dtyp
 
 def paged_read_fp8(k_pages: Tensor, v_pages: Tensor, k_scales: Tensor, v_scales: Tensor, table: Tensor, q_start: Tensor,
                    kv_len: Tensor, tokens: int, *, dtype: torch.dtype = torch.bfloat16) -> tuple[Tensor, Tensor]:
-    """What rows of an 8-bit cache stand for: (k, v) [tokens, kv_heads, head_dim] in ``dtype`` (bf16: exactly). Sequence b's
-    rows q_start[b] to q_start[b + 1] - 1 are those of its last slots, as ``paged_write_fp8`` takes them: with q_start the
-    running sums of kv_len, everything its sequences hold. ``tokens``: rows in all (q_start's last entry). Rows that belong
+    """What rows of an 8-bit cache stand for: (k, v) [tokens, kv_heads, head_dim] in ``dtype``: bf16 exactly under the
+    scale bytes 3 to 246, past them, and in fp16, rounded or infinite where the type does not hold the value. Sequence b's rows
+    q_start[b] to q_start[b + 1] - 1 are those of its last slots, as ``paged_write_fp8`` takes them: with q_start the running
+    sums of kv_len, everything its sequences hold. ``tokens``: rows in all (q_start's last entry). Rows that belong
     to no sequence, or to slots before a sequence's first, are not written."""
     a = (k_pages, v_pages, k_scales, v_scales, table, q_start, kv_len)
     host = _host()

@@ -1,5 +1,6 @@
-"""The 8-bit paged cache where its format ends: keys that the rotation takes past their type's range. Tables
-of 2 and 0 turn nothing and scale exactly, so rows are equal to their definition, code for code."""
+"""The 8-bit paged cache where its format ends: keys that the rotation takes past their type's range, and
+which values a read gives back exactly. Tables of 2 and 0 turn nothing and scale exactly, so rows are equal to their definition,
+code for code."""
 
 from __future__ import annotations
 
@@ -7,7 +8,7 @@ import pytest
 import torch
 
 from test_gpu_paged import BF16, DEV, F16, _gen, _ints
-from test_gpu_paged_fp8 import FP8, held
+from test_gpu_paged_fp8 import FP8, held, value_of
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +64,18 @@ def test_keys_that_the_rotation_takes_past_the_type(dtype, rot, interleaved, odd
     if dtype == F16:                                  # (bf16's products with such keys pass fp32)
         o, lse = paged_attention_fp8((q * 2.0 ** -9).to(dtype), *pool, table, start, length, n, n)
         assert bool(o.isfinite().all()) and bool(lse.isfinite().all())
+
+
+def test_bf16_reads_exactly_what_it_can_hold():
+    """Every finite code under the scale bytes 3 to 246 is a bf16 number, and read as it is; past them the nearest one, or
+    infinity."""
+    from gen_worker_amd.paged import paged_read_fp8
+
+    codes = torch.arange(256, device=DEV, dtype=torch.uint8).view(1, 1, 16, 16).expand(256, 1, 16, 16).contiguous()
+    scales = torch.arange(256, device=DEV, dtype=torch.uint8).view(256, 1, 1).expand(256, 1, 16).contiguous()
+    table = torch.arange(256, device=DEV, dtype=torch.int32).view(1, 256)
+    k, _ = paged_read_fp8(codes.view(FP8), codes.view(FP8), scales, scales, table, _ints([0, 4096]), _ints([4096]), 4096)
+    got, want = k.view(256, 16, 16).double(), value_of(codes, scales)[:, 0]
+    assert torch.equal(got[3:247].nan_to_num(), want[3:247].nan_to_num())
+    assert not torch.equal(got[2].nan_to_num(), want[2].nan_to_num()) and bool(got[247].isinf().any())
+    assert torch.equal(got.nan_to_num(), want.to(BF16).double().nan_to_num())
