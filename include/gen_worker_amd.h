@@ -702,8 +702,10 @@ int gwa_paged_evict_fp8(const gwa_paged_cache* cache, const gwa_paged_scales* sc
  * the first always stays. The token is the first i, in the vocabulary's order, at which
  * the kept weights up to and with w_i pass uniform * their sum; its logprob is
  * log(w_i / sum) (fp32). temperature 0 takes the largest (logprob 0).
- * Weights are integers of 2^-45 of the largest (of fewer bits over 131072 tokens),
- * formed in 64 bits, and so are sums: no order of summation changes a result.
+ * Weights are integers of a unit, 2^-45 of the largest (2^-(62 - bits) past 2^17 tokens, a
+ * vocabulary of `bits` bits), formed in 64 bits, and so are sums: no order of summation
+ * changes a result. What weighs less than half a unit is never drawn: all of it together is
+ * less than vocab / 2 units, 2^-29 of the largest weight at 2^17 tokens, 2^-15 at 2^24.
  * -inf and NaN are never drawn; a row that holds nothing else gives token -1 and
  * logprob NaN. Of several +inf each has weight 1, and nothing else has any.
  * Settings are arrays [rows] or, where the pointer is NULL, the number beside it; from

@@ -83,8 +83,9 @@ __device__ __forceinline__ void fill_table(double* table, int shift) {
 // A row's tokens by their weight exp((x - m) / temperature) = 2^y, y = (x - m) log2(e) / temperature in 64 bits. The weight
 // is an integer of 2^-shift: 2^y = 2^n 2^(j/512) 2^r, |r| <= 1/1024, by a table (which holds the 2^shift) and the series of
 // 2^r to r^3 (the rest is below 2^-46), rounded by an addition of 2^52. Bins are an eighth of a unit of y wide; the last is
-// for what weighs nothing: y < -47, -inf and NaN. Bins and their halves (`inside`) fall as x grows, never the other way. A token's weight and
-// bin have to be the same wherever they are formed, so the compiler may not choose where products and sums are fused.
+// for what weighs nothing: y < -47, -inf and NaN. Bins, and the SM_BINS parts of one (`inside`), fall as x grows, never the other
+// way. A token's weight and bin have to be the same wherever they are formed, so the compiler may not choose where products and
+// sums are fused.
 // m = +inf is held as 1e300: +inf is then at y = 0, all else far below.
 struct Scale {
   double c, m;

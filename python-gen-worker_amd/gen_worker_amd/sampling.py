@@ -109,8 +109,9 @@ def sample_tokens(logits: Tensor, uniform: Tensor, *, temperature: Union[float, 
 
     A setting is a number, or a tensor [rows] (top_k int32, the others fp32) with one for each row, whose values out of
     range count as the nearest in it (a NaN as 0). Settings are fp32. -inf and NaN are never drawn; a row with nothing else
-    gives token -1 and logprob NaN. Weights and sums are integers in 64 bits: the result does not depend on how the work is
-    split. No gradient is defined."""
+    gives token -1 and logprob NaN. Weights and sums are integers in 64 bits, of 2^-45 of the largest weight (2^-38 at
+    2^24 tokens; half of that or less is never drawn), so the result does not depend on how the work is split. No gradient is
+    defined."""
     each, numbers = settings(temperature, top_k, top_p, min_p)
     a = (logits, uniform, *each)
     _require(all(paged._tangent(x) is None for x in a), "no gradient is defined for a dual tensor's tangent")
