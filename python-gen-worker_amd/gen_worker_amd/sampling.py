@@ -18,6 +18,7 @@ from . import paged
 
 _DTYPES = {torch.bfloat16: nat.DT_BF16, torch.float16: nat.DT_F16, torch.float32: nat.DT_F32}
 MAX_VOCAB = 1 << 24
+MAX_TOP_K = (1 << 31) - 1
 
 
 class SamplingError(ValueError):
@@ -50,6 +51,7 @@ def _sample_body(logits: Tensor, uniform: Tensor, temperature: Optional[Tensor],
                            ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
                            ("min_p", min_p, torch.float32)):
         _column(what, t, dtype, rows, dev)
+    _require(0 <= all_top_k <= MAX_TOP_K, f"top_k must be 0 to {MAX_TOP_K}, got {all_top_k}")
     if vocab > 1 and logits.stride(1) != 1 or rows > 1 and logits.stride(0) < vocab:
         logits = logits.contiguous()
     tokens = torch.empty(rows, dtype=torch.int64, device=dev)
@@ -91,7 +93,7 @@ def _setting(value, plain, what: str, low, high):
 
 def settings(temperature, top_k, top_p, min_p) -> tuple[tuple, tuple]:
     """``sample_tokens``' settings, checked: (tensors, None for numbers; numbers, a default for tensors)."""
-    pairs = (_setting(temperature, 1.0, "temperature", 0.0, 3.0e38), _setting(top_k, 0, "top_k", 0, (1 << 31) - 1),
+    pairs = (_setting(temperature, 1.0, "temperature", 0.0, 3.0e38), _setting(top_k, 0, "top_k", 0, MAX_TOP_K),
              _setting(top_p, 1.0, "top_p", 0.0, 1.0), _setting(min_p, 0.0, "min_p", 0.0, 1.0))
     return tuple(t for t, _ in pairs), tuple(n for _, n in pairs)
 

@@ -142,3 +142,18 @@ def test_random_rows(vocab, dtype):
             # (a total off by d moves its logarithm by at most d / (total - d))
             d = e + (3 * e + border if border else 0.0) + total * 2.0 ** -44
             assert abs(float(lps[r]) - lp) <= 2.0 ** -24 * abs(lp) + d / (total - d), (s, r, t)
+
+
+def test_the_registered_op_refuses_a_top_k_past_32_bits():
+    """As the function does: 2^32 + 1 is not 1."""
+    from gen_worker_amd.sampling import SamplingError, sample_tokens
+
+    x, u = torch.randn(2, 50, generator=_gen(1), device=DEV), torch.tensor([0.1, 0.9], device=DEV)
+    op = torch.ops.cozy_gen_worker.sample_tokens
+    for k in ((1 << 32) + 1, 1 << 31, -1):
+        with pytest.raises(SamplingError, match="top_k"):
+            op(x, u, None, None, None, None, 1.0, k, 1.0, 0.0)
+        with pytest.raises(SamplingError, match="top_k"):
+            sample_tokens(x, u, top_k=k)
+    got = op(x, u, None, None, None, None, 1.0, (1 << 31) - 1, 1.0, 0.0)
+    assert all(torch.equal(a, b) for a, b in zip(got, sample_tokens(x, u)))
