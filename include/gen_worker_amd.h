@@ -679,7 +679,8 @@ int gwa_paged_write_fp8(const gwa_paged_cache* cache, const gwa_paged_scales* sc
 int gwa_paged_read_fp8(const gwa_paged_cache* cache, const gwa_paged_scales* scales, void* k_out, void* v_out,
                        int64_t tokens, void* stream);
 
-/* gwa_paged_attention over such a cache. */
+/* gwa_paged_attention over such a cache: k and v are what its rows stand for, rounded to the
+ * dtype before the products where it does not hold them. */
 int64_t gwa_paged_attention_fp8_workspace(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
                                           int64_t head_dim, int64_t max_q, int64_t max_kv, int64_t capacity,
                                           int gather);

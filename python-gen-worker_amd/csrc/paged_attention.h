@@ -196,9 +196,11 @@ __global__ __launch_bounds__(64) void paged_gather_rows_kernel(PagedArgs c, cons
 // every MFMA waited for the LDS read issued just ahead of it (1057 us); both waves of a SIMD in the same phase take 1013;
 // 128-key tiles spill and take 1710. Of an 8-bit cache (E8) the rows pass through registers, where they become 16-bit values
 // on their way to LDS, a tile ahead: one conversion for two values, again for each row tile; 2048 tokens over 16500 keys
-// (525 GFLOP) take 550 to 605 us where a 16-bit cache takes 515 to 540. Five sequences of up to 509 tokens over up to 4001
-// keys, 16 heads of 64: 35 us, in which nothing is busy (matrix cores 11 %, vector unit 27 %, LDS 7 %): a tile has half the work between the same two barriers, and
-// 2 waves a SIMD do not cover what each waits for (38 us of an 8-bit cache).
+// (525 GFLOP) take 550 to 567 us where a 16-bit cache takes 500 in the same run. Those registers come on top: at head_dim
+// 128 the form of 4 waves spills 30 of a lane (16 tokens for each of 32 sequences over up to 8192 keys, 32 heads over 8: 100
+// us, a 16-bit cache 102), that of 8 waves 3. Five sequences of up to 509 tokens over up to 4001 keys, 16 heads of 64: 34 us,
+// in which nothing is busy (matrix cores 11 %, vector unit 27 %, LDS 7 %): a tile has half the work between the same two
+// barriers, and 2 waves a SIMD do not cover what each waits for (37 us of an 8-bit cache).
 template <int D, int BN, int NW>
 struct TileShape {
   static constexpr int kRow = 2 * D, kRun = 1024 / kRow;  // row bytes; rows a 1 KB copy covers
@@ -672,10 +674,13 @@ __global__ __launch_bounds__(256) void paged_attn_join_parts_kernel(AttnArgs a) 
 // their join before the shares); 4 tokens each over up to 8192 keys 88 us with the join, 8 tokens 101 (floors 76 and 85); one
 // sequence of 701 keys, 32 heads over 8, 9 to 10 us and 3.9 for the join (medians): launch and four dependent loads.
 // Of an 8-bit cache (E8) two tiles are in flight in registers, K's codes as the operands need them and V's on to LDS as
-// 16-bit values. The 32 sequences of up to 32768 keys: 162 us, 4.9 TB/s (169 to 170 a call with the join); the same loads
+// 16-bit values. The 32 sequences of up to 32768 keys: 163 us, 4.9 TB/s (170 a call with the join); the same loads
 // without any work on them 153. One scale byte a lane, given out by lane moves, and places found by the wave: 179 us of a
-// call with every lane loading its rows' own. The sequence of 701 keys: 9.2 us and 3.8; a workgroup of 8 waves for all its
+// call with every lane loading its rows' own. The sequence of 701 keys: 9.0 us and 3.1; a workgroup of 8 waves for all its
 // keys, with no join: 11.6 to 12.5, so there is none.
+// Two row blocks (17 to 32 rows) at head_dim 128 do not fit an 8-bit cache's registers: two tiles in flight, V's operands read
+// ahead and O spill 125 to 128 of a lane (one block 5 to 15, heads of 64 at most 6, the 16-bit form none). 8 tokens for each of
+// 32 sequences over up to 8192 keys, 32 heads over 8: 240 us where a 16-bit cache takes 101; 4 tokens, one block: 58 and 80.
 constexpr int FW_KEYS = 32, FW_PAGES = 512;  // keys a tile; page ids staged at a time (whole tiles: page_size >= 8)
 constexpr int FW_WAVES = 4, FW_UNIT = FW_KEYS * FW_WAVES;
 // Where the segment of a run that starts at key s_lo ends, at k_hi at the latest: behind the FW_PAGES-th page from that of
@@ -940,7 +945,8 @@ __global__ __launch_bounds__(64 * FW_WAVES, E8 ? 2 : 1) void paged_attn_few_kern
       if constexpr (E8) {
         // tiles wave, wave + NW, ...: two in flight, in registers of their own. The loads go out whether or not there is such
         // a tile (past the end they repeat the last key), so that how many are outstanding is known wherever one is waited
-        // for: with conditions around them every wait is for all
+        // for: with conditions around them every wait is for all. (Two tiles' loads a wave are repeated so: next to nothing of
+        // a long run, half of all of a split of 256 keys, whose lines are in the caches then)
         FewRaw<D> w0, w1;
         auto tile = [&](int t, FewRaw<D>& w) __attribute__((always_inline)) {
           if (whole(t)) step(t, w, std::false_type{});
@@ -1337,7 +1343,7 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int
     const int64_t tt = p.tile_rows / group, tiles = ((max_q < 1 ? 1 : max_q) + tt - 1) / tt;
     const int64_t row_tiles = kv_heads * std::min(batch * tiles, tokens / tt + batch), units = (max_kv + 63) / 64;
     // (two workgroups a CU where they fit; 8-bit rows leave fewer bytes in flight a wave: 16 rows over up to 32768 keys of 32
-    // sequences take 170 us with two and 178 with one)
+    // sequences take 170 us with two and 178 with one, heads of 64 90 and 124)
     p.shares = p.tile_rows == 128 || (E8 && p.tile_rows == 16) ? 2 * kCus : kCus;
     // Many rows: a workgroup a row tile where that takes no longer. 64 keys take it about 2 us, and it goes through
     // whole rounds of workgroups; shares always end together, but take 8 us to find and to join and 6 % more for

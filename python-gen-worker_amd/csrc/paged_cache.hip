@@ -11,7 +11,7 @@ namespace {
 constexpr int RT_THREADS = 256;
 
 // A thread a unit; the tables' rows are shared by a token's heads in L1. 16411 tokens, 24 heads of 128, half of each head
-// rotated, bf16: 41 us for 202 MB, 4.9 TB/s; fp32 91 us for 403 MB, 4.4 TB/s.
+// rotated, bf16: 38 to 39 us for 202 MB, 5.2 TB/s; fp32 91 us for 403 MB, 4.4 TB/s.
 template <int DT, bool VEC>
 __global__ __launch_bounds__(RT_THREADS) void rotary_kernel(const void* x, int64_t ldxt, int64_t ldxh, void* y,
                                                             int64_t ldyt, int64_t ldyh, Rotation r, int64_t tokens,
@@ -25,7 +25,8 @@ __global__ __launch_bounds__(RT_THREADS) void rotary_kernel(const void* x, int64
 }
 
 // One workgroup a token: its query heads into q_out, its key and value heads into the token's slot, which the whole
-// workgroup looks up once. 10475 tokens with 16 + 2 x 16 heads of 64: 22 us for 130 MB, 5.9 TB/s; 48 tokens 4.3 us.
+// workgroup looks up once. 10475 tokens with 16 + 2 x 16 heads of 64: 22 us for 130 MB, 5.9 TB/s, on the same
+// inputs again and again; on three sets in turn 27 to 28. 48 tokens 4.3 us.
 template <int DT, bool VEC>
 __global__ __launch_bounds__(RT_THREADS) void paged_write_kernel(PagedArgs c, const uint16_t* q, int64_t ldqt,
                                                                  int64_t ldqh, const uint16_t* k, int64_t ldkt,
@@ -292,8 +293,9 @@ __global__ __launch_bounds__(EV_THREADS) void evict_select_kernel(PagedArgs c, i
 
 constexpr int EC_THREADS = 256;
 
-// Kept rows into the new pages: a row of k and v is head_dim / 8 pieces of 16 bytes, one piece of both a thread. 252 k rows of
-// 128 (257 MB read and written): 44 to 46 us, 5.6 to 5.8 TB/s.
+// Kept rows into the new pages: a row of k and v is head_dim / 8 pieces of 16 bytes (16 of an 8-bit cache), one piece of both
+// a thread. 252 k rows of 128 (257 MB read and written), the same ones again and again: 44 to 46 us, 5.6 to 5.8 TB/s; three
+// sets in turn: 55, of an 8-bit cache 32.
 __global__ __launch_bounds__(EC_THREADS) void evict_copy_kernel(PagedArgs c, const int32_t* new_table,
                                                                 int64_t new_stride, int new_capacity,
                                                                 const int32_t* kept, int budget, int pieces) {

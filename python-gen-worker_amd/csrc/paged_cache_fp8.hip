@@ -62,8 +62,8 @@ __device__ __forceinline__ float group_max(float x, int n) {
 // has a run of neighbouring tokens, whose codes and scale bytes share lines in its L2.
 // Bytes bound it, and on the way there the chain of dependent loads: the slot's three are scalar loads that no wait for a row
 // falls among (as vector loads behind the row's: 4 us more), and the tables' go out before the row's are waited for.
-// Measured: 10475 prompt tokens, 16 / 16 heads of 64, half of each rotated, fp16: 27 us, 4.0 TB/s; 8192 tokens, 32 / 8
-// heads of 128: 37.5 us, 4.9 TB/s, without VEC 100; 48 tokens of as many sequences 4.0 us, without VEC 8.0. Workgroups
+// Measured: 10475 prompt tokens, 16 / 16 heads of 64, half of each rotated, fp16: 27 to 28 us, 3.9 TB/s; 8192 tokens, 32 / 8
+// heads of 128: 37.5 us, 4.9 TB/s, without VEC 100; 48 tokens of as many sequences 4.5 us, without VEC 8.0. Workgroups
 // of 256 threads whatever the rows are: 34.5 us of the prompts where this form then took 31; two or four
 // tokens a workgroup: 31 to 38; a limit of 64 registers, for 8 waves a SIMD: spills, 30.
 template <int DT, bool VEC>

@@ -700,7 +700,7 @@ __device__ __forceinline__ float row_max(const SampleArgs& a, int64_t row) {
 }
 
 // second: every part's histogram, of tokens or of their weight, as sums up to each bin. Bound by the weights' arithmetic in
-// 64 bits, 31 vector instructions a logit (the logits come from the last-level cache): 256 rows of 131072 36 us, 3.7 TB/s; 64
+// 64 bits, 31 vector instructions a logit (the logits come from the last-level cache): 256 rows of 131072 35 us, 3.8 TB/s; 64
 // of bf16 10 us. All of a load's weights formed ahead of the branches: 35 to 36.5 and 11.
 template <int DT>
 __global__ __launch_bounds__(256) void sample_bins_kernel(SampleArgs a) {

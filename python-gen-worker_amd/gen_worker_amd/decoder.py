@@ -106,8 +106,9 @@ class PagedDecoder(nn.Module):
                  temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0,
                  seed: int = 0) -> list[list[int]]:
         """Answers of ``new_tokens`` tokens to each prompt, all in one batch: greedy, or with a ``temperature`` drawn
-        (``sample_tokens``) by random numbers of the ``seed``. ``budget``: keys a layer keeps of a sequence, the last
-        ``recent`` among them. ``dtype``: of the caches (``torch.float8_e4m3fn``: 8 bits)."""
+        (``sample_tokens``) by random numbers of the ``seed``: -1 where a step's logits are all -inf or NaN, after which the
+        rest of that answer means nothing. ``budget``: keys a layer keeps of a sequence, the last ``recent`` among them.
+        ``dtype``: of the caches (``torch.float8_e4m3fn``: 8 bits)."""
         if not prompts or not all(len(p) for p in prompts) or new_tokens < 1:
             raise PagedError("generate: every prompt needs a token, and the answer one")
         if max(len(p) for p in prompts) + new_tokens > self.cfg.positions:

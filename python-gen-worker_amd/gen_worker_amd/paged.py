@@ -408,7 +408,9 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, 
 
     Query head x reads kv head x // (heads / kv_heads). With ``causal`` token i of n in a sequence of L keys sees the
     first L - n + i + 1, else all L; a row that sees none, or scores of -inf alone, gives o = 0 and lse = -inf, one that
-    sees a NaN score NaN. ``scale`` defaults to head_dim^-0.5. ``max_q`` and ``max_kv``: the batch's largest new-token count and kv_len, which choose the launch.
+    sees a NaN score NaN. ``scale`` defaults to head_dim^-0.5. ``max_q`` and ``max_kv``: the batch's largest new-token count
+    and kv_len, which choose the launch. Scores, statistics and sums are fp32; at head_dim 64 and 128 the probabilities are
+    rounded to q's type for their product with the values, since the matrix cores' operands are.
     ``weights`` fp32 [pages, kv_heads, page_size]: every key's slot gets, added, the probability it drew from the
     sequence's new tokens over the kv head's query heads, in an order that does not depend on timing; sequences may
     share pages only without it. head_dim: a multiple of 8 up to 256 (the matrix cores serve 64 and 128, up to 256 query
@@ -589,8 +591,9 @@ def _(q, k_pages, v_pages, k_scales, v_scales, table, q_start, kv_len, max_q, ma
 def paged_attention_fp8(q: Tensor, k_pages: Tensor, v_pages: Tensor, k_scales: Tensor, v_scales: Tensor, table: Tensor,
                         q_start: Tensor, kv_len: Tensor, max_q: int, max_kv: int, *, scale: Optional[float] = None,
                         causal: bool = True, weights: Optional[Tensor] = None) -> tuple[Tensor, Tensor]:
-    """``paged_attention`` over an 8-bit cache (see ``paged_write_fp8``): keys and values are what its rows stand for, in
-    q's type (bf16 or fp16; a scale byte of 255 reads as NaN). head_dim: a multiple of 16 up to 256."""
+    """``paged_attention`` over an 8-bit cache (see ``paged_write_fp8``), its roundings among them: keys and values are what its
+    rows stand for, in q's type as ``paged_read_fp8`` gives them (bf16 or fp16; what fp16's subnormals do not hold is rounded
+    before the products; a scale byte of 255 reads as NaN). head_dim: a multiple of 16 up to 256."""
     if scale is None:
         scale = float(q.shape[-1]) ** -0.5
     _no_tangents("paged_attention_fp8", q, weights)
